@@ -318,6 +318,169 @@ tlh_status tlh_reshape_and_cache(const void *key, const void *value, void *k_cac
                                  const int64_t *slots, int32_t num_tokens, int32_t num_kv_heads, int32_t head_size,
                                  int32_t block_size, int64_t num_blocks, void *stream);
 
+/* ------------------------------------------------------ packed attention
+ * Causal attention of whole prompts packed one after another (a prefill of
+ * several sequences in one call, with no mask tensor and no padding). No
+ * counterpart in the reference, whose FLASH_ATTN_EXT takes a padded batch and a
+ * mask. `type` is TLH_TYPE_F16 or TLH_TYPE_BF16, of all four tensors:
+ *   q, out  [num_tokens][num_heads][head_size]
+ *   k, v    [num_tokens][num_kv_heads][head_size]
+ * a token's heads are contiguous, and q_stride, k_stride, v_stride and
+ * out_stride are the elements from one token to the next (multiples of 8; views
+ * of a fused QKV projection need no copy). Sequence s is the tokens
+ * seq_starts[s] .. seq_starts[s + 1] - 1 (i32 [num_seqs + 1] on the device, not
+ * decreasing; a sequence may be empty):
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (num_heads / num_kv_heads)]) v[j, ..]
+ * over the tokens j <= t of t's sequence. Scores, softmax and sums are f32; the
+ * softmax's numerators are rounded to the type for the product with v, the
+ * result once. A token sees nothing of the ones it does not attend to, whatever
+ * they hold (infinities and NaN too). Tokens behind the last sequence, and a
+ * sequence's tokens from max_seq_len on, are left as they were; starts outside
+ * [0, num_tokens] are taken as the nearer end. Pointers are 16-byte aligned;
+ * out must not overlap the inputs. head_size as for paged attention. */
+typedef struct tlh_packed_attention_args {
+    void *out;
+    const void *q;
+    const void *k;
+    const void *v;
+    const int32_t *seq_starts;
+    int64_t out_stride;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int32_t type;
+    int32_t num_seqs;
+    int32_t num_tokens;
+    int32_t max_seq_len;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_size;
+    float scale;
+} tlh_packed_attention_args;
+
+tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream);
+
+/* -------------------------------------------------------- tree attention
+ * Attention of a tree of drafted tokens over the paged cache (the verification
+ * step of speculative decoding; a chain of drafts is a tree too, and so is the
+ * next few tokens of a prompt). No counterpart in the reference. Layouts and
+ * geometry as for paged attention, the drafted tokens' keys and values already
+ * written to the cache (tlh_reshape_and_cache) as the last of context_lens:
+ *   q, out       f16 [num_rows][num_heads][head_size]
+ *   draft_starts i32 [num_seqs + 1]: sequence s has the rows draft_starts[s] ..
+ *                draft_starts[s + 1] - 1, n of them, at most max_drafts <= 64;
+ *                rows behind the last sequence are left as they were
+ *   draft_masks  i64 [num_rows]: bit j of a row's mask says that it sees its
+ *                sequence's drafted token j (its ancestors and itself)
+ * With L = context_lens[s], every row sees the tokens before L - n, and drafted
+ * token j at place L - n + j where its mask says so. f32 scores, softmax and
+ * sums, its numerators rounded to f16 for the product with v; a row that sees
+ * nothing gives zeros, and what a row does not see does not reach it, whatever
+ * it holds. num_blocks is the pools' length in blocks: tokens of a page
+ * outside it are not seen. Lengths are bounded by max_context_len, starts by
+ * num_rows, a sequence's rows by max_drafts. `scratch` holds the partials of a
+ * split context (tlh_tree_attention_scratch_bytes, 16-byte aligned; it may be
+ * NULL when that is 0); calls that share one must be stream-ordered. */
+typedef struct tlh_tree_attention_args {
+    void *out;
+    const void *q;
+    const void *k_cache;
+    const void *v_cache;
+    const int32_t *block_tables;
+    const int32_t *context_lens;
+    const int32_t *draft_starts;
+    const int64_t *draft_masks;
+    int64_t num_blocks;
+    int32_t num_seqs;
+    int32_t num_rows;
+    int32_t max_drafts;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_size;
+    int32_t block_size;
+    int32_t max_blocks_per_seq;
+    int32_t max_context_len;
+    float scale;
+} tlh_tree_attention_args;
+
+tlh_status tlh_tree_attention_scratch_bytes(const tlh_tree_attention_args *a, size_t *bytes);
+tlh_status tlh_tree_attention(const tlh_tree_attention_args *a, void *scratch, size_t scratch_bytes, void *stream);
+
+/* --------------------------------------------------------- cache moves
+ * Copies of whole pages in every layer's pools in one launch (a fork's
+ * copy-on-write, a defragmentation), as the reference's copy_blocks
+ * (crates/kernels/src/cuda/paged_attn.rs:423-504) does a layer at a time.
+ * `pools` is a host array of num_pools pool addresses (a layer's key pool and
+ * its value pool count as two), each of num_blocks blocks of block_bytes bytes
+ * (a multiple of 16; pools 16-byte aligned); pairs i64 [num_pairs][2] on the
+ * device: block src to block dst in each pool. A block may be the source of
+ * several pairs, but a destination must be neither another pair's destination
+ * nor any pair's source: pairs run in no order. A pair with a block outside
+ * [0, num_blocks) does nothing. */
+tlh_status tlh_copy_blocks(void *const *pools, int32_t num_pools, int64_t block_bytes, int64_t num_blocks,
+                           const int64_t *pairs, int32_t num_pairs, void *stream);
+
+/* Closes the gaps that rejected drafted tokens leave in a paged cache, in every
+ * layer in one launch (no counterpart in the reference). context_lens,
+ * draft_starts and max_drafts as tlh_tree_attention took them; bit j of
+ * keep[s] (i64 [num_seqs]) says that drafted token j of sequence s was
+ * accepted. The kept tokens' keys and values move, in order, to the places from
+ * L - n on, and new_lens[s] (i32, not context_lens itself) becomes the length
+ * with them. The drafted places must lie in pages that no other sequence of
+ * the call shares. A move from or to a page outside [0, num_blocks) is left
+ * out. k_caches and v_caches are host arrays of num_layers pool addresses in
+ * the paged-attention layouts (f16). */
+typedef struct tlh_compact_cache_args {
+    void *const *k_caches;
+    void *const *v_caches;
+    const int32_t *block_tables;
+    const int32_t *context_lens;
+    const int32_t *draft_starts;
+    const int64_t *keep;
+    int32_t *new_lens;
+    int64_t num_blocks;
+    int32_t num_layers;
+    int32_t num_seqs;
+    int32_t max_drafts;
+    int32_t num_kv_heads;
+    int32_t head_size;
+    int32_t block_size;
+    int32_t max_blocks_per_seq;
+} tlh_compact_cache_args;
+
+tlh_status tlh_compact_cache(const tlh_compact_cache_args *a, void *stream);
+
+/* ------------------------------------------------------- token logprobs
+ * What a server answers and accepts by, from the logits of `rows` positions
+ * (f32, f16 or bf16 [rows][vocab], row_stride elements from row to row, any
+ * alignment of the type; vocab <= 1000000). No counterpart in the reference.
+ *   logprobs[r]       log softmax(logits[r])[tokens[r]] (NaN for a token outside [0, vocab))
+ *   entropy[r]        -sum p log p, natural logarithm
+ *   top_ids[r][i], top_logprobs[r][i], i < top: the `top` largest logits from the
+ *                     largest down, equal ones by the lowest index (top <= 32, <= vocab)
+ * tokens and logprobs may be NULL together, entropy may be NULL, and the top
+ * arrays where top is 0. Logits may be -inf (a grammar's mask): those tokens
+ * have the log probability -inf. A row that is -inf throughout, or that holds
+ * +inf or NaN, has NaN for what is not defined; a NaN ranks above every number.
+ * `scratch` holds the rows' partial results (16-byte aligned); calls that share
+ * one must be stream-ordered. */
+typedef struct tlh_token_logprobs_args {
+    const void *logits;
+    const int32_t *tokens;
+    float *logprobs;
+    float *entropy;
+    float *top_logprobs;
+    int32_t *top_ids;
+    int64_t row_stride;
+    int32_t type;
+    int32_t rows;
+    int32_t vocab;
+    int32_t top;
+} tlh_token_logprobs_args;
+
+tlh_status tlh_token_logprobs_scratch_bytes(const tlh_token_logprobs_args *a, size_t *bytes);
+tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, size_t scratch_bytes, void *stream);
+
 /* ------------------------------------------------------------ executor
  * A graph of ggml nodes compiled once into a recorded list of launches on this
  * library's kernels and replayed per run, replacing the reference's

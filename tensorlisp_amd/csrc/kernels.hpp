@@ -404,4 +404,14 @@ tlh_status launch_reshape_and_cache(const void *key, const void *value, void *k_
                                     int block_size, int64_t num_blocks, hipStream_t stream, bool key_f32 = false,
                                     bool value_f32 = false);
 
+// The serving operators (arguments checked by the C ABI layer).
+tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream_t stream);
+size_t tree_attention_scratch_bytes(const tlh_tree_attention_args &a);
+tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch, hipStream_t stream);
+tlh_status launch_copy_blocks(void *const *pools, int num_pools, int64_t block_bytes, int64_t num_blocks,
+                              const int64_t *pairs, int num_pairs, hipStream_t stream);
+tlh_status launch_compact_cache(const tlh_compact_cache_args &a, hipStream_t stream);
+size_t token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int top);
+tlh_status launch_token_logprobs(const tlh_token_logprobs_args &a, void *scratch, hipStream_t stream);
+
 }  // namespace tlh

@@ -1156,6 +1156,162 @@ tlh_status tlh_reshape_and_cache(const void *key, const void *value, void *k_cac
                                     block_size, num_blocks, (hipStream_t)stream);
 }
 
+// ----------------------------------------------------- serving operators
+static bool paged_head_size(int h) {
+    return h == 64 || h == 80 || h == 96 || h == 112 || h == 128 || h == 192 || h == 256;
+}
+static bool paged_block_size(int b) { return b == 8 || b == 16 || b == 32; }
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// heads per grid unit and counts small enough for 32-bit products of them
+static tlh_status check_heads(const char *what, int heads, int kv_heads, int head_size) {
+    if (!paged_head_size(head_size))
+        return set_error(TLH_INVALID, "%s: unsupported head_size %d", what, head_size);
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || heads > 65535)
+        return set_error(TLH_INVALID, "%s: num_heads must be a multiple of num_kv_heads, at most 65535", what);
+    return TLH_OK;
+}
+
+tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream) {
+    if (!a) return set_error(TLH_INVALID, "packed_attention: null args");
+    if (a->type != TLH_TYPE_F16 && a->type != TLH_TYPE_BF16)
+        return set_error(TLH_UNSUPPORTED, "packed_attention: tensors of ggml type %d (%s); have f16, bf16", a->type,
+                         type_name(a->type));
+    const tlh_status st = check_heads("packed_attention", a->num_heads, a->num_kv_heads, a->head_size);
+    if (st != TLH_OK) return st;
+    if (a->num_seqs < 0 || a->num_tokens < 0 || a->max_seq_len < 0)
+        return set_error(TLH_INVALID, "packed_attention: negative count");
+    const int64_t qrow = (int64_t)a->num_heads * a->head_size, krow = (int64_t)a->num_kv_heads * a->head_size;
+    if (a->out_stride < qrow || a->q_stride < qrow || a->k_stride < krow || a->v_stride < krow ||
+        ((a->out_stride | a->q_stride | a->k_stride | a->v_stride) & 7) != 0)
+        return set_error(TLH_INVALID, "packed_attention: a token stride is shorter than its heads or no multiple of 8");
+    if (a->num_seqs == 0 || a->num_tokens == 0 || a->max_seq_len == 0) return TLH_OK;
+    if (!a->out || !a->q || !a->k || !a->v || !a->seq_starts)
+        return set_error(TLH_INVALID, "packed_attention: null pointer");
+    if (!aligned16(a->out) || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) ||
+        ((uintptr_t)a->seq_starts & 3))
+        return set_error(TLH_INVALID, "packed_attention: tensors must be 16-byte aligned");
+    return launch_packed_attention(*a, (hipStream_t)stream);
+}
+
+static tlh_status check_tree(const tlh_tree_attention_args *a) {
+    if (!a) return set_error(TLH_INVALID, "tree_attention: null args");
+    const tlh_status st = check_heads("tree_attention", a->num_heads, a->num_kv_heads, a->head_size);
+    if (st != TLH_OK) return st;
+    if (!paged_block_size(a->block_size))
+        return set_error(TLH_INVALID, "tree_attention: unsupported block_size %d (have 8, 16, 32)", a->block_size);
+    if (a->num_seqs < 0 || a->num_seqs > 65535 || a->num_rows < 0 || a->num_blocks < 0 || a->max_blocks_per_seq < 0 ||
+        a->max_context_len < 0)
+        return set_error(TLH_INVALID, "tree_attention: bad counts (at most 65535 sequences)");
+    if (a->max_drafts < 0 || a->max_drafts > 64)
+        return set_error(TLH_INVALID, "tree_attention: max_drafts %d outside 0..64", a->max_drafts);
+    if ((int64_t)a->max_blocks_per_seq * a->block_size < a->max_context_len)
+        return set_error(TLH_INVALID, "tree_attention: max_blocks_per_seq * block_size < max_context_len");
+    return TLH_OK;
+}
+
+tlh_status tlh_tree_attention_scratch_bytes(const tlh_tree_attention_args *a, size_t *bytes) {
+    if (!bytes) return set_error(TLH_INVALID, "tree_attention_scratch_bytes: null pointer");
+    const tlh_status st = check_tree(a);
+    if (st != TLH_OK) return st;
+    *bytes = tree_attention_scratch_bytes(*a);
+    return TLH_OK;
+}
+
+tlh_status tlh_tree_attention(const tlh_tree_attention_args *a, void *scratch, size_t scratch_bytes, void *stream) {
+    const tlh_status st = check_tree(a);
+    if (st != TLH_OK) return st;
+    if (a->num_seqs == 0 || a->num_rows == 0 || a->max_drafts == 0) return TLH_OK;
+    if (!a->out || !a->q || !a->context_lens || !a->draft_starts || !a->draft_masks ||
+        (a->max_context_len > 0 && (!a->k_cache || !a->v_cache || !a->block_tables)))
+        return set_error(TLH_INVALID, "tree_attention: null pointer");
+    if (!aligned16(a->out) || !aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
+        ((uintptr_t)a->draft_masks & 7) ||
+        (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens | (uintptr_t)a->draft_starts) & 3))
+        return set_error(TLH_INVALID, "tree_attention: q, out and the caches must be 16-byte aligned");
+    const size_t need = tree_attention_scratch_bytes(*a);
+    if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+        return set_error(TLH_INVALID, "tree_attention: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    return launch_tree_attention(*a, scratch, (hipStream_t)stream);
+}
+
+tlh_status tlh_copy_blocks(void *const *pools, int32_t num_pools, int64_t block_bytes, int64_t num_blocks,
+                           const int64_t *pairs, int32_t num_pairs, void *stream) {
+    if (num_pools < 0 || num_pairs < 0 || num_blocks < 0 || block_bytes <= 0 || block_bytes % 16 != 0 ||
+        block_bytes > ((int64_t)1 << 29) || num_blocks > INT64_MAX / block_bytes)
+        return set_error(TLH_INVALID, "copy_blocks: bad geometry (blocks are a multiple of 16 bytes, at most 512 MiB)");
+    if (num_pools == 0 || num_pairs == 0) return TLH_OK;
+    if (!pools || !pairs || ((uintptr_t)pairs & 7)) return set_error(TLH_INVALID, "copy_blocks: null or misaligned pointer");
+    for (int i = 0; i < num_pools; ++i)
+        if (!pools[i] || !aligned16(pools[i]))
+            return set_error(TLH_INVALID, "copy_blocks: pool %d is null or not 16-byte aligned", i);
+    return launch_copy_blocks(pools, num_pools, block_bytes, num_blocks, pairs, num_pairs, (hipStream_t)stream);
+}
+
+tlh_status tlh_compact_cache(const tlh_compact_cache_args *a, void *stream) {
+    if (!a) return set_error(TLH_INVALID, "compact_cache: null args");
+    if (!paged_head_size(a->head_size) || !paged_block_size(a->block_size) || a->num_kv_heads <= 0 ||
+        a->num_kv_heads > 65535)
+        return set_error(TLH_INVALID, "compact_cache: unsupported head_size %d, block_size %d or num_kv_heads %d",
+                         a->head_size, a->block_size, a->num_kv_heads);
+    if (a->num_layers < 0 || a->num_seqs < 0 || a->num_blocks < 0 || a->max_blocks_per_seq < 0 ||
+        (int64_t)a->max_blocks_per_seq * a->block_size > INT32_MAX)
+        return set_error(TLH_INVALID, "compact_cache: bad counts");
+    if (a->max_drafts < 0 || a->max_drafts > 64)
+        return set_error(TLH_INVALID, "compact_cache: max_drafts %d outside 0..64", a->max_drafts);
+    if (a->num_seqs == 0 || a->num_layers == 0) return TLH_OK;
+    if (!a->k_caches || !a->v_caches || !a->context_lens || !a->draft_starts || !a->keep || !a->new_lens ||
+        (a->max_blocks_per_seq > 0 && !a->block_tables))
+        return set_error(TLH_INVALID, "compact_cache: null pointer");
+    if ((const int32_t *)a->new_lens == a->context_lens)
+        return set_error(TLH_INVALID, "compact_cache: new_lens must not be context_lens");
+    if (((uintptr_t)a->keep & 7) || (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens |
+                                      (uintptr_t)a->draft_starts | (uintptr_t)a->new_lens) & 3))
+        return set_error(TLH_INVALID, "compact_cache: misaligned pointer");
+    for (int i = 0; i < a->num_layers; ++i)
+        if (!a->k_caches[i] || !a->v_caches[i] || !aligned16(a->k_caches[i]) || !aligned16(a->v_caches[i]))
+            return set_error(TLH_INVALID, "compact_cache: layer %d's pools are null or not 16-byte aligned", i);
+    return launch_compact_cache(*a, (hipStream_t)stream);
+}
+
+static tlh_status check_logprobs(const tlh_token_logprobs_args *a) {
+    if (!a) return set_error(TLH_INVALID, "token_logprobs: null args");
+    if (!float_type(a->type))
+        return set_error(TLH_UNSUPPORTED, "token_logprobs: logits of ggml type %d (%s); have f32, f16, bf16", a->type,
+                         type_name(a->type));
+    if (a->rows < 0 || a->vocab < 1 || a->vocab > 1000000)
+        return set_error(TLH_INVALID, "token_logprobs: %d rows, vocab %d outside 1..1000000", a->rows, a->vocab);
+    if (a->top < 0 || a->top > 32 || a->top > a->vocab)
+        return set_error(TLH_INVALID, "token_logprobs: top %d outside 0..min(32, vocab)", a->top);
+    if (a->row_stride < a->vocab)
+        return set_error(TLH_INVALID, "token_logprobs: row stride shorter than the vocabulary");
+    return TLH_OK;
+}
+
+tlh_status tlh_token_logprobs_scratch_bytes(const tlh_token_logprobs_args *a, size_t *bytes) {
+    if (!bytes) return set_error(TLH_INVALID, "token_logprobs_scratch_bytes: null pointer");
+    const tlh_status st = check_logprobs(a);
+    if (st != TLH_OK) return st;
+    *bytes = token_logprobs_scratch_bytes(a->rows, a->vocab, a->top);
+    return TLH_OK;
+}
+
+tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, size_t scratch_bytes, void *stream) {
+    const tlh_status st = check_logprobs(a);
+    if (st != TLH_OK) return st;
+    if (a->rows == 0) return TLH_OK;
+    if (!a->logits || (!a->tokens) != (!a->logprobs) || (a->top > 0 && (!a->top_logprobs || !a->top_ids)))
+        return set_error(TLH_INVALID, "token_logprobs: null pointer");
+    if (((uintptr_t)a->logits & (float_size(a->type) - 1)) ||
+        (((uintptr_t)a->tokens | (uintptr_t)a->logprobs | (uintptr_t)a->entropy | (uintptr_t)a->top_logprobs |
+          (uintptr_t)a->top_ids) & 3))
+        return set_error(TLH_INVALID, "token_logprobs: misaligned pointer");
+    const size_t need = token_logprobs_scratch_bytes(a->rows, a->vocab, a->top);
+    if (!scratch || scratch_bytes < need || !aligned16(scratch))
+        return set_error(TLH_INVALID, "token_logprobs: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    return launch_token_logprobs(*a, scratch, (hipStream_t)stream);
+}
+
 tlh_status tlh_flash_attn_ext_scratch_bytes(const tlh_op *op, size_t *bytes) {
     if (!bytes) return set_error(TLH_INVALID, "flash_attn_ext_scratch_bytes: null pointer");
     FlashAttnDesc d;

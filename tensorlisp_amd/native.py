@@ -40,6 +40,8 @@ EXPORTS = (
     "tlh_mul_mat_noalloc", "tlh_mul_mat_quantize", "tlh_mul_mat_compute", "tlh_mul_mat_id_scratch_bytes", "tlh_mul_mat_id",
     "tlh_quantize_act", "tlh_dequantize", "tlh_flash_attn_ext_scratch_bytes", "tlh_flash_attn_ext",
     "tlh_paged_attention_scratch_bytes", "tlh_paged_attention", "tlh_reshape_and_cache",
+    "tlh_packed_attention", "tlh_tree_attention_scratch_bytes", "tlh_tree_attention", "tlh_copy_blocks",
+    "tlh_compact_cache", "tlh_token_logprobs_scratch_bytes", "tlh_token_logprobs",
     "tlh_core_check", "tlh_core", "tlh_program_compile", "tlh_program_destroy", "tlh_copy", "tlh_memset",
     "tlh_read_floor",
     "tlh_program_input",
@@ -79,6 +81,37 @@ class TlhPagedArgs(C.Structure):
                 ("scale", C.c_float)]
 
 
+class TlhPackedArgs(C.Structure):
+    _fields_ = [("out", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("seq_starts", C.c_void_p), ("out_stride", C.c_int64), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("type", C.c_int32), ("num_seqs", C.c_int32),
+                ("num_tokens", C.c_int32), ("max_seq_len", C.c_int32), ("num_heads", C.c_int32),
+                ("num_kv_heads", C.c_int32), ("head_size", C.c_int32), ("scale", C.c_float)]
+
+
+class TlhTreeArgs(C.Structure):
+    _fields_ = [("out", C.c_void_p), ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("block_tables", C.c_void_p), ("context_lens", C.c_void_p), ("draft_starts", C.c_void_p),
+                ("draft_masks", C.c_void_p), ("num_blocks", C.c_int64), ("num_seqs", C.c_int32),
+                ("num_rows", C.c_int32), ("max_drafts", C.c_int32), ("num_heads", C.c_int32),
+                ("num_kv_heads", C.c_int32), ("head_size", C.c_int32), ("block_size", C.c_int32),
+                ("max_blocks_per_seq", C.c_int32), ("max_context_len", C.c_int32), ("scale", C.c_float)]
+
+
+class TlhCompactArgs(C.Structure):
+    _fields_ = [("k_caches", C.POINTER(C.c_void_p)), ("v_caches", C.POINTER(C.c_void_p)),
+                ("block_tables", C.c_void_p), ("context_lens", C.c_void_p), ("draft_starts", C.c_void_p),
+                ("keep", C.c_void_p), ("new_lens", C.c_void_p), ("num_blocks", C.c_int64), ("num_layers", C.c_int32),
+                ("num_seqs", C.c_int32), ("max_drafts", C.c_int32), ("num_kv_heads", C.c_int32),
+                ("head_size", C.c_int32), ("block_size", C.c_int32), ("max_blocks_per_seq", C.c_int32)]
+
+
+class TlhLogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("logprobs", C.c_void_p), ("entropy", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("top_ids", C.c_void_p), ("row_stride", C.c_int64), ("type", C.c_int32),
+                ("rows", C.c_int32), ("vocab", C.c_int32), ("top", C.c_int32)]
+
+
 assert C.sizeof(TlhOp) == 456, C.sizeof(TlhOp)
 
 
@@ -112,6 +145,13 @@ def load_library(path: Path = LIB_PATH) -> C.CDLL:
     L.tlh_paged_attention_scratch_bytes.argtypes = [C.POINTER(TlhPagedArgs), C.POINTER(C.c_size_t)]
     L.tlh_paged_attention.argtypes = [C.POINTER(TlhPagedArgs), vp, C.c_size_t, vp]
     L.tlh_reshape_and_cache.argtypes = [vp, vp, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, vp]
+    L.tlh_packed_attention.argtypes = [C.POINTER(TlhPackedArgs), vp]
+    L.tlh_tree_attention_scratch_bytes.argtypes = [C.POINTER(TlhTreeArgs), C.POINTER(C.c_size_t)]
+    L.tlh_tree_attention.argtypes = [C.POINTER(TlhTreeArgs), vp, C.c_size_t, vp]
+    L.tlh_copy_blocks.argtypes = [C.POINTER(C.c_void_p), C.c_int32, i64, i64, vp, C.c_int32, vp]
+    L.tlh_compact_cache.argtypes = [C.POINTER(TlhCompactArgs), vp]
+    L.tlh_token_logprobs_scratch_bytes.argtypes = [C.POINTER(TlhLogprobsArgs), C.POINTER(C.c_size_t)]
+    L.tlh_token_logprobs.argtypes = [C.POINTER(TlhLogprobsArgs), vp, C.c_size_t, vp]
     L.tlh_core_check.argtypes = [C.c_int, C.POINTER(TlhOp), C.c_int, C.c_int]
     L.tlh_core.argtypes = [C.c_int, C.POINTER(TlhOp), vp, vp, vp, vp, vp]
     i32p, i64p = C.POINTER(C.c_int32), C.POINTER(C.c_int64)
@@ -472,6 +512,253 @@ def reshape_and_cache(key, value, k_cache, v_cache, slots, num_kv_heads, block_s
     num_blocks = min(k_cache.numel(), v_cache.numel()) // (num_kv_heads * hs * block_size)
     check(lib().tlh_reshape_and_cache(_ptr(key), _ptr(value), _ptr(k_cache), _ptr(v_cache), _ptr(slots), tokens,
                                       num_kv_heads, hs, block_size, num_blocks, _stream(stream)))
+
+
+# --------------------------------------------------------- serving operators
+def _arg(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _tensor(t, dtype, shape, name: str, device=None):
+    """A contiguous tensor of this dtype and shape (None: any extent) on `device`."""
+    _arg(t.dtype == dtype and t.dim() == len(shape) and t.is_contiguous() and
+         all(w is None or n == w for n, w in zip(t.shape, shape)),
+         f"{name}: {t.dtype} {tuple(t.shape)}, not contiguous {dtype} {tuple('*' if w is None else w for w in shape)}")
+    _arg(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr()
+
+
+class _on:
+    """Runs a call on the tensors' device, on `stream` or that device's current stream."""
+
+    def __init__(self, device, stream):
+        self.device, self.stream, self.guard = device, stream, None
+
+    def __enter__(self):
+        import torch
+
+        if self.device.type != "cuda":
+            raise ValueError(f"tensors must be on the GPU, not on {self.device}")
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        if self.stream is not None and getattr(self.stream, "device", self.device) != self.device:
+            raise ValueError(f"the stream is on {self.stream.device}, the tensors are on {self.device}")
+        return _stream(self.stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _use_on(stream, *tensors):
+    """Tensors allocated on the current stream but used on another: the allocator must wait for that one."""
+    import torch
+
+    if stream is not None:
+        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(getattr(stream, "value", stream) or 0))
+        for t in tensors:
+            t.record_stream(s)
+
+
+def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=None, stream=None):
+    """Causal attention of prompts packed one after another: q (tokens, heads,
+    head size), k and v (tokens, kv heads, head size) f16 or bf16, tokens at any
+    stride that is a multiple of 8 elements (views of a fused projection),
+    seq_starts i32 (sequences + 1,) -> out (tokens, heads, head size). No
+    sequence may be longer than max_seq_len. Tokens behind the last sequence are
+    left as they were in `out`."""
+    import torch
+
+    tokens, heads, hs = q.shape
+    _arg(q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype,
+         f"q, k and v must be f16 or all bf16, not {q.dtype}, {k.dtype}, {v.dtype}")
+    _arg(k.dim() == 3 and k.shape == v.shape and k.shape[0] == tokens and k.shape[2] == hs,
+         f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    fresh = out is None
+    if fresh:
+        out = torch.empty((tokens, heads, hs), dtype=q.dtype, device=q.device)
+    _arg(out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and type")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        _arg(t.device == q.device, f"{name} is on {t.device}, not on {q.device}")
+        _arg(t.numel() == 0 or ((t.shape[2] == 1 or t.stride(2) == 1) and (t.shape[1] == 1 or t.stride(1) == hs)),
+             f"{name}: a token's heads must be contiguous")
+    a = TlhPackedArgs()
+    a.seq_starts = _tensor(seq_starts, torch.int32, (None,), "seq_starts", q.device)
+    _arg(seq_starts.shape[0] >= 1, "seq_starts must hold at least one start")
+    a.out, a.q, a.k, a.v = out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr()
+    one = tokens <= 1  # the stride of a single token means nothing
+    a.out_stride, a.q_stride = (heads * hs, heads * hs) if one else (out.stride(0), q.stride(0))
+    a.k_stride, a.v_stride = (k.shape[1] * hs, k.shape[1] * hs) if one else (k.stride(0), v.stride(0))
+    a.type = F16 if q.dtype == torch.float16 else BF16
+    a.num_seqs, a.num_tokens, a.max_seq_len = seq_starts.shape[0] - 1, tokens, max_seq_len
+    a.num_heads, a.num_kv_heads, a.head_size, a.scale = heads, k.shape[1], hs, scale
+    with _on(q.device, stream) as s:
+        check(lib().tlh_packed_attention(C.byref(a), s))
+    if fresh:
+        _use_on(stream, out)
+    return out
+
+
+class TreeAttention:
+    """Attention of drafted tokens over the paged cache, with its scratch, launched many times. A call
+    takes up to num_seqs sequences and num_rows drafted tokens in all, at most max_drafts (<= 64) of one
+    sequence; calls of one object must be stream-ordered (they share the scratch)."""
+
+    def __init__(self, num_seqs, num_rows, max_drafts, num_heads, num_kv_heads, head_size, block_size,
+                 max_blocks_per_seq, max_context_len, scale, device="cuda"):
+        import torch
+
+        a = self.args = TlhTreeArgs()
+        a.num_seqs, a.num_rows, a.max_drafts = num_seqs, num_rows, max_drafts
+        a.num_heads, a.num_kv_heads, a.head_size, a.block_size = num_heads, num_kv_heads, head_size, block_size
+        a.max_blocks_per_seq, a.max_context_len, a.scale = max_blocks_per_seq, max_context_len, scale
+        n = C.c_size_t()
+        check(lib().tlh_tree_attention_scratch_bytes(C.byref(a), C.byref(n)))
+        self.scratch_bytes = n.value
+        self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
+
+    def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream=None):
+        """q and out f16 (num_rows, heads, head size), the caches in the paged-attention layouts,
+        block_tables i32 (num_seqs, max_blocks_per_seq), context_lens i32 (num_seqs,) with the drafted
+        tokens, draft_starts i32 (num_seqs + 1,), draft_masks i64 (num_rows,): bit j = sees draft j."""
+        import torch
+
+        a, dev = self.args, self.scratch.device
+        rows, S, KV, D, bs = a.num_rows, a.num_seqs, a.num_kv_heads, a.head_size, a.block_size
+        a.q = _tensor(q, torch.float16, (rows, a.num_heads, D), "q", dev)
+        a.out = _tensor(out, torch.float16, (rows, a.num_heads, D), "out", dev)
+        a.k_cache = _tensor(k_cache, torch.float16, (None, KV, D // 8, bs, 8), "k_cache", dev)
+        a.v_cache = _tensor(v_cache, torch.float16, (k_cache.shape[0], KV, D, bs), "v_cache", dev)
+        a.block_tables = _tensor(block_tables, torch.int32, (S, a.max_blocks_per_seq), "block_tables", dev)
+        a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
+        a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
+        a.draft_masks = _tensor(draft_masks, torch.int64, (rows,), "draft_masks", dev)
+        a.num_blocks = k_cache.shape[0]
+        with _on(dev, stream) as s:
+            check(lib().tlh_tree_attention(C.byref(a), self.scratch.data_ptr(), self.scratch_bytes, s))
+        return out
+
+
+def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, max_drafts: int,
+                   max_context_len: int, scale: float, stream=None):
+    """One TreeAttention call: q f16 (rows, heads, head size) -> out alike (zeros in rows behind the last sequence)."""
+    import torch
+
+    rows, heads, hs = q.shape
+    node = TreeAttention(block_tables.shape[0], rows, max_drafts, heads, v_cache.shape[1], hs, v_cache.shape[3],
+                         block_tables.shape[1], max_context_len, scale, device=q.device)
+    q, out = q.contiguous(), torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
+    if stream is not None:  # the zeros and a copied q come from the current stream
+        s = torch.cuda.current_stream(q.device)
+        (stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream))).wait_stream(s)
+    node(out, q, k_cache, v_cache, block_tables.contiguous(), context_lens, draft_starts, draft_masks, stream)
+    _use_on(stream, out, q, node.scratch)
+    return out
+
+
+class KVPools:
+    """The key and value pools of a cache's layers (lists of f16 tensors in the
+    paged-attention layouts, one length in blocks), moved in all layers at once."""
+
+    def __init__(self, k_caches, v_caches, num_kv_heads: int, head_size: int, block_size: int):
+        import torch
+
+        _arg(len(k_caches) == len(v_caches) and len(k_caches) > 0, "as many key as value pools, at least one")
+        self.device, self.num_blocks = k_caches[0].device, k_caches[0].shape[0]
+        self.kv_heads, self.head_size, self.block_size = num_kv_heads, head_size, block_size
+        n, self.layers = self.num_blocks, len(k_caches)
+        ks = [_tensor(t, torch.float16, (n, num_kv_heads, head_size // 8, block_size, 8), "k_cache", self.device)
+              for t in k_caches]
+        vs = [_tensor(t, torch.float16, (n, num_kv_heads, head_size, block_size), "v_cache", self.device)
+              for t in v_caches]
+        self.tensors = (list(k_caches), list(v_caches))  # the pools live as long as their addresses are used
+        self._all = (C.c_void_p * (2 * self.layers))(*ks, *vs)
+        self._k, self._v = (C.c_void_p * self.layers)(*ks), (C.c_void_p * self.layers)(*vs)
+
+    def copy_blocks(self, pairs, stream=None) -> None:
+        """Block pairs[i, 0] to block pairs[i, 1] in every pool; pairs i64 (n, 2). No destination may be
+        another pair's destination or any pair's source; a pair outside the pools does nothing."""
+        import torch
+
+        p = _tensor(pairs, torch.int64, (None, 2), "pairs", self.device)
+        with _on(self.device, stream) as s:
+            check(lib().tlh_copy_blocks(self._all, 2 * self.layers, self.kv_heads * self.head_size * self.block_size * 2,
+                                        self.num_blocks, p, pairs.shape[0], s))
+
+    def compact(self, block_tables, context_lens, draft_starts, keep, new_lens, max_drafts: int, stream=None):
+        """Moves the kept drafted tokens (bit j of keep[s], i64 (sequences,)) of every sequence right behind
+        its committed ones in every layer; new_lens i32 (sequences,) receives the lengths with them."""
+        import torch
+
+        a, dev = TlhCompactArgs(), self.device
+        S = context_lens.shape[0]
+        a.k_caches, a.v_caches = self._k, self._v
+        a.block_tables = _tensor(block_tables, torch.int32, (S, None), "block_tables", dev)
+        a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
+        a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
+        a.keep = _tensor(keep, torch.int64, (S,), "keep", dev)
+        a.new_lens = _tensor(new_lens, torch.int32, (S,), "new_lens", dev)
+        a.num_blocks, a.num_layers, a.num_seqs, a.max_drafts = self.num_blocks, self.layers, S, max_drafts
+        a.num_kv_heads, a.head_size, a.block_size = self.kv_heads, self.head_size, self.block_size
+        a.max_blocks_per_seq = block_tables.shape[1]
+        with _on(dev, stream) as s:
+            check(lib().tlh_compact_cache(C.byref(a), s))
+        return new_lens
+
+
+class TokenLogprobs:
+    """Log probabilities of given tokens, entropies and the `top` likeliest tokens of up to `rows` rows of
+    logits, with the scratch; calls of one object must be stream-ordered (they share it)."""
+
+    def __init__(self, rows: int, vocab: int, top: int = 0, dtype=None, device="cuda"):
+        import torch
+
+        self.rows, self.dtype = rows, dtype or torch.float32
+        a = self.args = TlhLogprobsArgs()
+        a.type, a.rows, a.vocab, a.top = _ggml_type(torch.empty(0, dtype=self.dtype)), rows, vocab, top
+        a.row_stride = vocab
+        n = C.c_size_t()
+        check(lib().tlh_token_logprobs_scratch_bytes(C.byref(a), C.byref(n)))
+        self.scratch_bytes = n.value
+        self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
+
+    def __call__(self, logits, tokens, logprobs, entropy, top_logprobs=None, top_ids=None, stream=None):
+        """logits (n, vocab) with n <= rows, any row stride; tokens i32 (n,); logprobs and entropy f32 (n,);
+        top_logprobs f32 and top_ids i32 (n, top). tokens and logprobs, or entropy, may be None."""
+        import torch
+
+        a, dev, n = self.args, self.scratch.device, logits.shape[0]
+        _arg(logits.dtype == self.dtype and logits.dim() == 2 and n <= self.rows and logits.shape[1] == a.vocab and
+             logits.device == dev and (logits.shape[1] == 1 or logits.stride(1) == 1),
+             f"logits {logits.dtype} {tuple(logits.shape)} on {logits.device} for {self.rows} rows of {a.vocab} {self.dtype}")
+        a.rows, a.logits = n, logits.data_ptr()
+        a.row_stride = logits.stride(0) if n > 1 else a.vocab
+        a.tokens = _tensor(tokens, torch.int32, (n,), "tokens", dev) if tokens is not None else None
+        a.logprobs = _tensor(logprobs, torch.float32, (n,), "logprobs", dev) if logprobs is not None else None
+        a.entropy = _tensor(entropy, torch.float32, (n,), "entropy", dev) if entropy is not None else None
+        if a.top:
+            _arg(top_logprobs is not None and top_ids is not None, "top_logprobs and top_ids are needed where top > 0")
+            a.top_logprobs = _tensor(top_logprobs, torch.float32, (n, a.top), "top_logprobs", dev)
+            a.top_ids = _tensor(top_ids, torch.int32, (n, a.top), "top_ids", dev)
+        with _on(dev, stream) as s:
+            check(lib().tlh_token_logprobs(C.byref(a), self.scratch.data_ptr(), self.scratch_bytes, s))
+        return logprobs, entropy, top_logprobs, top_ids
+
+
+def token_logprobs(logits, tokens, top: int = 0, stream=None):
+    """logits (rows, vocab) f32 / f16 / bf16, tokens i32 (rows,) -> (logprobs (rows,), entropy (rows,),
+    top_logprobs (rows, top), top_ids i32 (rows, top))."""
+    import torch
+
+    n, dev = logits.shape[0], logits.device
+    node = TokenLogprobs(n, logits.shape[1], top, logits.dtype, device=dev)
+    f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
+    outs = (f(n), f(n), f(n, top), torch.empty((n, top), dtype=torch.int32, device=dev))
+    node(logits, tokens, *outs, stream=stream)
+    _use_on(stream, *outs, node.scratch)
+    return outs
 
 
 # ------------------------------------------------------------------ core ops
