@@ -49,6 +49,10 @@ __device__ __forceinline__ float lp_wave_sum(float v) {
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
+__device__ __forceinline__ float lp_wave_maxf(float v) {
+    for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
 // set bits of b below this lane
 __device__ __forceinline__ int lp_below(uint64_t b) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
@@ -62,6 +66,89 @@ template <int TY> __device__ __forceinline__ float lp_elem(const void *p, int64_
 
 // Scratch of chunk p of a row: m, S, T, one free word, then `top` entries.
 __host__ __device__ constexpr size_t lp_slot(int top) { return 16 + 8 * (size_t)top; }
+
+// One wave's part of a chunk: NV vectors of C elements a lane, the first of vector
+// i at element e0 + 256 C i of the row. EDGE: some elements may lie outside [0, V)
+// (they hold -inf, and are told from a row's own -inf by their index).
+template <int TY, int C, int NV, bool EDGE> struct LpWave {
+    const float (&x)[NV][C];
+    const void *base;  // the row
+    const int e0, V, lane;
+    __device__ int elem(int i, int c) const { return e0 + 256 * C * i + c; }
+    __device__ bool there(int i, int c) const { return !EDGE || (uint32_t)elem(i, c) < (uint32_t)V; }
+
+    // The `top` largest elements into out[0 .. top) in order, 0 past the last. `best`: the lane's largest.
+    // A row with a NaN or +inf (plain = false) and one with more elements above the threshold
+    // than the list holds are taken one maximum at a time.
+    __device__ void select(float best, int top, bool plain, uint64_t *list, uint64_t *out) const {
+        if (plain) {
+            // thr: the top-th largest of the lanes' maxima, bit by bit (-inf with fewer lanes than that)
+            const uint32_t k = lp_key(best);
+            uint32_t thr_key = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t cand = thr_key | 1u << bit;
+                if (__popcll(__builtin_amdgcn_ballot_w64(k >= cand)) >= top) thr_key = cand;
+            }
+            const float thr = lp_value(thr_key);
+            int above = 0, equal = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                uint64_t any = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c) any |= __builtin_amdgcn_ballot_w64(x[i][c] >= thr);
+                if (any == 0) continue;
+                int before = 0;  // of the lanes below: elements of the vector that equal thr
+                uint64_t eq[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    eq[c] = __builtin_amdgcn_ballot_w64(x[i][c] == thr && there(i, c));
+                    before += lp_below(eq[c]);
+                }
+                int eqs = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint64_t gt = __builtin_amdgcn_ballot_w64(x[i][c] > thr);
+                    const uint64_t entry = lp_entry(lp_key(x[i][c]), elem(i, c));
+                    const int ga = above + lp_below(gt);
+                    if ((gt >> lane) & 1 && ga < LP_CAP) list[ga] = entry;
+                    above += __popcll(gt);
+                    if ((eq[c] >> lane) & 1) {
+                        if (equal + before < top) list[LP_CAP + equal + before] = entry;
+                        ++before;
+                    }
+                    eqs += __popcll(eq[c]);
+                }
+                equal += eqs;
+            }
+            if (above <= LP_CAP) {
+                const int n = above + min(equal, top);
+                if (lane >= n && lane < top) out[lane] = 0;
+                __builtin_amdgcn_wave_barrier();
+                for (int e = lane; e < n; e += 64) {
+                    const uint64_t mine = list[e < above ? e : LP_CAP + e - above];
+                    int rank = 0;
+#pragma unroll 8
+                    for (int f = 0; f < n; ++f) rank += list[f < above ? f : LP_CAP + f - above] > mine;
+                    if (rank < top) out[rank] = mine;
+                }
+                return;
+            }
+        }
+        uint64_t last = ~(uint64_t)0;
+        for (int r = 0; r < top; ++r) {
+            uint64_t b = 0;
+#pragma unroll 1
+            for (int i = 0; i < NV * C; ++i) {  // read again: rare, and registers cannot be indexed in a loop
+                const int e = e0 + 256 * C * (i / C) + i % C;
+                if (e < 0 || e >= V) continue;
+                const uint64_t entry = lp_entry(lp_key(lp_elem<TY>(base, e)), e);
+                if (entry < last && entry > b) b = entry;
+            }
+            last = lp_wave_max(b);
+            if (lane == 0) out[r] = last;
+        }
+    }
+};
 
 template <int TY, int EPT>
 __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__ logits, int64_t row_stride, int V,
@@ -77,12 +164,14 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
     // Loads are aligned whatever the row's address: element 0 of the chunks'
     // numbering lies up to C - 1 elements before the row.
     const int mis = (int)(((uintptr_t)base & 15) / ES);
-    const int v0 = p * 256 * EPT + threadIdx.x * C - mis;  // the first of vector i's elements: v0 + 256 * C * i
+    const int first = p * 256 * EPT - mis;
+    const int e0 = first + threadIdx.x * C;
+    const bool edge = first < 0 || first + 256 * EPT > V;  // the chunk holds places outside the row
     float x[NV][C];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int e = v0 + 256 * C * i;
-        if (e >= 0 && e + C <= V) {
+        const int e = e0 + 256 * C * i;
+        if (!edge || (e >= 0 && e + C <= V)) {
             const uint4 w = *(const uint4 *)(base + (int64_t)e * ES);
             const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -95,135 +184,72 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
             for (int c = 0; c < C; ++c) x[i][c] = e + c >= 0 && e + c < V ? lp_elem<TY>(base, e + c) : -INFINITY;
         }
     }
-    auto there = [&](int i, int c) {
-        const int e = v0 + 256 * C * i + c;
-        return e >= 0 && e < V;
-    };
-    auto key_of = [&](int i, int c) { return there(i, c) ? lp_key(x[i][c]) : 0u; };
-
-    float m = -INFINITY;
+    float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) m = fmaxf(m, x[i][c]);
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int c = 0; c < C; ++c) best = fmaxf(best, x[i][c]);
+    const float m = lp_wave_maxf(best);
+    // exp(x - m) as 2^((x - m) log2 e). Below -1000 it is 0 anyway, and a -inf
+    // (x or, where all are, x - m = NaN) must not reach the product with it. A
+    // NaN among the logits is not in m; it passes both maxima and makes S NaN.
     float S = 0.0f, T = 0.0f;
-    // all -inf: S = 0. A NaN is not in the maximum, and makes S NaN unless m is -inf
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const float d = x[i][c] - m, e = __expf(d);
-            S += x[i][c] == -INFINITY ? 0.0f : e;
-            T += e > 0.0f && x[i][c] != -INFINITY ? e * d : 0.0f;
-        }
-    S = lp_wave_sum(S);
-    T = lp_wave_sum(T);
-    if (lane == 0) s_sum[wave][0] = m, s_sum[wave][1] = S, s_sum[wave][2] = T;
-
-    if (top > 0) {
-        uint32_t best = 0;
+    if (m != -INFINITY) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int c = 0; c < C; ++c) best = max(best, key_of(i, c));
-        // the top-th largest lane maximum, bit by bit
-        uint32_t thr = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = thr | 1u << bit;
-            if (__popcll(__builtin_amdgcn_ballot_w64(best >= cand)) >= top) thr = cand;
-        }
-        int above = 0, equal = 0;
-        uint64_t *list = s_list[wave];  // the elements above thr, and from LP_CAP on those that equal it
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            uint64_t gt[C], eq[C];
-            uint64_t any = 0;
-#pragma unroll
             for (int c = 0; c < C; ++c) {
-                const uint32_t k = key_of(i, c);
-                gt[c] = __builtin_amdgcn_ballot_w64(k > thr);
-                eq[c] = __builtin_amdgcn_ballot_w64(k == thr && k != 0);
-                any |= gt[c] | eq[c];
+                const float t = x[i][c] - m, d = t < -1000.0f ? -1000.0f : t;
+                const float e = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+                S += e;
+                T += e * d;
             }
-            if (any) {
-                int before = 0, gts = 0, eqs = 0;  // of the lanes below: elements equal to thr
+    } else {
 #pragma unroll
-                for (int c = 0; c < C; ++c) before += lp_below(eq[c]);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint64_t entry = lp_entry(key_of(i, c), v0 + 256 * C * i + c);
-                    const int ga = above + gts + lp_below(gt[c]);
-                    if ((gt[c] >> lane) & 1 && ga < LP_CAP) list[ga] = entry;
-                    gts += __popcll(gt[c]);
-                    if ((eq[c] >> lane) & 1) {
-                        if (equal + before < top) list[LP_CAP + equal + before] = entry;
-                        ++before;
-                    }
-                    eqs += __popcll(eq[c]);
-                }
-                above += gts;
-                equal += eqs;
-            }
-        }
-        if (lane < LP_MAX_TOP) s_top[wave][lane] = 0;
-        if (above <= LP_CAP) {
-            const int ne = min(equal, top), n = above + ne;
-            __builtin_amdgcn_wave_barrier();
-            for (int e = lane; e < n; e += 64) {
-                const uint64_t mine = list[e < above ? e : LP_CAP + e - above];
-                int rank = 0;
-                for (int f = 0; f < n; ++f) rank += list[f < above ? f : LP_CAP + f - above] > mine;
-                if (rank < top) s_top[wave][rank] = mine;
-            }
-        } else {  // one maximum at a time, each below the last
-            uint64_t last = ~(uint64_t)0;
-            for (int r = 0; r < top; ++r) {
-                uint64_t b = 0;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const uint32_t k = key_of(i, c);
-                        const uint64_t entry = k ? lp_entry(k, v0 + 256 * C * i + c) : 0;
-                        if (entry < last && entry > b) b = entry;
-                    }
-                last = lp_wave_max(b);
-                if (lane == 0) s_top[wave][r] = last;
-            }
-        }
+            for (int c = 0; c < C; ++c) S += x[i][c] == -INFINITY ? 0.0f : x[i][c];  // a NaN
+    }
+    S = lp_wave_sum(S);
+    T = lp_wave_sum(T);
+    if (lane == 0) s_sum[wave][0] = m, s_sum[wave][1] = S, s_sum[wave][2] = T;
+    if (top > 0) {
+        const bool plain = S == S;  // no NaN and no +inf
+        if (edge) LpWave<TY, C, NV, true>{x, base, e0, V, lane}.select(best, top, plain, s_list[wave], s_top[wave]);
+        else LpWave<TY, C, NV, false>{x, base, e0, V, lane}.select(best, top, plain, s_list[wave], s_top[wave]);
     }
     __syncthreads();
     uint8_t *slot = scratch + ((int64_t)row * P + p) * lp_slot(top);
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 255) {
         float M = -INFINITY, SS = 0.0f, TT = 0.0f;
+#pragma unroll
         for (int w = 0; w < 4; ++w) M = fmaxf(M, s_sum[w][0]);
+#pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float d = s_sum[w][0] - M, f = __expf(d);
-            if (s_sum[w][0] == -INFINITY) {
-                SS += s_sum[w][1];  // 0, or NaN
-                continue;
-            }
-            SS += f * s_sum[w][1];
-            TT += f * s_sum[w][2] + f * d * s_sum[w][1];
+            const bool none = s_sum[w][0] == -INFINITY;  // S is 0, or NaN
+            SS += none ? s_sum[w][1] : f * s_sum[w][1];
+            TT += none ? 0.0f : f * s_sum[w][2] + f * d * s_sum[w][1];
         }
         *(float4 *)slot = make_float4(M, SS, TT, 0.0f);
     }
     // merge the waves' sorted lists: an entry's rank is its place in its own
-    // list and the larger ones of the others
-    for (int e = threadIdx.x; e < 4 * top; e += 256) {
-        const int w = e / top, r = e % top;
+    // list and the larger ones of the others; a place past the last entry is 0
+    if (threadIdx.x < 4 * top) {
+        const int w = threadIdx.x & 3, r = threadIdx.x >> 2;
         const uint64_t mine = s_top[w][r];
-        int rank = r;
-        for (int o = 1; o < 4; ++o)
-            for (int f = 0; f < top; ++f) rank += s_top[(w + o) & 3][f] > mine;
+        int rank = r, present = 0;
+#pragma unroll 4
+        for (int f = 0; f < top; ++f)
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                const uint64_t other = s_top[o][f];
+                rank += o != w && other > mine;
+                present += other != 0;
+            }
         if (mine && rank < top) ((uint64_t *)(slot + 16))[rank] = mine;
+        if (w == 0 && r >= present) ((uint64_t *)(slot + 16))[r] = 0;
     }
-    // places past the chunk's last element
-    int present = 0;
-    for (int w = 0; w < 4; ++w)
-        for (int f = 0; f < top; ++f) present += s_top[w][f] != 0;
-    for (int r = present + threadIdx.x; r < top; r += 256) ((uint64_t *)(slot + 16))[r] = 0;
 }
 
 template <int TY>
@@ -259,16 +285,26 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
             a.logprobs[row] = lp;
         }
     }
+    // the lanes' lists are sorted: the largest head is the next entry; the two
+    // entries behind each head are on their way while a head is compared
     const uint64_t *list = (const uint64_t *)(slot + 16);
-    int at = 0;
-    uint64_t head = lane < P && top > 0 ? list[0] : 0;
+    auto entry = [&](int i) { return lane < P && i < top ? list[i] : (uint64_t)0; };
+    uint64_t head = entry(0), next = entry(1), after = entry(2);
+    int at = 2;
     for (int r = 0; r < top; ++r) {
-        const uint64_t best = lp_wave_max(head);
-        if (head == best && best) {  // entries are unique
-            a.top_logprobs[(int64_t)row * top + r] = (lp_value((uint32_t)(best >> 32)) - M) - lse;
-            a.top_ids[(int64_t)row * top + r] = (int32_t)~(uint32_t)best;
-            ++at;
-            head = at < top ? list[at] : 0;
+        const uint32_t best = lp_wave_max((uint32_t)(head >> 32));
+        uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)(head >> 32) == best);
+        if (__popcll(who) > 1) {  // equal logits: the lowest index, the largest complement
+            const uint32_t low = (uint32_t)(head >> 32) == best ? (uint32_t)head : 0u;
+            const uint32_t first = lp_wave_max(low);
+            who = __builtin_amdgcn_ballot_w64((uint32_t)(head >> 32) == best && (uint32_t)head == first);
+        }
+        if (head != 0 && (who >> lane) & 1) {
+            a.top_logprobs[(int64_t)row * top + r] = (lp_value(best) - M) - lse;
+            a.top_ids[(int64_t)row * top + r] = (int32_t)~(uint32_t)head;
+            head = next;
+            next = after;
+            after = entry(++at);
         }
     }
 }

@@ -234,30 +234,29 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
                 }
             }
             if (careful && !whole) {
+// through the wave's part of the merge buffer, which is free until the end
+                uint32_t *sp = (uint32_t *)&s_o[wave][0][0], *sv = sp + RT * 512;
+                static_assert((RT + 1) * 512 * 4 <= sizeof(s_o[0]), "operands of one dim block");
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) sp[512 * t + 64 * x + lane] = word4(pf[t][x / 4], x % 4);
+#pragma unroll
+                for (int d = 0; d < NB; ++d) {
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) sv[64 * x + lane] = word4(vf[d][x / 4], x % 4);
+                    __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-                for (int key = 0; key < 32; ++key) {
-                    const int w = 4 * (key >> 4) + ((key & 7) >> 1), from = 32 * ((key >> 3) & 1), odd = key & 1;
-                    float p[RT];
+                    for (int key = 0; key < 32; ++key) {
+                        const int at = 64 * (4 * (key >> 4) + ((key & 7) >> 1)) + 32 * ((key >> 3) & 1), sh = 16 * (key & 1);
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) {
-                        uint32_t pw = 0;
+                        for (int t = 0; t < RT; ++t) {
+                            const float p = h2f((uint16_t)(sp[512 * t + at + c] >> sh));
+                            if ((vis[t] >> key) & 1)
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) pw = x == w ? word4(pf[t][x / 4], x % 4) : pw;
-                        pw = __shfl(pw, c + from, 64);
-                        p[t] = h2f((uint16_t)(odd ? pw >> 16 : pw & 0xffffu));
-                    }
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        uint32_t vw = 0;
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) vw = x == w ? word4(vf[d][x / 4], x % 4) : vw;
-                        const float v1 = h2f((uint16_t)(odd ? vw >> 16 : vw & 0xffffu));
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float v = __shfl(v1, from + 8 * (i / 4) + 4 * h + i % 4, 64);
-#pragma unroll
-                            for (int t = 0; t < RT; ++t)
-                                if ((vis[t] >> key) & 1) O[t][d][i] += p[t] * v;
+                                for (int i = 0; i < 16; ++i)
+                                    O[t][d][i] += p * h2f((uint16_t)(sv[at + 8 * (i / 4) + 4 * h + i % 4] >> sh));
                         }
                     }
                 }
@@ -356,7 +355,6 @@ __global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a, int row
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     constexpr int E = (D + 63) / 64;
     float acc[E] = {};
-#pragma unroll 4
     for (int p = 0; p < np; ++p) {
         const float wp = __shfl(w, p, 64);
 #pragma unroll

@@ -515,18 +515,16 @@ def reshape_and_cache(key, value, k_cache, v_cache, slots, num_kv_heads, block_s
 
 
 # --------------------------------------------------------- serving operators
-def _arg(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _tensor(t, dtype, shape, name: str, device=None):
-    """A contiguous tensor of this dtype and shape (None: any extent) on `device`."""
-    _arg(t.dtype == dtype and t.dim() == len(shape) and t.is_contiguous() and
-         all(w is None or n == w for n, w in zip(t.shape, shape)),
-         f"{name}: {t.dtype} {tuple(t.shape)}, not contiguous {dtype} {tuple('*' if w is None else w for w in shape)}")
-    _arg(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+def _tensor(t, dtype, shape, name: str, device):
+    """The address of a contiguous tensor of this dtype and shape on `device`."""
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, not contiguous {dtype} {shape} on {device}")
     return t.data_ptr()
+
+
+def _extent(t) -> int:
+    """The first extent of a tensor that may have any."""
+    return t.shape[0] if t.dim() else 0
 
 
 class _on:
@@ -540,11 +538,13 @@ class _on:
 
         if self.device.type != "cuda":
             raise ValueError(f"tensors must be on the GPU, not on {self.device}")
+        if self.stream is not None and getattr(self.stream, "device", self.device) != self.device:
+            raise ValueError(f"the stream is on {self.stream.device}, the tensors are on {self.device}")
         if self.device.index != torch.cuda.current_device():
             self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        if self.stream is not None and getattr(self.stream, "device", self.device) != self.device:
-            raise ValueError(f"the stream is on {self.stream.device}, the tensors are on {self.device}")
+        if self.stream is None:  # current_stream's number, without the 2.7 us its Stream object takes
+            return torch._C._cuda_getCurrentRawStream(self.device.index)
         return _stream(self.stream)
 
     def __exit__(self, *exc):
@@ -562,6 +562,18 @@ def _use_on(stream, *tensors):
             t.record_stream(s)
 
 
+def _token_rows(t, heads: int, hs: int, name: str, device):
+    """(address, token stride) of a (tokens, heads, head size) view whose tokens' heads are contiguous."""
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    st, one = t.stride(), heads * hs
+    if t.shape[0] <= 1:  # the stride of a single token means nothing
+        st = (one, st[1], st[2])
+    if t.numel() and ((hs > 1 and st[2] != 1) or (heads > 1 and st[1] != hs)):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return t.data_ptr(), st[0] if t.numel() else one
+
+
 def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=None, stream=None):
     """Causal attention of prompts packed one after another: q (tokens, heads,
     head size), k and v (tokens, kv heads, head size) f16 or bf16, tokens at any
@@ -571,30 +583,30 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     left as they were in `out`."""
     import torch
 
-    tokens, heads, hs = q.shape
-    _arg(q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype,
-         f"q, k and v must be f16 or all bf16, not {q.dtype}, {k.dtype}, {v.dtype}")
-    _arg(k.dim() == 3 and k.shape == v.shape and k.shape[0] == tokens and k.shape[2] == hs,
-         f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    (tokens, heads, hs), dtype, dev = q.shape, q.dtype, q.device
+    if dtype not in (torch.float16, torch.bfloat16) or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"q, k and v must be f16 or all bf16, not {dtype}, {k.dtype}, {v.dtype}")
+    kv = k.shape[1] if k.dim() == 3 else 0
+    if k.shape != (tokens, kv, hs) or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     fresh = out is None
     if fresh:
-        out = torch.empty((tokens, heads, hs), dtype=q.dtype, device=q.device)
-    _arg(out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and type")
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        _arg(t.device == q.device, f"{name} is on {t.device}, not on {q.device}")
-        _arg(t.numel() == 0 or ((t.shape[2] == 1 or t.stride(2) == 1) and (t.shape[1] == 1 or t.stride(1) == hs)),
-             f"{name}: a token's heads must be contiguous")
+        out = torch.empty((tokens, heads, hs), dtype=dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != dtype:
+        raise ValueError("out must have q's shape and type")
     a = TlhPackedArgs()
-    a.seq_starts = _tensor(seq_starts, torch.int32, (None,), "seq_starts", q.device)
-    _arg(seq_starts.shape[0] >= 1, "seq_starts must hold at least one start")
-    a.out, a.q, a.k, a.v = out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr()
-    one = tokens <= 1  # the stride of a single token means nothing
-    a.out_stride, a.q_stride = (heads * hs, heads * hs) if one else (out.stride(0), q.stride(0))
-    a.k_stride, a.v_stride = (k.shape[1] * hs, k.shape[1] * hs) if one else (k.stride(0), v.stride(0))
-    a.type = F16 if q.dtype == torch.float16 else BF16
-    a.num_seqs, a.num_tokens, a.max_seq_len = seq_starts.shape[0] - 1, tokens, max_seq_len
-    a.num_heads, a.num_kv_heads, a.head_size, a.scale = heads, k.shape[1], hs, scale
-    with _on(q.device, stream) as s:
+    a.q, a.q_stride = _token_rows(q, heads, hs, "q", dev)
+    a.k, a.k_stride = _token_rows(k, kv, hs, "k", dev)
+    a.v, a.v_stride = _token_rows(v, kv, hs, "v", dev)
+    a.out, a.out_stride = _token_rows(out, heads, hs, "out", dev)
+    n = _extent(seq_starts)
+    a.seq_starts = _tensor(seq_starts, torch.int32, (n,), "seq_starts", dev)
+    if n < 1:
+        raise ValueError("seq_starts must hold at least one start")
+    a.type = F16 if dtype == torch.float16 else BF16
+    a.num_seqs, a.num_tokens, a.max_seq_len = n - 1, tokens, max_seq_len
+    a.num_heads, a.num_kv_heads, a.head_size, a.scale = heads, kv, hs, scale
+    with _on(dev, stream) as s:
         check(lib().tlh_packed_attention(C.byref(a), s))
     if fresh:
         _use_on(stream, out)
@@ -618,6 +630,7 @@ class TreeAttention:
         check(lib().tlh_tree_attention_scratch_bytes(C.byref(a), C.byref(n)))
         self.scratch_bytes = n.value
         self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
+        self.device, self.scratch_ptr = self.scratch.device, self.scratch.data_ptr()
 
     def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream=None):
         """q and out f16 (num_rows, heads, head size), the caches in the paged-attention layouts,
@@ -625,19 +638,19 @@ class TreeAttention:
         tokens, draft_starts i32 (num_seqs + 1,), draft_masks i64 (num_rows,): bit j = sees draft j."""
         import torch
 
-        a, dev = self.args, self.scratch.device
+        a, dev = TlhTreeArgs.from_buffer_copy(self.args), self.device  # a call's own: threads may share the node
         rows, S, KV, D, bs = a.num_rows, a.num_seqs, a.num_kv_heads, a.head_size, a.block_size
         a.q = _tensor(q, torch.float16, (rows, a.num_heads, D), "q", dev)
         a.out = _tensor(out, torch.float16, (rows, a.num_heads, D), "out", dev)
-        a.k_cache = _tensor(k_cache, torch.float16, (None, KV, D // 8, bs, 8), "k_cache", dev)
-        a.v_cache = _tensor(v_cache, torch.float16, (k_cache.shape[0], KV, D, bs), "v_cache", dev)
+        a.num_blocks = blocks = _extent(k_cache)
+        a.k_cache = _tensor(k_cache, torch.float16, (blocks, KV, D // 8, bs, 8), "k_cache", dev)
+        a.v_cache = _tensor(v_cache, torch.float16, (blocks, KV, D, bs), "v_cache", dev)
         a.block_tables = _tensor(block_tables, torch.int32, (S, a.max_blocks_per_seq), "block_tables", dev)
         a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
         a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
         a.draft_masks = _tensor(draft_masks, torch.int64, (rows,), "draft_masks", dev)
-        a.num_blocks = k_cache.shape[0]
         with _on(dev, stream) as s:
-            check(lib().tlh_tree_attention(C.byref(a), self.scratch.data_ptr(), self.scratch_bytes, s))
+            check(lib().tlh_tree_attention(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
         return out
 
 
@@ -665,9 +678,11 @@ class KVPools:
     def __init__(self, k_caches, v_caches, num_kv_heads: int, head_size: int, block_size: int):
         import torch
 
-        _arg(len(k_caches) == len(v_caches) and len(k_caches) > 0, "as many key as value pools, at least one")
+        if len(k_caches) != len(v_caches) or not k_caches:
+            raise ValueError("as many key as value pools, at least one")
         self.device, self.num_blocks = k_caches[0].device, k_caches[0].shape[0]
         self.kv_heads, self.head_size, self.block_size = num_kv_heads, head_size, block_size
+        self.block_bytes = num_kv_heads * head_size * block_size * 2
         n, self.layers = self.num_blocks, len(k_caches)
         ks = [_tensor(t, torch.float16, (n, num_kv_heads, head_size // 8, block_size, 8), "k_cache", self.device)
               for t in k_caches]
@@ -682,10 +697,10 @@ class KVPools:
         another pair's destination or any pair's source; a pair outside the pools does nothing."""
         import torch
 
-        p = _tensor(pairs, torch.int64, (None, 2), "pairs", self.device)
+        n = _extent(pairs)
+        p = _tensor(pairs, torch.int64, (n, 2), "pairs", self.device)
         with _on(self.device, stream) as s:
-            check(lib().tlh_copy_blocks(self._all, 2 * self.layers, self.kv_heads * self.head_size * self.block_size * 2,
-                                        self.num_blocks, p, pairs.shape[0], s))
+            check(lib().tlh_copy_blocks(self._all, 2 * self.layers, self.block_bytes, self.num_blocks, p, n, s))
 
     def compact(self, block_tables, context_lens, draft_starts, keep, new_lens, max_drafts: int, stream=None):
         """Moves the kept drafted tokens (bit j of keep[s], i64 (sequences,)) of every sequence right behind
@@ -693,16 +708,16 @@ class KVPools:
         import torch
 
         a, dev = TlhCompactArgs(), self.device
-        S = context_lens.shape[0]
+        S, width = _extent(context_lens), block_tables.shape[-1]
         a.k_caches, a.v_caches = self._k, self._v
-        a.block_tables = _tensor(block_tables, torch.int32, (S, None), "block_tables", dev)
+        a.block_tables = _tensor(block_tables, torch.int32, (S, width), "block_tables", dev)
         a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
         a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
         a.keep = _tensor(keep, torch.int64, (S,), "keep", dev)
         a.new_lens = _tensor(new_lens, torch.int32, (S,), "new_lens", dev)
         a.num_blocks, a.num_layers, a.num_seqs, a.max_drafts = self.num_blocks, self.layers, S, max_drafts
         a.num_kv_heads, a.head_size, a.block_size = self.kv_heads, self.head_size, self.block_size
-        a.max_blocks_per_seq = block_tables.shape[1]
+        a.max_blocks_per_seq = width
         with _on(dev, stream) as s:
             check(lib().tlh_compact_cache(C.byref(a), s))
         return new_lens
@@ -715,7 +730,7 @@ class TokenLogprobs:
     def __init__(self, rows: int, vocab: int, top: int = 0, dtype=None, device="cuda"):
         import torch
 
-        self.rows, self.dtype = rows, dtype or torch.float32
+        self.rows, self.vocab, self.dtype = rows, vocab, dtype or torch.float32
         a = self.args = TlhLogprobsArgs()
         a.type, a.rows, a.vocab, a.top = _ggml_type(torch.empty(0, dtype=self.dtype)), rows, vocab, top
         a.row_stride = vocab
@@ -723,27 +738,30 @@ class TokenLogprobs:
         check(lib().tlh_token_logprobs_scratch_bytes(C.byref(a), C.byref(n)))
         self.scratch_bytes = n.value
         self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
+        self.device, self.scratch_ptr = self.scratch.device, self.scratch.data_ptr()
 
     def __call__(self, logits, tokens, logprobs, entropy, top_logprobs=None, top_ids=None, stream=None):
         """logits (n, vocab) with n <= rows, any row stride; tokens i32 (n,); logprobs and entropy f32 (n,);
         top_logprobs f32 and top_ids i32 (n, top). tokens and logprobs, or entropy, may be None."""
         import torch
 
-        a, dev, n = self.args, self.scratch.device, logits.shape[0]
-        _arg(logits.dtype == self.dtype and logits.dim() == 2 and n <= self.rows and logits.shape[1] == a.vocab and
-             logits.device == dev and (logits.shape[1] == 1 or logits.stride(1) == 1),
-             f"logits {logits.dtype} {tuple(logits.shape)} on {logits.device} for {self.rows} rows of {a.vocab} {self.dtype}")
+        a, dev, n, vocab = TlhLogprobsArgs.from_buffer_copy(self.args), self.device, _extent(logits), self.vocab
+        if (logits.dtype != self.dtype or logits.shape != (n, vocab) or n > self.rows or logits.device != dev or
+                (vocab > 1 and logits.stride(1) != 1)):
+            raise ValueError(f"logits {logits.dtype} {tuple(logits.shape)} on {logits.device}, strides {logits.stride()}, "
+                             f"for up to {self.rows} rows of {vocab} {self.dtype} on {dev}")
         a.rows, a.logits = n, logits.data_ptr()
-        a.row_stride = logits.stride(0) if n > 1 else a.vocab
+        a.row_stride = logits.stride(0) if n > 1 else vocab
         a.tokens = _tensor(tokens, torch.int32, (n,), "tokens", dev) if tokens is not None else None
         a.logprobs = _tensor(logprobs, torch.float32, (n,), "logprobs", dev) if logprobs is not None else None
         a.entropy = _tensor(entropy, torch.float32, (n,), "entropy", dev) if entropy is not None else None
         if a.top:
-            _arg(top_logprobs is not None and top_ids is not None, "top_logprobs and top_ids are needed where top > 0")
+            if top_logprobs is None or top_ids is None:
+                raise ValueError("top_logprobs and top_ids are needed where top > 0")
             a.top_logprobs = _tensor(top_logprobs, torch.float32, (n, a.top), "top_logprobs", dev)
             a.top_ids = _tensor(top_ids, torch.int32, (n, a.top), "top_ids", dev)
         with _on(dev, stream) as s:
-            check(lib().tlh_token_logprobs(C.byref(a), self.scratch.data_ptr(), self.scratch_bytes, s))
+            check(lib().tlh_token_logprobs(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
         return logprobs, entropy, top_logprobs, top_ids
 
 
