@@ -13,7 +13,7 @@
 // to 32 RT rows that share a kv head (drafted tokens x the group's heads) and
 // one partition of the context; its waves take 32-key tiles in turn. Both
 // products' operands come from the pages straight into registers, 16 bytes a
-// lane, and need no LDS:
+// lane:
 //   S^T = K . Q^T     a lane's key row is one of 32, taken in an order that
 //                     makes S^T's registers 8 i .. 8 i + 7 the keys 16 i + 8 h ..
 //                     + 7 of the tile, in order;
@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
     constexpr int MD = NB > 1 ? 64 : 32;  // dims merged at a time
     __shared__ __attribute__((aligned(16))) float s_o[TA_WAVES][32][MD + 4];
     __shared__ float s_m[TA_WAVES][32 * RT], s_l[TA_WAVES][32 * RT];
+    __shared__ uint4 s_q[RT][NS][64];  // Q^T as the lanes take it: 16 bytes a lane, in order
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
     // with 8 kv heads a head's workgroups share an XCD, row blocks next to each other
@@ -78,19 +79,18 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
     const int ntiles = (t1 - t0 + 31) / 32;
     const int32_t *table = a.tables + (int64_t)s * a.max_blocks;
 
-    // this lane's rows: drafted token row / G, head row % G of the group
-    uint4 qf[RT][NS];
+    // this lane's rows: drafted token row / G, head row % G of the group. The four
+    // waves share Q in LDS: in registers it would leave too few for two waves a SIMD
     uint64_t mask[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = min(r0 + 32 * t + c, R - 1), i = row / a.G;
         const uint8_t *qr = (const uint8_t *)(a.q + ((int64_t)(sq.b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * h;
         mask[t] = (uint64_t)a.masks[sq.b + i];
-#pragma unroll
-        for (int st = 0; st < NS; ++st) {
+        for (int st = wave; st < NS; st += TA_WAVES) {
             const uint4 w = *(const uint4 *)(qr + 32 * st);
-            qf[t][st] = make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor,
-                                   (w.w & a.qand) ^ a.qxor);
+            s_q[t][st][lane] = make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor,
+                                          (w.w & a.qand) ^ a.qxor);
         }
     }
 
@@ -104,15 +104,20 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
         int id[PAGES];
         uint32_t good;  // bits of the tile's keys whose page is inside
     };
-    auto pages_of = [&](int base) {
-        Pages p;
+    // their ids are read two tiles ahead, so that no tile waits for the table
+    auto ids_of = [&](int k) {
+        Pages p = {};
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i)
+            p.id[i] = table[__builtin_amdgcn_readfirstlane(min((t0 + 32 * k) / BS + i, (L - 1) / BS))];
+        return p;
+    };
+    auto checked = [&](Pages p) {
         p.good = 0;
 #pragma unroll
         for (int i = 0; i < PAGES; ++i) {
-            const int at = __builtin_amdgcn_readfirstlane(min(base / BS + i, (L - 1) / BS));
-            const int id = table[at];
-            const bool ok = id >= 0 && id < a.num_blocks;
-            p.id[i] = __builtin_amdgcn_readfirstlane(ok ? id : 0);
+            const bool ok = p.id[i] >= 0 && p.id[i] < a.num_blocks;
+            p.id[i] = ok ? p.id[i] : 0;
             p.good |= ok ? (BS == 32 ? ~0u : ((1u << (BS & 31)) - 1) << (BS * i)) : 0u;
         }
         return p;
@@ -133,12 +138,14 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int key = 16 * i + 8 * h;
-            const uint8_t *vp = vbase + page_at(p, key) + (key % BS) * 2;
+            const uint8_t *vp = vbase + page_at(p, key) + (key % BS) * 2 + c * BS * 2;
 #pragma unroll
-            for (int d = 0; d < NB; ++d) vf[d][i] = *(const uint4 *)(vp + (int64_t)min(32 * d + c, D - 1) * BS * 2);
+            for (int d = 0; d < NB; ++d)  // dims past the last repeat it
+                vf[d][i] = *(const uint4 *)(vp + (32 * d + 31 < D ? 32 * d : min(32 * d + c, D - 1) - c) * BS * 2);
         }
     };
 
+    __syncthreads();
     f32x16 O[RT][NB];
     float m[RT], l[RT];
     // A value that is not finite would turn the zero weight of a key that a row does
@@ -155,22 +162,23 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
         }
         Pages pg = {}, pn = {};
         if (wave < ntiles) {
-            pg = pages_of(t0 + 32 * wave);
+            pg = checked(ids_of(wave));
+            pn = ids_of(wave + TA_WAVES);
             load_k(pg);
             load_v(pg);
         }
         for (int k = wave; k < ntiles; k += TA_WAVES) {
             const int base = t0 + 32 * k;
-            const bool more = k + TA_WAVES < ntiles;
-            pn = more ? pages_of(base + 32 * TA_WAVES) : pg;
+            pn = checked(pn);
+            const Pages after = ids_of(k + 2 * TA_WAVES);
             f32x16 S[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t) S[t] = (f32x16){};
 #pragma unroll
             for (int st = 0; st < NS; ++st)
 #pragma unroll
-                for (int t = 0; t < RT; ++t) S[t] = mfma32<false>(kf[st], qf[t][st], S[t]);
-            load_k(pn);  // past the last tile: its own again
+                for (int t = 0; t < RT; ++t) S[t] = mfma32<false>(kf[st], s_q[t][st][lane], S[t]);
+            load_k(pn);  // past the last tile: the last page again
             const bool whole = base + 32 <= prefix && pg.good == ~0u;
             uint32_t vis[RT];
             uint32_t there = ~0u;  // keys that are in the cache
@@ -270,6 +278,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
             }
             load_v(pn);
             pg = pn;
+            pn = after;
         }
         if (careful || !some_masked) break;
         bool bad = false;
