@@ -43,6 +43,11 @@ template <bool BF> __device__ __forceinline__ float unpack16(uint32_t h) {
 }
 __device__ __forceinline__ uint32_t word4(const uint4 &v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 
+// 16 bytes a lane from global memory straight to LDS: lane l's land at lds + 16 l
+__device__ __forceinline__ void to_lds(const void *g, void *lds) {
+    __builtin_amdgcn_global_load_lds(g, (lds_void *)lds, 16, 0, 0);
+}
+
 // a lane's value and its partner's (l ^ 32)
 __device__ __forceinline__ float max_halves(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
             const int64_t key = min(t * KT + kk, n - 1);
             int ck = lp ^ Gm::kswz(kk), cv = lp ^ Gm::vswz(kk);
             if (Gm::C < CP) ck = ck < Gm::C ? ck : 0, cv = cv < Gm::C ? cv : 0;
-            __builtin_amdgcn_global_load_lds(kb + key * a.sk + 16 * ck, (lds_void *)(T + (4 * i + wave) * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(vb + key * a.sv + 16 * cv, (lds_void *)(T + Gm::TILE + (4 * i + wave) * 1024), 16, 0, 0);
+            to_lds(kb + key * a.sk + 16 * ck, T + (4 * i + wave) * 1024);
+            to_lds(vb + key * a.sv + 16 * cv, T + Gm::TILE + (4 * i + wave) * 1024);
         }
     };
 

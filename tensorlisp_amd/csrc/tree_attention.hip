@@ -9,19 +9,24 @@
 // A row that sees nothing gives zeros.
 //
 // Bound by one read of the keys and values while the rows are few; by the
-// matrix cores with a tree of tens of tokens. A workgroup of four waves takes up
-// to 32 RT rows that share a kv head (drafted tokens x the group's heads) and
-// one partition of the context; its waves take 32-key tiles in turn. Both
-// products' operands come from the pages straight into registers, 16 bytes a
-// lane:
+// matrix cores and the exponentials with a tree of tens of tokens. The rows of a
+// (sequence, kv head) are its drafted tokens x the group's heads; a wave owns 32:
 //   S^T = K . Q^T     a lane's key row is one of 32, taken in an order that
 //                     makes S^T's registers 8 i .. 8 i + 7 the keys 16 i + 8 h ..
 //                     + 7 of the tile, in order;
 //   O^T += V^T . P^T  so P is the operand as it is, and V^T's is 8 consecutive
 //                     places of one dim.
-// The next tile's keys are requested when this one's have been multiplied, its
-// values when this one's have, so that with two waves a SIMD a tile is always
-// in flight. Partitions are merged by a second launch.
+// Either operand is 16 bytes a lane that lie together in the page, so the pages
+// are read as they are. Two forms:
+//  * up to 64 rows: a workgroup takes 32 rows and one partition of the context,
+//    its four waves 32-key tiles in turn, straight into registers: the next
+//    tile's keys are requested when this one's have been multiplied, its values
+//    when this one's have, so with two waves a SIMD a tile is always in flight;
+//    the waves merge at the end;
+//  * more rows: a workgroup takes 128 rows, and its four waves share 64-key
+//    tiles in LDS (double-buffered, loaded straight from the pages in the order
+//    in which the lanes take them), so a page is read a quarter as often.
+// Partitions are merged by a second launch.
 #include <algorithm>
 
 #include "mfma32.hpp"
@@ -29,7 +34,7 @@
 namespace tlh {
 
 constexpr int TA_WAVES = 4, TA_KEYS = 32 * TA_WAVES;  // keys a workgroup takes a round
-constexpr int TA_WGS = 1024;                          // workgroups a split aims for
+constexpr int TA_WGS = 1024, TA_WGS_SHARED = 512;     // workgroups a split aims for
 constexpr int TA_MAX_PARTS = 64;                      // a lane each in the merge
 
 struct TaArgs {
@@ -37,9 +42,9 @@ struct TaArgs {
     const uint16_t *q, *kc, *vc;
     const int32_t *tables, *lens, *starts;
     const int64_t *masks;
-    float *part;  // [s][kv head][row block][partition][row][m, l, -, -, D]
+    float *part;  // [s][kv head][block of 32 rows][partition][row][m, l, -, -, D]
     int64_t num_blocks;
-    int S, H, KV, G, rows, max_drafts, max_blocks, max_ctx, P, part_len, RB;
+    int S, H, KV, G, rows, max_drafts, max_blocks, max_ctx, P, part_len, RB;  // RB: blocks of 32 rows
     float cs;             // |scale| * log2(e); 1 where the scale is 0
     uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
@@ -56,63 +61,39 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int s) {
     return q;
 }
 
-template <int D, int BS, int RT>
-__global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_tree_attn(const TaArgs a) {
-    constexpr int NS = D / 16, NB = (D + 31) / 32, PAGES = 32 / BS;
-    constexpr int MD = NB > 1 ? 64 : 32;  // dims merged at a time
-    __shared__ __attribute__((aligned(16))) float s_o[TA_WAVES][32][MD + 4];
-    __shared__ float s_m[TA_WAVES][32 * RT], s_l[TA_WAVES][32 * RT];
-    __shared__ uint4 s_q[RT][NS][64];  // Q^T as the lanes take it: 16 bytes a lane, in order
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = lane >> 5, c = lane & 31;
-    // with 8 kv heads a head's workgroups share an XCD, row blocks next to each other
-    const int hk = blockIdx.x % a.KV;
-    const int rb = (blockIdx.x / a.KV) % a.RB;
-    const int s = (blockIdx.x / a.KV / a.RB) % a.S;
-    const int part = blockIdx.x / a.KV / a.RB / a.S;
-    const TaSeq sq = ta_seq(a, s);
-    const int n = sq.n, L = sq.L, R = n * a.G, r0 = rb * 32 * RT;
-    const int t0 = part * a.part_len;
-    if (r0 >= R || (part > 0 && t0 >= L)) return;
-    const int t1 = min(L, t0 + a.part_len);
-    const int prefix = L - n;
-    const int ntiles = (t1 - t0 + 31) / 32;
-    const int32_t *table = a.tables + (int64_t)s * a.max_blocks;
+// What the two forms share: a wave's 32 rows of one (sequence, kv head).
+template <int D, int BS> struct TaWave {
+    static constexpr int NS = D / 16, NB = (D + 31) / 32, PAGES = 32 / BS;
+    const TaArgs &a;
+    const int lane, h, c;
+    const int32_t *table;
+    const int64_t page_bytes;
+    const uint8_t *kbase, *vbase;
+    const int kappa;  // the key of S^T's row c: bits 2 and 3 of c exchanged
+    const int prefix, L;
+    uint64_t mask = 0;  // of this lane's row
 
-    // this lane's rows: drafted token row / G, head row % G of the group. The four
-    // waves share Q in LDS: in registers it would leave too few for two waves a SIMD
-    uint64_t mask[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int row = min(r0 + 32 * t + c, R - 1), i = row / a.G;
-        const uint8_t *qr = (const uint8_t *)(a.q + ((int64_t)(sq.b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * h;
-        mask[t] = (uint64_t)a.masks[sq.b + i];
-        for (int st = wave; st < NS; st += TA_WAVES) {
-            const uint4 w = *(const uint4 *)(qr + 32 * st);
-            s_q[t][st][lane] = make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor,
-                                          (w.w & a.qand) ^ a.qxor);
-        }
-    }
+    __device__ TaWave(const TaArgs &a_, int lane_, int s, int hk, const TaSeq &sq)
+        : a(a_), lane(lane_), h(lane_ >> 5), c(lane_ & 31), table(a_.tables + (int64_t)s * a_.max_blocks),
+          page_bytes((int64_t)a_.KV * D * BS * 2), kbase((const uint8_t *)a_.kc + (int64_t)hk * D * BS * 2),
+          vbase((const uint8_t *)a_.vc + (int64_t)hk * D * BS * 2),
+          kappa((c & 0x13) | (c & 4) << 1 | (c & 8) >> 1), prefix(sq.L - sq.n), L(sq.L) {}
 
-    const int64_t page_bytes = (int64_t)a.KV * D * BS * 2;
-    const uint8_t *kbase = (const uint8_t *)a.kc + (int64_t)hk * D * BS * 2;
-    const uint8_t *vbase = (const uint8_t *)a.vc + (int64_t)hk * D * BS * 2;
-    // the key of S^T's row c: bits 2 and 3 of c exchanged
-    const int kappa = (c & 0x13) | (c & 4) << 1 | (c & 8) >> 1;
-    // a tile's pages (the last one's again past the context), and whether any is outside the pools
+    // The pages of the tile at key `base` (past the context its last one again). Their
+    // ids are read ahead of their use, so that no tile waits for the table; one
+    // outside the pools is taken as page 0, its keys as not there.
     struct Pages {
         int id[PAGES];
         uint32_t good;  // bits of the tile's keys whose page is inside
     };
-    // their ids are read two tiles ahead, so that no tile waits for the table
-    auto ids_of = [&](int k) {
+    __device__ Pages ids_of(int base) const {
         Pages p = {};
 #pragma unroll
         for (int i = 0; i < PAGES; ++i)
-            p.id[i] = table[__builtin_amdgcn_readfirstlane(min((t0 + 32 * k) / BS + i, (L - 1) / BS))];
+            p.id[i] = table[__builtin_amdgcn_readfirstlane(min(base / BS + i, (L - 1) / BS))];
         return p;
-    };
-    auto checked = [&](Pages p) {
+    }
+    __device__ Pages checked(Pages p) const {
         p.good = 0;
 #pragma unroll
         for (int i = 0; i < PAGES; ++i) {
@@ -121,239 +102,438 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 && RT == 1 ? 2 : 1) k_
             p.good |= ok ? (BS == 32 ? ~0u : ((1u << (BS & 31)) - 1) << (BS * i)) : 0u;
         }
         return p;
-    };
-    auto page_at = [&](const Pages &p, int key) {  // of key `key` of the tile
+    }
+    __device__ int64_t page_at(const Pages &p, int key) const {  // of key `key` of the tile
         int id = p.id[0];
 #pragma unroll
         for (int i = 1; i < PAGES; ++i) id = key / BS == i ? p.id[i] : id;
         return (int64_t)id * page_bytes;
-    };
-    uint4 kf[NS], vf[NB][2];
-    auto load_k = [&](const Pages &p) {
-        const uint8_t *kp = kbase + page_at(p, kappa) + h * BS * 16 + (kappa % BS) * 16;
-#pragma unroll
-        for (int st = 0; st < NS; ++st) kf[st] = *(const uint4 *)(kp + st * BS * 32);
-    };
-    auto load_v = [&](const Pages &p) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int key = 16 * i + 8 * h;
-            const uint8_t *vp = vbase + page_at(p, key) + (key % BS) * 2 + c * BS * 2;
-#pragma unroll
-            for (int d = 0; d < NB; ++d)  // dims past the last repeat it
-                vf[d][i] = *(const uint4 *)(vp + (32 * d + 31 < D ? 32 * d : min(32 * d + c, D - 1) - c) * BS * 2);
-        }
-    };
+    }
+    // this lane's 16 bytes of the keys' step st are k_at() + k_step(st), of the values'
+    // keys 16 i + 8 h .. + 7 and dims 32 d .. + 31 v_at(i) + v_step(d)
+    __device__ const uint8_t *k_at(const Pages &p) const {
+        return kbase + page_at(p, kappa) + h * BS * 16 + (kappa % BS) * 16;
+    }
+    __device__ static int k_step(int st) { return st * BS * 32; }
+    __device__ const uint8_t *v_at(const Pages &p, int i) const {
+        const int key = 16 * i + 8 * h;
+        return vbase + page_at(p, key) + (key % BS) * 2 + c * BS * 2;
+    }
+    __device__ int v_step(int d) const {  // dims past the last repeat it
+        return (32 * d + 31 < D ? 32 * d : min(32 * d + c, D - 1) - c) * BS * 2;
+    }
 
-    __syncthreads();
-    f32x16 O[RT][NB];
-    float m[RT], l[RT];
+    __device__ const uint8_t *set_row(int b, int hk, int row) {  // -> this lane's part of the row's q
+        const int i = row / a.G;
+        mask = (uint64_t)a.masks[b + i];
+        return (const uint8_t *)(a.q + ((int64_t)(b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * h;
+    }
+    __device__ uint4 signed_q(uint4 w) const {
+        return make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor, (w.w & a.qand) ^ a.qxor);
+    }
+
+    f32x16 O[NB];
+    float m, l;  // the exponents' reference (an unscaled score), this half's sum
     // A value that is not finite would turn the zero weight of a key that a row does
     // not see into NaN. So where a wave's sums come out not finite, it takes its tiles
     // again, carefully: in those with masked keys it adds each seen key's product by itself.
-    bool careful = false, some_masked = false;
-    for (;;) {
+    bool some_masked = false;
+    __device__ void reset() {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            m[t] = -INFINITY;
-            l[t] = 0.0f;
+        for (int d = 0; d < NB; ++d) O[d] = (f32x16){};
+        m = -INFINITY;
+        l = 0.0f;
+    }
+    __device__ bool bad() const {
+        bool x = false;
 #pragma unroll
-            for (int d = 0; d < NB; ++d) O[t][d] = (f32x16){};
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x = x || !(fabsf(O[d][i]) < INFINITY);
+        return x;
+    }
+
+    struct Seen {
+        bool whole;       // every row sees every key of the tile
+        uint32_t there;   // keys that are in the cache
+        uint32_t vis;     // keys that this lane's row sees
+    };
+    __device__ Seen seen(int base, uint32_t good) {
+        Seen s = {base + 32 <= prefix && good == ~0u, ~0u, ~0u};
+        if (!s.whole) {
+            some_masked = true;
+            s.there = L <= base ? 0u : good & (L - base >= 32 ? ~0u : (1u << (L - base)) - 1);
+            const int d = base - prefix;
+            const uint32_t see = d >= 64    ? 0u
+                                 : d >= 0   ? (uint32_t)(mask >> d)
+                                 : d <= -32 ? ~0u
+                                            : (uint32_t)(mask << -d) | ((1u << -d) - 1);
+            s.vis = see & s.there;
         }
-        Pages pg = {}, pn = {};
+        return s;
+    }
+    // scores -> numerators (f16), the running maximum and sum
+    __device__ void softmax(f32x16 &S, const Seen &s, uint4 (&pf)[2]) {
+        if (!s.whole) {
+            const uint32_t mine = s.vis >> (8 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[i] = -INFINITY;
+        }
+        float mx = S[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[i]);
+        mx = max_halves(mx);
+        // the reference moves only when the maximum has grown by more than 2^8
+        const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f);
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+            const float alpha = grow ? __builtin_amdgcn_exp2f((m - mx) * a.cs) : 1.0f;
+            m = grow ? mx : m;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) O[d][i] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * a.cs;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[8 * i + e] * a.cs - mc);
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            pf[i] = pack8<false>(p);
+        }
+    }
+    // places that hold no token's value may hold anything
+    __device__ uint4 live_v(uint4 v, int i, uint32_t there) const {
+        const uint32_t on = there >> (16 * i + 8 * h);
+        auto keep = [&](int e) { return ((on >> e) & 1 ? 0xffffu : 0u) | ((on >> e) & 2 ? 0xffff0000u : 0u); };
+        return make_uint4(v.x & keep(0), v.y & keep(2), v.z & keep(4), v.w & keep(6));
+    }
+    // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
+    // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
+    __device__ void careful_pv(int d, const Seen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+            const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
+            if (!((s.vis >> key) & 1)) continue;
+            const float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                O[d][x] += p * h2f((uint16_t)(sv[sv_step * i + 4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
+        }
+    }
+};
+
+template <int D, int BS>
+__global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(const TaArgs a) {
+    using W = TaWave<D, BS>;
+    constexpr int NS = W::NS, NB = W::NB;
+    constexpr int MD = NB > 1 ? 64 : 32;  // dims merged at a time
+    __shared__ __attribute__((aligned(16))) float s_o[TA_WAVES][32][MD + 4];
+    __shared__ float s_m[TA_WAVES][32], s_l[TA_WAVES][32];
+    __shared__ uint4 s_q[NS][64];  // Q^T as the lanes take it: 16 bytes a lane, in order
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // with 8 kv heads a head's workgroups share an XCD, row blocks next to each other
+    const int hk = blockIdx.x % a.KV;
+    const int rb = (blockIdx.x / a.KV) % a.RB;
+    const int s = (blockIdx.x / a.KV / a.RB) % a.S;
+    const int part = blockIdx.x / a.KV / a.RB / a.S;
+    const TaSeq sq = ta_seq(a, s);
+    const int L = sq.L, R = sq.n * a.G, r0 = 32 * rb;
+    const int t0 = part * a.part_len;
+    if (r0 >= R || (part > 0 && t0 >= L)) return;
+    const int ntiles = (min(L, t0 + a.part_len) - t0 + 31) / 32;
+    W w(a, lane, s, hk, sq);
+    const int c = w.c, h = w.h;
+    {
+        // the four waves share Q in LDS: in registers it would leave too few for two waves a SIMD
+        const uint8_t *qr = w.set_row(sq.b, hk, min(r0 + c, R - 1));
+        for (int st = wave; st < NS; st += TA_WAVES) s_q[st][lane] = w.signed_q(*(const uint4 *)(qr + 32 * st));
+    }
+    uint4 kf[NS], vf[NB][2];
+    auto load_k = [&](const typename W::Pages &p) {
+        const uint8_t *kp = w.k_at(p);
+#pragma unroll
+        for (int st = 0; st < NS; ++st) kf[st] = *(const uint4 *)(kp + W::k_step(st));
+    };
+    auto load_v = [&](const typename W::Pages &p) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint8_t *vp = w.v_at(p, i);
+#pragma unroll
+            for (int d = 0; d < NB; ++d) vf[d][i] = *(const uint4 *)(vp + w.v_step(d));
+        }
+    };
+    __syncthreads();
+    bool careful = false;
+    for (;;) {
+        w.reset();
+        typename W::Pages pg = {}, pn = {};
         if (wave < ntiles) {
-            pg = checked(ids_of(wave));
-            pn = ids_of(wave + TA_WAVES);
+            pg = w.checked(w.ids_of(t0 + 32 * wave));
+            pn = w.ids_of(t0 + 32 * (wave + TA_WAVES));
             load_k(pg);
             load_v(pg);
         }
         for (int k = wave; k < ntiles; k += TA_WAVES) {
             const int base = t0 + 32 * k;
-            pn = checked(pn);
-            const Pages after = ids_of(k + 2 * TA_WAVES);
-            f32x16 S[RT];
+            pn = w.checked(pn);
+            const typename W::Pages after = w.ids_of(base + 64 * TA_WAVES);
+            f32x16 S = (f32x16){};
 #pragma unroll
-            for (int t = 0; t < RT; ++t) S[t] = (f32x16){};
-#pragma unroll
-            for (int st = 0; st < NS; ++st)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) S[t] = mfma32<false>(kf[st], s_q[t][st][lane], S[t]);
+            for (int st = 0; st < NS; ++st) S = mfma32<false>(kf[st], s_q[st][lane], S);
             load_k(pn);  // past the last tile: the last page again
-            const bool whole = base + 32 <= prefix && pg.good == ~0u;
-            uint32_t vis[RT];
-            uint32_t there = ~0u;  // keys that are in the cache
-            if (!whole) {
-                some_masked = true;
-                there = pg.good & (L - base >= 32 ? ~0u : (1u << (L - base)) - 1);
-                const int d = base - prefix;
+            const typename W::Seen see = w.seen(base, pg.good);
+            uint4 pf[2];
+            w.softmax(S, see, pf);
+            if (see.there != ~0u) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    const uint32_t see = d >= 64    ? 0u
-                                         : d >= 0   ? (uint32_t)(mask[t] >> d)
-                                         : d <= -32 ? ~0u
-                                                    : (uint32_t)(mask[t] << -d) | ((1u << -d) - 1);
-                    vis[t] = see & there;
-                    const uint32_t mine = vis[t] >> (8 * h);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[t][i] = -INFINITY;
-                }
+                    for (int d = 0; d < NB; ++d) vf[d][i] = w.live_v(vf[d][i], i, see.there);
             }
-            uint4 pf[RT][2];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                float mx = S[t][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[t][i]);
-                mx = max_halves(mx);
-                // the reference moves only when the maximum has grown by more than 2^8
-                const bool grow = mx > m[t] && !((mx - m[t]) * a.cs <= 8.0f);
-                if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-                    const float alpha = grow ? __builtin_amdgcn_exp2f((m[t] - mx) * a.cs) : 1.0f;
-                    m[t] = grow ? mx : m[t];
-                    l[t] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < NB; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) O[t][d][i] *= alpha;
-                }
-                const float mc = m[t] == -INFINITY ? 0.0f : m[t] * a.cs;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float p[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[t][8 * i + e] * a.cs - mc);
-                    l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                    pf[t][i] = pack8<false>(p);
-                }
-            }
-            if (!whole && there != ~0u) {  // places that hold no token's value may hold anything
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t live = there >> (16 * i + 8 * h);
-                    auto keep = [&](int e) { return ((live >> e) & 1 ? 0xffffu : 0u) | ((live >> e) & 2 ? 0xffff0000u : 0u); };
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        vf[d][i].x &= keep(0);
-                        vf[d][i].y &= keep(2);
-                        vf[d][i].z &= keep(4);
-                        vf[d][i].w &= keep(6);
-                    }
-                }
-            }
-            if (careful && !whole) {
-// through the wave's part of the merge buffer, which is free until the end
-                uint32_t *sp = (uint32_t *)&s_o[wave][0][0], *sv = sp + RT * 512;
-                static_assert((RT + 1) * 512 * 4 <= sizeof(s_o[0]), "operands of one dim block");
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) sp[512 * t + 64 * x + lane] = word4(pf[t][x / 4], x % 4);
+            if (careful && !see.whole) {
+                // through the wave's part of the merge buffer, which is free until the end
+                uint4 *sp = (uint4 *)&s_o[wave][0][0], *sv = sp + 128;
+                static_assert(256 * 16 <= sizeof(s_o[0]), "operands of one dim block");
+                sp[lane] = pf[0], sp[64 + lane] = pf[1];
 #pragma unroll
                 for (int d = 0; d < NB; ++d) {
                     __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) sv[64 * x + lane] = word4(vf[d][x / 4], x % 4);
+                    sv[lane] = vf[d][0], sv[64 + lane] = vf[d][1];
                     __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-                    for (int key = 0; key < 32; ++key) {
-                        const int at = 64 * (4 * (key >> 4) + ((key & 7) >> 1)) + 32 * ((key >> 3) & 1), sh = 16 * (key & 1);
-#pragma unroll
-                        for (int t = 0; t < RT; ++t) {
-                            const float p = h2f((uint16_t)(sp[512 * t + at + c] >> sh));
-                            if ((vis[t] >> key) & 1)
-#pragma unroll
-                                for (int i = 0; i < 16; ++i)
-                                    O[t][d][i] += p * h2f((uint16_t)(sv[at + 8 * (i / 4) + 4 * h + i % 4] >> sh));
-                        }
-                    }
+                    w.careful_pv(d, see, (const uint32_t *)sp, (const uint32_t *)sv, 256);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int d = 0; d < NB; ++d)
-#pragma unroll
-                        for (int t = 0; t < RT; ++t) O[t][d] = mfma32<false>(vf[d][i], pf[t][i], O[t][d]);
+                    for (int d = 0; d < NB; ++d) w.O[d] = mfma32<false>(vf[d][i], pf[i], w.O[d]);
             }
             load_v(pn);
             pg = pn;
             pn = after;
         }
-        if (careful || !some_masked) break;
-        bool bad = false;
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int d = 0; d < NB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) bad = bad || !(fabsf(O[t][d][i]) < INFINITY);
-        if (__builtin_amdgcn_ballot_w64(bad) == 0) break;
+        if (careful || !w.some_masked || __builtin_amdgcn_ballot_w64(w.bad()) == 0) break;
         careful = true;
     }
 
-    // merge the waves: row c of row tile t, MD dims at a time
+    // merge the waves, MD dims at a time
+    const float lt = sum_halves(w.l);
+    if (h == 0) s_m[wave][c] = w.m, s_l[wave][c] = lt;
+    float *slot = a.part + ((((int64_t)s * a.KV + hk) * a.RB + rb) * a.P + part) * 32 * (D + 4);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const float lt = sum_halves(l[t]);
-        if (h == 0) s_m[wave][32 * t + c] = m[t], s_l[wave][32 * t + c] = lt;
-    }
-    float *slot = a.part + ((((int64_t)s * a.KV + hk) * a.RB + rb) * a.P + part) * (32 * RT) * (D + 4);
+    for (int d0 = 0; d0 < NB; d0 += MD / 32) {
+        if (d0 > 0) lds_barrier();  // the last part has been read
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+        for (int d = d0; d < d0 + MD / 32 && d < NB; ++d)
 #pragma unroll
-        for (int d0 = 0; d0 < NB; d0 += MD / 32) {
-            if (t + d0 > 0) lds_barrier();  // the last part has been read
+            for (int j = 0; j < 4; ++j)
+                *(float4 *)&s_o[wave][c][32 * (d - d0) + 8 * j + 4 * h] =
+                    make_float4(w.O[d][4 * j], w.O[d][4 * j + 1], w.O[d][4 * j + 2], w.O[d][4 * j + 3]);
+        lds_barrier();
+        for (int e = threadIdx.x; e < 32 * (MD / 4); e += 64 * TA_WAVES) {
+            const int row = e / (MD / 4), dd = 4 * (e % (MD / 4)), dim = 32 * d0 + dd, rr = r0 + row;
+            if (rr >= R || dim >= D) continue;
+            float M = -INFINITY;
 #pragma unroll
-            for (int d = d0; d < d0 + MD / 32 && d < NB; ++d)
+            for (int x = 0; x < TA_WAVES; ++x) M = fmaxf(M, s_m[x][row]);
+            float sum = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *(float4 *)&s_o[wave][c][32 * (d - d0) + 8 * j + 4 * h] =
-                        make_float4(O[t][d][4 * j], O[t][d][4 * j + 1], O[t][d][4 * j + 2], O[t][d][4 * j + 3]);
-            lds_barrier();
-            for (int e = threadIdx.x; e < 32 * (MD / 4); e += 64 * TA_WAVES) {
-                const int row = e / (MD / 4), dd = 4 * (e % (MD / 4)), dim = 32 * d0 + dd, rr = r0 + 32 * t + row;
-                if (rr >= R || dim >= D) continue;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < TA_WAVES; ++w) M = fmaxf(M, s_m[w][32 * t + row]);
-                float sum = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < TA_WAVES; ++w) {
-                    const float mw = s_m[w][32 * t + row];
-                    const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * a.cs);
-                    const float4 x = *(const float4 *)&s_o[w][row][dd];
-                    if (mw == -INFINITY && !(s_l[w][32 * t + row] != 0.0f)) continue;  // saw nothing
-                    sum += f * s_l[w][32 * t + row];
-                    o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
-                }
-                if (a.P == 1) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    uint16_t *dst = a.out + ((int64_t)(sq.b + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + dim;
-                    const float x[8] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv, 0, 0, 0, 0};
-                    const uint4 w = pack8<false>(x);
-                    *(uint2 *)dst = make_uint2(w.x, w.y);
-                } else {
-                    float *dst = slot + (int64_t)(32 * t + row) * (D + 4);
-                    *(float4 *)(dst + 4 + dim) = o;
-                    if (dim == 0) *(float2 *)dst = make_float2(M, sum);
-                }
+            for (int x = 0; x < TA_WAVES; ++x) {
+                const float mw = s_m[x][row];
+                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * a.cs);
+                const float4 v = *(const float4 *)&s_o[x][row][dd];
+                if (mw == -INFINITY && !(s_l[x][row] != 0.0f)) continue;  // saw nothing
+                sum += f * s_l[x][row];
+                o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+            }
+            if (a.P == 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                uint16_t *dst = a.out + ((int64_t)(sq.b + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + dim;
+                const float x[8] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv, 0, 0, 0, 0};
+                const uint4 v = pack8<false>(x);
+                *(uint2 *)dst = make_uint2(v.x, v.y);
+            } else {
+                float *dst = slot + (int64_t)row * (D + 4);
+                *(float4 *)(dst + 4 + dim) = o;
+                if (dim == 0) *(float2 *)dst = make_float2(M, sum);
             }
         }
+    }
+}
+
+// The form for many rows. Tiles of KT keys in LDS as the operands' 1-KiB fragments
+// (64 lanes x 16 bytes): of every 32 keys the NS steps of K, then of V^T the two
+// halves of keys x NB dim blocks.
+template <int D> struct TaShared {
+    static constexpr int KT = D <= 128 ? 64 : 32;
+    static constexpr int TILE = KT / 32 * (D / 16 + 2 * ((D + 31) / 32)) * 1024;
+};
+
+template <int D, int BS>
+__global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_shared(const TaArgs a) {
+    using W = TaWave<D, BS>;
+    constexpr int NS = W::NS, NB = W::NB;
+    using Sh = TaShared<D>;
+    constexpr int KT = Sh::KT, SUBS = KT / 32, KF = SUBS * NS;
+    __shared__ __attribute__((aligned(16))) uint8_t T0[Sh::TILE], T1[Sh::TILE];
+    __shared__ uint4 s_p[TA_WAVES][128];  // the careful pass's P
+    __shared__ int s_flag[TA_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row_groups = (a.RB + TA_WAVES - 1) / TA_WAVES;
+    const int hk = blockIdx.x % a.KV;
+    const int rg = (blockIdx.x / a.KV) % row_groups;
+    const int s = (blockIdx.x / a.KV / row_groups) % a.S;
+    const int part = blockIdx.x / a.KV / row_groups / a.S;
+    const TaSeq sq = ta_seq(a, s);
+    const int L = sq.L, R = sq.n * a.G, rb = rg * TA_WAVES + wave, r0 = 32 * rb;
+    const int t0 = part * a.part_len;
+    if (rg * TA_WAVES * 32 >= R || (part > 0 && t0 >= L)) return;
+    const int ntiles = (min(L, t0 + a.part_len) - t0 + KT - 1) / KT;
+    const bool mine = r0 < R;  // some wave of the workgroup has rows, this one may not
+    W w(a, lane, s, hk, sq);
+    const int c = w.c, h = w.h;
+    typename W::Pages pg[SUBS], pn[SUBS];  // of the tile in turn and the next one
+    auto ids = [&](int t, typename W::Pages (&p)[SUBS]) {
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) p[u] = w.ids_of(t0 + KT * t + 32 * u);
+    };
+    // wave w loads the fragments w, w + 4, ... of K and of V
+    auto load_tile = [&](const typename W::Pages *p, uint8_t *T) {
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+            const uint8_t *kp = w.k_at(p[u]);
+#pragma unroll
+            for (int x = 0; x < (NS + TA_WAVES - 1) / TA_WAVES; ++x) {
+                const int st = TA_WAVES * x + wave;
+                if (NS % TA_WAVES == 0 || st < NS)
+                    to_lds(kp + W::k_step(st), T + (u * NS + st) * 1024);
+            }
+#pragma unroll
+            for (int x = 0; x < (2 * NB + TA_WAVES - 1) / TA_WAVES; ++x) {
+                const int f = TA_WAVES * x + wave, i = f & 1, d = f >> 1;
+                if (2 * NB % TA_WAVES == 0 || f < 2 * NB)
+                    to_lds(w.v_at(p[u], i) + w.v_step(d), T + (KF + (2 * u + i) * NB + d) * 1024);
+            }
+        }
+    };
+    uint4 qf[NS];
+    {
+        const uint8_t *qr = w.set_row(sq.b, hk, min(r0 + c, R - 1));
+#pragma unroll
+        for (int st = 0; st < NS; ++st) qf[st] = w.signed_q(*(const uint4 *)(qr + 32 * st));
+    }
+    bool careful = false;
+    auto tile = [&](int t, const uint8_t (&T)[Sh::TILE], uint8_t (&Tn)[Sh::TILE]) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): tile t has landed
+        lds_barrier();                       // for every wave, and the other buffer is free
+        uint32_t good[SUBS];
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) good[u] = pg[u].good;
+        if (t + 1 < ntiles) {
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) pg[u] = w.checked(pn[u]);
+            load_tile(pg, Tn);
+            ids(t + 2, pn);
+        }
+        if (!mine) return;
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+            const int base = t0 + KT * t + 32 * u;
+            f32x16 S = (f32x16){};
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+                S = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S);
+            const typename W::Seen see = w.seen(base, good[u]);
+            uint4 pf[2];
+            w.softmax(S, see, pf);
+            const uint8_t *V = T + (KF + u * 2 * NB) * 1024;
+            if (careful && !see.whole) {
+                __builtin_amdgcn_wave_barrier();
+                s_p[wave][lane] = pf[0], s_p[wave][64 + lane] = pf[1];
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int d = 0; d < NB; ++d)
+                    w.careful_pv(d, see, (const uint32_t *)s_p[wave], (const uint32_t *)(V + d * 1024), 256 * NB);
+            } else if (see.there != ~0u) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int d = 0; d < NB; ++d)
+                        w.O[d] = mfma32<false>(w.live_v(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), i, see.there),
+                                               pf[i], w.O[d]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int d = 0; d < NB; ++d)
+                        w.O[d] = mfma32<false>(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), pf[i], w.O[d]);
+            }
+        }
+    };
+    for (;;) {
+        w.reset();
+        if (ntiles > 0) {
+            ids(0, pg);
+            ids(1, pn);
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) pg[u] = w.checked(pg[u]);
+            load_tile(pg, T0);
+        }
+        for (int t = 0; t < ntiles; t += 2) {
+            tile(t, T0, T1);
+            if (t + 1 < ntiles) tile(t + 1, T1, T0);
+        }
+        if (careful) break;
+        const bool again = mine && w.some_masked && __builtin_amdgcn_ballot_w64(w.bad() && r0 + c < R) != 0;
+        if (lane == 0) s_flag[wave] = again;
+        lds_barrier();  // and every wave is done with both buffers
+        careful = (s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3]) != 0;
+        if (!careful) break;
+    }
+    const int rr = r0 + c;
+    const float sum = sum_halves(w.l);
+    if (rr >= R) return;
+    if (a.P == 1) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t *dst = a.out + ((int64_t)(sq.b + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + 4 * h;
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (32 * d + 8 * j >= D) continue;
+                const float x[8] = {w.O[d][4 * j] * inv, w.O[d][4 * j + 1] * inv, w.O[d][4 * j + 2] * inv,
+                                    w.O[d][4 * j + 3] * inv, 0, 0, 0, 0};
+                const uint4 v = pack8<false>(x);
+                *(uint2 *)(dst + 32 * d + 8 * j) = make_uint2(v.x, v.y);
+            }
+    } else {
+        float *dst = a.part + (((((int64_t)s * a.KV + hk) * a.RB + rb) * a.P + part) * 32 + c) * (D + 4);
+        if (h == 0) *(float2 *)dst = make_float2(w.m, sum);
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (32 * d + 8 * j < D)
+                    *(float4 *)(dst + 4 + 32 * d + 8 * j + 4 * h) =
+                        make_float4(w.O[d][4 * j], w.O[d][4 * j + 1], w.O[d][4 * j + 2], w.O[d][4 * j + 3]);
+    }
 }
 
 // One wave a row: lane p holds partition p's weight, the lanes then take the dims.
 template <int D>
-__global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a, int rows_a_block) {
+__global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a) {
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), hk = blockIdx.y, s = blockIdx.z;
     const TaSeq sq = ta_seq(a, s);
     if (row >= sq.n * a.G) return;
     const int np = (sq.L + a.part_len - 1) / a.part_len;
-    const int64_t step = (int64_t)rows_a_block * (D + 4);
-    const float *base = a.part + ((((int64_t)s * a.KV + hk) * a.RB + row / rows_a_block) * a.P) * step +
-                        (int64_t)(row % rows_a_block) * (D + 4);
+    const int64_t step = 32 * (D + 4);
+    const float *base = a.part + ((((int64_t)s * a.KV + hk) * a.RB + row / 32) * a.P) * step + (row % 32) * (D + 4);
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < np) ml = *(const float2 *)(base + lane * step);
     float M = ml.x;
@@ -376,53 +556,48 @@ __global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a, int row
         if (lane + 64 * e < D) dst[lane + 64 * e] = f2h(acc[e] * inv);
 }
 
-// Row tiles a wave: two where a sequence may have more than 32 rows (the second
-// one's products use the same key and value registers), if they fit.
-static int ta_row_tiles(const tlh_tree_attention_args &a) {
-    return a.head_size <= 128 && a.max_drafts * (a.num_heads / a.num_kv_heads) > 32 ? 2 : 1;
-}
-static int64_t ta_row_blocks(const tlh_tree_attention_args &a) {
-    const int64_t per = 32 * ta_row_tiles(a);
-    return ((int64_t)a.max_drafts * (a.num_heads / a.num_kv_heads) + per - 1) / per;
-}
+static int64_t ta_max_rows(const tlh_tree_attention_args &a) { return (int64_t)a.max_drafts * (a.num_heads / a.num_kv_heads); }
+// More than two blocks of 32 rows share their tiles.
+static bool ta_shared(const tlh_tree_attention_args &a) { return ta_max_rows(a) > 64; }
+static int64_t ta_row_blocks(const tlh_tree_attention_args &a) { return (ta_max_rows(a) + 31) / 32; }
 static int64_t ta_rounds(const tlh_tree_attention_args &a) { return ((int64_t)a.max_context_len + TA_KEYS - 1) / TA_KEYS; }
-// partitions: as many as make TA_WGS workgroups, each of at least one round of keys
+// partitions: as many as make the workgroups aimed for, each of at least one round of keys
 static int ta_parts(const tlh_tree_attention_args &a, int &part_len) {
-    const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * ta_row_blocks(a);
+    const bool sh = ta_shared(a);
+    const int64_t blocks = sh ? (ta_row_blocks(a) + TA_WAVES - 1) / TA_WAVES : ta_row_blocks(a);
+    const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * blocks;
     const int64_t rounds = std::max<int64_t>(ta_rounds(a), 1);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>({TA_WGS / std::max<int64_t>(base, 1), TA_MAX_PARTS, rounds}));
+    const int64_t want = std::max<int64_t>(
+        1, std::min<int64_t>({(sh ? TA_WGS_SHARED : TA_WGS) / std::max<int64_t>(base, 1), TA_MAX_PARTS, rounds}));
     const int64_t each = (rounds + want - 1) / want;
     part_len = (int)(each * TA_KEYS);
     return (int)((rounds + each - 1) / each);
 }
 
-// A slot of 32 RT rows a workgroup. Counted so that the size never shrinks as
-// any of the counts grows: one buffer for the largest call serves every smaller one.
+// A slot of 32 rows for every block of rows and partition. Counted so that the size
+// never shrinks as any of the counts grows (one buffer for the largest call serves
+// every smaller one): a split makes at most TA_WGS slots more than there are blocks,
+// or TA_WGS_SHARED times the four blocks of a workgroup.
 size_t tree_attention_scratch_bytes(const tlh_tree_attention_args &a) {
     if (ta_rounds(a) <= 1) return 0;
     const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * ta_row_blocks(a);
-    const int64_t slots = std::min(base * std::min<int64_t>(ta_rounds(a), TA_MAX_PARTS), base + TA_WGS);
-    return (size_t)slots * 32 * ta_row_tiles(a) * (a.head_size + 4) * sizeof(float);
+    const int64_t slots = std::min(base * std::min<int64_t>(ta_rounds(a), TA_MAX_PARTS),
+                                   base + std::max(TA_WGS, TA_WAVES * TA_WGS_SHARED));
+    return (size_t)slots * 32 * (a.head_size + 4) * sizeof(float);
 }
 
-template <int D, int BS, int RT> static void launch_ta3(const TaArgs &t, unsigned blocks, hipStream_t stream) {
-    hipLaunchKernelGGL((k_tree_attn<D, BS, RT>), dim3(blocks), dim3(64 * TA_WAVES), 0, stream, t);
+template <int D, int BS> static void launch_ta2(const TaArgs &t, bool shared, unsigned blocks, hipStream_t stream) {
+    if (shared) hipLaunchKernelGGL((k_tree_attn_shared<D, BS>), dim3(blocks), dim3(64 * TA_WAVES), 0, stream, t);
+    else hipLaunchKernelGGL((k_tree_attn<D, BS>), dim3(blocks), dim3(64 * TA_WAVES), 0, stream, t);
 }
-template <int D, int BS> static void launch_ta2(const TaArgs &t, int rt, unsigned blocks, hipStream_t stream) {
-    if constexpr (D <= 128) {
-        if (rt == 2) return launch_ta3<D, BS, 2>(t, blocks, stream);
-    }
-    launch_ta3<D, BS, 1>(t, blocks, stream);
-}
-template <int D> static void launch_ta(const TaArgs &t, int bs, int rt, unsigned blocks, hipStream_t stream) {
+template <int D> static void launch_ta(const TaArgs &t, int bs, bool shared, unsigned blocks, hipStream_t stream) {
     switch (bs) {
-    case 8: launch_ta2<D, 8>(t, rt, blocks, stream); break;
-    case 16: launch_ta2<D, 16>(t, rt, blocks, stream); break;
-    default: launch_ta2<D, 32>(t, rt, blocks, stream); break;
+    case 8: launch_ta2<D, 8>(t, shared, blocks, stream); break;
+    case 16: launch_ta2<D, 16>(t, shared, blocks, stream); break;
+    default: launch_ta2<D, 32>(t, shared, blocks, stream); break;
     }
     if (t.P > 1)
-        hipLaunchKernelGGL((k_tree_attn_merge<D>), dim3((t.max_drafts * t.G + 3) / 4, t.KV, t.S), dim3(256), 0, stream, t,
-                           32 * rt);
+        hipLaunchKernelGGL((k_tree_attn_merge<D>), dim3((t.max_drafts * t.G + 3) / 4, t.KV, t.S), dim3(256), 0, stream, t);
 }
 
 tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch, hipStream_t stream) {
@@ -434,22 +609,22 @@ tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch
     t.num_blocks = a.num_blocks;
     t.S = a.num_seqs, t.H = a.num_heads, t.KV = a.num_kv_heads, t.G = a.num_heads / a.num_kv_heads;
     t.rows = a.num_rows, t.max_drafts = a.max_drafts, t.max_blocks = a.max_blocks_per_seq, t.max_ctx = a.max_context_len;
-    const int rt = ta_row_tiles(a);
+    const bool sh = ta_shared(a);
     const int64_t rb = ta_row_blocks(a);
     t.P = ta_parts(a, t.part_len);
     t.RB = (int)rb;
     t.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
     t.qand = a.scale == 0.0f ? 0u : ~0u, t.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
-    const int64_t blocks = (int64_t)t.P * t.S * rb * t.KV;
+    const int64_t blocks = (int64_t)t.P * t.S * (sh ? (rb + TA_WAVES - 1) / TA_WAVES : rb) * t.KV;
     if (blocks > INT32_MAX) return set_error(TLH_INVALID, "tree_attention: too many sequences and heads for one launch");
     switch (a.head_size) {
-    case 64: launch_ta<64>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    case 80: launch_ta<80>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    case 96: launch_ta<96>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    case 112: launch_ta<112>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    case 128: launch_ta<128>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    case 192: launch_ta<192>(t, a.block_size, rt, (unsigned)blocks, stream); break;
-    default: launch_ta<256>(t, a.block_size, rt, (unsigned)blocks, stream); break;
+    case 64: launch_ta<64>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    case 80: launch_ta<80>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    case 96: launch_ta<96>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    case 112: launch_ta<112>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    case 128: launch_ta<128>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    case 192: launch_ta<192>(t, a.block_size, sh, (unsigned)blocks, stream); break;
+    default: launch_ta<256>(t, a.block_size, sh, (unsigned)blocks, stream); break;
     }
     return check_launch("tree_attention");
 }
