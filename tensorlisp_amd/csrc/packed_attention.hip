@@ -16,9 +16,10 @@
 //                   sum cost one exchange with lane l ^ 32 a tile;
 //   O^T += V^T . P^T  P comes from S^T's registers as they are; V^T from LDS by
 //                   transposing reads of four keys x 16 dims.
-// Workgroups are ordered by query position, last first (they see the most
-// keys), then by sequence, then by kv head, so that with 8 kv heads a head's K
-// and V stay in one XCD's L2.
+// Workgroups are ordered by sequence, then by query position, last first (they see
+// the most keys), then by kv head: those that run together read the same K and V,
+// and with 8 kv heads a head's stay in one XCD's L2. (By position first, which
+// ends more evenly, 16 prompts of 100..2000 took 400 us instead of 300.)
 //
 // The softmax is lazy: the exponents' reference moves only when a row's maximum
 // has grown by more than 2^8, so the numerators stay below 2^8 (inside f16) and
@@ -62,10 +63,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
     __shared__ __attribute__((aligned(16))) uint8_t T0[2 * Gm::TILE], T1[2 * Gm::TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
-    // workgroup -> (query tile, last first; sequence; group of heads)
+    // workgroup -> (sequence; query tile, last first; group of heads)
     const int hg = blockIdx.x % a.HG;
-    const int s = (blockIdx.x / a.HG) % a.S;
-    const int qt = a.levels - 1 - (int)(blockIdx.x / a.HG / a.S);
+    const int qt = a.levels - 1 - (int)(blockIdx.x / a.HG % a.levels);
+    const int s = blockIdx.x / a.HG / a.levels;
     const int b0 = max(0, min(a.starts[s], a.tokens)), b1 = max(0, min(a.starts[s + 1], a.tokens));
     const int n = min(b1 - b0, a.max_len);
     const int qpw = 32 * (4 / a.gw);
