@@ -227,28 +227,42 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
                 // (past the last dim: repeats of other dims' values)
                 if (32 * d + 8 * (i / 4) < D) bad = bad || !(fabsf(O[d][i]) < INFINITY);
             }
-        if (careful) break;
+        if (careful) {
+            lds_barrier();
+            break;
+        }
         int *flags = (int *)T0;
         const int mine = __builtin_amdgcn_ballot_w64(bad && qi < n) != 0;
         lds_barrier();
         if (lane == 0) flags[wave] = mine;
         lds_barrier();
-        careful = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
-        if (!careful) break;
+        const bool any = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
         lds_barrier();
+        if (!any) break;
+        careful = true;
         load_tile(0, T0);
     }
-    if (qi < n) {
-        uint8_t *o = a.out + (int64_t)(b0 + qi) * a.so + (int64_t)head * D * 2 + 8 * h;
+    // The wave's 32 rows leave through its quarter of the buffers (free since the
+    // flags' barriers), so that a row is written in one piece: 16-byte chunks of row r
+    // at position chunk ^ (r % CP), then whole rows, 64 / CP at a time.
+    uint8_t *R = (wave & 2 ? T1 : T0) + (wave & 1) * Gm::TILE;
+    static_assert(32 * CP * 16 <= Gm::TILE, "a wave's rows");
 #pragma unroll
-        for (int d = 0; d < NB; ++d)
+    for (int d = 0; d < NB; ++d)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (32 * d + 8 * j >= D) continue;
-                const float x[8] = {O[d][4 * j], O[d][4 * j + 1], O[d][4 * j + 2], O[d][4 * j + 3], 0, 0, 0, 0};
-                const uint4 w = pack8<BF>(x);
-                *(uint2 *)(o + 64 * d + 16 * j) = make_uint2(w.x, w.y);
-            }
+        for (int j = 0; j < 4; ++j) {
+            if (32 * d + 8 * j >= D) continue;
+            const float x[8] = {O[d][4 * j], O[d][4 * j + 1], O[d][4 * j + 2], O[d][4 * j + 3], 0, 0, 0, 0};
+            const uint4 w = pack8<BF>(x);
+            *(uint2 *)(R + c * CP * 16 + 16 * ((4 * d + j) ^ (c & (CP - 1))) + 8 * h) = make_uint2(w.x, w.y);
+        }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < CP / 2; ++i) {
+        const int r = i * (64 / CP) + lk, chunk = lp ^ (r & (CP - 1));
+        if (q0 + r < n && (Gm::C == CP || chunk < Gm::C))
+            *(uint4 *)(a.out + (int64_t)(b0 + q0 + r) * a.so + (int64_t)head * D * 2 + 16 * chunk) =
+                *(const uint4 *)(R + r * CP * 16 + 16 * lp);
     }
 }
 
