@@ -240,7 +240,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
         lds_barrier();
         if (!any) break;
         careful = true;
-        load_tile(0, T0);
+        int again = 0;
+        asm volatile("" : "+s"(again));  // its addresses formed here: kept from the start, they spill
+        load_tile(again, T0);
     }
     // The wave's 32 rows leave through its quarter of the buffers (free since the
     // flags' barriers), so that a row is written in one piece: 16-byte chunks of row r
