@@ -172,17 +172,21 @@ template <int D, int BS> struct TaWave {
         }
         return s;
     }
-    // scores -> numerators (f16), the running maximum and sum
-    __device__ void softmax(f32x16 &S, const Seen &s, uint4 (&pf)[2]) {
-        if (!s.whole) {
-            const uint32_t mine = s.vis >> (8 * h);
+    // scores of U x 32 keys -> numerators (f16), the running maximum and sum
+    template <int U> __device__ void softmax(f32x16 (&S)[U], const Seen (&s)[U], uint4 (&pf)[2 * U]) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[i] = -INFINITY;
-        }
-        float mx = S[0];
+        for (int u = 0; u < U; ++u)
+            if (!s[u].whole) {
+                const uint32_t mine = s[u].vis >> (8 * h);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[i]);
+                for (int i = 0; i < 16; ++i)
+                    if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[u][i] = -INFINITY;
+            }
+        float mx = S[0][0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[u][i]);
         mx = max_halves(mx);
         // the reference moves only when the maximum has grown by more than 2^8
         const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f);
@@ -197,13 +201,15 @@ template <int D, int BS> struct TaWave {
         }
         const float mc = m == -INFINITY ? 0.0f : m * a.cs;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float p[8];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[8 * i + e] * a.cs - mc);
-            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            pf[i] = pack8<false>(p);
-        }
+            for (int i = 0; i < 2; ++i) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[u][8 * i + e] * a.cs - mc);
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                pf[2 * u + i] = pack8<false>(p);
+            }
     }
     // places that hold no token's value may hold anything
     __device__ uint4 live_v(uint4 v, int i, uint32_t there) const {
@@ -281,13 +287,13 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
             const int base = t0 + 32 * k;
             pn = w.checked(pn);
             const typename W::Pages after = w.ids_of(base + 64 * TA_WAVES);
-            f32x16 S = (f32x16){};
+            f32x16 S[1] = {(f32x16){}};
 #pragma unroll
-            for (int st = 0; st < NS; ++st) S = mfma32<false>(kf[st], s_q[st][lane], S);
+            for (int st = 0; st < NS; ++st) S[0] = mfma32<false>(kf[st], s_q[st][lane], S[0]);
             load_k(pn);  // past the last tile: the last page again
-            const typename W::Seen see = w.seen(base, pg.good);
+            const typename W::Seen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
             uint4 pf[2];
-            w.softmax(S, see, pf);
+            w.softmax(S, sees, pf);
             if (see.there != ~0u) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -441,44 +447,50 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
             ids(t + 2, pn);
         }
         if (!mine) return;
+f32x16 S[SUBS];
+        typename W::Seen see[SUBS];
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
-            const int base = t0 + KT * t + 32 * u;
-            f32x16 S = (f32x16){};
+            S[u] = (f32x16){};
 #pragma unroll
             for (int st = 0; st < NS; ++st)
-                S = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S);
-            const typename W::Seen see = w.seen(base, good[u]);
-            uint4 pf[2];
-            w.softmax(S, see, pf);
+                S[u] = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S[u]);
+            see[u] = w.seen(t0 + KT * t + 32 * u, good[u]);
+        }
+        uint4 pf[2 * SUBS];
+        w.softmax(S, see, pf);
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
             const uint8_t *V = T + (KF + u * 2 * NB) * 1024;
-            if (careful && !see.whole) {
+            if (careful && !see[u].whole) {
                 __builtin_amdgcn_wave_barrier();
-                s_p[wave][lane] = pf[0], s_p[wave][64 + lane] = pf[1];
+                s_p[wave][lane] = pf[2 * u], s_p[wave][64 + lane] = pf[2 * u + 1];
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int d = 0; d < NB; ++d)
-                    w.careful_pv(d, see, (const uint32_t *)s_p[wave], (const uint32_t *)(V + d * 1024), 256 * NB);
-            } else if (see.there != ~0u) {
-#pragma unroll
+                    w.careful_pv(d, see[u], (const uint32_t *)s_p[wave], (const uint32_t *)(V + d * 1024), 256 * NB);
+            } else if (see[u].there != ~0u) {
+#pragma unroll 1
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int d = 0; d < NB; ++d)
-                        w.O[d] = mfma32<false>(w.live_v(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), i, see.there),
-                                               pf[i], w.O[d]);
+                        w.O[d] = mfma32<false>(w.live_v(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), i, see[u].there),
+                                               i ? pf[2 * u + 1] : pf[2 * u], w.O[d]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int d = 0; d < NB; ++d)
-                        w.O[d] = mfma32<false>(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), pf[i], w.O[d]);
+                        w.O[d] = mfma32<false>(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), pf[2 * u + i], w.O[d]);
             }
         }
     };
     for (;;) {
         w.reset();
         if (ntiles > 0) {
-            ids(0, pg);
+            int first = 0;
+            asm volatile("" : "+s"(first));  // its addresses formed here: kept for another pass, they spill
+            ids(first, pg);
             ids(1, pn);
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) pg[u] = w.checked(pg[u]);
