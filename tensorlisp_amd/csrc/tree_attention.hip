@@ -18,15 +18,15 @@
 //                     places of one dim.
 // Either operand is 16 bytes a lane that lie together in the page, so the pages
 // are read as they are. Two forms:
-//  * up to 64 rows: a workgroup takes 32 rows and one partition of the context,
-//    its four waves 32-key tiles in turn, straight into registers: the next
-//    tile's keys are requested when this one's have been multiplied, its values
-//    when this one's have, so with two waves a SIMD a tile is always in flight;
-//    the waves merge at the end;
-//  * more rows: a workgroup takes 128 rows, and its four waves share 64-key
-//    tiles in LDS (double-buffered, loaded straight from the pages in the order
-//    in which the lanes take them), so a page is read a quarter as often.
-// Partitions are merged by a second launch.
+//  * a workgroup takes 32 rows and one partition of the context, its four waves
+//    32-key tiles in turn, straight into registers: the next tile's keys are
+//    requested when this one's have been multiplied, its values when this one's
+//    have, so with two waves a SIMD a tile is always in flight; the waves merge
+//    at the end, the partitions in a second launch;
+//  * with many rows, and sequences enough to fill the machine without a split: a
+//    workgroup takes 128 rows, and its four waves share 64-key tiles in LDS
+//    (double-buffered, loaded straight from the pages in the order in which the
+//    lanes take them), so a page is read a quarter as often.
 #include <algorithm>
 
 #include "mfma32.hpp"
@@ -34,7 +34,8 @@
 namespace tlh {
 
 constexpr int TA_WAVES = 4, TA_KEYS = 32 * TA_WAVES;  // keys a workgroup takes a round
-constexpr int TA_WGS = 1024, TA_WGS_SHARED = 512;     // workgroups a split aims for
+constexpr int TA_WGS = 1024;                          // workgroups a split aims for
+constexpr int TA_WGS_SHARED = 512;                    // workgroups that fill the machine (two a CU)
 constexpr int TA_MAX_PARTS = 64;                      // a lane each in the merge
 
 struct TaArgs {
@@ -45,6 +46,7 @@ struct TaArgs {
     float *part;  // [s][kv head][block of 32 rows][partition][row][m, l, -, -, D]
     int64_t num_blocks;
     int S, H, KV, G, rows, max_drafts, max_blocks, max_ctx, P, part_len, RB;  // RB: blocks of 32 rows
+    int sort;  // sequences go longest first
     float cs;             // |scale| * log2(e); 1 where the scale is 0
     uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
@@ -59,6 +61,25 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int s) {
     q.n = min(e - q.b, a.max_drafts);
     q.L = a.num_blocks > 0 ? max(0, min(a.lens[s], a.max_ctx)) : 0;
     return q;
+}
+
+// The o-th longest sequence's index (the o-th, without a.sort): with more workgroups
+// than run at once, long sequences that start last would end alone. Every lane of the
+// wave calls; lane i ranks sequence i (S <= 64).
+__device__ __forceinline__ int ta_pick(const TaArgs &a, int o, int lane) {
+    if (!a.sort) return o;
+    int key = -1;
+    if (lane < a.S) {
+        const TaSeq q = ta_seq(a, lane);
+        key = q.n > 0 ? q.L : 0;
+    }
+    int rank = 0;
+    for (int j = 0; j < a.S; ++j) {
+        const int other = __builtin_amdgcn_readlane(key, j);
+        rank += other > key || (other == key && j < lane);
+    }
+    const uint64_t who = __builtin_amdgcn_ballot_w64(lane < a.S && rank == o);
+    return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
 }
 
 // What the two forms share: a wave's 32 rows of one (sequence, kv head).
@@ -237,6 +258,9 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
     using W = TaWave<D, BS>;
     constexpr int NS = W::NS, NB = W::NB;
     constexpr int MD = NB > 1 ? 64 : 32;  // dims merged at a time
+    // Loads a tile ahead, where two waves' registers hold O, the keys and the values; above
+    // 128 dims a tile's values are requested when its keys have been multiplied.
+    constexpr bool AHEAD = D <= 128;
     __shared__ __attribute__((aligned(16))) float s_o[TA_WAVES][32][MD + 4];
     __shared__ float s_m[TA_WAVES][32], s_l[TA_WAVES][32];
     __shared__ uint4 s_q[NS][64];  // Q^T as the lanes take it: 16 bytes a lane, in order
@@ -244,7 +268,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
     // with 8 kv heads a head's workgroups share an XCD, row blocks next to each other
     const int hk = blockIdx.x % a.KV;
     const int rb = (blockIdx.x / a.KV) % a.RB;
-    const int s = (blockIdx.x / a.KV / a.RB) % a.S;
+    const int s = ta_pick(a, (blockIdx.x / a.KV / a.RB) % a.S, lane);
     const int part = blockIdx.x / a.KV / a.RB / a.S;
     const TaSeq sq = ta_seq(a, s);
     const int L = sq.L, R = sq.n * a.G, r0 = 32 * rb;
@@ -280,17 +304,21 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
         if (wave < ntiles) {
             pg = w.checked(w.ids_of(t0 + 32 * wave));
             pn = w.ids_of(t0 + 32 * (wave + TA_WAVES));
-            load_k(pg);
-            load_v(pg);
+            if (AHEAD) {
+                load_k(pg);
+                load_v(pg);
+            }
         }
         for (int k = wave; k < ntiles; k += TA_WAVES) {
             const int base = t0 + 32 * k;
             pn = w.checked(pn);
             const typename W::Pages after = w.ids_of(base + 64 * TA_WAVES);
+            if (!AHEAD) load_k(pg);
             f32x16 S[1] = {(f32x16){}};
 #pragma unroll
             for (int st = 0; st < NS; ++st) S[0] = mfma32<false>(kf[st], s_q[st][lane], S[0]);
-            load_k(pn);  // past the last tile: the last page again
+            if (AHEAD) load_k(pn);  // past the last tile: the last page again
+            else load_v(pg);
             const typename W::Seen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
             uint4 pf[2];
             w.softmax(S, sees, pf);
@@ -318,7 +346,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
 #pragma unroll
                     for (int d = 0; d < NB; ++d) w.O[d] = mfma32<false>(vf[d][i], pf[i], w.O[d]);
             }
-            load_v(pn);
+            if (AHEAD) load_v(pn);
             pg = pn;
             pn = after;
         }
@@ -393,20 +421,18 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
     const int row_groups = (a.RB + TA_WAVES - 1) / TA_WAVES;
     const int hk = blockIdx.x % a.KV;
     const int rg = (blockIdx.x / a.KV) % row_groups;
-    const int s = (blockIdx.x / a.KV / row_groups) % a.S;
-    const int part = blockIdx.x / a.KV / row_groups / a.S;
+    const int s = ta_pick(a, (blockIdx.x / a.KV / row_groups) % a.S, lane);
     const TaSeq sq = ta_seq(a, s);
-    const int L = sq.L, R = sq.n * a.G, rb = rg * TA_WAVES + wave, r0 = 32 * rb;
-    const int t0 = part * a.part_len;
-    if (rg * TA_WAVES * 32 >= R || (part > 0 && t0 >= L)) return;
-    const int ntiles = (min(L, t0 + a.part_len) - t0 + KT - 1) / KT;
+    const int L = sq.L, R = sq.n * a.G, r0 = 32 * (rg * TA_WAVES + wave);
+    if (rg * TA_WAVES * 32 >= R) return;
+    const int ntiles = (L + KT - 1) / KT;
     const bool mine = r0 < R;  // some wave of the workgroup has rows, this one may not
     W w(a, lane, s, hk, sq);
     const int c = w.c, h = w.h;
     typename W::Pages pg[SUBS], pn[SUBS];  // of the tile in turn and the next one
     auto ids = [&](int t, typename W::Pages (&p)[SUBS]) {
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u) p[u] = w.ids_of(t0 + KT * t + 32 * u);
+        for (int u = 0; u < SUBS; ++u) p[u] = w.ids_of(KT * t + 32 * u);
     };
     // wave w loads the fragments w, w + 4, ... of K and of V
     auto load_tile = [&](const typename W::Pages *p, uint8_t *T) {
@@ -455,7 +481,7 @@ f32x16 S[SUBS];
 #pragma unroll
             for (int st = 0; st < NS; ++st)
                 S[u] = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S[u]);
-            see[u] = w.seen(t0 + KT * t + 32 * u, good[u]);
+            see[u] = w.seen(KT * t + 32 * u, good[u]);
         }
         uint4 pf[2 * SUBS];
         w.softmax(S, see, pf);
@@ -510,30 +536,18 @@ f32x16 S[SUBS];
     const int rr = r0 + c;
     const float sum = sum_halves(w.l);
     if (rr >= R) return;
-    if (a.P == 1) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t *dst = a.out + ((int64_t)(sq.b + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + 4 * h;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t *dst = a.out + ((int64_t)(sq.b + rr / a.G) * a.H + hk * a.G + rr % a.G) * D + 4 * h;
 #pragma unroll
-        for (int d = 0; d < NB; ++d)
+    for (int d = 0; d < NB; ++d)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (32 * d + 8 * j >= D) continue;
-                const float x[8] = {w.O[d][4 * j] * inv, w.O[d][4 * j + 1] * inv, w.O[d][4 * j + 2] * inv,
-                                    w.O[d][4 * j + 3] * inv, 0, 0, 0, 0};
-                const uint4 v = pack8<false>(x);
-                *(uint2 *)(dst + 32 * d + 8 * j) = make_uint2(v.x, v.y);
-            }
-    } else {
-        float *dst = a.part + (((((int64_t)s * a.KV + hk) * a.RB + rb) * a.P + part) * 32 + c) * (D + 4);
-        if (h == 0) *(float2 *)dst = make_float2(w.m, sum);
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (32 * d + 8 * j < D)
-                    *(float4 *)(dst + 4 + 32 * d + 8 * j + 4 * h) =
-                        make_float4(w.O[d][4 * j], w.O[d][4 * j + 1], w.O[d][4 * j + 2], w.O[d][4 * j + 3]);
-    }
+        for (int j = 0; j < 4; ++j) {
+            if (32 * d + 8 * j >= D) continue;
+            const float x[8] = {w.O[d][4 * j] * inv, w.O[d][4 * j + 1] * inv, w.O[d][4 * j + 2] * inv,
+                                w.O[d][4 * j + 3] * inv, 0, 0, 0, 0};
+            const uint4 v = pack8<false>(x);
+            *(uint2 *)(dst + 32 * d + 8 * j) = make_uint2(v.x, v.y);
+        }
 }
 
 // One wave a row: lane p holds partition p's weight, the lanes then take the dims.
@@ -569,32 +583,38 @@ __global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a) {
 }
 
 static int64_t ta_max_rows(const tlh_tree_attention_args &a) { return (int64_t)a.max_drafts * (a.num_heads / a.num_kv_heads); }
-// More than two blocks of 32 rows share their tiles.
-static bool ta_shared(const tlh_tree_attention_args &a) { return ta_max_rows(a) > 64; }
 static int64_t ta_row_blocks(const tlh_tree_attention_args &a) { return (ta_max_rows(a) + 31) / 32; }
+static int64_t ta_shared_wgs(const tlh_tree_attention_args &a) {
+    return (int64_t)a.num_seqs * a.num_kv_heads * ((ta_row_blocks(a) + TA_WAVES - 1) / TA_WAVES);
+}
+// Shared tiles for more than two blocks of 32 rows, where they make two workgroups a
+// CU without a split. 32/8 heads of 128, trees of 64, us (shared, own tiles): 32
+// sequences of 4096 200, 259, of 512..4096 172, 159; 64 of 1000 123, 177. With fewer
+// workgroups a split's partials cost more than the shared reads save: 16 of 512..4096
+// 102, 83, 8 of 100..8000 97, 85.
+static bool ta_shared(const tlh_tree_attention_args &a) {
+    return ta_row_blocks(a) > 2 && ta_shared_wgs(a) >= TA_WGS_SHARED;
+}
 static int64_t ta_rounds(const tlh_tree_attention_args &a) { return ((int64_t)a.max_context_len + TA_KEYS - 1) / TA_KEYS; }
-// partitions: as many as make the workgroups aimed for, each of at least one round of keys
+// partitions: as many as make no more than TA_WGS workgroups, each of at least one round of keys
 static int ta_parts(const tlh_tree_attention_args &a, int &part_len) {
-    const bool sh = ta_shared(a);
-    const int64_t blocks = sh ? (ta_row_blocks(a) + TA_WAVES - 1) / TA_WAVES : ta_row_blocks(a);
-    const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * blocks;
+    const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * ta_row_blocks(a);
     const int64_t rounds = std::max<int64_t>(ta_rounds(a), 1);
-    const int64_t want = std::max<int64_t>(
-        1, std::min<int64_t>({(sh ? TA_WGS_SHARED : TA_WGS) / std::max<int64_t>(base, 1), TA_MAX_PARTS, rounds}));
+    const int64_t want = ta_shared(a) ? 1
+                                      : std::max<int64_t>(1, std::min<int64_t>({TA_WGS / std::max<int64_t>(base, 1),
+                                                                                TA_MAX_PARTS, rounds}));
     const int64_t each = (rounds + want - 1) / want;
     part_len = (int)(each * TA_KEYS);
     return (int)((rounds + each - 1) / each);
 }
 
-// A slot of 32 rows for every block of rows and partition. Counted so that the size
-// never shrinks as any of the counts grows (one buffer for the largest call serves
-// every smaller one): a split makes at most TA_WGS slots more than there are blocks,
-// or TA_WGS_SHARED times the four blocks of a workgroup.
+// A slot of 32 rows for every block of rows and partition, at most TA_WGS of them
+// where there are several partitions. The size never shrinks as any of the counts
+// grows: one buffer for the largest call serves every smaller one.
 size_t tree_attention_scratch_bytes(const tlh_tree_attention_args &a) {
     if (ta_rounds(a) <= 1) return 0;
     const int64_t base = (int64_t)a.num_seqs * a.num_kv_heads * ta_row_blocks(a);
-    const int64_t slots = std::min(base * std::min<int64_t>(ta_rounds(a), TA_MAX_PARTS),
-                                   base + std::max(TA_WGS, TA_WAVES * TA_WGS_SHARED));
+    const int64_t slots = std::min<int64_t>(base * std::min<int64_t>(ta_rounds(a), TA_MAX_PARTS), TA_WGS);
     return (size_t)slots * 32 * (a.head_size + 4) * sizeof(float);
 }
 
@@ -627,7 +647,8 @@ tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch
     t.RB = (int)rb;
     t.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
     t.qand = a.scale == 0.0f ? 0u : ~0u, t.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
-    const int64_t blocks = (int64_t)t.P * t.S * (sh ? (rb + TA_WAVES - 1) / TA_WAVES : rb) * t.KV;
+    const int64_t blocks = sh ? ta_shared_wgs(a) : (int64_t)t.P * t.S * rb * t.KV;
+    t.sort = t.S > 1 && t.S <= 64 && blocks > 2 * device_cus();
     if (blocks > INT32_MAX) return set_error(TLH_INVALID, "tree_attention: too many sequences and heads for one launch");
     switch (a.head_size) {
     case 64: launch_ta<64>(t, a.block_size, sh, (unsigned)blocks, stream); break;

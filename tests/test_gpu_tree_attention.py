@@ -237,3 +237,65 @@ def test_nothing_to_do(gpu):
     check(run(c), c)
     c["starts"] = [0, 0, 0]
     assert (run(c, max_drafts=4) == 7).all()
+
+
+# --------------------------------------------------- many rows share tiles
+# more than 64 rows of a kv head (drafted tokens x group) and at least 512 workgroups
+# of 128 rows: the form whose four waves read one tile from LDS
+def shared_case(hs, bs, seed, contexts=(0, 5, 150, 64, 33, 1, 97, 40), drafts=(40, 1, 33, 64, 7, 40, 0, 35), **kw):
+    n = 512 // (32 * len(contexts))
+    return build(64, 32, hs, bs, list(contexts) * n, list(drafts) * n, seed, **kw)
+
+
+@pytest.mark.parametrize("hs,bs", [(128, 16), (64, 8), (256, 32), (80, 16), (112, 32), (192, 8), (96, 8), (64, 32)])
+def test_many_rows_against_64_bits(gpu, hs, bs):
+    c = shared_case(hs, bs, 60 + hs)
+    check(run(c), c)
+
+
+def test_many_rows_little_or_nothing_seen_and_bad_pages(gpu):
+    c = shared_case(128, 16, 61)
+    r = np.random.default_rng(61)
+    c["masks"] = [int(m) if i % 3 else 0 for i, m in enumerate(r.integers(0, 2 ** 62, len(c["masks"])))]
+    check(run(c), c)
+    c["table"][2, 1], c["table"][2, 9], c["table"][10, 0], c["table"][3, :] = -5, 10 ** 6, 2 ** 31 - 1, -1
+    check(run(c), c)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_many_rows_what_is_not_seen_does_not_reach_them(gpu, bad):
+    hs, bs = 128, 16
+    c = shared_case(hs, bs, 62)
+    for s, L in enumerate(c["lens"]):
+        page, off = c["table"][s, (L - 1) // bs], (L - 1) % bs + 1
+        c["kc"][page, :, :, off:], c["vc"][page, :, :, off:] = bad, bad
+    check(run(c), c)
+    hit = []
+    for s in (0, 3):  # drafted token 4: the rows that see it are not finite, no others
+        p = c["lens"][s] - (c["starts"][s + 1] - c["starts"][s]) + 4
+        c["kc"][c["table"][s, p // bs], :, :, p % bs] = bad
+        c["vc"][c["table"][s, p // bs], :, :, p % bs] = bad
+        hit += [i for i in range(c["starts"][s], c["starts"][s + 1]) if c["masks"][i] >> 4 & 1]
+    out = run(c)
+    others = [i for i in range(c["starts"][-1]) if i not in hit]
+    check(out, c, others)
+    assert not torch.isfinite(out[hit]).all(-1).any()
+
+
+def test_many_rows_long_contexts_and_max_drafts(gpu):
+    c = build(64, 32, 64, 16, [1500] + [20] * 15, [36] * 16, 63)
+    check(run(c), c)
+    c = build(64, 32, 64, 16, [30] * 16, [40] * 16, 64, masks=chain_masks(40) * 16)
+    out = run(c, max_drafts=35)  # places 5..39 of the drafted ones are rows 0..34's
+    for s in range(16):
+        assert (out[40 * s + 35:40 * s + 40] == 7).all()
+    assert torch.equal(out, run(c, max_drafts=35))
+
+
+def test_many_sequences_longest_first(gpu):
+    """More workgroups than run at once: sequences go by length, whatever their order."""
+    r = np.random.default_rng(65)
+    c = build(32, 32, 64, 16, [int(x) for x in r.integers(0, 300, 64)], [int(x) for x in r.integers(0, 4, 64)], 65)
+    check(run(c), c)
+    c = build(16, 16, 64, 8, [int(x) for x in r.integers(0, 40, 130)], [2] * 130, 66)
+    check(run(c), c)
