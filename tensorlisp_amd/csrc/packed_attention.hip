@@ -99,14 +99,20 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
     f32x16 O[NB];
     float m, l;  // this lane's query: the exponents' reference (an unscaled score); this half's sum
     load_tile(0, T0);
-    uint4 qf[NS];
+    // Q as the lanes take it: in registers, above 192 dims (where O leaves none: 4000
+    // tokens, 16/8 heads of 256, 392 us with it in registers, 256 without) in LDS
+    constexpr bool QREG = D <= 192;
+    __shared__ uint4 s_q[QREG ? 1 : 4][QREG ? 1 : NS][QREG ? 1 : 64];
+    uint4 qf[QREG ? NS : 1];
     {
         const uint8_t *qr = a.q + (int64_t)(b0 + min(qi, n - 1)) * a.sq + (int64_t)head * D * 2 + 16 * h;
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
             const uint4 w = *(const uint4 *)(qr + 32 * st);
-            qf[st] = make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor,
-                                (w.w & a.qand) ^ a.qxor);
+            const uint4 q = make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor,
+                                       (w.w & a.qand) ^ a.qxor);
+            if constexpr (QREG) qf[st] = q;
+            else s_q[wave][st][lane] = q;
         }
     }
     // a transposing read takes key tr_key of four and 4 of 16 dims from each of 16
@@ -132,7 +138,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
             const int kk = 32 * b + c;
 #pragma unroll
             for (int st = 0; st < NS; ++st)
-                S[b] = mfma32<BF>(*(const uint4 *)(T + kk * CP * 16 + 16 * ((2 * st + h) ^ Gm::kswz(kk))), qf[st], S[b]);
+                S[b] = mfma32<BF>(*(const uint4 *)(T + kk * CP * 16 + 16 * ((2 * st + h) ^ Gm::kswz(kk))),
+                                  QREG ? qf[QREG ? st : 0] : s_q[QREG ? 0 : wave][QREG ? 0 : st][QREG ? 0 : lane], S[b]);
         }
         const bool diagonal = k0 + KT - 1 > q0;  // some key lies after some query
         if (diagonal) {
