@@ -36,10 +36,14 @@ tlh_status launch_copy_blocks(void *const *pools, int num_pools, int64_t block_b
         const int n = std::min(POOLS_A_LAUNCH, num_pools - p0);
         PoolPtrs pp = {};
         for (int i = 0; i < n; ++i) pp.p[i] = (uint8_t *)pools[p0 + i];
-        const dim3 grid(num_pairs, n, (unsigned)((block_bytes + COPY_PIECE - 1) / COPY_PIECE));
-        hipLaunchKernelGGL(k_copy_blocks, grid, dim3(256), 0, stream, pp, block_bytes, num_blocks, pairs);
-        const tlh_status st = check_launch("copy_blocks");
-        if (st != TLH_OK) return st;
+        for (int r0 = 0; r0 < num_pairs; r0 += 1 << 22) {  // grid x
+            const dim3 grid(std::min(num_pairs - r0, 1 << 22), n, (unsigned)((block_bytes + COPY_PIECE - 1) / COPY_PIECE));
+            hipLaunchKernelGGL(k_copy_blocks, grid, dim3(256), 0, stream, pp, block_bytes, num_blocks,
+                               pairs + 2 * (int64_t)r0);
+            const tlh_status st = check_launch("copy_blocks");
+            if (st != TLH_OK) return st;
+            if (num_pairs - r0 <= 1 << 22) break;
+        }
     }
     return TLH_OK;
 }

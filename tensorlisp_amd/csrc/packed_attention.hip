@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
     const int h = lane >> 5, c = lane & 31;
     // workgroup -> (sequence; query tile, last first; group of heads)
     const int hg = blockIdx.x % a.HG;
-    const int qt = a.levels - 1 - (int)(blockIdx.x / a.HG % a.levels);
-    const int s = blockIdx.x / a.HG / a.levels;
+    const int qt = a.levels - 1 - (int)(blockIdx.x / a.HG);
+    const int s = blockIdx.y;
     const int b0 = max(0, min(a.starts[s], a.tokens)), b1 = max(0, min(a.starts[s + 1], a.tokens));
     const int n = min(b1 - b0, a.max_len);
     const int qpw = 32 * (4 / a.gw);
@@ -275,11 +275,15 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
     }
 }
 
-template <int D>
-static tlh_status launch_pk(const PkArgs &p, bool bf, int64_t blocks, hipStream_t stream) {
-    if (bf) hipLaunchKernelGGL((k_packed_attn<D, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((k_packed_attn<D, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    return check_launch("packed_attention");
+template <int D> static tlh_status launch_pk(PkArgs p, bool bf, hipStream_t stream) {
+    for (int left = p.S; left > 0; left -= 65535, p.starts += 65535) {  // grid y
+        const dim3 grid((unsigned)(p.HG * p.levels), std::min(left, 65535));
+        if (bf) hipLaunchKernelGGL((k_packed_attn<D, true>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((k_packed_attn<D, false>), grid, dim3(256), 0, stream, p);
+        const tlh_status st = check_launch("packed_attention");
+        if (st != TLH_OK) return st;
+    }
+    return TLH_OK;
 }
 
 tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream_t stream) {
@@ -293,21 +297,20 @@ tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream
     p.gw = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     p.HG = a.num_heads / p.gw;
     const int qpw = 32 * (4 / p.gw);
-    p.levels = (p.max_len + qpw - 1) / qpw;
+    p.levels = (p.max_len - 1) / qpw + 1;
     p.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * PK_LOG2E;
     p.qand = a.scale == 0.0f ? 0u : ~0u, p.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
-    const int64_t blocks = (int64_t)p.levels * p.S * p.HG;
-    if ((int64_t)p.S * p.HG > INT32_MAX || blocks > INT32_MAX)
-        return set_error(TLH_INVALID, "packed_attention: too many sequences of max_seq_len for one launch");
+    if ((int64_t)p.levels * p.HG >= 1 << 24)  // x 256 threads
+        return set_error(TLH_INVALID, "packed_attention: max_seq_len x num_heads too large for one launch");
     const bool bf = a.type == TLH_TYPE_BF16;
     switch (a.head_size) {
-    case 64: return launch_pk<64>(p, bf, blocks, stream);
-    case 80: return launch_pk<80>(p, bf, blocks, stream);
-    case 96: return launch_pk<96>(p, bf, blocks, stream);
-    case 112: return launch_pk<112>(p, bf, blocks, stream);
-    case 128: return launch_pk<128>(p, bf, blocks, stream);
-    case 192: return launch_pk<192>(p, bf, blocks, stream);
-    default: return launch_pk<256>(p, bf, blocks, stream);
+    case 64: return launch_pk<64>(p, bf, stream);
+    case 80: return launch_pk<80>(p, bf, stream);
+    case 96: return launch_pk<96>(p, bf, stream);
+    case 112: return launch_pk<112>(p, bf, stream);
+    case 128: return launch_pk<128>(p, bf, stream);
+    case 192: return launch_pk<192>(p, bf, stream);
+    default: return launch_pk<256>(p, bf, stream);
     }
 }
 

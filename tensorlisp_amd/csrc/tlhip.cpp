@@ -1254,7 +1254,7 @@ tlh_status tlh_compact_cache(const tlh_compact_cache_args *a, void *stream) {
         a->num_kv_heads > 65535)
         return set_error(TLH_INVALID, "compact_cache: unsupported head_size %d, block_size %d or num_kv_heads %d",
                          a->head_size, a->block_size, a->num_kv_heads);
-    if (a->num_layers < 0 || a->num_seqs < 0 || a->num_blocks < 0 || a->max_blocks_per_seq < 0 ||
+    if (a->num_layers < 0 || a->num_seqs < 0 || a->num_seqs > 1 << 23 || a->num_blocks < 0 || a->max_blocks_per_seq < 0 ||
         (int64_t)a->max_blocks_per_seq * a->block_size > INT32_MAX)
         return set_error(TLH_INVALID, "compact_cache: bad counts");
     if (a->max_drafts < 0 || a->max_drafts > 64)
@@ -1263,8 +1263,10 @@ tlh_status tlh_compact_cache(const tlh_compact_cache_args *a, void *stream) {
     if (!a->k_caches || !a->v_caches || !a->context_lens || !a->draft_starts || !a->keep || !a->new_lens ||
         (a->max_blocks_per_seq > 0 && !a->block_tables))
         return set_error(TLH_INVALID, "compact_cache: null pointer");
-    if ((const int32_t *)a->new_lens == a->context_lens)
-        return set_error(TLH_INVALID, "compact_cache: new_lens must not be context_lens");
+    const int32_t *nl = a->new_lens;
+    if ((nl < a->context_lens + a->num_seqs && a->context_lens < nl + a->num_seqs) ||
+        (nl < a->draft_starts + a->num_seqs + 1 && a->draft_starts < nl + a->num_seqs))
+        return set_error(TLH_INVALID, "compact_cache: new_lens must not overlap context_lens or draft_starts");
     if (((uintptr_t)a->keep & 7) || (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens |
                                       (uintptr_t)a->draft_starts | (uintptr_t)a->new_lens) & 3))
         return set_error(TLH_INVALID, "compact_cache: misaligned pointer");
@@ -1279,8 +1281,9 @@ static tlh_status check_logprobs(const tlh_token_logprobs_args *a) {
     if (!float_type(a->type))
         return set_error(TLH_UNSUPPORTED, "token_logprobs: logits of ggml type %d (%s); have f32, f16, bf16", a->type,
                          type_name(a->type));
-    if (a->rows < 0 || a->vocab < 1 || a->vocab > 1000000)
-        return set_error(TLH_INVALID, "token_logprobs: %d rows, vocab %d outside 1..1000000", a->rows, a->vocab);
+    if (a->rows < 0 || a->rows > 1 << 24 || a->vocab < 1 || a->vocab > 1000000)
+        return set_error(TLH_INVALID, "token_logprobs: %d rows outside 0..2^24 or vocab %d outside 1..1000000", a->rows,
+                         a->vocab);
     if (a->top < 0 || a->top > 32 || a->top > a->vocab)
         return set_error(TLH_INVALID, "token_logprobs: top %d outside 0..min(32, vocab)", a->top);
     if (a->row_stride < a->vocab)

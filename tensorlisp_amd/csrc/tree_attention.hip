@@ -649,7 +649,8 @@ tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch
     t.qand = a.scale == 0.0f ? 0u : ~0u, t.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
     const int64_t blocks = sh ? ta_shared_wgs(a) : (int64_t)t.P * t.S * rb * t.KV;
     t.sort = t.S > 1 && t.S <= 64 && blocks > 2 * device_cus();
-    if (blocks > INT32_MAX) return set_error(TLH_INVALID, "tree_attention: too many sequences and heads for one launch");
+    if (blocks >= 1 << 24)  // x 256 threads
+        return set_error(TLH_INVALID, "tree_attention: too many sequences and heads for one launch");
     switch (a.head_size) {
     case 64: launch_ta<64>(t, a.block_size, sh, (unsigned)blocks, stream); break;
     case 80: launch_ta<80>(t, a.block_size, sh, (unsigned)blocks, stream); break;

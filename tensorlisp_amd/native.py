@@ -580,7 +580,7 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     stride that is a multiple of 8 elements (views of a fused projection),
     seq_starts i32 (sequences + 1,) -> out (tokens, heads, head size). No
     sequence may be longer than max_seq_len. Tokens behind the last sequence are
-    left as they were in `out`."""
+    left as they were in `out` (without one, as the new tensor holds them)."""
     import torch
 
     (tokens, heads, hs), dtype, dev = q.shape, q.dtype, q.device

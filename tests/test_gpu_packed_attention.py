@@ -211,3 +211,29 @@ def test_numbers_of_sequences_and_tokens_at_zero(gpu):
     N.packed_attention(q, k, v, dev([0, 10]), 0, 0.1, out=out)
     assert (out == 7).all()
     assert N.packed_attention(q[:0], k[:0], v[:0], dev([0, 0]), 5, 0.1).shape == (0, 4, 64)
+
+
+def test_more_sequences_than_a_grid_dimension(gpu):
+    r = np.random.default_rng(18)
+    lens = [int(n) for n in r.integers(0, 3, 70001)]
+    q, k, v = inputs(1, 1, 64, sum(lens), F16, 18)
+    starts = starts_of(lens)
+    out = N.packed_attention(q, k, v, dev(starts), 2, 0.125)
+    s = (q[1:, 0].float() * k[:-1, 0].float()).sum(1) * 0.125  # a second token's two scores
+    own = (q[:, 0].float() * k[:, 0].float()).sum(1) * 0.125
+    want = v[:, 0].float().clone()
+    second = torch.zeros(sum(lens), dtype=torch.bool, device="cuda")
+    second[[a + 1 for a, n in zip(starts, lens) if n == 2]] = True
+    p = torch.sigmoid(own[1:] - s)[:, None]  # the weight of the token itself
+    want[1:] = torch.where(second[1:, None], p * v[1:, 0].float() + (1 - p) * v[:-1, 0].float(), want[1:])
+    # f16: the result's rounding, the weights' rounding, and f32 scores
+    tol = 2.0 ** -11 * 2.1 * v.float().abs().max() + 1e-4
+    assert (out[:, 0].float() - want).abs().max() <= tol
+
+
+def test_scales_below_zero_and_zero(gpu):
+    q, k, v = inputs(4, 2, 128, 150, F16, 19)
+    out = N.packed_attention(q, k, v, dev([0, 150]), 150, -0.2)
+    check(out, -q, k, v, [0, 150], 0.2)
+    out = N.packed_attention(q, k, v, dev([0, 150]), 150, 0.0)
+    check(out, q * 0, k, v, [0, 150], 1.0)

@@ -299,3 +299,12 @@ def test_many_sequences_longest_first(gpu):
     check(run(c), c)
     c = build(16, 16, 64, 8, [int(x) for x in r.integers(0, 40, 130)], [2] * 130, 66)
     check(run(c), c)
+
+
+def test_scales_below_zero_and_zero(gpu):
+    c = build(8, 2, 128, 16, [300], [20], 67)
+    c["scale"] = -0.2
+    out = run(c)
+    check(out, {**c, "q": -c["q"], "scale": 0.2})
+    c["scale"] = 0.0
+    check(run(c), {**c, "q": c["q"] * 0, "scale": 1.0})

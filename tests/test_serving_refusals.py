@@ -220,3 +220,19 @@ def test_python_checks_name_the_tensor():
         lp(rows(2, 100, dtype=torch.float32), i32(2), rows(2, dtype=torch.float32), None)
     with pytest.raises(N.TlhError, match="top"):
         N.TokenLogprobs(2, 10, 11, torch.float32, device="cpu")
+
+
+def test_sizes_past_one_launch_are_refused():
+    """Grids of more threads than a launch takes, told before it."""
+    assert status(N.lib().tlh_packed_attention, C.byref(packed(num_tokens=2 ** 31 - 1, max_seq_len=2 ** 31 - 1)), None)[0] == "INVALID"
+    assert status(N.lib().tlh_tree_attention, C.byref(tree(num_seqs=65535, num_heads=2048, num_kv_heads=1024)), P, BIG, None)[0] == "INVALID"
+    assert compact(num_seqs=1 << 24) == "INVALID"
+    assert logprobs(rows=(1 << 24) + 1) == "INVALID"
+
+
+def test_compact_cache_lengths_must_not_overlap():
+    base = 0x100000
+    for at in (0, 4, 12, -4, -12):
+        assert compact(num_seqs=4, context_lens=base, new_lens=base + at, draft_starts=base + 4096) == "INVALID", at
+        assert compact(num_seqs=4, draft_starts=base, new_lens=base + at, context_lens=base + 4096) == "INVALID", at
+    assert compact(num_seqs=4, draft_starts=base, new_lens=base + 16, context_lens=base + 4096) == "INVALID"
