@@ -269,6 +269,15 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
     const int top = a.top;
     const uint8_t *slot = scratch + ((int64_t)row * P + min(lane, P - 1)) * lp_slot(top);
     const float4 st = *(const float4 *)slot;
+    // what is needed later starts on its way here
+    const uint64_t *list = (const uint64_t *)(slot + 16);
+    auto entry = [&](int i) { return lane < P && i < top ? list[i] : (uint64_t)0; };
+    uint64_t ahead[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ahead[i] = entry(i);
+    const int token = a.logprobs ? a.tokens[row] : -1;
+    const bool known = token >= 0 && token < a.vocab;
+    const float x = known ? lp_elem<TY>(a.logits, (int64_t)row * a.row_stride + token) : 0.0f;
     float M = lane < P ? st.x : -INFINITY;
     for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     float S = 0.0f, T = 0.0f;
@@ -286,28 +295,18 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
     const float lse = logf(S);
     if (lane == 0) {
         if (a.entropy) a.entropy[row] = lse - T / S;
-        if (a.logprobs) {
-            const int t = a.tokens[row];
-            float lp = __uint_as_float(0x7fc00000u);
-            if (t >= 0 && t < a.vocab) lp = (lp_elem<TY>(a.logits, (int64_t)row * a.row_stride + t) - M) - lse;
-            a.logprobs[row] = lp;
-        }
+        if (a.logprobs) a.logprobs[row] = known ? (x - M) - lse : __uint_as_float(0x7fc00000u);
     }
     // The lanes' lists are sorted. As in a chunk: the top-th largest of their first four
     // entries is a threshold (0 with fewer of them), and the few that reach it are ranked
     // by counting.
     __shared__ uint64_t s_list[4][LP_MERGE];
     uint64_t *l = s_list[threadIdx.x >> 6];
-    const uint64_t *list = (const uint64_t *)(slot + 16);
-    auto entry = [&](int i) { return lane < P && i < top ? list[i] : (uint64_t)0; };
     auto put = [&](int r, uint64_t e) {
         a.top_logprobs[(int64_t)row * top + r] = (lp_value((uint32_t)(e >> 32)) - M) - lse;
         a.top_ids[(int64_t)row * top + r] = (int32_t)~(uint32_t)e;
     };
     if (top == 0) return;
-    uint64_t ahead[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ahead[i] = entry(i);
     uint32_t thr = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t cand = thr | 1u << bit;

@@ -560,21 +560,35 @@ __global__ void __launch_bounds__(256) k_tree_attn_merge(const TaArgs a) {
     const int np = (sq.L + a.part_len - 1) / a.part_len;
     const int64_t step = 32 * (D + 4);
     const float *base = a.part + ((((int64_t)s * a.KV + hk) * a.RB + row / 32) * a.P) * step + (row % 32) * (D + 4);
+    constexpr int E = (D + 63) / 64, AT_ONCE = 8;
+    // the first partitions' sums are on their way while the weights are formed
+    float o[AT_ONCE][E];
+    auto load = [&](int p0) {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e)  // (past the last partition or dim: an element that gets no weight, or no place)
+                o[i][e] = base[max(min(p0 + i, np - 1), 0) * step + 4 + min(lane + 64 * e, D - 1)];
+    };
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < np) ml = *(const float2 *)(base + lane * step);
+    if (np > 0) load(0);
     float M = ml.x;
-    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
     const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - M) * a.cs);
     float sum = w * ml.y;
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i, 64);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    constexpr int E = (D + 63) / 64;
     float acc[E] = {};
-    for (int p = 0; p < np; ++p) {
-        const float wp = __shfl(w, p, 64);
+    for (int p0 = 0; p0 < np; p0 += AT_ONCE) {
+        if (p0 > 0) load(p0);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lane + 64 * e < D) acc[e] += wp * base[p * step + 4 + lane + 64 * e];
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (p0 + i >= np) break;
+            const float wp = __shfl(w, p0 + i, 64);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += wp * o[i][e];
+        }
     }
     uint16_t *dst = a.out + ((int64_t)(sq.b + row / a.G) * a.H + hk * a.G + row % a.G) * D;
 #pragma unroll
