@@ -7,17 +7,18 @@
 // The bound is one read of the logits. A workgroup takes a chunk of a row into
 // registers, so the chunk's maximum is known before its exponentials (one pass,
 // no rescaling) and its largest elements are found without a second read:
-//  * the top-th largest of the 256 lanes' maxima is a threshold (at least `top`
-//    elements of the chunk reach it, few more do); every wave lists its elements
-//    above it and the first `top` that equal it, and the listed ones are ranked by
-//    counting (a threshold from each wave's own 64 maxima lists four times as many:
-//    777 x 128256, top 20, 130 us instead of 97);
-//  * a vocabulary-wide run of equal logits (a grammar's -inf mask) costs no
-//    more: ties are taken in index order and only up to `top`;
+//  * the top-th largest of the 256 lanes' maxima is a threshold: at least `top`
+//    elements of the chunk reach it, and few more do. Every wave lists its own, and the
+//    listed ones are ranked by counting (a threshold from each wave's 64 maxima lists
+//    four times as many: 777 x 128256, top 20, 130 us instead of 86; without the
+//    alternatives it is 70);
+//  * where more reach it than the list holds, as in a vocabulary-wide run of equal
+//    logits (a grammar's -inf mask), ties are taken in index order and only up to
+//    `top` (112 us with 999 of 1000 masked);
 //  * more elements above the threshold than the list holds (the largest ones
-//    crowded into few lanes) are taken one maximum at a time instead.
-// A second launch folds the chunks' sums and merges their sorted lists, one
-// wave a row with one list a lane.
+//    crowded into few lanes) are taken one maximum at a time instead, read again.
+// A second launch folds the chunks' sums and merges their sorted lists the same
+// way, one wave a row with one list a lane.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -81,11 +82,28 @@ template <int TY, int C, int NV, bool EDGE> struct LpWave {
     __device__ int elem(int i, int c) const { return e0 + 256 * C * i + c; }
     __device__ bool there(int i, int c) const { return !EDGE || (uint32_t)elem(i, c) < (uint32_t)V; }
 
-    // Lists the elements above thr (a value) and the first `top` that equal it; -> how many.
-    // A wave with a NaN or +inf (plain = false) and one with more elements above thr than
-    // the list holds take their `top` largest one maximum at a time instead.
-    __device__ int list_top(float thr, int top, bool plain, uint64_t *list) const {
+    // Lists the elements that reach thr (a value); where they are more than the list holds,
+    // those above it and the first `top` that equal it; -> how many. A wave with a NaN or
+    // +inf (plain = false) and one with too many above thr take their `top` largest one
+    // maximum at a time instead.
+    __device__ __forceinline__ int list_top(float thr, int top, bool plain, uint64_t *list) const {
         if (plain) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                uint64_t any = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c) any |= __builtin_amdgcn_ballot_w64(x[i][c] >= thr);
+                if (any == 0 || n > LP_CAP) continue;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint64_t who = __builtin_amdgcn_ballot_w64(x[i][c] >= thr && there(i, c));
+                    const int at = n + lp_below(who);
+                    if ((who >> lane) & 1 && at < LP_CAP) list[at] = lp_entry(lp_key(x[i][c]), elem(i, c));
+                    n += __popcll(who);
+                }
+            }
+            if (n <= LP_CAP) return n;
             int above = 0, equal = 0;
             const float over = lp_value(lp_key(thr) + 1);  // the next number
 #pragma unroll
@@ -149,7 +167,7 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
     constexpr int C = TY == TLH_TYPE_F32 ? 4 : 8;  // elements of a 16-byte load
     constexpr int ES = 16 / C, NV = EPT / C;
     __shared__ uint64_t s_list[4][LP_CAP + LP_MAX_TOP];
-    __shared__ uint32_t s_best[256];
+    __shared__ uint32_t s_best[256], s_thr;
     __shared__ int s_n[4];
     __shared__ float s_sum[4][3];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -210,17 +228,23 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
     if (top > 0) {
         s_best[threadIdx.x] = lp_key(best);
         __syncthreads();
-        // thr: the top-th largest of the lanes' maxima, bit by bit (-inf with fewer lanes than that)
-        uint32_t k[4], thr = 0;
+        // thr: the top-th largest of the lanes' maxima, bit by bit (-inf with fewer lanes than
+        // that), by one wave
+        if (wave == 0) {
+            uint32_t k[4], t = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) k[w] = s_best[64 * w + lane];
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = thr | 1u << bit;
-            int n = 0;
+            for (int w = 0; w < 4; ++w) k[w] = s_best[64 * w + lane];
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t cand = t | 1u << bit;
+                int n = 0;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) n += __popcll(__builtin_amdgcn_ballot_w64(k[w] >= cand));
-            if (n >= top) thr = cand;
+                for (int w = 0; w < 4; ++w) n += __popcll(__builtin_amdgcn_ballot_w64(k[w] >= cand));
+                if (n >= top) t = cand;
+            }
+            if (lane == 0) s_thr = t;
         }
+        __syncthreads();
+        const uint32_t thr = s_thr;
         const bool plain = S == S;  // no NaN and no +inf
         const int n = edge ? LpWave<TY, C, NV, true>{x, base, e0, V, lane}.list_top(lp_value(thr), top, plain, s_list[wave])
                            : LpWave<TY, C, NV, false>{x, base, e0, V, lane}.list_top(lp_value(thr), top, plain, s_list[wave]);

@@ -94,7 +94,7 @@ template <int D, int BS> struct TaWave {
     const int prefix, L;
     uint64_t mask = 0;  // of this lane's row
 
-    __device__ TaWave(const TaArgs &a_, int lane_, int s, int hk, const TaSeq &sq)
+    __device__ __forceinline__ TaWave(const TaArgs &a_, int lane_, int s, int hk, const TaSeq &sq)
         : a(a_), lane(lane_), h(lane_ >> 5), c(lane_ & 31), table(a_.tables + (int64_t)s * a_.max_blocks),
           page_bytes((int64_t)a_.KV * D * BS * 2), kbase((const uint8_t *)a_.kc + (int64_t)hk * D * BS * 2),
           vbase((const uint8_t *)a_.vc + (int64_t)hk * D * BS * 2),
@@ -107,14 +107,14 @@ template <int D, int BS> struct TaWave {
         int id[PAGES];
         uint32_t good;  // bits of the tile's keys whose page is inside
     };
-    __device__ Pages ids_of(int base) const {
+    __device__ __forceinline__ Pages ids_of(int base) const {
         Pages p = {};
 #pragma unroll
         for (int i = 0; i < PAGES; ++i)
             p.id[i] = table[__builtin_amdgcn_readfirstlane(min(base / BS + i, (L - 1) / BS))];
         return p;
     }
-    __device__ Pages checked(Pages p) const {
+    __device__ __forceinline__ Pages checked(Pages p) const {
         p.good = 0;
 #pragma unroll
         for (int i = 0; i < PAGES; ++i) {
@@ -124,7 +124,7 @@ template <int D, int BS> struct TaWave {
         }
         return p;
     }
-    __device__ int64_t page_at(const Pages &p, int key) const {  // of key `key` of the tile
+    __device__ __forceinline__ int64_t page_at(const Pages &p, int key) const {  // of key `key` of the tile
         int id = p.id[0];
 #pragma unroll
         for (int i = 1; i < PAGES; ++i) id = key / BS == i ? p.id[i] : id;
@@ -132,24 +132,24 @@ template <int D, int BS> struct TaWave {
     }
     // this lane's 16 bytes of the keys' step st are k_at() + k_step(st), of the values'
     // keys 16 i + 8 h .. + 7 and dims 32 d .. + 31 v_at(i) + v_step(d)
-    __device__ const uint8_t *k_at(const Pages &p) const {
+    __device__ __forceinline__ const uint8_t *k_at(const Pages &p) const {
         return kbase + page_at(p, kappa) + h * BS * 16 + (kappa % BS) * 16;
     }
-    __device__ static int k_step(int st) { return st * BS * 32; }
-    __device__ const uint8_t *v_at(const Pages &p, int i) const {
+    static __device__ __forceinline__ int k_step(int st) { return st * BS * 32; }
+    __device__ __forceinline__ const uint8_t *v_at(const Pages &p, int i) const {
         const int key = 16 * i + 8 * h;
         return vbase + page_at(p, key) + (key % BS) * 2 + c * BS * 2;
     }
-    __device__ int v_step(int d) const {  // dims past the last repeat it
+    __device__ __forceinline__ int v_step(int d) const {  // dims past the last repeat it
         return (32 * d + 31 < D ? 32 * d : min(32 * d + c, D - 1) - c) * BS * 2;
     }
 
-    __device__ const uint8_t *set_row(int b, int hk, int row) {  // -> this lane's part of the row's q
+    __device__ __forceinline__ const uint8_t *set_row(int b, int hk, int row) {  // -> this lane's part of the row's q
         const int i = row / a.G;
         mask = (uint64_t)a.masks[b + i];
         return (const uint8_t *)(a.q + ((int64_t)(b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * h;
     }
-    __device__ uint4 signed_q(uint4 w) const {
+    __device__ __forceinline__ uint4 signed_q(uint4 w) const {
         return make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor, (w.w & a.qand) ^ a.qxor);
     }
 
@@ -159,13 +159,13 @@ template <int D, int BS> struct TaWave {
     // not see into NaN. So where a wave's sums come out not finite, it takes its tiles
     // again, carefully: in those with masked keys it adds each seen key's product by itself.
     bool some_masked = false;
-    __device__ void reset() {
+    __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int d = 0; d < NB; ++d) O[d] = (f32x16){};
         m = -INFINITY;
         l = 0.0f;
     }
-    __device__ bool bad() const {
+    __device__ __forceinline__ bool bad() const {
         bool x = false;
 #pragma unroll
         for (int d = 0; d < NB; ++d)
@@ -179,7 +179,7 @@ template <int D, int BS> struct TaWave {
         uint32_t there;   // keys that are in the cache
         uint32_t vis;     // keys that this lane's row sees
     };
-    __device__ Seen seen(int base, uint32_t good) {
+    __device__ __forceinline__ Seen seen(int base, uint32_t good) {
         Seen s = {base + 32 <= prefix && good == ~0u, ~0u, ~0u};
         if (!s.whole) {
             some_masked = true;
@@ -194,7 +194,7 @@ template <int D, int BS> struct TaWave {
         return s;
     }
     // scores of U x 32 keys -> numerators (f16), the running maximum and sum
-    template <int U> __device__ void softmax(f32x16 (&S)[U], const Seen (&s)[U], uint4 (&pf)[2 * U]) {
+    template <int U> __device__ __forceinline__ void softmax(f32x16 (&S)[U], const Seen (&s)[U], uint4 (&pf)[2 * U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (!s[u].whole) {
@@ -233,14 +233,14 @@ template <int D, int BS> struct TaWave {
             }
     }
     // places that hold no token's value may hold anything
-    __device__ uint4 live_v(uint4 v, int i, uint32_t there) const {
+    __device__ __forceinline__ uint4 live_v(uint4 v, int i, uint32_t there) const {
         const uint32_t on = there >> (16 * i + 8 * h);
         auto keep = [&](int e) { return ((on >> e) & 1 ? 0xffffu : 0u) | ((on >> e) & 2 ? 0xffff0000u : 0u); };
         return make_uint4(v.x & keep(0), v.y & keep(2), v.z & keep(4), v.w & keep(6));
     }
     // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
     // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
-    __device__ void careful_pv(int d, const Seen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
+    __device__ __forceinline__ void careful_pv(int d, const Seen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
 #pragma unroll 1
         for (int key = 0; key < 32; ++key) {
             const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
