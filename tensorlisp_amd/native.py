@@ -552,12 +552,19 @@ class _on:
             self.guard.__exit__(*exc)
 
 
-def _use_on(stream, *tensors):
-    """Tensors allocated on the current stream but used on another: the allocator must wait for that one."""
+def _torch_stream(stream, device):
+    """A stream as the calls take it (torch's, or a hipStream_t) as torch's."""
     import torch
 
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    return torch.cuda.ExternalStream(stream, device=device)
+
+
+def _use_on(stream, *tensors):
+    """Tensors allocated on the current stream but used on another: the allocator must wait for that one."""
     if stream is not None:
-        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(getattr(stream, "value", stream) or 0))
+        s = _torch_stream(stream, tensors[0].device)
         for t in tensors:
             t.record_stream(s)
 
@@ -664,8 +671,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts
                          block_tables.shape[1], max_context_len, scale, device=q.device)
     q, out = q.contiguous(), torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
     if stream is not None:  # the zeros and a copied q come from the current stream
-        s = torch.cuda.current_stream(q.device)
-        (stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream))).wait_stream(s)
+        _torch_stream(stream, q.device).wait_stream(torch.cuda.current_stream(q.device))
     node(out, q, k_cache, v_cache, block_tables.contiguous(), context_lens, draft_starts, draft_masks, stream)
     _use_on(stream, out, q, node.scratch)
     return out

@@ -180,3 +180,23 @@ def test_two_nodes_at_once(gpu):
             nodes[i](outs[i], *ins[i], stream=streams[i])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+
+
+def test_streams_given_by_number(gpu):
+    """A hipStream_t as a number, as the other entry points take it."""
+    g = torch.Generator(device="cuda").manual_seed(93)
+    q = torch.randn((40, H, D), generator=g, device="cuda").half()
+    k = torch.randn((40, KV, D), generator=g, device="cuda").half()
+    x, t = torch.randn((3, 9000), generator=g, device="cuda"), i32([1, 2, 3])
+    kc = torch.randn((8, KV, D // 8, BS, 8), generator=g, device="cuda").half()
+    vc = torch.randn((8, KV, D, BS), generator=g, device="cuda").half()
+    tree = (q[:4], kc, vc, i32([[3, 1, 7]]), i32([44]), i32([0, 4]), signed([1, 3, 7, 15]).cuda(), 4, 48, 0.1)
+    want = (N.packed_attention(q, k, k, i32([0, 40]), 40, 0.1), N.tree_attention(*tree), *N.token_logprobs(x, t, 3))
+    starts = i32([0, 40])
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (s, s.cuda_stream):
+        got = (N.packed_attention(q, k, k, starts, 40, 0.1, stream=stream), N.tree_attention(*tree, stream=stream),
+               *N.token_logprobs(x, t, 3, stream=stream))
+        s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
