@@ -14,7 +14,7 @@
 //    alternatives it is 70);
 //  * where more reach it than the list holds, as in a vocabulary-wide run of equal
 //    logits (a grammar's -inf mask), ties are taken in index order and only up to
-//    `top` (112 us with 999 of 1000 masked);
+//    `top` (109 us with 999 of 1000 masked);
 //  * more elements above the threshold than the list holds (the largest ones
 //    crowded into few lanes) are taken one maximum at a time instead, read again.
 // A second launch folds the chunks' sums and merges their sorted lists the same
@@ -26,8 +26,10 @@
 namespace tlh {
 
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_CAP = 256;       // listed elements above a wave's threshold
-constexpr int LP_MERGE = 128;     // listed entries of a row in the merge
+constexpr int LP_FEW = 64;        // elements that reach the threshold, a wave: listed as they are
+constexpr int LP_CAP = 256;       // elements above it, where more reach it
+constexpr int LP_MERGE = 256;     // listed entries of a row in the merge
+constexpr int LP_AHEAD = 4;       // entries of a list that make the merge's threshold
 constexpr int LP_LISTS = 64;      // chunks of a row, at most: a lane each in the merge
 // elements of a chunk: 64 (or 16, for few rows) of each of 256 lanes
 constexpr int LP_CHUNK = 64 * 256, LP_CHUNK_SMALL = 16 * 256;
@@ -82,8 +84,8 @@ template <int TY, int C, int NV, bool EDGE> struct LpWave {
     __device__ int elem(int i, int c) const { return e0 + 256 * C * i + c; }
     __device__ bool there(int i, int c) const { return !EDGE || (uint32_t)elem(i, c) < (uint32_t)V; }
 
-    // Lists the elements that reach thr (a value); where they are more than the list holds,
-    // those above it and the first `top` that equal it; -> how many. A wave with a NaN or
+    // Lists the elements that reach thr (a value); where they are more than a few, those
+    // above it and the first `top` that equal it; -> how many. A wave with a NaN or
     // +inf (plain = false) and one with too many above thr take their `top` largest one
     // maximum at a time instead.
     __device__ __forceinline__ int list_top(float thr, int top, bool plain, uint64_t *list) const {
@@ -94,16 +96,16 @@ template <int TY, int C, int NV, bool EDGE> struct LpWave {
                 uint64_t any = 0;
 #pragma unroll
                 for (int c = 0; c < C; ++c) any |= __builtin_amdgcn_ballot_w64(x[i][c] >= thr);
-                if (any == 0 || n > LP_CAP) continue;
+                if (any == 0 || n > LP_FEW) continue;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     const uint64_t who = __builtin_amdgcn_ballot_w64(x[i][c] >= thr && there(i, c));
                     const int at = n + lp_below(who);
-                    if ((who >> lane) & 1 && at < LP_CAP) list[at] = lp_entry(lp_key(x[i][c]), elem(i, c));
+                    if ((who >> lane) & 1 && at < LP_FEW) list[at] = lp_entry(lp_key(x[i][c]), elem(i, c));
                     n += __popcll(who);
                 }
             }
-            if (n <= LP_CAP) return n;
+            if (n <= LP_FEW) return n;
             int above = 0, equal = 0;
             const float over = lp_value(lp_key(thr) + 1);  // the next number
 #pragma unroll
@@ -296,9 +298,9 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
     // what is needed later starts on its way here
     const uint64_t *list = (const uint64_t *)(slot + 16);
     auto entry = [&](int i) { return lane < P && i < top ? list[i] : (uint64_t)0; };
-    uint64_t ahead[4];
+    uint64_t ahead[LP_AHEAD];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ahead[i] = entry(i);
+    for (int i = 0; i < LP_AHEAD; ++i) ahead[i] = entry(i);
     const int token = a.logprobs ? a.tokens[row] : -1;
     const bool known = token >= 0 && token < a.vocab;
     const float x = known ? lp_elem<TY>(a.logits, (int64_t)row * a.row_stride + token) : 0.0f;
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
         if (a.entropy) a.entropy[row] = lse - T / S;
         if (a.logprobs) a.logprobs[row] = known ? (x - M) - lse : __uint_as_float(0x7fc00000u);
     }
-    // The lanes' lists are sorted. As in a chunk: the top-th largest of their first four
+    // The lanes' lists are sorted. As in a chunk: the top-th largest of their first
     // entries is a threshold (0 with fewer of them), and the few that reach it are ranked
     // by counting.
     __shared__ uint64_t s_list[4][LP_MERGE];
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
         const uint32_t cand = thr | 1u << bit;
         int reach = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reach += __popcll(__builtin_amdgcn_ballot_w64((uint32_t)(ahead[i] >> 32) >= cand));
+        for (int i = 0; i < LP_AHEAD; ++i) reach += __popcll(__builtin_amdgcn_ballot_w64((uint32_t)(ahead[i] >> 32) >= cand));
         if (reach >= top) thr = cand;
     }
     int n = 0;
@@ -349,8 +351,8 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
         if (in && at < LP_MERGE) l[at] = e;
         n += __popcll(who);
 #pragma unroll
-        for (int j = 0; j < 3; ++j) ahead[j] = ahead[j + 1];
-        ahead[3] = entry(i + 4);
+        for (int j = 0; j + 1 < LP_AHEAD; ++j) ahead[j] = ahead[j + 1];
+        ahead[LP_AHEAD - 1] = entry(i + LP_AHEAD);
     }
     if (n <= LP_MERGE) {
         __builtin_amdgcn_wave_barrier();
@@ -383,9 +385,15 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
     }
 }
 
+// A small vocabulary's chunk of 64 a lane would be mostly empty: 1393 rows of 2601, 29
+// us with it, 16 with 16.
+static bool lp_small(int64_t vocab) { return vocab <= 2 * LP_CHUNK_SMALL; }
 static int lp_ept(int64_t rows, int64_t vocab) {
     // few rows: shorter chunks, so that more CUs share them
-    return rows * ((vocab + LP_CHUNK - 1) / LP_CHUNK) < 256 && vocab + 7 <= (int64_t)LP_CHUNK_SMALL * LP_LISTS ? 16 : 64;
+    return lp_small(vocab) || (rows * ((vocab + LP_CHUNK - 1) / LP_CHUNK) < 256 &&
+                               vocab + 7 <= (int64_t)LP_CHUNK_SMALL * LP_LISTS)
+               ? 16
+               : 64;
 }
 static int lp_chunks(int64_t vocab, int ept) {
     return (int)((vocab + 7 + 256 * ept - 1) / (256 * ept));  // up to 7 places before a row that is not aligned
@@ -394,7 +402,10 @@ static int lp_chunks(int64_t vocab, int ept) {
 // Room for either chunk length, so that the size grows with the rows and one
 // buffer for the largest batch serves every smaller one.
 size_t token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int top) {
-    return ((size_t)rows * lp_chunks(vocab, 64) + (size_t)std::min<int64_t>(rows, 256) * lp_chunks(vocab, 16)) * lp_slot(top);
+    const size_t chunks = lp_small(vocab) ? (size_t)rows * lp_chunks(vocab, 16)
+                                          : (size_t)rows * lp_chunks(vocab, 64) +
+                                                (size_t)std::min<int64_t>(rows, 256) * lp_chunks(vocab, 16);
+    return chunks * lp_slot(top);
 }
 
 template <int TY> static void launch_lp(const tlh_token_logprobs_args &a, void *scratch, hipStream_t stream) {

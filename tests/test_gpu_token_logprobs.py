@@ -192,3 +192,15 @@ def test_on_another_stream_and_captured(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, N.token_logprobs(x, t, 5)))
+
+
+@pytest.mark.parametrize("rows,vocab,top", [(6, 128256, 5), (16, 21236, 8), (68, 19835, 32), (300, 8192, 32), (300, 8193, 32),
+                                            (20, 4090, 20), (3, 8190, 7)])
+@pytest.mark.parametrize("masked", [0.0, 0.999])
+def test_ends_of_chunks(gpu, rows, vocab, top, masked):
+    """Last chunks that hold a few vectors, masked ones among them, and vocabularies about the chunk lengths."""
+    x = logits(rows, vocab, torch.float32, 82)
+    off = torch.rand((rows, vocab), generator=torch.Generator().manual_seed(83)) < masked
+    off[:, 0] = False
+    x.masked_fill_(off.cuda(), float("-inf"))
+    check(x, torch.zeros(rows, dtype=torch.int32, device="cuda"), top)
