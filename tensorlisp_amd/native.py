@@ -670,10 +670,11 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts
     node = TreeAttention(block_tables.shape[0], rows, max_drafts, heads, v_cache.shape[1], hs, v_cache.shape[3],
                          block_tables.shape[1], max_context_len, scale, device=q.device)
     q, out = q.contiguous(), torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
-    if stream is not None:  # the zeros and a copied q come from the current stream
+    block_tables = block_tables.contiguous()
+    if stream is not None:  # the zeros and the copies come from the current stream
         _torch_stream(stream, q.device).wait_stream(torch.cuda.current_stream(q.device))
-    node(out, q, k_cache, v_cache, block_tables.contiguous(), context_lens, draft_starts, draft_masks, stream)
-    _use_on(stream, out, q, node.scratch)
+    node(out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream)
+    _use_on(stream, out, q, block_tables, node.scratch)
     return out
 
 

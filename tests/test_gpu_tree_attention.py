@@ -308,3 +308,21 @@ def test_scales_below_zero_and_zero(gpu):
     check(out, {**c, "q": -c["q"], "scale": 0.2})
     c["scale"] = 0.0
     check(run(c), {**c, "q": c["q"] * 0, "scale": 1.0})
+
+
+def test_one_call_form_with_views(gpu):
+    """Non-contiguous q and block tables are copied, also for a call on another stream."""
+    c = build(8, 2, 128, 16, [100, 30], [5, 9], 68, width=9)
+    q = torch.zeros((14, 16, 128), dtype=torch.float16, device="cuda")
+    q[:, ::2] = c["q"].cuda()
+    wide = i32(np.repeat(c["table"], 2, 1))[:, ::2]
+    dev = (c["kc"].cuda(), c["vc"].cuda(), wide, i32(c["lens"]), i32(c["starts"]), signed(c["masks"]).cuda(), 9, 105,
+           c["scale"])
+    check(N.tree_attention(q[:, ::2], *dev), c)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        out = N.tree_attention(q[:, ::2], *dev, stream=s)
+        torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda")  # the allocator may hand out what the call let go
+    s.synchronize()
+    check(out, c)
