@@ -669,12 +669,15 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts
     rows, heads, hs = q.shape
     node = TreeAttention(block_tables.shape[0], rows, max_drafts, heads, v_cache.shape[1], hs, v_cache.shape[3],
                          block_tables.shape[1], max_context_len, scale, device=q.device)
-    q, out = q.contiguous(), torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
-    block_tables = block_tables.contiguous()
-    if stream is not None:  # the zeros and the copies come from the current stream
-        _torch_stream(stream, q.device).wait_stream(torch.cuda.current_stream(q.device))
+    out = torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
+    side = None
+    if stream is not None:  # the zeros come from the current stream; the copies are the call's, on its own
+        side = _torch_stream(stream, q.device)
+        side.wait_stream(torch.cuda.current_stream(q.device))
+    with torch.cuda.stream(side):
+        q, block_tables = q.contiguous(), block_tables.contiguous()
     node(out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream)
-    _use_on(stream, out, q, block_tables, node.scratch)
+    _use_on(stream, out, node.scratch)
     return out
 
 

@@ -326,3 +326,24 @@ def test_one_call_form_with_views(gpu):
         torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda")  # the allocator may hand out what the call let go
     s.synchronize()
     check(out, c)
+
+
+def test_one_call_form_copies_on_the_calls_stream(gpu):
+    """Views that the call's own stream is still to fill are copied behind that work."""
+    c = build(8, 2, 128, 16, [100, 30], [5, 9], 69, width=9)
+    q = torch.zeros((14, 16, 128), dtype=torch.float16, device="cuda")
+    table = torch.zeros((2, 18), dtype=torch.int32, device="cuda")
+    cq, ctable = c["q"].cuda(), i32(c["table"])
+    dev = (c["kc"].cuda(), c["vc"].cuda(), table[:, ::2], i32(c["lens"]), i32(c["starts"]), signed(c["masks"]).cuda(), 9,
+           105, c["scale"])
+    busy = torch.ones((4096, 4096), dtype=torch.float16, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(40):  # some ms
+            torch.mm(busy, busy)
+        q[:, ::2] = cq
+        table[:, ::2] = ctable
+    out = N.tree_attention(q[:, ::2], *dev, stream=s)
+    s.synchronize()
+    check(out, c)
