@@ -60,6 +60,12 @@ __device__ __forceinline__ float lp_wave_maxf(float v) {
     for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
+// x - m, whose exponential is 0 below -1000 anyway: a -inf (x, or the difference of
+// numbers far apart) must not reach the product with it
+__device__ __forceinline__ float lp_apart(float x, float m) {
+    const float d = x - m;
+    return d < -1000.0f ? -1000.0f : d;
+}
 // set bits of b below this lane
 __device__ __forceinline__ int lp_below(uint64_t b) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
@@ -204,16 +210,15 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
 #pragma unroll
         for (int c = 0; c < C; ++c) best = fmaxf(best, x[i][c]);
     const float m = lp_wave_maxf(best);
-    // exp(x - m) as 2^((x - m) log2 e). Below -1000 it is 0 anyway, and a -inf
-    // (x or, where all are, x - m = NaN) must not reach the product with it. A
-    // NaN among the logits is not in m; it passes both maxima and makes S NaN.
+    // exp(x - m) as 2^((x - m) log2 e). A NaN among the logits is not in m; it passes
+    // both maxima and makes S NaN.
     float S = 0.0f, T = 0.0f;
     if (m != -INFINITY) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const float t = x[i][c] - m, d = t < -1000.0f ? -1000.0f : t;
+                const float d = lp_apart(x[i][c], m);
                 const float e = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
                 S += e;
                 T += e * d;
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(256) k_token_logprobs(const void *__restrict__
         for (int w = 0; w < 4; ++w) M = fmaxf(M, s_sum[w][0]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float d = s_sum[w][0] - M, f = __expf(d);
+            const float d = lp_apart(s_sum[w][0], M), f = __expf(d);
             const bool none = s_sum[w][0] == -INFINITY;  // S is 0, or NaN
             SS += none ? s_sum[w][1] : f * s_sum[w][1];
             TT += none ? 0.0f : f * s_sum[w][2] + f * d * s_sum[w][1];
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(256) k_token_logprobs_merge(const tlh_token_lo
         if (st.x == -INFINITY) {
             S = st.y;  // 0, or NaN
         } else {
-            const float d = st.x - M, f = __expf(d);
+            const float d = lp_apart(st.x, M), f = __expf(d);
             S = f * st.y;
             T = f * st.z + f * d * st.y;
         }

@@ -204,3 +204,18 @@ def test_ends_of_chunks(gpu, rows, vocab, top, masked):
     off[:, 0] = False
     x.masked_fill_(off.cuda(), float("-inf"))
     check(x, torch.zeros(rows, dtype=torch.int32, device="cuda"), top)
+
+
+@pytest.mark.parametrize("vocab", [500, 5000, 40000, 200000])
+def test_numbers_too_far_apart_to_subtract(gpu, vocab):
+    """Whole waves, and whole chunks, at one end of the range, the maximum at the other: their difference overflows."""
+    x = torch.full((2, vocab), -3e38, dtype=torch.float32, device="cuda")
+    x[0, vocab // 2] = x[0, vocab - 1] = 3e38
+    x[1, 3] = x[1, 4] = x[1, vocab // 3] = 3e38
+    t = torch.tensor([vocab - 1, 4], dtype=torch.int32, device="cuda")
+    lp, ent, tl, ti = N.token_logprobs(x, t, 2)
+    want = torch.log(torch.tensor([2.0, 3.0], dtype=torch.float64))  # two and three equal ones, the rest 0
+    close(ent, want, torch.full((2,), 2.0 ** -18, dtype=torch.float64))
+    close(lp, -want, torch.full((2,), 2.0 ** -18, dtype=torch.float64))
+    close(tl, -want[:, None].expand(2, 2), torch.full((2, 2), 2.0 ** -18, dtype=torch.float64))
+    assert ti.tolist() == [[vocab // 2, vocab - 1], [3, 4]]
