@@ -1205,6 +1205,8 @@ static tlh_status check_tree(const tlh_tree_attention_args *a) {
         return set_error(TLH_INVALID, "tree_attention: bad counts (at most 65535 sequences)");
     if (a->max_drafts < 0 || a->max_drafts > 64)
         return set_error(TLH_INVALID, "tree_attention: max_drafts %d outside 0..64", a->max_drafts);
+    if (a->max_context_len > 1 << 30)  // the kernels look a few tiles past it, in 32 bits
+        return set_error(TLH_INVALID, "tree_attention: max_context_len %d above 2^30", a->max_context_len);
     if ((int64_t)a->max_blocks_per_seq * a->block_size < a->max_context_len)
         return set_error(TLH_INVALID, "tree_attention: max_blocks_per_seq * block_size < max_context_len");
     return TLH_OK;

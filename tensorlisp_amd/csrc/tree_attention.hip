@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
             ids(t + 2, pn);
         }
         if (!mine) return;
-f32x16 S[SUBS];
+        f32x16 S[SUBS];
         typename W::Seen see[SUBS];
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {

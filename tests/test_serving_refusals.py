@@ -236,3 +236,12 @@ def test_compact_cache_lengths_must_not_overlap():
         assert compact(num_seqs=4, context_lens=base, new_lens=base + at, draft_starts=base + 4096) == "INVALID", at
         assert compact(num_seqs=4, draft_starts=base, new_lens=base + at, context_lens=base + 4096) == "INVALID", at
     assert compact(num_seqs=4, draft_starts=base, new_lens=base + 16, context_lens=base + 4096) == "INVALID"
+
+
+def test_tree_attention_refuses_contexts_past_its_integers():
+    """A tile's lookahead past the last token is formed in 32 bits."""
+    n = C.c_size_t()
+    for ctx, want in ((1 << 30, "OK"), ((1 << 30) + 1, "INVALID"), ((1 << 31) - 1, "INVALID")):
+        a = tree(max_context_len=ctx, max_blocks_per_seq=1 << 27)
+        assert status(N.lib().tlh_tree_attention_scratch_bytes, C.byref(a), C.byref(n))[0] == want
+    assert status(N.lib().tlh_tree_attention, C.byref(a), P, BIG, None)[0] == "INVALID"
