@@ -561,6 +561,18 @@ def _torch_stream(stream, device):
     return torch.cuda.ExternalStream(stream, device=device)
 
 
+def _behind_current(stream, device):
+    """A call's own tensors come from the current stream's pool, where queued work may still use the memory they were
+    given: the call's `stream` waits for that work. -> the stream as torch's, None for the current one."""
+    import torch
+
+    if stream is None:
+        return None
+    side = _torch_stream(stream, device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    return side
+
+
 def _use_on(stream, *tensors):
     """Tensors allocated on the current stream but used on another: the allocator must wait for that one."""
     if stream is not None:
@@ -587,7 +599,8 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     stride that is a multiple of 8 elements (views of a fused projection),
     seq_starts i32 (sequences + 1,) -> out (tokens, heads, head size). No
     sequence may be longer than max_seq_len. Tokens behind the last sequence are
-    left as they were in `out` (without one, as the new tensor holds them)."""
+    left as they were in `out` (without one, as the new tensor holds them, and
+    `stream` waits for the current stream's work, which may still use its memory)."""
     import torch
 
     (tokens, heads, hs), dtype, dev = q.shape, q.dtype, q.device
@@ -614,6 +627,8 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     a.num_seqs, a.num_tokens, a.max_seq_len = n - 1, tokens, max_seq_len
     a.num_heads, a.num_kv_heads, a.head_size, a.scale = heads, kv, hs, scale
     with _on(dev, stream) as s:
+        if fresh:
+            _behind_current(stream, dev)
         check(lib().tlh_packed_attention(C.byref(a), s))
     if fresh:
         _use_on(stream, out)
@@ -663,18 +678,16 @@ class TreeAttention:
 
 def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, max_drafts: int,
                    max_context_len: int, scale: float, stream=None):
-    """One TreeAttention call: q f16 (rows, heads, head size) -> out alike (zeros in rows behind the last sequence)."""
+    """One TreeAttention call: q f16 (rows, heads, head size) -> out alike (zeros in rows behind the last sequence).
+    `stream` waits for the current stream's work."""
     import torch
 
     rows, heads, hs = q.shape
     node = TreeAttention(block_tables.shape[0], rows, max_drafts, heads, v_cache.shape[1], hs, v_cache.shape[3],
                          block_tables.shape[1], max_context_len, scale, device=q.device)
     out = torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
-    side = None
-    if stream is not None:  # the zeros come from the current stream; the copies are the call's, on its own
-        side = _torch_stream(stream, q.device)
-        side.wait_stream(torch.cuda.current_stream(q.device))
-    with torch.cuda.stream(side):
+    # the zeros come from the current stream; the copies are the call's, on its own
+    with torch.cuda.stream(_behind_current(stream, q.device)):
         q, block_tables = q.contiguous(), block_tables.contiguous()
     node(out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream)
     _use_on(stream, out, node.scratch)
@@ -777,13 +790,15 @@ class TokenLogprobs:
 
 def token_logprobs(logits, tokens, top: int = 0, stream=None):
     """logits (rows, vocab) f32 / f16 / bf16, tokens i32 (rows,) -> (logprobs (rows,), entropy (rows,),
-    top_logprobs (rows, top), top_ids i32 (rows, top))."""
+    top_logprobs (rows, top), top_ids i32 (rows, top)). `stream` waits for the current stream's work, which
+    may still use the new tensors' memory."""
     import torch
 
     n, dev = logits.shape[0], logits.device
     node = TokenLogprobs(n, logits.shape[1], top, logits.dtype, device=dev)
     f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
     outs = (f(n), f(n), f(n, top), torch.empty((n, top), dtype=torch.int32, device=dev))
+    _behind_current(stream, dev)
     node(logits, tokens, *outs, stream=stream)
     _use_on(stream, *outs, node.scratch)
     return outs

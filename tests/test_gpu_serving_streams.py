@@ -1,0 +1,74 @@
+"""GPU: the serving operators on other streams than the current one, with work still queued on either."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tensorlisp_amd import native as N
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def normal(seed, *shape):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda").half()
+
+
+@pytest.fixture
+def busy(gpu):
+    """Queues some ms of work on the current stream."""
+    m = torch.ones((4096, 4096), dtype=torch.float16, device="cuda")
+    o = torch.empty_like(m)
+    torch.mm(m, m, out=o)
+    torch.cuda.synchronize()
+
+    def queue():
+        for _ in range(40):
+            torch.mm(m, m, out=o)
+
+    return queue
+
+
+def packed_case():
+    q, k, starts = normal(1, 700, 8, 128), normal(2, 700, 2, 128), i32(0, 300, 700)
+    return lambda stream=None: (N.packed_attention(q, k, k, starts, 400, 0.1, stream=stream),)
+
+
+def logprobs_case():
+    x, t = normal(3, 64, 30000).float(), torch.arange(64, dtype=torch.int32, device="cuda")
+    return lambda stream=None: N.token_logprobs(x, t, 20, stream=stream)
+
+
+@pytest.mark.parametrize("case,sizes", [
+    # the memory that the calls' own tensors may be given, in bytes: outputs and scratch
+    (packed_case, [700 * 8 * 128 * 2]), (logprobs_case, [64 * 4, 64 * 4, 64 * 80, 64 * 80]),
+], ids=["packed", "logprobs"])
+def test_memory_that_queued_work_still_uses(busy, case, sizes):
+    """Blocks just let go are read by work queued on the current stream while a call on another stream gets them."""
+    call = case()
+    want = call()
+    if case is logprobs_case:
+        sizes = sizes + [N.TokenLogprobs(64, 30000, 20).scratch_bytes]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    kept = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes]
+    let_go = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes]
+    torch.cuda.synchronize()
+    for t in let_go:
+        t.fill_(7)
+    busy()
+    for a, b in zip(kept, let_go):
+        a.copy_(b)
+    at = {t.data_ptr() for t in let_go}
+    t = b = None
+    let_go.clear()
+    got = call(s)
+    assert any(x.data_ptr() in at for x in got)  # the test's point
+    torch.cuda.synchronize()
+    assert all((t == 7).all() for t in kept)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,0 +1,86 @@
+"""The serving operators' order of allocations, waits and launches on streams, on the CPU: the streams are stand-ins
+that write down what is asked of them, and no kernel is launched."""
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+import torch
+
+from tensorlisp_amd import native as N
+
+
+class Stream:
+    def __init__(self, log, name):
+        self.log, self.name = log, name
+
+    def wait_stream(self, other):
+        self.log.append(f"{self.name} waits for {other}")
+
+
+class Library:
+    """The library, with the launches written down instead."""
+
+    def __init__(self, real, log):
+        self.real, self.log = real, log
+
+    def __getattr__(self, name):
+        if name in ("tlh_packed_attention", "tlh_tree_attention", "tlh_token_logprobs"):
+            return lambda *a: self.log.append("launch") or 0
+        return getattr(self.real, name)
+
+
+@pytest.fixture
+def log(monkeypatch):
+    out, lib, empty = [], N.lib(), torch.empty
+    monkeypatch.setattr(N, "lib", lambda: Library(lib, out))
+    monkeypatch.setattr(N, "_on", lambda device, stream: contextlib.nullcontext(0 if stream is None else stream))
+    monkeypatch.setattr(N, "_torch_stream", lambda stream, device: Stream(out, f"stream {stream}"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "the current stream")
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: out.append(f"recorded on {s.name}"))
+
+    def logged(*a, **kw):
+        out.append("allocation")
+        return empty(*a, **kw)
+
+    monkeypatch.setattr(torch, "empty", logged)
+    return out
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def packed(stream, out=None):
+    q, k = torch.zeros((4, 8, 64), dtype=torch.float16), torch.zeros((4, 2, 64), dtype=torch.float16)
+    N.packed_attention(q, k, k, i32(0, 4), 4, 0.1, out=out, stream=stream)
+
+
+def logprobs(stream):
+    N.token_logprobs(torch.zeros((2, 100)), i32(1, 2), 3, stream=stream)
+
+
+def tree(stream):
+    kc, vc = torch.zeros((5, 2, 8, 16, 8), dtype=torch.float16), torch.zeros((5, 2, 64, 16), dtype=torch.float16)
+    N.tree_attention(torch.zeros((3, 8, 64), dtype=torch.float16), kc, vc, torch.zeros((1, 4), dtype=torch.int32), i32(7),
+                     i32(0, 3), torch.zeros(3, dtype=torch.int64), 3, 60, 0.1, stream=stream)
+
+
+@pytest.mark.parametrize("call", [packed, logprobs, tree])
+def test_new_tensors_are_used_behind_the_current_streams_work(log, call):
+    """What a call allocates comes from the current stream's pool: its memory may still be in use there."""
+    call(77)
+    wait = log.index("stream 77 waits for the current stream")
+    assert wait < log.index("launch") and "allocation" not in log[wait:]
+
+
+@pytest.mark.parametrize("call", [packed, logprobs, tree])
+def test_calls_on_the_current_stream_wait_for_nothing(log, call):
+    call(None)
+    assert "launch" in log and not [x for x in log if "waits" in x or "recorded" in x]
+
+
+def test_given_outputs_need_no_wait(log):
+    packed(77, out=torch.zeros((4, 8, 64), dtype=torch.float16))
+    assert log == ["launch"]
