@@ -558,6 +558,8 @@ def _torch_stream(stream, device):
 
     if isinstance(stream, torch.cuda.Stream):
         return stream
+    if not stream:  # the default stream's number, which ExternalStream takes for none and makes a new stream
+        return torch.cuda.default_stream(device)
     return torch.cuda.ExternalStream(stream, device=device)
 
 

@@ -72,3 +72,23 @@ def test_memory_that_queued_work_still_uses(busy, case, sizes):
     torch.cuda.synchronize()
     assert all((t == 7).all() for t in kept)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_views_that_the_default_stream_is_still_to_fill(busy):
+    """Stream 0 by its number: the one-call form copies views there, behind the work queued there."""
+    q, kc, vc = normal(4, 6, 8, 64), normal(5, 40, 2, 8, 16, 8), normal(6, 40, 2, 64, 16)
+    table, masks = torch.arange(39, -1, -1, dtype=torch.int32, device="cuda")[None], torch.tensor(
+        [1, 3, 7, 9, 17, 33], device="cuda")
+    rest = (i32(601), i32(0, 6), masks, 6, 640, 0.1)
+    want = N.tree_attention(q, kc, vc, table, *rest)
+    wide, wide_table = torch.zeros((6, 16, 64), dtype=torch.float16, device="cuda"), torch.zeros(
+        (1, 80), dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy()
+    wide[:, ::2] = q
+    wide_table[:, ::2] = table
+    with torch.cuda.stream(s):
+        out = N.tree_attention(wide[:, ::2], kc, vc, wide_table[:, ::2], *rest, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

@@ -84,3 +84,10 @@ def test_calls_on_the_current_stream_wait_for_nothing(log, call):
 def test_given_outputs_need_no_wait(log):
     packed(77, out=torch.zeros((4, 8, 64), dtype=torch.float16))
     assert log == ["launch"]
+
+
+def test_stream_number_zero_is_the_default_stream(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: f"the default stream of {device}")
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda n, device=None: f"stream {n} of {device}")
+    assert N._torch_stream(0, "cuda:1") == "the default stream of cuda:1"
+    assert N._torch_stream(5, "cuda:1") == "stream 5 of cuda:1"
