@@ -527,8 +527,15 @@ def _extent(t) -> int:
     return t.shape[0] if t.dim() else 0
 
 
+def _current(device) -> int:
+    """current_stream's number, without the 2.7 us its Stream object takes."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class _on:
-    """Runs a call on the tensors' device, on `stream` or that device's current stream."""
+    """Runs a call on the tensors' device, on `stream` or that device's current stream: that stream's number."""
 
     def __init__(self, device, stream):
         self.device, self.stream, self.guard = device, stream, None
@@ -543,9 +550,9 @@ class _on:
         if self.device.index != torch.cuda.current_device():
             self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        if self.stream is None:  # current_stream's number, without the 2.7 us its Stream object takes
-            return torch._C._cuda_getCurrentRawStream(self.device.index)
-        return _stream(self.stream)
+        if self.stream is None:
+            return _current(self.device)
+        return int(getattr(self.stream, "cuda_stream", self.stream))
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -637,24 +644,53 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     return out
 
 
-class TreeAttention:
+class _ScratchNode:
+    """A node that owns its scratch, which it allocates on the current stream; its calls may run on others. Calls
+    of one node must be stream-ordered, and a captured call keeps using the scratch: keep the node with the graph."""
+
+    def _allocate(self, nbytes: int, device):
+        import torch
+
+        self.scratch_bytes = nbytes
+        self.scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self.device, self.scratch_ptr = self.scratch.device, self.scratch.data_ptr()
+        self._home = _current(self.device) if self.device.type == "cuda" else 0
+        self._streams = {self._home}  # those that may use it
+
+    def _use_scratch(self, stream: int):
+        """Called before a launch on `stream`. On another stream's first call, that one waits for the work queued on
+        the scratch's own, which may still use its memory, and the allocator learns that it uses the scratch."""
+        if stream in self._streams:
+            return
+        side, home = (_torch_stream(n, self.device) for n in (stream, self._home))
+        # (a capture cannot wait for work outside it, and begins with the device idle)
+        if not _capturing(side) and not _capturing(home):
+            side.wait_stream(home)
+            self._streams.add(stream)
+        self.scratch.record_stream(side)
+
+
+def _capturing(stream) -> bool:
+    import torch
+
+    with torch.cuda.stream(stream):  # (the default stream cannot be captured, nor asked while others are)
+        return stream.cuda_stream != 0 and torch.cuda.is_current_stream_capturing()
+
+
+class TreeAttention(_ScratchNode):
     """Attention of drafted tokens over the paged cache, with its scratch, launched many times. A call
     takes up to num_seqs sequences and num_rows drafted tokens in all, at most max_drafts (<= 64) of one
     sequence; calls of one object must be stream-ordered (they share the scratch)."""
 
     def __init__(self, num_seqs, num_rows, max_drafts, num_heads, num_kv_heads, head_size, block_size,
                  max_blocks_per_seq, max_context_len, scale, device="cuda"):
-        import torch
-
         a = self.args = TlhTreeArgs()
         a.num_seqs, a.num_rows, a.max_drafts = num_seqs, num_rows, max_drafts
         a.num_heads, a.num_kv_heads, a.head_size, a.block_size = num_heads, num_kv_heads, head_size, block_size
         a.max_blocks_per_seq, a.max_context_len, a.scale = max_blocks_per_seq, max_context_len, scale
         n = C.c_size_t()
         check(lib().tlh_tree_attention_scratch_bytes(C.byref(a), C.byref(n)))
-        self.scratch_bytes = n.value
-        self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
-        self.device, self.scratch_ptr = self.scratch.device, self.scratch.data_ptr()
+        self._allocate(n.value, device)
 
     def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream=None):
         """q and out f16 (num_rows, heads, head size), the caches in the paged-attention layouts,
@@ -674,6 +710,7 @@ class TreeAttention:
         a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
         a.draft_masks = _tensor(draft_masks, torch.int64, (rows,), "draft_masks", dev)
         with _on(dev, stream) as s:
+            self._use_scratch(s)
             check(lib().tlh_tree_attention(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
         return out
 
@@ -692,7 +729,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, context_lens, draft_starts
     with torch.cuda.stream(_behind_current(stream, q.device)):
         q, block_tables = q.contiguous(), block_tables.contiguous()
     node(out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream)
-    _use_on(stream, out, node.scratch)
+    _use_on(stream, out)
     return out
 
 
@@ -748,7 +785,7 @@ class KVPools:
         return new_lens
 
 
-class TokenLogprobs:
+class TokenLogprobs(_ScratchNode):
     """Log probabilities of given tokens, entropies and the `top` likeliest tokens of up to `rows` rows of
     logits, with the scratch; calls of one object must be stream-ordered (they share it)."""
 
@@ -761,9 +798,7 @@ class TokenLogprobs:
         a.row_stride = vocab
         n = C.c_size_t()
         check(lib().tlh_token_logprobs_scratch_bytes(C.byref(a), C.byref(n)))
-        self.scratch_bytes = n.value
-        self.scratch = torch.empty(max(n.value, 16), dtype=torch.uint8, device=device)
-        self.device, self.scratch_ptr = self.scratch.device, self.scratch.data_ptr()
+        self._allocate(n.value, device)
 
     def __call__(self, logits, tokens, logprobs, entropy, top_logprobs=None, top_ids=None, stream=None):
         """logits (n, vocab) with n <= rows, any row stride; tokens i32 (n,); logprobs and entropy f32 (n,);
@@ -786,6 +821,7 @@ class TokenLogprobs:
             a.top_logprobs = _tensor(top_logprobs, torch.float32, (n, a.top), "top_logprobs", dev)
             a.top_ids = _tensor(top_ids, torch.int32, (n, a.top), "top_ids", dev)
         with _on(dev, stream) as s:
+            self._use_scratch(s)
             check(lib().tlh_token_logprobs(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
         return logprobs, entropy, top_logprobs, top_ids
 
@@ -802,7 +838,7 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None):
     outs = (f(n), f(n), f(n, top), torch.empty((n, top), dtype=torch.int32, device=dev))
     _behind_current(stream, dev)
     node(logits, tokens, *outs, stream=stream)
-    _use_on(stream, *outs, node.scratch)
+    _use_on(stream, *outs)
     return outs
 
 

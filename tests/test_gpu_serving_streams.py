@@ -92,3 +92,89 @@ def test_views_that_the_default_stream_is_still_to_fill(busy):
         out = N.tree_attention(wide[:, ::2], kc, vc, wide_table[:, ::2], *rest, stream=0)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def tree_node():
+    """The partials of 1024 workgroups: 8 sequences x 2 kv heads in 64 partitions."""
+    q, kc, vc = normal(7, 64, 8, 128), normal(8, 8 * 513, 2, 16, 16, 8), normal(9, 8 * 513, 2, 128, 16)
+    table = torch.randperm(8 * 513, device="cuda", dtype=torch.int32).view(8, 513)
+    args = (q, kc, vc, table, i32(*[8200 - 100 * i for i in range(8)]), i32(*range(0, 65, 8)),
+            torch.tensor([(1 << (i % 8 + 1)) - 1 for i in range(64)], device="cuda"))
+    return (lambda: N.TreeAttention(8, 64, 8, 8, 2, 128, 16, 513, 8208, 0.1),
+            lambda node, outs, stream: node(outs[0], *args, stream=stream), [torch.empty_like(q)])
+
+
+def logprobs_node():
+    x, t = normal(3, 64, 30000).float(), torch.arange(64, dtype=torch.int32, device="cuda")
+    outs = [torch.empty(64, device="cuda"), torch.empty(64, device="cuda"), torch.empty((64, 20), device="cuda"),
+            torch.empty((64, 20), dtype=torch.int32, device="cuda")]
+    return (lambda: N.TokenLogprobs(64, 30000, 20), lambda node, outs, stream: node(x, t, *outs, stream=stream), outs)
+
+
+@pytest.mark.parametrize("case", [tree_node, logprobs_node])
+def test_a_new_nodes_scratch_in_memory_that_queued_work_still_uses(busy, case):
+    make, call, want = case()
+    node = make()
+    n, got = node.scratch.numel(), [torch.zeros_like(t) for t in want]
+    call(node, want, None)
+    node = None
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    kept = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    let_go = torch.empty(n, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    let_go.fill_(7)
+    busy()
+    kept.copy_(let_go)
+    at, let_go = let_go.data_ptr(), None
+    node = make()
+    assert node.scratch_ptr == at  # the test's point
+    call(node, got, s)
+    torch.cuda.synchronize()
+    assert (kept == 7).all()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("given", [True, False], ids=["given stream", "current stream"])
+@pytest.mark.parametrize("case", [tree_node, logprobs_node])
+def test_a_node_let_go_behind_a_call_on_another_stream(busy, case, given):
+    make, call, want = case()
+    node = make()
+    call(node, want, None)
+    n, got = node.scratch.numel(), [torch.zeros_like(t) for t in want]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        busy()
+        if not given:
+            call(node, got, None)
+    if given:
+        call(node, got, s)
+    at, node = node.scratch_ptr, None
+    others = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    assert all(t.data_ptr() != at for t in others)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("case", [tree_node, logprobs_node])
+def test_a_node_captured_before_any_call(gpu, case):
+    """The first call is in a graph, on another stream than the node was made on; then eager ones on more streams."""
+    make, call, want = case()
+    call(make(), want, None)
+    node, got = make(), [torch.zeros_like(t) for t in want]
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        call(node, got, None)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        other = [torch.zeros_like(t) for t in want]
+        torch.cuda.synchronize()
+        call(node, other, s)
+        s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
