@@ -693,13 +693,17 @@ class TreeAttention(_ScratchNode):
         self._allocate(n.value, device)
 
     def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, draft_starts, draft_masks, stream=None):
-        """q and out f16 (num_rows, heads, head size), the caches in the paged-attention layouts,
-        block_tables i32 (num_seqs, max_blocks_per_seq), context_lens i32 (num_seqs,) with the drafted
-        tokens, draft_starts i32 (num_seqs + 1,), draft_masks i64 (num_rows,): bit j = sees draft j."""
+        """q and out f16 (rows, heads, head size) with rows <= num_rows, the caches in the paged-attention
+        layouts, block_tables i32 (sequences, max_blocks_per_seq) with sequences <= num_seqs, context_lens
+        i32 (sequences,) with the drafted tokens, draft_starts i32 (sequences + 1,), draft_masks i64
+        (rows,): bit j = sees draft j."""
         import torch
 
         a, dev = TlhTreeArgs.from_buffer_copy(self.args), self.device  # a call's own: threads may share the node
-        rows, S, KV, D, bs = a.num_rows, a.num_seqs, a.num_kv_heads, a.head_size, a.block_size
+        rows, S, KV, D, bs = _extent(out), _extent(block_tables), a.num_kv_heads, a.head_size, a.block_size
+        if rows > a.num_rows or S > a.num_seqs:
+            raise ValueError(f"out of {rows} rows and block_tables of {S} sequences, for up to {a.num_rows} and {a.num_seqs}")
+        a.num_rows, a.num_seqs = rows, S
         a.q = _tensor(q, torch.float16, (rows, a.num_heads, D), "q", dev)
         a.out = _tensor(out, torch.float16, (rows, a.num_heads, D), "out", dev)
         a.num_blocks = blocks = _extent(k_cache)

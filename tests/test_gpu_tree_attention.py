@@ -347,3 +347,15 @@ def test_one_call_form_copies_on_the_calls_stream(gpu):
     out = N.tree_attention(q[:, ::2], *dev, stream=s)
     s.synchronize()
     check(out, c)
+
+
+def test_a_node_takes_smaller_calls(gpu):
+    """One node for a batch that shrinks: fewer sequences and rows each time, split more, in the same scratch."""
+    contexts, drafts = [700, 30, 2000, 411, 0, 1500], [5, 1, 9, 3, 8, 2]
+    node = N.TreeAttention(6, 28, 9, 8, 2, 128, 16, 200, 3200, 128 ** -0.5)
+    for n in (6, 5, 3, 2, 1):
+        c = build(8, 2, 128, 16, contexts[:n], drafts[:n], 70, width=200)
+        out = torch.full((len(c["q"]), 8, 128), 7.0, dtype=torch.float16, device="cuda")
+        node(out, c["q"].cuda(), c["kc"].cuda(), c["vc"].cuda(), i32(c["table"]), i32(c["lens"]), i32(c["starts"]),
+             signed(c["masks"]).cuda())
+        check(out, c)

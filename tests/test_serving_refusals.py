@@ -245,3 +245,25 @@ def test_tree_attention_refuses_contexts_past_its_integers():
         a = tree(max_context_len=ctx, max_blocks_per_seq=1 << 27)
         assert status(N.lib().tlh_tree_attention_scratch_bytes, C.byref(a), C.byref(n))[0] == want
     assert status(N.lib().tlh_tree_attention, C.byref(a), P, BIG, None)[0] == "INVALID"
+
+
+def test_a_tree_node_takes_smaller_calls_and_refuses_larger_ones():
+    kc, vc = rows(5, 2, 8, 16, 8), rows(5, 2, 64, 16)
+    node = N.TreeAttention(3, 10, 8, 8, 2, 64, 16, 4, 64, 0.1, device="cpu")
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+
+    def call(n, seqs, **kw):
+        a = dict(out=rows(n, 8, 64), q=rows(n, 8, 64), k_cache=kc, v_cache=vc, block_tables=i32(seqs, 4),
+                 context_lens=i32(seqs), draft_starts=i32(seqs + 1), draft_masks=torch.zeros(n, dtype=torch.int64))
+        node(**{**a, **kw})
+
+    for n, seqs in ((10, 3), (7, 3), (10, 1), (1, 1), (0, 3), (0, 0)):
+        with pytest.raises(ValueError, match="on the GPU"):  # everything before that fits
+            call(n, seqs)
+    for n, seqs in ((11, 3), (10, 4)):
+        with pytest.raises(ValueError, match="up to"):
+            call(n, seqs)
+    for name, bad in (("q", rows(6, 8, 64)), ("draft_masks", torch.zeros(8, dtype=torch.int64)), ("context_lens", i32(3)),
+                      ("draft_starts", i32(2)), ("block_tables", i32(2, 3))):
+        with pytest.raises(ValueError, match=name):
+            call(7, 2, **{name: bad})
