@@ -527,6 +527,13 @@ def _extent(t) -> int:
     return t.shape[0] if t.dim() else 0
 
 
+def _int32(value, name: str) -> int:
+    """A count as the calls take it: ctypes would cut a larger one to 32 bits without a word."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} {value} does not fit 32 bits")
+    return value
+
+
 def _current(device) -> int:
     """current_stream's number, without the 2.7 us its Stream object takes."""
     import torch
@@ -633,7 +640,7 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     if n < 1:
         raise ValueError("seq_starts must hold at least one start")
     a.type = F16 if dtype == torch.float16 else BF16
-    a.num_seqs, a.num_tokens, a.max_seq_len = n - 1, tokens, max_seq_len
+    a.num_seqs, a.num_tokens, a.max_seq_len = n - 1, _int32(tokens, "tokens"), _int32(max_seq_len, "max_seq_len")
     a.num_heads, a.num_kv_heads, a.head_size, a.scale = heads, kv, hs, scale
     with _on(dev, stream) as s:
         if fresh:
@@ -685,9 +692,12 @@ class TreeAttention(_ScratchNode):
     def __init__(self, num_seqs, num_rows, max_drafts, num_heads, num_kv_heads, head_size, block_size,
                  max_blocks_per_seq, max_context_len, scale, device="cuda"):
         a = self.args = TlhTreeArgs()
-        a.num_seqs, a.num_rows, a.max_drafts = num_seqs, num_rows, max_drafts
-        a.num_heads, a.num_kv_heads, a.head_size, a.block_size = num_heads, num_kv_heads, head_size, block_size
-        a.max_blocks_per_seq, a.max_context_len, a.scale = max_blocks_per_seq, max_context_len, scale
+        counts = dict(num_seqs=num_seqs, num_rows=num_rows, max_drafts=max_drafts, num_heads=num_heads,
+                      num_kv_heads=num_kv_heads, head_size=head_size, block_size=block_size,
+                      max_blocks_per_seq=max_blocks_per_seq, max_context_len=max_context_len)
+        for name, value in counts.items():
+            setattr(a, name, _int32(value, name))
+        a.scale = scale
         n = C.c_size_t()
         check(lib().tlh_tree_attention_scratch_bytes(C.byref(a), C.byref(n)))
         self._allocate(n.value, device)
@@ -763,7 +773,7 @@ class KVPools:
         another pair's destination or any pair's source; a pair outside the pools does nothing."""
         import torch
 
-        n = _extent(pairs)
+        n = _int32(_extent(pairs), "pairs")
         p = _tensor(pairs, torch.int64, (n, 2), "pairs", self.device)
         with _on(self.device, stream) as s:
             check(lib().tlh_copy_blocks(self._all, 2 * self.layers, self.block_bytes, self.num_blocks, p, n, s))
@@ -781,7 +791,8 @@ class KVPools:
         a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
         a.keep = _tensor(keep, torch.int64, (S,), "keep", dev)
         a.new_lens = _tensor(new_lens, torch.int32, (S,), "new_lens", dev)
-        a.num_blocks, a.num_layers, a.num_seqs, a.max_drafts = self.num_blocks, self.layers, S, max_drafts
+        a.num_blocks, a.num_layers, a.num_seqs = self.num_blocks, self.layers, S
+        a.max_drafts = _int32(max_drafts, "max_drafts")
         a.num_kv_heads, a.head_size, a.block_size = self.kv_heads, self.head_size, self.block_size
         a.max_blocks_per_seq = width
         with _on(dev, stream) as s:
@@ -798,7 +809,8 @@ class TokenLogprobs(_ScratchNode):
 
         self.rows, self.vocab, self.dtype = rows, vocab, dtype or torch.float32
         a = self.args = TlhLogprobsArgs()
-        a.type, a.rows, a.vocab, a.top = _ggml_type(torch.empty(0, dtype=self.dtype)), rows, vocab, top
+        a.type = _ggml_type(torch.empty(0, dtype=self.dtype))
+        a.rows, a.vocab, a.top = _int32(rows, "rows"), _int32(vocab, "vocab"), _int32(top, "top")
         a.row_stride = vocab
         n = C.c_size_t()
         check(lib().tlh_token_logprobs_scratch_bytes(C.byref(a), C.byref(n)))

@@ -267,3 +267,27 @@ def test_a_tree_node_takes_smaller_calls_and_refuses_larger_ones():
                       ("draft_starts", i32(2)), ("block_tables", i32(2, 3))):
         with pytest.raises(ValueError, match=name):
             call(7, 2, **{name: bad})
+
+
+@pytest.mark.parametrize("more", [1 << 31, (1 << 32) + 4, -(1 << 32) + 4])
+def test_counts_past_32_bits_are_refused(more):
+    """Cut to 32 bits most of these would be a count that fits."""
+    q, k, starts = rows(4, 8, 64), rows(4, 2, 64), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="max_seq_len .* 32 bits"):
+        N.packed_attention(q, k, k, starts, more, 0.1)
+    names = ("num_seqs", "num_rows", "max_drafts", "num_heads", "num_kv_heads", "head_size", "block_size",
+             "max_blocks_per_seq", "max_context_len")
+    good = dict(zip(names, (1, 3, 3, 8, 2, 64, 16, 4, 64)))
+    N.TreeAttention(**good, scale=0.1, device="cpu")
+    for name in names:
+        with pytest.raises(ValueError, match=f"{name} .* 32 bits"):
+            N.TreeAttention(**{**good, name: more}, scale=0.1, device="cpu")
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    pools = N.KVPools([rows(5, 2, 8, 16, 8)], [rows(5, 2, 64, 16)], 2, 64, 16)
+    with pytest.raises(ValueError, match="max_drafts .* 32 bits"):
+        pools.compact(i32(1, 4), i32(1), i32(2), torch.zeros(1, dtype=torch.int64), i32(1), more)
+    for at, name in enumerate(("rows", "vocab", "top")):
+        args = [2, 100, 3]
+        args[at] = more
+        with pytest.raises(ValueError, match=f"{name} .* 32 bits"):
+            N.TokenLogprobs(*args, torch.float32, device="cpu")
