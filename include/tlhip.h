@@ -334,7 +334,8 @@ tlh_status tlh_reshape_and_cache(const void *key, const void *value, void *k_cac
  * decreasing; a sequence may be empty):
  *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (num_heads / num_kv_heads)]) v[j, ..]
  * over the tokens j <= t of t's sequence. Scores, softmax and sums are f32; the
- * softmax's numerators are rounded to the type for the product with v, the
+ * softmax's numerators are rounded to the type for the product with v (in f16
+ * those below 2^-21 of the row's largest change by up to 2^-32 of it), the
  * result once. A token sees nothing of the ones it does not attend to, whatever
  * they hold (infinities and NaN too). Tokens behind the last sequence, and a
  * sequence's tokens from max_seq_len on, are left as they were; starts outside
@@ -376,7 +377,8 @@ tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream
  *                sequence's drafted token j (its ancestors and itself)
  * With L = context_lens[s], every row sees the tokens before L - n, and drafted
  * token j at place L - n + j where its mask says so. f32 scores, softmax and
- * sums, its numerators rounded to f16 for the product with v; a row that sees
+ * sums, its numerators rounded to f16 for the product with v (those below 2^-21
+ * of the row's largest change by up to 2^-32 of it); a row that sees
  * nothing gives zeros, and what a row does not see does not reach it, whatever
  * it holds. num_blocks is the pools' length in blocks: tokens of a page
  * outside it are not seen. Lengths are bounded by max_context_len (at most

@@ -8,6 +8,8 @@
 // keys {16 i + 8 (e / 4) + 4 h + e % 4}, e < 8.
 #pragma once
 
+#include <algorithm>
+
 #include "kernels.hpp"
 
 namespace tlh {
@@ -25,6 +27,15 @@ template <bool BF> __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f3
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+// A softmax's numerators in f16 have their reference 7 (of an exponent of 2) below the
+// maximum that set it, so that maximum's own is 2^7, and none is above 2^15, half of f16's
+// range, as the reference lags by no more than 8. What f16 rounds to 0, or to a multiple of
+// its smallest number 2^-24, is then off by at most 2^-32 of the largest a key: 2^-15 over
+// 131072 keys, not the 2^-8 of numerators that begin at 1.
+constexpr float F16_LIFT = 7.0f;
+// ... in scores (finite where the scale nearly vanishes and no numerator does)
+inline float f16_lift(float cs) { return std::min(F16_LIFT / cs, 1e30f); }
 
 // eight f32 rounded to nearest even
 template <bool BF> __device__ __forceinline__ uint4 pack8(const float (&p)[8]) {

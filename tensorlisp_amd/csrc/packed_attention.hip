@@ -27,8 +27,8 @@
 // (4000 tokens, 16/8 heads) 256 us, 510.
 //
 // The softmax is lazy: the exponents' reference moves only when a row's maximum
-// has grown by more than 2^8, so the numerators stay below 2^8 (inside f16) and
-// most tiles rescale nothing; it does not change the quotient.
+// has grown by more than 2^8, so most tiles rescale nothing. In f16 it is set below
+// the maximum (F16_LIFT): numerators of up to 2^15. It does not change the quotient.
 #include <algorithm>
 
 #include "mfma32.hpp"
@@ -58,6 +58,7 @@ struct PkArgs {
     int64_t so, sq, sk, sv;  // bytes from token to token
     int S, tokens, max_len, G, gw, HG, levels;
     float cs;             // |scale| * log2(e); 1 where the scale is 0
+    float lift;           // how far below the maximum the exponents' reference is set, in scores
     uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
 
@@ -160,10 +161,11 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[b][i]);
         mx = max_halves(mx);
-        const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f);
+        const bool grow = mx > m && !((mx - m) * a.cs <= (BF ? 8.0f : 8.0f + F16_LIFT));
         if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float alpha = grow ? __builtin_amdgcn_exp2f((m - mx) * a.cs) : 1.0f;
-            m = grow ? mx : m;
+            const float ref = BF ? mx : mx - a.lift;
+            const float alpha = grow ? __builtin_amdgcn_exp2f((m - ref) * a.cs) : 1.0f;
+            m = grow ? ref : m;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < NB; ++d)
@@ -304,6 +306,7 @@ tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream
     const int qpw = 32 * (4 / p.gw);
     p.levels = (p.max_len - 1) / qpw + 1;
     p.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * PK_LOG2E;
+    p.lift = f16_lift(p.cs);
     p.qand = a.scale == 0.0f ? 0u : ~0u, p.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
     if ((int64_t)p.levels * p.HG >= 1 << 24)  // x 256 threads
         return set_error(TLH_INVALID, "packed_attention: max_seq_len x num_heads too large for one launch");

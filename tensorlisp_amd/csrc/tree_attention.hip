@@ -52,6 +52,7 @@ struct TaArgs {
     int S, H, KV, G, rows, max_drafts, max_blocks, max_ctx, P, part_len, RB;  // RB: blocks of 32 rows
     int sort;  // sequences go longest first
     float cs;             // |scale| * log2(e); 1 where the scale is 0
+    float lift;           // how far below the maximum the exponents' reference is set, in scores
     uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
 
@@ -214,10 +215,11 @@ template <int D, int BS> struct TaWave {
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[u][i]);
         mx = max_halves(mx);
         // the reference moves only when the maximum has grown by more than 2^8
-        const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f);
+        const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f + F16_LIFT);
         if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float alpha = grow ? __builtin_amdgcn_exp2f((m - mx) * a.cs) : 1.0f;
-            m = grow ? mx : m;
+            const float ref = mx - a.lift;
+            const float alpha = grow ? __builtin_amdgcn_exp2f((m - ref) * a.cs) : 1.0f;
+            m = grow ? ref : m;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < NB; ++d)
@@ -664,6 +666,7 @@ tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch
     t.P = ta_parts(a, t.part_len);
     t.RB = (int)rb;
     t.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
+    t.lift = f16_lift(t.cs);
     t.qand = a.scale == 0.0f ? 0u : ~0u, t.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
     const int64_t blocks = sh ? ta_shared_wgs(a) : (int64_t)t.P * t.S * rb * t.KV;
     t.sort = t.S > 1 && t.S <= 64 && blocks > 2 * device_cus();

@@ -125,3 +125,20 @@ def tables(r, lens, bs, spare=2, width=None):
         t[s, :n] = ids[at:at + n]
         at += n
     return t, blocks
+
+
+def one_large_and_many_tiny(n, D, seed):
+    """k and v (n, D) f16 and the weights' logarithm: with q = (1, 0, ..) and scale 1 every key but the first weighs 2^-25.09
+    of it, which f16 rounds to 0, and carries the values: half of the dims 1 throughout, half normal."""
+    g = torch.Generator().manual_seed(seed)
+    k, v = torch.zeros((n, D), dtype=torch.float16), torch.randn((n, D), generator=g).half()
+    k[0, 0] = 17.390625  # 25.0894 ln 2
+    v[:, :D // 2] = 1.0
+    v[0] = 0.0
+    return k, v
+
+
+def tiny_bound(out, A, d, keys, vmax):
+    """f16, with numerators of at least 2^7 for the largest: those below 2^-14 are off by at most 2^-25, 2^-32 of it."""
+    eps = torch.finfo(torch.float16).eps
+    return (out.abs() + A) * eps / 2 * 1.01 + 2 * d * A + 2.0 ** -32 * keys * vmax + 2.0 ** -24

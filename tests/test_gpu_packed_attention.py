@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from serving_refs import packed_reference
+from serving_refs import attend, one_large_and_many_tiny, packed_reference, tiny_bound
 from tensorlisp_amd import native as N
 
 pytestmark = pytest.mark.gpu
@@ -237,3 +237,17 @@ def test_scales_below_zero_and_zero(gpu):
     check(out, -q, k, v, [0, 150], 0.2)
     out = N.packed_attention(q, k, v, dev([0, 150]), 150, 0.0)
     check(out, q * 0, k, v, [0, 150], 1.0)
+
+
+@pytest.mark.parametrize("n", [5000, 131072])
+def test_weights_below_f16s_smallest(gpu, n):
+    """One key of weight 1 and n - 1 of 2^-25 each, which together are up to 4e-3 of the result."""
+    k, v = one_large_and_many_tiny(n, 64, 20)
+    q = torch.zeros((n, 1, 64), dtype=F16, device="cuda")
+    q[:, :, 0] = 1.0
+    out = N.packed_attention(q, k[:, None].cuda(), v[:, None].cuda(), dev([0, n]), n, 1.0)[:, 0].cpu().double()
+    rows = torch.tensor([1, 700, n // 2, n - 33, n - 1])
+    see = torch.arange(n)[None] <= rows[:, None]
+    want, A, d = attend(q[:5, 0].cpu().double(), k.double(), v.double(), see, 1.0)
+    err, tol = (out[rows] - want).abs(), tiny_bound(want, A, d, n, float(v.abs().max()))
+    assert (err <= tol).all(), float((err / tol).max())

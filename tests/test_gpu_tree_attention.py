@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from serving_refs import chain_masks, pools, random_tree, signed, tables, tree_reference
+from serving_refs import (attend, chain_masks, one_large_and_many_tiny, pools, random_tree, signed, tables, tiny_bound,
+                          tree_reference)
 from tensorlisp_amd import native as N
 
 pytestmark = pytest.mark.gpu
@@ -359,3 +360,29 @@ def test_a_node_takes_smaller_calls(gpu):
         node(out, c["q"].cuda(), c["kc"].cuda(), c["vc"].cuda(), i32(c["table"]), i32(c["lens"]), i32(c["starts"]),
              signed(c["masks"]).cuda())
         check(out, c)
+
+
+@pytest.mark.parametrize("n,heads,kv,seqs,drafts", [
+    (131072, 8, 1, 1, 4), (131072, 4, 4, 3, 1), (32768, 64, 32, 16, 64),  # the last in the form of shared tiles
+])
+def test_weights_below_f16s_smallest(gpu, n, heads, kv, seqs, drafts):
+    """One key of weight 1 and n - 1 of 2^-25 each, which together are up to 4e-3 of the result. The sequences share
+    their pages, and the heads their values."""
+    D, bs = 64, 32
+    k, v = one_large_and_many_tiny(n, D, 71)
+    kc = k.view(n // bs, 1, bs, D // 8, 8).transpose(2, 3).expand(-1, kv, -1, -1, -1).cuda().contiguous()
+    vc = v.view(n // bs, 1, bs, D).transpose(2, 3).expand(-1, kv, -1, -1).cuda().contiguous()
+    q = torch.zeros((seqs * drafts, heads, D), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    masks = chain_masks(drafts) * seqs
+    table = np.tile(np.arange(n // bs), (seqs, 1))
+    node = N.TreeAttention(seqs, seqs * drafts, drafts, heads, kv, D, bs, n // bs, n, 1.0)
+    out = node(torch.empty_like(q), q, kc, vc, i32(table), i32([n] * seqs), i32(range(0, seqs * drafts + 1, drafts)),
+               signed(masks).cuda()).cpu().double()
+    see = torch.arange(n)[None] <= n - drafts + torch.arange(drafts)[:, None]
+    want, A, d = attend(q[:drafts, 0].cpu().double(), k.double(), v.double(), see, 1.0)
+    tol = tiny_bound(want, A, d, n, float(v.abs().max()))
+    for s in range(seqs):
+        for h in range(heads):
+            err = (out[s * drafts:(s + 1) * drafts, h] - want).abs()
+            assert (err <= tol).all(), (s, h, float((err / tol).max()))
