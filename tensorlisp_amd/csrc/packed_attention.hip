@@ -28,7 +28,8 @@
 //
 // The softmax is lazy: the exponents' reference moves only when a row's maximum
 // has grown by more than 2^8, so most tiles rescale nothing. In f16 it is set below
-// the maximum (F16_LIFT): numerators of up to 2^15. It does not change the quotient.
+// the maximum (F16_LIFT): numerators of up to 2^15. It does not change the quotient
+// (bf16's sums of products that leave f32's range for it are taken again, smaller).
 #include <algorithm>
 
 #include "mfma32.hpp"
@@ -36,6 +37,7 @@
 namespace tlh {
 
 constexpr float PK_LOG2E = 1.4426950408889634f;
+constexpr float PK_BF_DROP = 40.0f;  // see the careful pass
 
 template <int D> struct PkGeom {
     static constexpr int KT = D <= 128 ? 64 : 32;                 // keys per tile
@@ -58,7 +60,7 @@ struct PkArgs {
     int64_t so, sq, sk, sv;  // bytes from token to token
     int S, tokens, max_len, G, gw, HG, levels;
     float cs;             // |scale| * log2(e); 1 where the scale is 0
-    float lift;           // how far below the maximum the exponents' reference is set, in scores
+    float lift;           // how far below the maximum the exponents' reference is set, in scores (bf16: carefully)
     uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
 
@@ -128,8 +130,12 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
     const int tr_at = (4 * h + tr_key) * CP * 16 + 8 * (lane & 1);
     // A value that is not finite would turn the zero weight of a masked key into NaN.
     // So where a result comes out not finite, the pass is run again, carefully: tiles
-    // with masked keys then add each visible key's product by itself.
+    // with masked keys then add each visible key's product by itself. In bf16, whose
+    // values reach the end of f32's range, the sums of products may also have left it:
+    // the reference is then set 40 above a row's maximum, so that the numerators of 2^31
+    // keys, each below 2^-32, come to less than 1, and no sum to more than the largest value.
     bool careful = false;
+    float lift = BF ? 0.0f : a.lift, top = BF ? 8.0f : 8.0f + F16_LIFT;
 
     auto tile = [&](int t, const uint8_t (&T)[2 * Gm::TILE], uint8_t (&Tn)[2 * Gm::TILE]) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): tile t has landed
@@ -161,9 +167,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[b][i]);
         mx = max_halves(mx);
-        const bool grow = mx > m && !((mx - m) * a.cs <= (BF ? 8.0f : 8.0f + F16_LIFT));
+        const bool grow = mx > -INFINITY && !((mx - m) * a.cs <= top);
         if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float ref = BF ? mx : mx - a.lift;
+            const float ref = mx - lift;
             const float alpha = grow ? __builtin_amdgcn_exp2f((m - ref) * a.cs) : 1.0f;
             m = grow ? ref : m;
             l *= alpha;
@@ -254,6 +260,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_packed_attn(const PkA
         lds_barrier();
         if (!any) break;
         careful = true;
+        if (BF) lift = a.lift, top = 8.0f - PK_BF_DROP;
         int again = 0;
         asm volatile("" : "+s"(again));  // its addresses formed here: kept from the start, they spill
         load_tile(again, T0);
@@ -306,7 +313,7 @@ tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream
     const int qpw = 32 * (4 / p.gw);
     p.levels = (p.max_len - 1) / qpw + 1;
     p.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * PK_LOG2E;
-    p.lift = f16_lift(p.cs);
+    p.lift = a.type == TLH_TYPE_BF16 ? -std::min(PK_BF_DROP / p.cs, 1e30f) : f16_lift(p.cs);
     p.qand = a.scale == 0.0f ? 0u : ~0u, p.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
     if ((int64_t)p.levels * p.HG >= 1 << 24)  // x 256 threads
         return set_error(TLH_INVALID, "packed_attention: max_seq_len x num_heads too large for one launch");

@@ -251,3 +251,38 @@ def test_weights_below_f16s_smallest(gpu, n):
     want, A, d = attend(q[:5, 0].cpu().double(), k.double(), v.double(), see, 1.0)
     err, tol = (out[rows] - want).abs(), tiny_bound(want, A, d, n, float(v.abs().max()))
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("hs", [64, 80, 128, 256])
+def test_bf16_values_near_the_end_of_the_range(gpu, hs):
+    """Sums of the numerators' products with v leave f32's range before they are divided by the numerators' sum."""
+    q, k, v = (t.clone() for t in inputs(4, 2, hs, 330, BF16, 21))
+    v[:200] *= 1e38 / 4  # normal: up to 1e38
+    v[200:] = torch.where(v[200:] < 0, -torch.finfo(BF16).max, torch.finfo(BF16).max)
+    for starts in ([0, 200, 330], [0, 330], [0, 1, 2, 5, 330]):
+        out = N.packed_attention(q, k, v, dev(starts), 330, hs ** -0.5)
+        check(out, q, k, v, starts, hs ** -0.5)
+    q[:], k[:] = 0.0, 0.0  # every key alike
+    v[:] = 2e38
+    out = N.packed_attention(q, k, v, dev([0, 330]), 330, 1.0)
+    check(out, q, k, v, [0, 330], 1.0)
+    v[:] = torch.finfo(BF16).max
+    out = N.packed_attention(q, k, v, dev([0, 330]), 330, 1.0)
+    check(out, q, k, v, [0, 330], 1.0)
+
+
+def test_bf16_large_values_behind_a_lagging_maximum(gpu):
+    """Scores that grow to just below what moves the exponents' reference, 2^8, and values near 2^120."""
+    n, hs = 300, 128
+    q, k, v = (t.clone() for t in inputs(2, 1, hs, n, BF16, 22))
+    q[:], k[:] = 0.0, 0.0
+    q[:, :, 0] = 1.0
+    k[:, :, 0] = torch.linspace(0, 5.5, n, device="cuda")[:, None]  # 2^7.9 at the end
+    v *= 1.5e36
+    v[5] = float("inf")  # some rows see this too, and are not finite
+    out = N.packed_attention(q, k, v, dev([0, n]), n, 1.0)
+    assert not torch.isfinite(out[5:]).any()
+    check(out[:5], q[:5], k[:5], v[:5], [0, 5], 1.0)
+    v[5] = 1e38
+    out = N.packed_attention(q, k, v, dev([0, n]), n, 1.0)
+    check(out, q, k, v, [0, n], 1.0)
