@@ -340,7 +340,8 @@ tlh_status tlh_reshape_and_cache(const void *key, const void *value, void *k_cac
  * they hold (infinities and NaN too). Tokens behind the last sequence, and a
  * sequence's tokens from max_seq_len on, are left as they were; starts outside
  * [0, num_tokens] are taken as the nearer end. Pointers are 16-byte aligned;
- * out must not overlap the inputs. head_size as for paged attention. */
+ * no row of out may overlap one of q, k or v (other columns of the same rows
+ * do not). head_size as for paged attention. */
 typedef struct tlh_packed_attention_args {
     void *out;
     const void *q;

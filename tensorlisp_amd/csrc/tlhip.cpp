@@ -8,6 +8,7 @@
 // N <= 16 -> int8-MFMA few-column kernel, else the GEMM.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -1172,6 +1173,25 @@ static tlh_status check_heads(const char *what, int heads, int kv_heads, int hea
     return TLH_OK;
 }
 
+// whether n rows of a_len bytes every a_step from a and n of b_len every b_step from b (no step
+// shorter than its row) have a byte in common
+static bool rows_overlap(const void *a, int64_t a_step, int64_t a_len, const void *b, int64_t b_step, int64_t b_len,
+                         int64_t n) {
+    const __int128 at = (intptr_t)a, bt = (intptr_t)b;
+    if (at + (__int128)(n - 1) * a_step + a_len <= bt || bt + (__int128)(n - 1) * b_step + b_len <= at) return false;
+    if (a_step == b_step) {  // parts of the same rows, as of a fused projection's
+        const int64_t d = (int64_t)(((bt - at) % a_step + a_step) % a_step);
+        return d < a_len || d + b_len > a_step;
+    }
+    for (int64_t i = 0; i < n; ++i) {  // b's last row that begins before a's i-th ends, and whether it reaches into that
+        const __int128 row = at + (__int128)i * a_step - bt;
+        if (row + a_len <= 0) continue;
+        const __int128 j = std::min<__int128>((row + a_len - 1) / b_step, n - 1);
+        if (j * b_step + b_len > row) return true;
+    }
+    return false;
+}
+
 tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream) {
     if (!a) return set_error(TLH_INVALID, "packed_attention: null args");
     if (a->type != TLH_TYPE_F16 && a->type != TLH_TYPE_BF16)
@@ -1191,6 +1211,10 @@ tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream
     if (!aligned16(a->out) || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) ||
         ((uintptr_t)a->seq_starts & 3))
         return set_error(TLH_INVALID, "packed_attention: tensors must be 16-byte aligned");
+    if (rows_overlap(a->out, 2 * a->out_stride, 2 * qrow, a->q, 2 * a->q_stride, 2 * qrow, a->num_tokens) ||
+        rows_overlap(a->out, 2 * a->out_stride, 2 * qrow, a->k, 2 * a->k_stride, 2 * krow, a->num_tokens) ||
+        rows_overlap(a->out, 2 * a->out_stride, 2 * qrow, a->v, 2 * a->v_stride, 2 * krow, a->num_tokens))
+        return set_error(TLH_INVALID, "packed_attention: out overlaps q, k or v");
     return launch_packed_attention(*a, (hipStream_t)stream);
 }
 

@@ -614,7 +614,8 @@ def packed_attention(q, k, v, seq_starts, max_seq_len: int, scale: float, out=No
     head size), k and v (tokens, kv heads, head size) f16 or bf16, tokens at any
     stride that is a multiple of 8 elements (views of a fused projection),
     seq_starts i32 (sequences + 1,) -> out (tokens, heads, head size). No
-    sequence may be longer than max_seq_len. Tokens behind the last sequence are
+    sequence may be longer than max_seq_len, and `out` must be apart from the
+    others (other columns of one buffer's rows are). Tokens behind the last sequence are
     left as they were in `out` (without one, as the new tensor holds them, and
     `stream` waits for the current stream's work, which may still use its memory)."""
     import torch

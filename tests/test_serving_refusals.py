@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import random
 
 import pytest
 import torch
@@ -291,3 +292,59 @@ def test_counts_past_32_bits_are_refused(more):
         args[at] = more
         with pytest.raises(ValueError, match=f"{name} .* 32 bits"):
             N.TokenLogprobs(*args, torch.float32, device="cpu")
+
+
+def test_packed_attention_out_must_be_apart():
+    """Rows of out that share a byte with rows of q, k or v are told apart from those that lie between them. (Calls
+    that pass are refused behind that, for more workgroups than a launch takes.)"""
+    H, KV, n, base = 32768, 8192, 1 << 16, 1 << 44
+    qrow, krow = 64 * H, 64 * KV  # elements
+
+    def refused(o, q, k, v, so, sq, sk, sv):
+        st, text = status(N.lib().tlh_packed_attention, C.byref(packed(
+            out=base + 2 * o, q=base + 2 * q, k=base + 2 * k, v=base + 2 * v, out_stride=so, q_stride=sq, k_stride=sk,
+            v_stride=sv, num_heads=H, num_kv_heads=KV, num_tokens=n, max_seq_len=n)), None)
+        assert st == "INVALID" and ("overlaps" in text or "too large for one launch" in text), text
+        return "overlaps" in text
+
+    wide, far = 2 * qrow + 2 * krow, 1 << 40
+    # columns of one buffer's rows: q, k, v, out in turn
+    at = dict(q=0, k=qrow, v=qrow + krow, o=qrow + 2 * krow)
+    steps = dict(so=wide, sq=wide, sk=wide, sv=wide)
+    assert not refused(**at, **steps)
+    for name in "qkv":  # any of them, from either side, and whole
+        for by in (8, -8):
+            assert refused(**{**at, "o": at[name] + by}, **steps)
+        assert refused(**{**at, "o": at[name]}, **steps)
+    assert refused(**{**at, "o": at["o"] + 8}, **steps)  # into the next row's q
+    # tensors of their own, one behind the other
+    own = dict(so=qrow, sq=qrow, sk=krow, sv=krow)
+    ends = dict(q=0, o=n * qrow, k=2 * n * qrow, v=2 * n * qrow + n * krow)
+    assert not refused(**ends, **own)
+    for o in (n * qrow - 8, n * qrow + 8):
+        assert refused(**{**ends, "o": o}, **own)
+    # rows at another step than q's, against the bytes
+    r = random.Random(5)
+    seen = set()
+    for _ in range(40):
+        so, sq = qrow * r.choice([2, 3, 4]) + 8 * r.randrange(4), qrow * r.choice([2, 3, 4, 6]) + 8 * r.randrange(4)
+        o, q = r.randrange(0, 4 * qrow, 8), r.randrange(0, 4 * qrow, 8)
+        if r.random() < 0.5:  # between q's rows, as long as the steps are whole multiples
+            so, sq, o, q = 4 * qrow, 2 * qrow, qrow * r.choice([1, 3]), 0
+        want = False
+        j = 0
+        for i in range(n):
+            while j < n and q + j * sq + qrow <= o + i * so:
+                j += 1
+            if j < n and q + j * sq < o + i * so + qrow:
+                want = True
+                break
+        assert refused(o, q, far, far + n * krow, so, sq, krow, krow) == want
+        seen.add(want)
+    assert seen == {True, False}
+
+
+def test_packed_attention_past_one_launch_is_told_as_such():
+    a = packed(num_tokens=2 ** 31 - 1, max_seq_len=2 ** 31 - 1, out=1 << 50)
+    assert status(N.lib().tlh_packed_attention, C.byref(a), None) == (
+        "INVALID", "packed_attention: max_seq_len x num_heads too large for one launch")
