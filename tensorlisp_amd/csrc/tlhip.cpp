@@ -1173,6 +1173,10 @@ static tlh_status check_heads(const char *what, int heads, int kv_heads, int hea
     return TLH_OK;
 }
 
+static bool overlap(const void *a, __int128 a_len, const void *b, __int128 b_len) {
+    return (intptr_t)a < (intptr_t)b + b_len && (intptr_t)b < (intptr_t)a + a_len;
+}
+
 // whether n rows of a_len bytes every a_step from a and n of b_len every b_step from b (no step
 // shorter than its row) have a byte in common
 static bool rows_overlap(const void *a, int64_t a_step, int64_t a_len, const void *b, int64_t b_step, int64_t b_len,
@@ -1255,6 +1259,10 @@ tlh_status tlh_tree_attention(const tlh_tree_attention_args *a, void *scratch, s
         ((uintptr_t)a->draft_masks & 7) ||
         (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens | (uintptr_t)a->draft_starts) & 3))
         return set_error(TLH_INVALID, "tree_attention: q, out and the caches must be 16-byte aligned");
+    const __int128 rows = (__int128)a->num_rows * a->num_heads * a->head_size * 2;
+    const __int128 pool = (__int128)a->num_blocks * a->num_kv_heads * a->head_size * a->block_size * 2;
+    if (overlap(a->out, rows, a->q, rows) || overlap(a->out, rows, a->k_cache, pool) || overlap(a->out, rows, a->v_cache, pool))
+        return set_error(TLH_INVALID, "tree_attention: out overlaps q or the caches");
     const size_t need = tree_attention_scratch_bytes(*a);
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return set_error(TLH_INVALID, "tree_attention: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);

@@ -348,3 +348,21 @@ def test_packed_attention_past_one_launch_is_told_as_such():
     a = packed(num_tokens=2 ** 31 - 1, max_seq_len=2 ** 31 - 1, out=1 << 50)
     assert status(N.lib().tlh_packed_attention, C.byref(a), None) == (
         "INVALID", "packed_attention: max_seq_len x num_heads too large for one launch")
+
+
+def test_tree_attention_out_must_be_apart():
+    """(Calls that pass are refused behind that, for want of scratch.)"""
+    rows, pool, base = 10 * 8 * 128 * 2, 100 * 2 * 128 * 16 * 2, 1 << 40
+    at = dict(q=base, k_cache=base + rows, v_cache=base + rows + pool)
+
+    def refused(out, **kw):
+        a = tree(**{**at, **kw}, out=out, max_context_len=8192, max_blocks_per_seq=512)
+        st, text = status(N.lib().tlh_tree_attention, C.byref(a), None, 0, None)
+        assert st == "INVALID" and ("overlaps" in text or "scratch" in text), text
+        return "overlaps" in text
+
+    assert not refused(base - rows) and not refused(base + rows + 2 * pool)
+    for out in (base - rows + 16, base, base + rows - 16, base + rows, base + rows + pool - 16, base + rows + 2 * pool - 16):
+        assert refused(out), out
+    assert not refused(base + rows + 2 * pool, num_blocks=0) and not refused(base + rows + 16, num_blocks=0)
+    assert refused(base + (1 << 50), num_blocks=1 << 62)
