@@ -431,7 +431,7 @@ tlh_status tlh_copy_blocks(void *const *pools, int32_t num_pools, int64_t block_
  * draft_starts and max_drafts as tlh_tree_attention took them; bit j of
  * keep[s] (i64 [num_seqs]) says that drafted token j of sequence s was
  * accepted. The kept tokens' keys and values move, in order, to the places from
- * L - n on, and new_lens[s] (i32, apart from context_lens) becomes the length
+ * L - n on, and new_lens[s] (i32, apart from what is read) becomes the length
  * with them. The drafted places must lie in pages that no other sequence of
  * the call shares. A move from or to a page outside [0, num_blocks) is left
  * out. k_caches and v_caches are host arrays of num_layers pool addresses in

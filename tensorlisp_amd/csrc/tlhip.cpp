@@ -1297,10 +1297,13 @@ tlh_status tlh_compact_cache(const tlh_compact_cache_args *a, void *stream) {
     if (!a->k_caches || !a->v_caches || !a->context_lens || !a->draft_starts || !a->keep || !a->new_lens ||
         (a->max_blocks_per_seq > 0 && !a->block_tables))
         return set_error(TLH_INVALID, "compact_cache: null pointer");
-    const int32_t *nl = a->new_lens;
-    if ((nl < a->context_lens + a->num_seqs && a->context_lens < nl + a->num_seqs) ||
-        (nl < a->draft_starts + a->num_seqs + 1 && a->draft_starts < nl + a->num_seqs))
-        return set_error(TLH_INVALID, "compact_cache: new_lens must not overlap context_lens or draft_starts");
+    // one workgroup of a sequence writes its new length while others still read what they go by
+    const int64_t S = a->num_seqs, lens = 4 * S;
+    if (overlap(a->new_lens, lens, a->context_lens, lens) || overlap(a->new_lens, lens, a->draft_starts, lens + 4) ||
+        overlap(a->new_lens, lens, a->keep, 8 * S) ||
+        overlap(a->new_lens, lens, a->block_tables, 4 * S * a->max_blocks_per_seq))
+        return set_error(TLH_INVALID,
+                         "compact_cache: new_lens must not overlap context_lens, draft_starts, keep or block_tables");
     if (((uintptr_t)a->keep & 7) || (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens |
                                       (uintptr_t)a->draft_starts | (uintptr_t)a->new_lens) & 3))
         return set_error(TLH_INVALID, "compact_cache: misaligned pointer");

@@ -366,3 +366,19 @@ def test_tree_attention_out_must_be_apart():
         assert refused(out), out
     assert not refused(base + rows + 2 * pool, num_blocks=0) and not refused(base + rows + 16, num_blocks=0)
     assert refused(base + (1 << 50), num_blocks=1 << 62)
+
+
+def test_compact_cache_lengths_must_be_apart_from_all_that_is_read():
+    """(Calls that pass are refused behind that, for a layer without pools.)"""
+    base = 0x100000
+
+    def refused(new_lens, **kw):
+        got = compact(num_seqs=4, new_lens=new_lens, pools=(P, None), **kw)
+        assert got == "INVALID"
+        return "overlap" in N.lib().tlh_last_error().decode()
+
+    for name, size in (("keep", 32), ("block_tables", 64), ("context_lens", 16), ("draft_starts", 20)):
+        for at in (-12, 0, 4, size - 4):
+            assert refused(base + at, **{name: base}), (name, at)
+        for at in (-16, size):
+            assert not refused(base + at, **{name: base}), (name, at)
