@@ -383,10 +383,12 @@ tlh_status tlh_packed_attention(const tlh_packed_attention_args *a, void *stream
  * nothing gives zeros, and what a row does not see does not reach it, whatever
  * it holds. num_blocks is the pools' length in blocks: tokens of a page
  * outside it are not seen. Lengths are bounded by max_context_len (at most
- * 2^30), starts by num_rows, a sequence's rows by max_drafts. out must not
- * overlap the inputs. `scratch` holds the partials of a split context
- * (tlh_tree_attention_scratch_bytes, 16-byte aligned; it may be NULL when that
- * is 0); calls that share one must be stream-ordered. */
+ * 2^30), starts by num_rows. Of a sequence with more than max_drafts rows the
+ * first max_drafts are computed, as if it had no others (n = max_drafts: their
+ * drafted places are the context's last max_drafts), and the rest are left as
+ * they were. out must not overlap the inputs. `scratch` holds the partials of a
+ * split context (tlh_tree_attention_scratch_bytes, 16-byte aligned; it may be
+ * NULL when that is 0); calls that share one must be stream-ordered. */
 typedef struct tlh_tree_attention_args {
     void *out;
     const void *q;

@@ -386,3 +386,24 @@ def test_weights_below_f16s_smallest(gpu, n, heads, kv, seqs, drafts):
         for h in range(heads):
             err = (out[s * drafts:(s + 1) * drafts, h] - want).abs()
             assert (err <= tol).all(), (s, h, float((err / tol).max()))
+
+
+def cut(c, most):
+    """The case of which only the first `most` rows of each sequence are left, and which rows those are."""
+    at = [i for a, b in zip(c["starts"][:-1], c["starts"][1:]) for i in range(a, min(b, a + most))]
+    counts = [min(b - a, most) for a, b in zip(c["starts"][:-1], c["starts"][1:])]
+    return {**c, "q": c["q"][at], "masks": [c["masks"][i] for i in at], "starts": [0] + [int(n) for n in np.cumsum(counts)]}, at
+
+
+@pytest.mark.parametrize("heads,kv,contexts,drafts,most", [
+    (8, 2, [40, 90, 700], [5, 3, 9], 3), (8, 2, [0, 2, 33], [64, 40, 35], 34),
+    (64, 32, [30, 0, 150, 7] * 4, [40, 64, 36, 33] * 4, 35),  # the form of shared tiles
+])
+def test_rows_up_to_max_drafts(gpu, heads, kv, contexts, drafts, most):
+    """A sequence's first max_drafts rows are computed as if it had no others."""
+    c = build(heads, kv, 128, 16, contexts, drafts, 72)
+    out = run(c, max_drafts=most)
+    less, at = cut(c, most)
+    check(out[at], less)
+    rest = [i for i in range(len(out)) if i not in at]
+    assert rest and (out[rest] == 7).all()

@@ -382,3 +382,14 @@ def test_compact_cache_lengths_must_be_apart_from_all_that_is_read():
             assert refused(base + at, **{name: base}), (name, at)
         for at in (-16, size):
             assert not refused(base + at, **{name: base}), (name, at)
+
+
+def test_a_split_contexts_scratch_is_asked_for_and_checked():
+    n = C.c_size_t()
+    a = tree(max_context_len=8192, max_blocks_per_seq=512)
+    assert status(N.lib().tlh_tree_attention_scratch_bytes, C.byref(a), C.byref(n))[0] == "OK"
+    assert n.value > 0
+    a.out = 1 << 40
+    for scratch, nbytes in ((P, n.value - 1), (None, n.value), (P + 8, n.value)):
+        st, text = status(N.lib().tlh_tree_attention, C.byref(a), scratch, nbytes, None)
+        assert st == "INVALID" and "scratch" in text
