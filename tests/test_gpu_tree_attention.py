@@ -407,3 +407,51 @@ def test_rows_up_to_max_drafts(gpu, heads, kv, contexts, drafts, most):
     check(out[at], less)
     rest = [i for i in range(len(out)) if i not in at]
     assert rest and (out[rest] == 7).all()
+
+
+def spoil(c, s, drafted, bad):
+    """Makes drafted token `drafted` of sequence s not finite -> the rows that see it."""
+    bs, n = c["vc"].shape[3], c["starts"][s + 1] - c["starts"][s]
+    p = c["lens"][s] - n + drafted
+    c["kc"][c["table"][s, p // bs], :, :, p % bs] = bad
+    c["vc"][c["table"][s, p // bs], :, :, p % bs] = bad
+    return [i for i in range(c["starts"][s], c["starts"][s + 1]) if c["masks"][i] >> drafted & 1]
+
+
+def check_spoilt(out, c, hit):
+    assert hit
+    check(out, c, [i for i in range(c["starts"][-1]) if i not in hit])
+    assert not torch.isfinite(out[hit]).all(-1).any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+@pytest.mark.parametrize("hs,bs", [(64, 8), (64, 32), (80, 16), (96, 32), (112, 8), (128, 32), (192, 16), (256, 8), (256, 32)])
+def test_many_rows_of_any_size_and_what_they_do_not_see(gpu, hs, bs, bad):
+    """The shared tiles' careful pass in its other geometries: 32-key tiles above 128 dims, dims repeated in the last
+    block, pages smaller and larger than 16 tokens."""
+    c = shared_case(hs, bs, 73 + hs)
+    hit = spoil(c, 0, 4, bad) + spoil(c, 3, 40, bad)
+    check_spoilt(run(c), c, hit)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv,hs,bs,contexts,drafts", [
+    (8, 2, 128, 16, [2000], [9]), (8, 2, 64, 8, [900, 3000], [6, 20]), (4, 2, 80, 32, [1500], [40]),
+    (8, 1, 192, 8, [1111], [12]), (4, 1, 256, 16, [700, 2500], [7, 33]), (4, 4, 112, 32, [130, 5000], [5, 64]),
+])
+def test_split_contexts_and_what_is_not_seen(gpu, heads, kv, hs, bs, contexts, drafts, bad):
+    """Own tiles over several partitions: the last one is taken carefully, the merge joins it to the others."""
+    c = build(heads, kv, hs, bs, contexts, drafts, 74)
+    hit = [i for s, n in enumerate(drafts) for i in spoil(c, s, n // 2, bad)]
+    check_spoilt(run(c), c, hit)
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (64, 32)])
+def test_pages_outside_and_values_not_finite(gpu, heads, kv):
+    """A page outside the pools in the middle of a context (its tile is taken as masked) whose neighbours are not finite:
+    those are seen by every row of the sequence, and by no other sequence."""
+    c = build(heads, kv, 64, 8, [300, 200] * 8, [40, 36] * 8, 75)
+    c["vc"][c["table"][0, 4], :, :, 3] = float("inf")
+    c["table"][0, 5] = -1
+    hit = list(range(40))
+    check_spoilt(run(c), c, hit)
