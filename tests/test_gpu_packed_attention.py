@@ -286,3 +286,16 @@ def test_bf16_large_values_behind_a_lagging_maximum(gpu):
     v[5] = 1e38
     out = N.packed_attention(q, k, v, dev([0, n]), n, 1.0)
     check(out, q, k, v, [0, n], 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv,hs", [(4, 2, 64), (5, 5, 80), (4, 1, 96), (6, 2, 112), (8, 2, 192), (3, 1, 256)])
+def test_later_tokens_reach_nothing_at_any_size(gpu, heads, kv, hs, bad, dtype):
+    """The careful pass where rows hold 8, 16 or 32 chunks and dims are repeated, with 1, 2 and 4 heads a workgroup."""
+    q, k, v = (t.clone() for t in inputs(heads, kv, hs, 210, dtype, 23))
+    k[57], v[57], v[161] = bad, bad, bad
+    out = N.packed_attention(q, k, v, dev([0, 100, 210]), 110, hs ** -0.5)
+    for a, b, first in ((0, 100, 57), (100, 210, 161)):
+        check(out[a:first], q[a:first], k[a:first], v[a:first], [0, first - a], hs ** -0.5)
+        assert not torch.isfinite(out[first:b]).all(-1).any()
