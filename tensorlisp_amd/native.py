@@ -584,8 +584,9 @@ def _behind_current(stream, device):
 
     if stream is None:
         return None
-    side = _torch_stream(stream, device)
-    side.wait_stream(torch.cuda.current_stream(device))
+    side, current = _torch_stream(stream, device), torch.cuda.current_stream(device)
+    if side != current:
+        side.wait_stream(current)
     return side
 
 

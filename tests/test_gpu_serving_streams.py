@@ -94,14 +94,18 @@ def test_views_that_the_default_stream_is_still_to_fill(busy):
     assert torch.equal(out, want)
 
 
-def tree_node():
-    """The partials of 1024 workgroups: 8 sequences x 2 kv heads in 64 partitions."""
+def tree_inputs():
     q, kc, vc = normal(7, 64, 8, 128), normal(8, 8 * 513, 2, 16, 16, 8), normal(9, 8 * 513, 2, 128, 16)
     table = torch.randperm(8 * 513, device="cuda", dtype=torch.int32).view(8, 513)
-    args = (q, kc, vc, table, i32(*[8200 - 100 * i for i in range(8)]), i32(*range(0, 65, 8)),
+    return (q, kc, vc, table, i32(*[8200 - 100 * i for i in range(8)]), i32(*range(0, 65, 8)),
             torch.tensor([(1 << (i % 8 + 1)) - 1 for i in range(64)], device="cuda"))
+
+
+def tree_node():
+    """The partials of 1024 workgroups: 8 sequences x 2 kv heads in 64 partitions."""
+    args = tree_inputs()
     return (lambda: N.TreeAttention(8, 64, 8, 8, 2, 128, 16, 513, 8208, 0.1),
-            lambda node, outs, stream: node(outs[0], *args, stream=stream), [torch.empty_like(q)])
+            lambda node, outs, stream: node(outs[0], *args, stream=stream), [torch.empty_like(args[0])])
 
 
 def logprobs_node():
@@ -178,3 +182,33 @@ def test_a_node_captured_before_any_call(gpu, case):
         call(node, other, s)
         s.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+def tree_one_call():
+    args = tree_inputs()
+    return lambda stream=None: (N.tree_attention(*args, 8, 8208, 0.1, stream=stream),)
+
+
+@pytest.mark.parametrize("where", ["current", "number", "forked"])
+@pytest.mark.parametrize("case", [packed_case, logprobs_case, tree_one_call])
+def test_one_call_forms_captured(gpu, case, where):
+    """On the capture's own stream, given as itself or by number, and on one that the capture forks to."""
+    call = case()
+    want = call()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        if where == "forked":
+            side.wait_stream(here)
+            got = call(side)
+            here.wait_stream(side)
+        else:
+            got = call(here if where == "current" else here.cuda_stream)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
