@@ -21,10 +21,10 @@
 // and with 8 kv heads a head's stay in one XCD's L2. (By position first, which
 // ends more evenly, 16 prompts of 100..2000 took 400 us instead of 300.)
 //
-// Measured: one prompt of 8191 tokens, 32/8 heads of 128, bf16, 571 to 608 us, 900 to 960
+// Measured: one prompt of 8191 tokens, 32/8 heads of 128, bf16, 559 to 608 us, 900 to 980
 // TFLOP/s (a library product of 8192^3 reaches 1145 on this card); 16 prompts of
-// 100..2000 264 to 279 us, 690 TFLOP/s; heads of 64 (8191 tokens) 346 us, 790; of 256
-// (4000 tokens, 16/8 heads) 256 us, 510.
+// 100..2000 264 to 279 us, 690 TFLOP/s, in any order of their lengths; heads of 64 (8191
+// tokens) 334 to 353 us, 780 to 820; of 256 (4000 tokens, 16/8 heads) 252 us, 520.
 //
 // The softmax is lazy: the exponents' reference moves only when a row's maximum
 // has grown by more than 2^8, so most tiles rescale nothing. In f16 it is set below

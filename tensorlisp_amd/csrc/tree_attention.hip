@@ -30,7 +30,8 @@
 //
 // Measured, 32/8 heads of 128: 32 trees of 1..8 tokens over 512..8192 127 us (4.5 TB/s);
 // 16 of 63 over 512..4096 84 to 89 us; 32 of 64 over 4096 200 to 217 us (shared tiles, 640
-// to 700 TFLOP/s); 1 of 7 over 600 11 to 12 us in two launches.
+// to 700 TFLOP/s); 1 of 7 over 600 10 to 12 us in two launches. These are of nodes made for
+// the longest context; made for 131072 tokens the first takes 5% more, the last 3 us.
 #include <algorithm>
 
 #include "mfma32.hpp"
