@@ -3,9 +3,10 @@
  * hot path: GGML_OP_MUL_MAT over GGUF block-quantized weights (Q8_0, Q4_0,
  * Q4_K, Q5_K, Q6_K; decode GEMV for N <= 16 columns, MFMA GEMM for prefill),
  * paged-attention decode over an f16 block-table KV cache, dense
- * GGML_OP_FLASH_ATTN_EXT over f16 K/V, and what a server that drafts tokens
- * needs beside them (packed prompts, drafted trees, page moves, log
- * probabilities).
+ * GGML_OP_FLASH_ATTN_EXT over f16 K/V, and what a server that mixes prompts,
+ * single and drafted tokens needs beside them (packed prompts, pieces of prompts
+ * over pages, drafted trees, heads' norms and rotation with the cache write,
+ * page moves, log probabilities, verification of drafts).
  *
  * This is the surface a `native-hip` feature binds from Rust
  * (crates/kernels/src/hip/ + crates/tensorlisp/src/native_hip.rs), in place of
@@ -488,6 +489,171 @@ typedef struct tlh_token_logprobs_args {
 
 tlh_status tlh_token_logprobs_scratch_bytes(const tlh_token_logprobs_args *a, size_t *bytes);
 tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, size_t scratch_bytes, void *stream);
+
+/* ------------------------------------------------------- chunk attention
+ * Causal attention of the sequences' new tokens over the paged cache: one token
+ * of a sequence that decodes, or any number of a prompt that comes in pieces or
+ * follows a cached prefix, mixed in one call. No counterpart in the reference.
+ * Layouts and geometry as for paged attention, the new tokens' keys and values
+ * already written to the cache as the last of context_lens:
+ *   q, out       f16 [num_rows][num_heads][head_size], a token's heads contiguous,
+ *                q_stride and out_stride elements from token to token (multiples of 8)
+ *   row_starts   i32 [num_seqs + 1]: sequence s has the rows row_starts[s] ..
+ *                row_starts[s + 1] - 1, n of them, at most max_rows; rows behind the
+ *                last sequence are left as they were
+ * With L = context_lens[s], row i of the sequence is the token at place L - n + i and
+ * sees the tokens up to itself, with window > 0 the last `window` of them. f32 scores,
+ * softmax and sums, its numerators rounded to f16 for the product with v (those below
+ * 2^-21 of the row's largest change by up to 2^-32 of it); a row that sees nothing (a
+ * place below 0, pages that are not there) gives zeros, and what a row does not see does
+ * not reach it, whatever it holds. num_blocks is the pools' length in blocks: tokens
+ * of a page outside it are not seen. Lengths are bounded by max_context_len (at most
+ * 2^30), starts by num_rows. Of a sequence with more than max_rows rows the first
+ * max_rows are computed, as if it had no others, and the rest are left as they were.
+ * No row of out may overlap a row of q (other columns of the same rows do not) or the
+ * caches. `scratch` holds the partials of split contexts (tlh_chunk_attention_scratch_bytes,
+ * which never shrinks as a count grows, 16-byte aligned; it may be NULL when that is
+ * 0); calls that share one must be stream-ordered. */
+typedef struct tlh_chunk_attention_args {
+    void *out;
+    const void *q;
+    const void *k_cache;
+    const void *v_cache;
+    const int32_t *block_tables;
+    const int32_t *context_lens;
+    const int32_t *row_starts;
+    int64_t out_stride;
+    int64_t q_stride;
+    int64_t num_blocks;
+    int32_t num_seqs;
+    int32_t num_rows;
+    int32_t max_rows;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_size;
+    int32_t block_size;
+    int32_t max_blocks_per_seq;
+    int32_t max_context_len;
+    int32_t window;
+    float scale;
+} tlh_chunk_attention_args;
+
+tlh_status tlh_chunk_attention_scratch_bytes(const tlh_chunk_attention_args *a, size_t *bytes);
+tlh_status tlh_chunk_attention(const tlh_chunk_attention_args *a, void *scratch, size_t scratch_bytes, void *stream);
+
+/* ------------------------------------------------------------- head rope
+ * What lies between the Q, K, V projections and attention, in one pass: the norms
+ * of the query and key heads, their rotation by the tokens' positions, and the
+ * write of keys and values to the paged cache. No counterpart in the reference,
+ * which runs RMS_NORM, ROPE and the cache write as nodes of their own.
+ *   q      [num_tokens][num_heads][head_size], k, v [num_tokens][num_kv_heads][head_size],
+ *          of `type` (f32, f16 or bf16), a token's heads contiguous, *_stride elements
+ *          from token to token
+ *   q_norm, k_norm  f32 [head_size] or NULL: a head x becomes
+ *          x / sqrt(mean(x^2) + eps) * norm
+ *   then its first n_dims dims are rotated in pairs (mode 0: 2p and 2p + 1, mode 2:
+ *          p and p + n_dims / 2, as TLH_CORE_ROPE): pair p by the angle
+ *          positions[pair_axis[p]][token] * freqs[p], cos and sin times attn_factor;
+ *          positions i32 [num_axes][num_tokens] (1 axis: text; 2 to 4: images, video),
+ *          freqs f32 [n_dims / 2]; n_dims 0 rotates nothing. The angle is formed and
+ *          reduced in 64 bits, so far positions keep their fraction.
+ *   q_out  out_type (f16 or bf16) [num_tokens][num_heads][head_size]; k_out and v_out
+ *          alike, each may be NULL: rounded once from f32
+ *   k_cache, v_cache, slots: all NULL, or (out_type f16) the pools of
+ *          tlh_reshape_and_cache and each token's slot there, num_blocks blocks long; a
+ *          negative slot or one past the pools writes nothing; slots must differ
+ * head_size as for paged attention; tensors 16-byte aligned, strides multiples of 16
+ * bytes. No output may overlap an input or another output (columns of the same
+ * rows that differ do not). */
+typedef struct tlh_head_rope_args {
+    const void *q;
+    const void *k;
+    const void *v;
+    const int32_t *positions;
+    const float *freqs;
+    const float *q_norm;
+    const float *k_norm;
+    void *q_out;
+    void *k_out;
+    void *v_out;
+    void *k_cache;
+    void *v_cache;
+    const int64_t *slots;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t q_out_stride;
+    int64_t k_out_stride;
+    int64_t v_out_stride;
+    int64_t num_blocks;
+    int32_t type;
+    int32_t out_type;
+    int32_t num_tokens;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_size;
+    int32_t block_size;
+    int32_t n_dims;
+    int32_t mode;
+    int32_t num_axes;
+    float eps;
+    float attn_factor;
+    uint8_t pair_axis[128];
+} tlh_head_rope_args;
+
+tlh_status tlh_head_rope(const tlh_head_rope_args *a, void *stream);
+
+/* ---------------------------------------------------------- draft verify
+ * Verification of drafted tokens against the model's probabilities from given random
+ * numbers, so that what is answered is distributed as the model alone would have it
+ * (a chain of drafts a sequence). No counterpart in the reference.
+ *   target  logits (f32, f16 or bf16) [num_drafts + num_seqs][vocab]: sequence s with
+ *           the drafted tokens b = draft_starts[s] .. draft_starts[s + 1] - 1, n of
+ *           them, at most max_drafts, has the rows b + s .. b + s + n: row b + s + i is
+ *           what the model says at the place of its draft i, the last one behind them
+ *   draft   logits of the drafting model, same type [num_drafts][vocab], or NULL where
+ *           tokens were proposed outright (copied from the prompt): q is then 1 at them
+ *   p, q    softmax(logits / temperatures[s]); a temperature that is not above 0 is
+ *           greedy: p is 1 at the largest logit, the lowest index among equal ones,
+ *           that token alone is accepted, and the drafter's logits are not looked at
+ * Draft i with token x is accepted if accept_at[b + i] * q(x) < p(x) and those before it
+ * are; accept_probs[b + i] = min(1, p(x) / q(x)) (NULL: not wanted; p(x) > 0 where q(x)
+ * is 0). accepted[s] counts them. The next token is drawn from what p has above q at the first one
+ * refused (from p where that is nothing), or from the row behind the drafts: the
+ * lowest index where the running sum exceeds sample_at[s] times the whole (the last with
+ * a weight above 0 where none does). out_tokens[s], i32 [max_drafts + 1], receives the
+ * accepted ones, this one, and -1 behind them. All of it is computed in 64 bits: a running sum over
+ * a vocabulary decides between neighbours that f32 cannot tell apart.
+ * Logits may be -inf (a mask). A row with a NaN, with +inf at a temperature above 0, or
+ * with nothing but -inf is no distribution: a draft that needs it is refused (accept
+ * probability NaN), and a token that would be drawn from it is -1. A token outside
+ * [0, vocab) has p = q = 0. Of a sequence with more than max_drafts drafts the first max_drafts are
+ * looked at, as if it had no others. Row strides in elements, any alignment of the type;
+ * vocab <= 1000000, max_drafts <= 1024. `scratch` (16-byte aligned) holds the rows'
+ * sums; calls that share one must be stream-ordered. The outputs must not overlap the
+ * inputs or each other. */
+typedef struct tlh_draft_verify_args {
+    const void *target;
+    const void *draft;
+    const int32_t *tokens;
+    const int32_t *draft_starts;
+    const float *temperatures;
+    const float *accept_at;
+    const float *sample_at;
+    int32_t *accepted;
+    int32_t *out_tokens;
+    float *accept_probs;
+    int64_t target_stride;
+    int64_t draft_stride;
+    int32_t type;
+    int32_t num_seqs;
+    int32_t num_drafts;
+    int32_t max_drafts;
+    int32_t vocab;
+} tlh_draft_verify_args;
+
+tlh_status tlh_draft_verify_scratch_bytes(const tlh_draft_verify_args *a, size_t *bytes);
+tlh_status tlh_draft_verify(const tlh_draft_verify_args *a, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------------------ executor
  * A graph of ggml nodes compiled once into a recorded list of launches on this

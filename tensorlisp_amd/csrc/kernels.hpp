@@ -408,6 +408,11 @@ tlh_status launch_reshape_and_cache(const void *key, const void *value, void *k_
 tlh_status launch_packed_attention(const tlh_packed_attention_args &a, hipStream_t stream);
 size_t tree_attention_scratch_bytes(const tlh_tree_attention_args &a);
 tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch, hipStream_t stream);
+size_t chunk_attention_scratch_bytes(const tlh_chunk_attention_args &a);
+tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scratch, hipStream_t stream);
+tlh_status launch_head_rope(const tlh_head_rope_args &a, hipStream_t stream);
+size_t draft_verify_scratch_bytes(const tlh_draft_verify_args &a);
+tlh_status launch_draft_verify(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream);
 tlh_status launch_copy_blocks(void *const *pools, int num_pools, int64_t block_bytes, int64_t num_blocks,
                               const int64_t *pairs, int num_pairs, hipStream_t stream);
 tlh_status launch_compact_cache(const tlh_compact_cache_args &a, hipStream_t stream);

@@ -1269,6 +1269,204 @@ tlh_status tlh_tree_attention(const tlh_tree_attention_args *a, void *scratch, s
     return launch_tree_attention(*a, scratch, (hipStream_t)stream);
 }
 
+static tlh_status check_chunk(const tlh_chunk_attention_args *a) {
+    if (!a) return set_error(TLH_INVALID, "chunk_attention: null args");
+    const tlh_status st = check_heads("chunk_attention", a->num_heads, a->num_kv_heads, a->head_size);
+    if (st != TLH_OK) return st;
+    if (!paged_block_size(a->block_size))
+        return set_error(TLH_INVALID, "chunk_attention: unsupported block_size %d (have 8, 16, 32)", a->block_size);
+    if (a->num_seqs < 0 || a->num_seqs > 65535 || a->num_rows < 0 || a->max_rows < 0 || a->num_blocks < 0 ||
+        a->max_blocks_per_seq < 0 || a->max_context_len < 0 || a->window < 0)
+        return set_error(TLH_INVALID, "chunk_attention: bad counts (at most 65535 sequences)");
+    if (a->max_context_len > 1 << 30)  // the kernels look a few tiles past it, in 32 bits
+        return set_error(TLH_INVALID, "chunk_attention: max_context_len %d above 2^30", a->max_context_len);
+    if ((int64_t)a->max_blocks_per_seq * a->block_size < a->max_context_len)
+        return set_error(TLH_INVALID, "chunk_attention: max_blocks_per_seq * block_size < max_context_len");
+    if ((int64_t)a->num_rows * a->num_heads > 1 << 30)
+        return set_error(TLH_INVALID, "chunk_attention: num_rows x num_heads above 2^30");
+    return TLH_OK;
+}
+
+tlh_status tlh_chunk_attention_scratch_bytes(const tlh_chunk_attention_args *a, size_t *bytes) {
+    if (!bytes) return set_error(TLH_INVALID, "chunk_attention_scratch_bytes: null pointer");
+    const tlh_status st = check_chunk(a);
+    if (st != TLH_OK) return st;
+    *bytes = chunk_attention_scratch_bytes(*a);
+    return TLH_OK;
+}
+
+tlh_status tlh_chunk_attention(const tlh_chunk_attention_args *a, void *scratch, size_t scratch_bytes, void *stream) {
+    const tlh_status st = check_chunk(a);
+    if (st != TLH_OK) return st;
+    const int64_t row = (int64_t)a->num_heads * a->head_size;
+    if (a->out_stride < row || a->q_stride < row || ((a->out_stride | a->q_stride) & 7) != 0 ||
+        std::max(a->out_stride, a->q_stride) > INT64_MAX >> 32)
+        return set_error(TLH_INVALID, "chunk_attention: a token stride is shorter than its heads or no multiple of 8");
+    if (a->num_seqs == 0 || a->num_rows == 0 || a->max_rows == 0) return TLH_OK;
+    if (!a->out || !a->q || !a->context_lens || !a->row_starts ||
+        (a->max_context_len > 0 && (!a->k_cache || !a->v_cache || !a->block_tables)))
+        return set_error(TLH_INVALID, "chunk_attention: null pointer");
+    if (!aligned16(a->out) || !aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
+        (((uintptr_t)a->block_tables | (uintptr_t)a->context_lens | (uintptr_t)a->row_starts) & 3))
+        return set_error(TLH_INVALID, "chunk_attention: q, out and the caches must be 16-byte aligned");
+    const __int128 all = ((__int128)(a->num_rows - 1) * a->out_stride + row) * 2;
+    const __int128 pool = (__int128)a->num_blocks * a->num_kv_heads * a->head_size * a->block_size * 2;
+    if (rows_overlap(a->out, 2 * a->out_stride, 2 * row, a->q, 2 * a->q_stride, 2 * row, a->num_rows) ||
+        overlap(a->out, all, a->k_cache, pool) || overlap(a->out, all, a->v_cache, pool))
+        return set_error(TLH_INVALID, "chunk_attention: out overlaps q or the caches");
+    const size_t need = chunk_attention_scratch_bytes(*a);
+    if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+        return set_error(TLH_INVALID, "chunk_attention: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    return launch_chunk_attention(*a, scratch, (hipStream_t)stream);
+}
+
+tlh_status tlh_head_rope(const tlh_head_rope_args *a, void *stream) {
+    if (!a) return set_error(TLH_INVALID, "head_rope: null args");
+    if (a->type != TLH_TYPE_F32 && a->type != TLH_TYPE_F16 && a->type != TLH_TYPE_BF16)
+        return set_error(TLH_UNSUPPORTED, "head_rope: heads of ggml type %d (%s); have f32, f16, bf16", a->type,
+                         type_name(a->type));
+    if (a->out_type != TLH_TYPE_F16 && a->out_type != TLH_TYPE_BF16)
+        return set_error(TLH_UNSUPPORTED, "head_rope: output of ggml type %d (%s); have f16, bf16", a->out_type,
+                         type_name(a->out_type));
+    const tlh_status st = check_heads("head_rope", a->num_heads, a->num_kv_heads, a->head_size);
+    if (st != TLH_OK) return st;
+    const bool cached = a->k_cache || a->v_cache || a->slots;
+    if (cached && (!a->k_cache || !a->v_cache || (!a->slots && a->num_tokens > 0)))
+        return set_error(TLH_INVALID, "head_rope: k_cache, v_cache and slots go together");
+    if (cached && a->out_type != TLH_TYPE_F16)
+        return set_error(TLH_UNSUPPORTED, "head_rope: the caches are f16, the output is %s", type_name(a->out_type));
+    if (cached && (!paged_block_size(a->block_size) || a->num_blocks < 0 || a->num_blocks > INT64_MAX / 32))
+        return set_error(TLH_INVALID, "head_rope: unsupported block_size %d (have 8, 16, 32) or bad num_blocks", a->block_size);
+    if (a->num_tokens < 0) return set_error(TLH_INVALID, "head_rope: negative count");
+    if (a->n_dims < 0 || a->n_dims > a->head_size || (a->n_dims & 1) || (a->mode != 0 && a->mode != 2))
+        return set_error(TLH_INVALID, "head_rope: n_dims %d (even, at most head_size) or mode %d (0 or 2)", a->n_dims, a->mode);
+    if (a->num_axes < 1 || a->num_axes > 4)
+        return set_error(TLH_INVALID, "head_rope: num_axes %d outside 1..4", a->num_axes);
+    for (int p = 0; p < a->n_dims / 2; ++p)
+        if (a->pair_axis[p] >= a->num_axes)
+            return set_error(TLH_INVALID, "head_rope: pair %d takes axis %d of %d", p, a->pair_axis[p], a->num_axes);
+    const int64_t qrow = (int64_t)a->num_heads * a->head_size, krow = (int64_t)a->num_kv_heads * a->head_size;
+    const int es = a->type == TLH_TYPE_F32 ? 4 : 2;
+    struct Rows {
+        const char *name;
+        const void *p;
+        int64_t stride, row;
+        int es;
+    };
+    const Rows in[] = {{"q", a->q, a->q_stride, qrow, es}, {"k", a->k, a->k_stride, krow, es}, {"v", a->v, a->v_stride, krow, es}};
+    const Rows out[] = {{"q_out", a->q_out, a->q_out_stride, qrow, 2}, {"k_out", a->k_out, a->k_out_stride, krow, 2},
+                        {"v_out", a->v_out, a->v_out_stride, krow, 2}};
+    auto ragged = [](const Rows &r) { return r.stride < r.row || ((r.stride * r.es) & 15) != 0 || r.stride > INT64_MAX >> 32; };
+    for (const Rows &r : in)
+        if (ragged(r)) return set_error(TLH_INVALID, "head_rope: %s's token stride is shorter than its heads or no multiple of 16 bytes", r.name);
+    for (const Rows &r : out)
+        if (r.p && ragged(r)) return set_error(TLH_INVALID, "head_rope: %s's token stride is shorter than its heads or no multiple of 16 bytes", r.name);
+    if (a->num_tokens == 0) return TLH_OK;
+    if (!a->q || !a->k || !a->v || !a->q_out || (a->n_dims > 0 && (!a->positions || !a->freqs)))
+        return set_error(TLH_INVALID, "head_rope: null pointer");
+    for (const Rows &r : in)
+        if (!aligned16(r.p)) return set_error(TLH_INVALID, "head_rope: %s must be 16-byte aligned", r.name);
+    for (const Rows &r : out)
+        if (!aligned16(r.p)) return set_error(TLH_INVALID, "head_rope: %s must be 16-byte aligned", r.name);
+    if (!aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->q_norm) || !aligned16(a->k_norm) ||
+        (((uintptr_t)a->positions | (uintptr_t)a->freqs) & 3) || ((uintptr_t)a->slots & 7))
+        return set_error(TLH_INVALID, "head_rope: misaligned pointer (caches and norms: 16 bytes)");
+    const __int128 pool = (__int128)a->num_blocks * krow * a->block_size * 2, n = a->num_tokens;
+    const struct {
+        const void *p;
+        __int128 bytes;
+    } small[] = {{a->positions, a->n_dims ? 4 * n * a->num_axes : 0}, {a->freqs, 2 * a->n_dims}, {a->q_norm, a->q_norm ? 4 * a->head_size : 0},
+                 {a->k_norm, a->k_norm ? 4 * a->head_size : 0}, {a->slots, cached ? 8 * n : 0}};
+    auto whole = [&](const Rows &r) { return ((__int128)(n - 1) * r.stride + r.row) * r.es; };
+    for (int i = 0; i < 3; ++i) {
+        const Rows &o = out[i];
+        if (!o.p) continue;
+        for (const Rows &r : in)
+            if (rows_overlap(o.p, o.es * o.stride, o.es * o.row, r.p, r.es * r.stride, r.es * r.row, n))
+                return set_error(TLH_INVALID, "head_rope: %s overlaps %s", o.name, r.name);
+        for (int j = 0; j < i; ++j)
+            if (out[j].p && rows_overlap(o.p, 2 * o.stride, 2 * o.row, out[j].p, 2 * out[j].stride, 2 * out[j].row, n))
+                return set_error(TLH_INVALID, "head_rope: %s overlaps %s", o.name, out[j].name);
+        for (const auto &x : small)
+            if (x.bytes > 0 && overlap(o.p, whole(o), x.p, x.bytes))
+                return set_error(TLH_INVALID, "head_rope: %s overlaps positions, freqs, norms or slots", o.name);
+        if (cached && (overlap(o.p, whole(o), a->k_cache, pool) || overlap(o.p, whole(o), a->v_cache, pool)))
+            return set_error(TLH_INVALID, "head_rope: %s overlaps the caches", o.name);
+    }
+    if (cached) {
+        for (const Rows &r : in)
+            if (overlap(r.p, whole(r), a->k_cache, pool) || overlap(r.p, whole(r), a->v_cache, pool))
+                return set_error(TLH_INVALID, "head_rope: the caches overlap %s", r.name);
+        for (const auto &x : small)
+            if (x.bytes > 0 && (overlap(x.p, x.bytes, a->k_cache, pool) || overlap(x.p, x.bytes, a->v_cache, pool)))
+                return set_error(TLH_INVALID, "head_rope: the caches overlap positions, freqs, norms or slots");
+        if (overlap(a->k_cache, pool, a->v_cache, pool)) return set_error(TLH_INVALID, "head_rope: the caches overlap");
+    }
+    return launch_head_rope(*a, (hipStream_t)stream);
+}
+
+static tlh_status check_verify(const tlh_draft_verify_args *a) {
+    if (!a) return set_error(TLH_INVALID, "draft_verify: null args");
+    if (a->type != TLH_TYPE_F32 && a->type != TLH_TYPE_F16 && a->type != TLH_TYPE_BF16)
+        return set_error(TLH_UNSUPPORTED, "draft_verify: logits of ggml type %d (%s); have f32, f16, bf16", a->type,
+                         type_name(a->type));
+    if (a->num_seqs < 0 || a->num_seqs > 65535 || a->num_drafts < 0 || a->num_drafts > 1 << 23 || a->vocab < 1 ||
+        a->vocab > 1000000)
+        return set_error(TLH_INVALID, "draft_verify: %d sequences outside 0..65535, %d drafts outside 0..2^23 or vocab %d outside "
+                         "1..1000000", a->num_seqs, a->num_drafts, a->vocab);
+    if (a->max_drafts < 0 || a->max_drafts > 1024)
+        return set_error(TLH_INVALID, "draft_verify: max_drafts %d outside 0..1024", a->max_drafts);
+    return TLH_OK;
+}
+
+tlh_status tlh_draft_verify_scratch_bytes(const tlh_draft_verify_args *a, size_t *bytes) {
+    if (!bytes) return set_error(TLH_INVALID, "draft_verify_scratch_bytes: null pointer");
+    const tlh_status st = check_verify(a);
+    if (st != TLH_OK) return st;
+    *bytes = draft_verify_scratch_bytes(*a);
+    return TLH_OK;
+}
+
+tlh_status tlh_draft_verify(const tlh_draft_verify_args *a, void *scratch, size_t scratch_bytes, void *stream) {
+    const tlh_status st = check_verify(a);
+    if (st != TLH_OK) return st;
+    if (a->target_stride < a->vocab || (a->draft && a->draft_stride < a->vocab) || a->target_stride > INT64_MAX >> 32 ||
+        (a->draft && a->draft_stride > INT64_MAX >> 32))
+        return set_error(TLH_INVALID, "draft_verify: row stride shorter than the vocabulary");
+    if (a->num_seqs == 0) return TLH_OK;
+    if (!a->target || !a->draft_starts || !a->temperatures || !a->sample_at || !a->accepted || !a->out_tokens ||
+        (a->num_drafts > 0 && (!a->tokens || !a->accept_at)))
+        return set_error(TLH_INVALID, "draft_verify: null pointer");
+    const int es = a->type == TLH_TYPE_F32 ? 4 : 2;
+    if ((((uintptr_t)a->target | (uintptr_t)a->draft) & (es - 1)) ||
+        (((uintptr_t)a->tokens | (uintptr_t)a->draft_starts | (uintptr_t)a->temperatures | (uintptr_t)a->accept_at |
+          (uintptr_t)a->sample_at | (uintptr_t)a->accepted | (uintptr_t)a->out_tokens | (uintptr_t)a->accept_probs) & 3))
+        return set_error(TLH_INVALID, "draft_verify: misaligned pointer");
+    struct Range {
+        const void *p;
+        __int128 bytes;
+    };
+    const __int128 S = a->num_seqs, R = a->num_drafts;
+    const Range in[] = {{a->target, ((R + S - 1) * a->target_stride + a->vocab) * es},
+                        {a->draft, a->draft && R > 0 ? ((R - 1) * a->draft_stride + a->vocab) * es : 0},
+                        {a->tokens, 4 * R}, {a->accept_at, 4 * R}, {a->draft_starts, 4 * (S + 1)},
+                        {a->temperatures, 4 * S}, {a->sample_at, 4 * S}};
+    const Range out[] = {{a->accepted, 4 * S}, {a->out_tokens, 4 * S * (a->max_drafts + 1)}, {a->accept_probs, a->accept_probs ? 4 * R : 0}};
+    for (int i = 0; i < 3; ++i) {
+        if (out[i].bytes == 0) continue;
+        for (const Range &r : in)
+            if (r.bytes > 0 && overlap(out[i].p, out[i].bytes, r.p, r.bytes))
+                return set_error(TLH_INVALID, "draft_verify: an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (out[j].bytes > 0 && overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return set_error(TLH_INVALID, "draft_verify: two outputs overlap");
+    }
+    const size_t need = draft_verify_scratch_bytes(*a);
+    if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+        return set_error(TLH_INVALID, "draft_verify: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    return launch_draft_verify(*a, scratch, (hipStream_t)stream);
+}
+
 tlh_status tlh_copy_blocks(void *const *pools, int32_t num_pools, int64_t block_bytes, int64_t num_blocks,
                            const int64_t *pairs, int32_t num_pairs, void *stream) {
     if (num_pools < 0 || num_pairs < 0 || num_blocks < 0 || block_bytes <= 0 || block_bytes % 16 != 0 ||

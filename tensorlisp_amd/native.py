@@ -42,6 +42,8 @@ EXPORTS = (
     "tlh_paged_attention_scratch_bytes", "tlh_paged_attention", "tlh_reshape_and_cache",
     "tlh_packed_attention", "tlh_tree_attention_scratch_bytes", "tlh_tree_attention", "tlh_copy_blocks",
     "tlh_compact_cache", "tlh_token_logprobs_scratch_bytes", "tlh_token_logprobs",
+    "tlh_chunk_attention_scratch_bytes", "tlh_chunk_attention", "tlh_head_rope", "tlh_draft_verify_scratch_bytes",
+    "tlh_draft_verify",
     "tlh_core_check", "tlh_core", "tlh_program_compile", "tlh_program_destroy", "tlh_copy", "tlh_memset",
     "tlh_read_floor",
     "tlh_program_input",
@@ -112,6 +114,32 @@ class TlhLogprobsArgs(C.Structure):
                 ("rows", C.c_int32), ("vocab", C.c_int32), ("top", C.c_int32)]
 
 
+class TlhChunkArgs(C.Structure):
+    _fields_ = [("out", C.c_void_p), ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("block_tables", C.c_void_p), ("context_lens", C.c_void_p), ("row_starts", C.c_void_p),
+                ("out_stride", C.c_int64), ("q_stride", C.c_int64), ("num_blocks", C.c_int64), ("num_seqs", C.c_int32),
+                ("num_rows", C.c_int32), ("max_rows", C.c_int32), ("num_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+                ("head_size", C.c_int32), ("block_size", C.c_int32), ("max_blocks_per_seq", C.c_int32),
+                ("max_context_len", C.c_int32), ("window", C.c_int32), ("scale", C.c_float)]
+
+
+class TlhHeadRopeArgs(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in ("q", "k", "v", "positions", "freqs", "q_norm", "k_norm", "q_out", "k_out", "v_out",
+                                          "k_cache", "v_cache", "slots")] + \
+               [(f, C.c_int64) for f in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride", "v_out_stride",
+                                         "num_blocks")] + \
+               [(f, C.c_int32) for f in ("type", "out_type", "num_tokens", "num_heads", "num_kv_heads", "head_size",
+                                         "block_size", "n_dims", "mode", "num_axes")] + \
+               [("eps", C.c_float), ("attn_factor", C.c_float), ("pair_axis", C.c_uint8 * 128)]
+
+
+class TlhVerifyArgs(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in ("target", "draft", "tokens", "draft_starts", "temperatures", "accept_at",
+                                          "sample_at", "accepted", "out_tokens", "accept_probs")] + \
+               [("target_stride", C.c_int64), ("draft_stride", C.c_int64)] + \
+               [(f, C.c_int32) for f in ("type", "num_seqs", "num_drafts", "max_drafts", "vocab")]
+
+
 assert C.sizeof(TlhOp) == 456, C.sizeof(TlhOp)
 
 
@@ -152,6 +180,11 @@ def load_library(path: Path = LIB_PATH) -> C.CDLL:
     L.tlh_compact_cache.argtypes = [C.POINTER(TlhCompactArgs), vp]
     L.tlh_token_logprobs_scratch_bytes.argtypes = [C.POINTER(TlhLogprobsArgs), C.POINTER(C.c_size_t)]
     L.tlh_token_logprobs.argtypes = [C.POINTER(TlhLogprobsArgs), vp, C.c_size_t, vp]
+    L.tlh_chunk_attention_scratch_bytes.argtypes = [C.POINTER(TlhChunkArgs), C.POINTER(C.c_size_t)]
+    L.tlh_chunk_attention.argtypes = [C.POINTER(TlhChunkArgs), vp, C.c_size_t, vp]
+    L.tlh_head_rope.argtypes = [C.POINTER(TlhHeadRopeArgs), vp]
+    L.tlh_draft_verify_scratch_bytes.argtypes = [C.POINTER(TlhVerifyArgs), C.POINTER(C.c_size_t)]
+    L.tlh_draft_verify.argtypes = [C.POINTER(TlhVerifyArgs), vp, C.c_size_t, vp]
     L.tlh_core_check.argtypes = [C.c_int, C.POINTER(TlhOp), C.c_int, C.c_int]
     L.tlh_core.argtypes = [C.c_int, C.POINTER(TlhOp), vp, vp, vp, vp, vp]
     i32p, i64p = C.POINTER(C.c_int32), C.POINTER(C.c_int64)
@@ -856,6 +889,238 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None):
     outs = (f(n), f(n), f(n, top), torch.empty((n, top), dtype=torch.int32, device=dev))
     _behind_current(stream, dev)
     node(logits, tokens, *outs, stream=stream)
+    _use_on(stream, *outs)
+    return outs
+
+
+class ChunkAttention(_ScratchNode):
+    """Causal attention of the sequences' new tokens over the paged cache, one or thousands a sequence, with its
+    scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. A call takes up to
+    num_seqs sequences and num_rows new tokens in all, at most max_rows of one sequence; calls of one object must be
+    stream-ordered (they share the scratch)."""
+
+    def __init__(self, num_seqs, num_rows, max_rows, num_heads, num_kv_heads, head_size, block_size,
+                 max_blocks_per_seq, max_context_len, scale, window: int = 0, device="cuda"):
+        a = self.args = TlhChunkArgs()
+        counts = dict(num_seqs=num_seqs, num_rows=num_rows, max_rows=max_rows, num_heads=num_heads,
+                      num_kv_heads=num_kv_heads, head_size=head_size, block_size=block_size,
+                      max_blocks_per_seq=max_blocks_per_seq, max_context_len=max_context_len, window=window)
+        for name, value in counts.items():
+            setattr(a, name, _int32(value, name))
+        a.scale = scale
+        n = C.c_size_t()
+        check(lib().tlh_chunk_attention_scratch_bytes(C.byref(a), C.byref(n)))
+        self._allocate(n.value, device)
+
+    def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, row_starts, stream=None):
+        """q and out f16 (rows, heads, head size) with rows <= num_rows, tokens at any stride that is a multiple of 8
+        elements, the caches in the paged-attention layouts, block_tables i32 (sequences, max_blocks_per_seq) with
+        sequences <= num_seqs, context_lens i32 (sequences,) with the new tokens, row_starts i32 (sequences + 1,)."""
+        import torch
+
+        a, dev = TlhChunkArgs.from_buffer_copy(self.args), self.device  # a call's own: threads may share the node
+        rows, S, H, KV, D, bs = (_extent(out), _extent(block_tables), a.num_heads, a.num_kv_heads, a.head_size,
+                                 a.block_size)
+        if rows > a.num_rows or S > a.num_seqs:
+            raise ValueError(f"out of {rows} rows and block_tables of {S} sequences, for up to {a.num_rows} and {a.num_seqs}")
+        for name, t in (("q", q), ("out", out)):
+            if t.dtype != torch.float16 or t.shape != (rows, H, D):
+                raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not {torch.float16} {(rows, H, D)}")
+        a.num_rows, a.num_seqs = rows, S
+        a.q, a.q_stride = _token_rows(q, H, D, "q", dev)
+        a.out, a.out_stride = _token_rows(out, H, D, "out", dev)
+        a.num_blocks = blocks = _extent(k_cache)
+        a.k_cache = _tensor(k_cache, torch.float16, (blocks, KV, D // 8, bs, 8), "k_cache", dev)
+        a.v_cache = _tensor(v_cache, torch.float16, (blocks, KV, D, bs), "v_cache", dev)
+        a.block_tables = _tensor(block_tables, torch.int32, (S, a.max_blocks_per_seq), "block_tables", dev)
+        a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
+        a.row_starts = _tensor(row_starts, torch.int32, (S + 1,), "row_starts", dev)
+        with _on(dev, stream) as s:
+            self._use_scratch(s)
+            check(lib().tlh_chunk_attention(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
+        return out
+
+
+def chunk_attention(q, k_cache, v_cache, block_tables, context_lens, row_starts, max_rows: int, max_context_len: int,
+                    scale: float, window: int = 0, stream=None):
+    """One ChunkAttention call: q f16 (rows, heads, head size) -> out alike, contiguous (zeros in rows behind the last
+    sequence). `stream` waits for the current stream's work."""
+    import torch
+
+    rows, heads, hs = q.shape
+    node = ChunkAttention(block_tables.shape[0], rows, max_rows, heads, v_cache.shape[1], hs, v_cache.shape[3],
+                          block_tables.shape[1], max_context_len, scale, window, device=q.device)
+    out = torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
+    # the zeros come from the current stream; the copy is the call's, on its own
+    with torch.cuda.stream(_behind_current(stream, q.device)):
+        block_tables = block_tables.contiguous()
+    node(out, q, k_cache, v_cache, block_tables, context_lens, row_starts, stream)
+    _use_on(stream, out)
+    return out
+
+
+def rope_freqs(n_dims: int, freq_base: float = 10000.0, freq_scale: float = 1.0, freq_factors=None, device="cuda"):
+    """HeadRope's frequencies, f32 (n_dims / 2,): freq_scale * freq_base^(-2 p / n_dims) / freq_factors[p]."""
+    import torch
+
+    p = torch.arange(n_dims // 2, dtype=torch.float64)
+    f = freq_scale * float(freq_base) ** (-2.0 * p / n_dims)
+    if freq_factors is not None:
+        f = f / freq_factors.detach().cpu().double()
+    return f.float().to(device)
+
+
+def rope_sections(sections, interleaved: bool = False):
+    """HeadRope's pair_axes where sections[a] pairs take axis a: one section after another, or in turn (pair p takes
+    axis p % axes while that has pairs left, axis 0 then)."""
+    axes = len(sections)
+    if not interleaved:
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    return [p % axes if p < axes * sections[p % axes] else 0 for p in range(sum(sections))]
+
+
+class HeadRope:
+    """The norms of the query and key heads, their rotation by the tokens' positions and the write of keys and values
+    to the paged cache, in one launch. freqs f32 (n_dims / 2,) on the GPU: pair p turns by its position times freqs[p];
+    pair_axes: the axis each pair takes its position from (None: one axis); mode 0 pairs dims 2p and 2p + 1, 2 (neox)
+    p and p + n_dims / 2; dims from n_dims on are not rotated. attn_factor multiplies cos and sin."""
+
+    def __init__(self, num_heads: int, num_kv_heads: int, head_size: int, freqs, pair_axes=None, mode: int = 2,
+                 eps: float = 1e-6, attn_factor: float = 1.0):
+        import torch
+
+        pairs = _extent(freqs)
+        a = self.args = TlhHeadRopeArgs()
+        a.num_heads, a.num_kv_heads = _int32(num_heads, "num_heads"), _int32(num_kv_heads, "num_kv_heads")
+        a.head_size, a.n_dims, a.mode = _int32(head_size, "head_size"), 2 * pairs, _int32(mode, "mode")
+        a.eps, a.attn_factor = eps, attn_factor
+        self.device, self.freqs = freqs.device, freqs  # freqs live as long as their address is used
+        a.freqs = _tensor(freqs, torch.float32, (pairs,), "freqs", self.device)
+        axes = [0] * pairs if pair_axes is None else [int(x) for x in pair_axes]
+        if len(axes) != pairs or pairs > 128 or any(not 0 <= x < 4 for x in axes):
+            raise ValueError(f"pair_axes must give one of four axes for each of {pairs} (at most 128) pairs")
+        a.num_axes = max(axes, default=0) + 1
+        a.pair_axis = (C.c_uint8 * 128)(*axes)
+
+    def __call__(self, q, k, v, positions, q_out, q_norm=None, k_norm=None, k_out=None, v_out=None, k_cache=None,
+                 v_cache=None, slots=None, stream=None):
+        """q (tokens, heads, head size), k and v (tokens, kv heads, head size) f32, f16 or bf16, tokens at any stride
+        that is a multiple of 16 bytes (views of a fused projection), positions i32 (tokens,) or (axes, tokens); q_norm
+        and k_norm f32 (head size,) or None -> q_out, and k_out and v_out where given (f16 or bf16); k_cache, v_cache
+        and slots i64 (tokens,) as reshape_and_cache takes them (then the outputs are f16)."""
+        import torch
+
+        a, dev = TlhHeadRopeArgs.from_buffer_copy(self.args), self.device
+        H, KV, D, n = a.num_heads, a.num_kv_heads, a.head_size, _extent(q)
+        if q.dtype != k.dtype or q.dtype != v.dtype or q.shape != (n, H, D) or k.shape != (n, KV, D) or v.shape != k.shape:
+            raise ValueError(f"q {q.dtype} {tuple(q.shape)}, k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)}, "
+                             f"for {H} heads and {KV} kv heads of {D}")
+        a.num_tokens, a.type, a.out_type = _int32(n, "tokens"), _ggml_type(q), _ggml_type(q_out)
+        a.q, a.q_stride = _token_rows(q, H, D, "q", dev)
+        a.k, a.k_stride = _token_rows(k, KV, D, "k", dev)
+        a.v, a.v_stride = _token_rows(v, KV, D, "v", dev)
+        outs = [("q_out", q_out, H, "q_out_stride"), ("k_out", k_out, KV, "k_out_stride"), ("v_out", v_out, KV, "v_out_stride")]
+        for name, t, heads, stride in outs:
+            if t is None:
+                setattr(a, stride, heads * D)
+                continue
+            if t.dtype != q_out.dtype or t.shape != (n, heads, D):
+                raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not {q_out.dtype} {(n, heads, D)}")
+            p, st = _token_rows(t, heads, D, name, dev)
+            setattr(a, name, p), setattr(a, stride, st)
+        if a.n_dims:
+            one = positions.dim() == 1 and a.num_axes == 1
+            a.positions = _tensor(positions, torch.int32, (n,) if one else (a.num_axes, n), "positions", dev)
+        if q_norm is not None:
+            a.q_norm = _tensor(q_norm, torch.float32, (D,), "q_norm", dev)
+        if k_norm is not None:
+            a.k_norm = _tensor(k_norm, torch.float32, (D,), "k_norm", dev)
+        if k_cache is not None or v_cache is not None or slots is not None:
+            if k_cache is None or v_cache is None or slots is None:
+                raise ValueError("k_cache, v_cache and slots go together")
+            a.num_blocks = blocks = _extent(k_cache)
+            a.block_size = bs = v_cache.shape[-1] if v_cache.dim() else 0
+            a.k_cache = _tensor(k_cache, torch.float16, (blocks, KV, D // 8, bs, 8), "k_cache", dev)
+            a.v_cache = _tensor(v_cache, torch.float16, (blocks, KV, D, bs), "v_cache", dev)
+            a.slots = _tensor(slots, torch.int64, (n,), "slots", dev)
+        with _on(dev, stream) as s:
+            check(lib().tlh_head_rope(C.byref(a), s))
+        return q_out
+
+
+class DraftVerify(_ScratchNode):
+    """Verification of drafted tokens (a chain a sequence) against the model's probabilities from given random numbers,
+    with the scratch. A call takes up to num_seqs sequences and num_drafts drafted tokens in all, at most max_drafts of
+    one sequence; drafter: whether a drafting model's logits come with them (else tokens were proposed outright). Calls
+    of one object must be stream-ordered (they share the scratch)."""
+
+    def __init__(self, num_seqs: int, num_drafts: int, max_drafts: int, vocab: int, dtype=None, drafter: bool = True,
+                 device="cuda"):
+        import torch
+
+        self.dtype, self.vocab, self.drafter = dtype or torch.float32, vocab, drafter
+        a = self.args = TlhVerifyArgs()
+        a.type = _ggml_type(torch.empty(0, dtype=self.dtype))
+        for name, value in dict(num_seqs=num_seqs, num_drafts=num_drafts, max_drafts=max_drafts, vocab=vocab).items():
+            setattr(a, name, _int32(value, name))
+        a.target_stride = a.draft_stride = vocab
+        a.draft = 16 if drafter else None  # (the size asks only whether there is one)
+        n = C.c_size_t()
+        check(lib().tlh_draft_verify_scratch_bytes(C.byref(a), C.byref(n)))
+        self._allocate(n.value, device)
+
+    def _logits(self, t, rows: int, name: str):
+        if (t.dtype != self.dtype or t.shape != (rows, self.vocab) or t.device != self.device or
+                (self.vocab > 1 and t.numel() and t.stride(1) != 1)):
+            raise ValueError(f"{name} {t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}, "
+                             f"not {rows} rows of {self.vocab} {self.dtype} on {self.device}")
+        return t.data_ptr(), t.stride(0) if rows > 1 else self.vocab
+
+    def __call__(self, target, draft, tokens, draft_starts, temperatures, accept_at, sample_at, accepted, out_tokens,
+                 accept_probs=None, stream=None):
+        """target (drafts + sequences, vocab): sequence s has the rows of its n drafted tokens and one more, from
+        draft_starts[s] + s on; draft (drafts, vocab) or None; tokens i32 (drafts,), draft_starts i32 (sequences + 1,),
+        temperatures f32 (sequences,) (0: greedy), accept_at f32 (drafts,) and sample_at f32 (sequences,) uniform in
+        [0, 1) -> accepted i32 (sequences,), out_tokens i32 (sequences, max_drafts + 1): the accepted tokens, the next
+        one, -1 behind; accept_probs f32 (drafts,) or None."""
+        import torch
+
+        a, dev = TlhVerifyArgs.from_buffer_copy(self.args), self.device
+        R, S = _extent(tokens), _extent(temperatures)
+        if R > a.num_drafts or S > a.num_seqs:
+            raise ValueError(f"{R} drafted tokens of {S} sequences, for up to {a.num_drafts} and {a.num_seqs}")
+        if (draft is not None) != self.drafter:
+            raise ValueError("a drafting model's logits come with every call of a node made for them, and with no other")
+        a.num_drafts, a.num_seqs = R, S
+        a.target, a.target_stride = self._logits(target, R + S, "target")
+        if draft is not None:
+            a.draft, a.draft_stride = self._logits(draft, R, "draft")
+        a.tokens = _tensor(tokens, torch.int32, (R,), "tokens", dev)
+        a.draft_starts = _tensor(draft_starts, torch.int32, (S + 1,), "draft_starts", dev)
+        a.temperatures = _tensor(temperatures, torch.float32, (S,), "temperatures", dev)
+        a.accept_at = _tensor(accept_at, torch.float32, (R,), "accept_at", dev)
+        a.sample_at = _tensor(sample_at, torch.float32, (S,), "sample_at", dev)
+        a.accepted = _tensor(accepted, torch.int32, (S,), "accepted", dev)
+        a.out_tokens = _tensor(out_tokens, torch.int32, (S, a.max_drafts + 1), "out_tokens", dev)
+        a.accept_probs = _tensor(accept_probs, torch.float32, (R,), "accept_probs", dev) if accept_probs is not None else None
+        with _on(dev, stream) as s:
+            self._use_scratch(s)
+            check(lib().tlh_draft_verify(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
+        return accepted, out_tokens, accept_probs
+
+
+def draft_verify(target, draft, tokens, draft_starts, temperatures, accept_at, sample_at, max_drafts: int, stream=None):
+    """One DraftVerify call -> (accepted i32 (sequences,), out_tokens i32 (sequences, max_drafts + 1), accept_probs f32
+    (drafts,), NaN for drafts of no sequence). `stream` waits for the current stream's work, which may still use the
+    new tensors' memory."""
+    import torch
+
+    S, R, dev = temperatures.shape[0], tokens.shape[0], target.device
+    node = DraftVerify(S, R, max_drafts, target.shape[1], target.dtype, draft is not None, device=dev)
+    outs = (torch.empty(S, dtype=torch.int32, device=dev), torch.empty((S, max_drafts + 1), dtype=torch.int32, device=dev),
+            torch.full((R,), float("nan"), device=dev))
+    _behind_current(stream, dev)
+    node(target, draft, tokens, draft_starts, temperatures, accept_at, sample_at, *outs, stream=stream)
     _use_on(stream, *outs)
     return outs
 
