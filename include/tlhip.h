@@ -499,8 +499,8 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  *   q, out       f16 [num_rows][num_heads][head_size], a token's heads contiguous,
  *                q_stride and out_stride elements from token to token (multiples of 8)
  *   row_starts   i32 [num_seqs + 1]: sequence s has the rows row_starts[s] ..
- *                row_starts[s + 1] - 1, n of them, at most max_rows; rows behind the
- *                last sequence are left as they were
+ *                row_starts[s + 1] - 1, n of them, at most max_rows (starts do not
+ *                decrease); rows behind the last sequence are left as they were
  * With L = context_lens[s], row i of the sequence is the token at place L - n + i and
  * sees the tokens up to itself, with window > 0 the last `window` of them. f32 scores,
  * softmax and sums, its numerators rounded to f16 for the product with v (those below

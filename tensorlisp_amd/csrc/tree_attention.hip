@@ -34,7 +34,7 @@
 // the longest context; made for 131072 tokens the first takes 5% more, the last 3 us.
 #include <algorithm>
 
-#include "mfma32.hpp"
+#include "paged_wave.hpp"
 
 namespace tlh {
 
@@ -43,18 +43,14 @@ constexpr int TA_WGS = 1024;                          // workgroups a split aims
 constexpr int TA_WGS_SHARED = 512;                    // workgroups that fill the machine (two a CU)
 constexpr int TA_MAX_PARTS = 64;                      // a lane each in the merge
 
-struct TaArgs {
+struct TaArgs : PagedArgs {
     uint16_t *out;
-    const uint16_t *q, *kc, *vc;
-    const int32_t *tables, *lens, *starts;
+    const uint16_t *q;
+    const int32_t *lens, *starts;
     const int64_t *masks;
     float *part;  // [s][kv head][block of 32 rows][partition][row][m, l, -, -, D]
-    int64_t num_blocks;
-    int S, H, KV, G, rows, max_drafts, max_blocks, max_ctx, P, part_len, RB;  // RB: blocks of 32 rows
+    int S, H, G, rows, max_drafts, max_ctx, P, part_len, RB;  // RB: blocks of 32 rows
     int sort;  // sequences go longest first
-    float cs;             // |scale| * log2(e); 1 where the scale is 0
-    float lift;           // how far below the maximum the exponents' reference is set, in scores
-    uint32_t qand, qxor;  // q's words: negated where the scale is negative, zeroed where it is 0
 };
 
 struct TaSeq {
@@ -88,177 +84,27 @@ __device__ __forceinline__ int ta_pick(const TaArgs &a, int o, int lane) {
     return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
 }
 
-// What the two forms share: a wave's 32 rows of one (sequence, kv head).
-template <int D, int BS> struct TaWave {
-    static constexpr int NS = D / 16, NB = (D + 31) / 32, PAGES = 32 / BS;
-    const TaArgs &a;
-    const int lane, h, c;
-    const int32_t *table;
-    const int64_t page_bytes;
-    const uint8_t *kbase, *vbase;
-    const int kappa;  // the key of S^T's row c: bits 2 and 3 of c exchanged
-    const int prefix, L;
+// Row i of a sequence sees the `prefix` tokens before the drafted ones and drafted token j
+// where bit j of its mask is set.
+struct TaRule {
+    int prefix;
     uint64_t mask = 0;  // of this lane's row
-
-    __device__ __forceinline__ TaWave(const TaArgs &a_, int lane_, int s, int hk, const TaSeq &sq)
-        : a(a_), lane(lane_), h(lane_ >> 5), c(lane_ & 31), table(a_.tables + (int64_t)s * a_.max_blocks),
-          page_bytes((int64_t)a_.KV * D * BS * 2), kbase((const uint8_t *)a_.kc + (int64_t)hk * D * BS * 2),
-          vbase((const uint8_t *)a_.vc + (int64_t)hk * D * BS * 2),
-          kappa((c & 0x13) | (c & 4) << 1 | (c & 8) >> 1), prefix(sq.L - sq.n), L(sq.L) {}
-
-    // The pages of the tile at key `base` (past the context its last one again). Their
-    // ids are read ahead of their use, so that no tile waits for the table; one
-    // outside the pools is taken as page 0, its keys as not there.
-    struct Pages {
-        int id[PAGES];
-        uint32_t good;  // bits of the tile's keys whose page is inside
-    };
-    __device__ __forceinline__ Pages ids_of(int base) const {
-        Pages p = {};
-#pragma unroll
-        for (int i = 0; i < PAGES; ++i)
-            p.id[i] = table[__builtin_amdgcn_readfirstlane(min(base / BS + i, (L - 1) / BS))];
-        return p;
-    }
-    __device__ __forceinline__ Pages checked(Pages p) const {
-        p.good = 0;
-#pragma unroll
-        for (int i = 0; i < PAGES; ++i) {
-            const bool ok = p.id[i] >= 0 && p.id[i] < a.num_blocks;
-            p.id[i] = ok ? p.id[i] : 0;
-            p.good |= ok ? (BS == 32 ? ~0u : ((1u << (BS & 31)) - 1) << (BS * i)) : 0u;
-        }
-        return p;
-    }
-    __device__ __forceinline__ int64_t page_at(const Pages &p, int key) const {  // of key `key` of the tile
-        int id = p.id[0];
-#pragma unroll
-        for (int i = 1; i < PAGES; ++i) id = key / BS == i ? p.id[i] : id;
-        return (int64_t)id * page_bytes;
-    }
-    // this lane's 16 bytes of the keys' step st are k_at() + k_step(st), of the values'
-    // keys 16 i + 8 h .. + 7 and dims 32 d .. + 31 v_at(i) + v_step(d)
-    __device__ __forceinline__ const uint8_t *k_at(const Pages &p) const {
-        return kbase + page_at(p, kappa) + h * BS * 16 + (kappa % BS) * 16;
-    }
-    static __device__ __forceinline__ int k_step(int st) { return st * BS * 32; }
-    __device__ __forceinline__ const uint8_t *v_at(const Pages &p, int i) const {
-        const int key = 16 * i + 8 * h;
-        return vbase + page_at(p, key) + (key % BS) * 2 + c * BS * 2;
-    }
-    __device__ __forceinline__ int v_step(int d) const {  // dims past the last repeat it
-        return (32 * d + 31 < D ? 32 * d : min(32 * d + c, D - 1) - c) * BS * 2;
-    }
-
-    __device__ __forceinline__ const uint8_t *set_row(int b, int hk, int row) {  // -> this lane's part of the row's q
-        const int i = row / a.G;
-        mask = (uint64_t)a.masks[b + i];
-        return (const uint8_t *)(a.q + ((int64_t)(b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * h;
-    }
-    __device__ __forceinline__ uint4 signed_q(uint4 w) const {
-        return make_uint4((w.x & a.qand) ^ a.qxor, (w.y & a.qand) ^ a.qxor, (w.z & a.qand) ^ a.qxor, (w.w & a.qand) ^ a.qxor);
-    }
-
-    f32x16 O[NB];
-    float m, l;  // the exponents' reference (an unscaled score), this half's sum
-    // A value that is not finite would turn the zero weight of a key that a row does
-    // not see into NaN. So where a wave's sums come out not finite, it takes its tiles
-    // again, carefully: in those with masked keys it adds each seen key's product by itself.
-    bool some_masked = false;
-    __device__ __forceinline__ void reset() {
-#pragma unroll
-        for (int d = 0; d < NB; ++d) O[d] = (f32x16){};
-        m = -INFINITY;
-        l = 0.0f;
-    }
-    __device__ __forceinline__ bool bad() const {
-        bool x = false;
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x = x || !(fabsf(O[d][i]) < INFINITY);
-        return x;
-    }
-
-    struct Seen {
-        bool whole;       // every row sees every key of the tile
-        uint32_t there;   // keys that are in the cache
-        uint32_t vis;     // keys that this lane's row sees
-    };
-    __device__ __forceinline__ Seen seen(int base, uint32_t good) {
-        Seen s = {base + 32 <= prefix && good == ~0u, ~0u, ~0u};
-        if (!s.whole) {
-            some_masked = true;
-            s.there = L <= base ? 0u : good & (L - base >= 32 ? ~0u : (1u << (L - base)) - 1);
-            const int d = base - prefix;
-            const uint32_t see = d >= 64    ? 0u
-                                 : d >= 0   ? (uint32_t)(mask >> d)
-                                 : d <= -32 ? ~0u
-                                            : (uint32_t)(mask << -d) | ((1u << -d) - 1);
-            s.vis = see & s.there;
-        }
-        return s;
-    }
-    // scores of U x 32 keys -> numerators (f16), the running maximum and sum
-    template <int U> __device__ __forceinline__ void softmax(f32x16 (&S)[U], const Seen (&s)[U], uint4 (&pf)[2 * U]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (!s[u].whole) {
-                const uint32_t mine = s[u].vis >> (8 * h);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[u][i] = -INFINITY;
-            }
-        float mx = S[0][0];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[u][i]);
-        mx = max_halves(mx);
-        // the reference moves only when the maximum has grown by more than 2^8
-        const bool grow = mx > m && !((mx - m) * a.cs <= 8.0f + F16_LIFT);
-        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float ref = mx - a.lift;
-            const float alpha = grow ? __builtin_amdgcn_exp2f((m - ref) * a.cs) : 1.0f;
-            m = grow ? ref : m;
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < NB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) O[d][i] *= alpha;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * a.cs;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[u][8 * i + e] * a.cs - mc);
-                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                pf[2 * u + i] = pack8<false>(p);
-            }
-    }
-    // places that hold no token's value may hold anything
-    __device__ __forceinline__ uint4 live_v(uint4 v, int i, uint32_t there) const {
-        const uint32_t on = there >> (16 * i + 8 * h);
-        auto keep = [&](int e) { return ((on >> e) & 1 ? 0xffffu : 0u) | ((on >> e) & 2 ? 0xffff0000u : 0u); };
-        return make_uint4(v.x & keep(0), v.y & keep(2), v.z & keep(4), v.w & keep(6));
-    }
-    // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
-    // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
-    __device__ __forceinline__ void careful_pv(int d, const Seen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
-#pragma unroll 1
-        for (int key = 0; key < 32; ++key) {
-            const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
-            if (!((s.vis >> key) & 1)) continue;
-            const float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                O[d][x] += p * h2f((uint16_t)(sv[sv_step * i + 4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
-        }
+    __device__ __forceinline__ bool whole(int base) const { return base + 32 <= prefix; }
+    __device__ __forceinline__ uint32_t sees(int base) const {
+        const int d = base - prefix;
+        return d >= 64    ? 0u
+               : d >= 0   ? (uint32_t)(mask >> d)
+               : d <= -32 ? ~0u
+                          : (uint32_t)(mask << -d) | ((1u << -d) - 1);
     }
 };
+template <int D, int BS> using TaWave = PagedWave<D, BS, TaRule>;
+// -> this lane's part of the row's q
+template <int D> __device__ __forceinline__ const uint8_t *ta_row(const TaArgs &a, TaRule &rule, int half, int b, int hk, int row) {
+    const int i = row / a.G;
+    rule.mask = (uint64_t)a.masks[b + i];
+    return (const uint8_t *)(a.q + ((int64_t)(b + i) * a.H + hk * a.G + row % a.G) * D) + 16 * half;
+}
 
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(const TaArgs a) {
@@ -282,11 +128,11 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
     const int t0 = part * a.part_len;
     if (r0 >= R || (part > 0 && t0 >= L)) return;
     const int ntiles = (min(L, t0 + a.part_len) - t0 + 31) / 32;
-    W w(a, lane, s, hk, sq);
+    W w(a, lane, s, hk, L, TaRule{L - sq.n});
     const int c = w.c, h = w.h;
     {
         // the four waves share Q in LDS: in registers it would leave too few for two waves a SIMD
-        const uint8_t *qr = w.set_row(sq.b, hk, min(r0 + c, R - 1));
+        const uint8_t *qr = ta_row<D>(a, w.rule, h, sq.b, hk, min(r0 + c, R - 1));
         for (int st = wave; st < NS; st += TA_WAVES) s_q[st][lane] = w.signed_q(*(const uint4 *)(qr + 32 * st));
     }
     uint4 kf[NS], vf[NB][2];
@@ -326,7 +172,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
             for (int st = 0; st < NS; ++st) S[0] = mfma32<false>(kf[st], s_q[st][lane], S[0]);
             if (AHEAD) load_k(pn);  // past the last tile: the last page again
             else load_v(pg);
-            const typename W::Seen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
+            const PagedSeen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
             uint4 pf[2];
             w.softmax(S, sees, pf);
             if (see.there != ~0u) {
@@ -407,19 +253,11 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn(c
     }
 }
 
-// The form for many rows. Tiles of KT keys in LDS as the operands' 1-KiB fragments
-// (64 lanes x 16 bytes): of every 32 keys the NS steps of K, then of V^T the two
-// halves of keys x NB dim blocks.
-template <int D> struct TaShared {
-    static constexpr int KT = D <= 128 ? 64 : 32;
-    static constexpr int TILE = KT / 32 * (D / 16 + 2 * ((D + 31) / 32)) * 1024;
-};
-
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_shared(const TaArgs a) {
     using W = TaWave<D, BS>;
     constexpr int NS = W::NS, NB = W::NB;
-    using Sh = TaShared<D>;
+    using Sh = PagedTile<D>;
     constexpr int KT = Sh::KT, SUBS = KT / 32, KF = SUBS * NS;
     __shared__ __attribute__((aligned(16))) uint8_t T0[Sh::TILE], T1[Sh::TILE];
     __shared__ uint4 s_p[TA_WAVES][128];  // the careful pass's P
@@ -434,7 +272,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
     if (rg * TA_WAVES * 32 >= R) return;
     const int ntiles = (L + KT - 1) / KT;
     const bool mine = r0 < R;  // some wave of the workgroup has rows, this one may not
-    W w(a, lane, s, hk, sq);
+    W w(a, lane, s, hk, L, TaRule{L - sq.n});
     const int c = w.c, h = w.h;
     typename W::Pages pg[SUBS], pn[SUBS];  // of the tile in turn and the next one
     auto ids = [&](int t, typename W::Pages (&p)[SUBS]) {
@@ -462,7 +300,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
     };
     uint4 qf[NS];
     {
-        const uint8_t *qr = w.set_row(sq.b, hk, min(r0 + c, R - 1));
+        const uint8_t *qr = ta_row<D>(a, w.rule, h, sq.b, hk, min(r0 + c, R - 1));
 #pragma unroll
         for (int st = 0; st < NS; ++st) qf[st] = w.signed_q(*(const uint4 *)(qr + 32 * st));
     }
@@ -481,7 +319,7 @@ __global__ void __launch_bounds__(64 * TA_WAVES, D <= 128 ? 2 : 1) k_tree_attn_s
         }
         if (!mine) return;
         f32x16 S[SUBS];
-        typename W::Seen see[SUBS];
+        PagedSeen see[SUBS];
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
             S[u] = (f32x16){};
@@ -666,9 +504,7 @@ tlh_status launch_tree_attention(const tlh_tree_attention_args &a, void *scratch
     const int64_t rb = ta_row_blocks(a);
     t.P = ta_parts(a, t.part_len);
     t.RB = (int)rb;
-    t.cs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
-    t.lift = f16_lift(t.cs);
-    t.qand = a.scale == 0.0f ? 0u : ~0u, t.qxor = a.scale < 0.0f ? 0x80008000u : 0u;
+    set_scale(t, a.scale);
     const int64_t blocks = sh ? ta_shared_wgs(a) : (int64_t)t.P * t.S * rb * t.KV;
     t.sort = t.S > 1 && t.S <= 64 && blocks > 2 * device_cus();
     if (blocks >= 1 << 24)  // x 256 threads
