@@ -38,6 +38,7 @@ struct CaArgs : PagedArgs {
     int64_t so, sq;  // bytes from token to token
     const int32_t *lens, *starts;
     float *part;     // [slot][slot_rows][m, l, -, -, D]
+    struct CaItem *list;
     int S, G, rows, max_rows, max_ctx, window, wgs, slots, slot_rows;
 };
 
@@ -56,15 +57,16 @@ __device__ __forceinline__ CaSeq ca_seq(const CaArgs &a, int s) {
 // A sequence's items a kv head and the 64-key tiles that the largest of them sees
 struct CaWork {
     int items, tiles, wide;
+    CaSeq q;
 };
 __host__ __device__ __forceinline__ int ca_tiles(int L, int G, int window, int rows) {
     const int64_t span = (int64_t)window + (rows - 1) / G + 1;  // keys that some row of a block of `rows` sees
     return L <= span ? (L + 63) / 64 : (int)((span + 63) / 64) + 1;
 }
 __device__ __forceinline__ CaWork ca_work(const CaArgs &a, int s) {
-    CaWork w = {0, 0, 0};
+    CaWork w = {};
     if (s >= a.S) return w;
-    const CaSeq q = ca_seq(a, s);
+    const CaSeq q = w.q = ca_seq(a, s);
     const int R = q.n * a.G;
     w.wide = R > CA_NARROW;
     const int per = w.wide ? 128 : 32;
@@ -73,25 +75,41 @@ __device__ __forceinline__ CaWork ca_work(const CaArgs &a, int s) {
     return w;
 }
 
-template <typename T> __device__ __forceinline__ T ca_sum(T v) {
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+// The sum of the lanes up to each (the last lane holds that of all), within the vector
+// unit: a shuffle through LDS for each of the six steps would make the plan 4 us long.
+__device__ __forceinline__ int ca_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // the lane 1 before, in rows of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // 2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // 4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // rows 1 and 3: the last lane of the row before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 2 and 3: lane 31
     return v;
 }
-__device__ __forceinline__ int ca_parts(int tiles, int each) { return max(1, min(CA_MAX_PARTS, (tiles + each - 1) / each)); }
+__device__ __forceinline__ int ca_sum(int v) { return __builtin_amdgcn_readlane(ca_scan(v), 63); }
+// ceil(tiles / each), at least 1 and at most CA_MAX_PARTS
+__device__ __forceinline__ int ca_parts(int tiles, int each, float inv) {
+    if (tiles >= (int64_t)CA_MAX_PARTS * each) return CA_MAX_PARTS;
+    const int q = (int)((float)tiles * inv);  // off by at most 1
+    const int r = tiles - q * each;
+    return max(1, q + (r > 0) + (r > each) - (r <= -each));
+}
 
-// What workgroup `block` of the launch (of the merge: of the items that have partitions)
-// does. Every lane calls; a lane looks at one sequence of 64 at a time.
+// What a workgroup does. Every lane calls; a lane looks at one sequence of 64 at a time.
 struct CaPlan {
     int s, local, parts, items, wide, slot;  // s < 0: nothing; slot: the sequence's first
+    int list, lists;                         // the first of the sequence's split items, and how many there are in all
+    CaSeq q;
 };
-template <bool MERGE> __device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) {
+__device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) {
     const CaWork first = ca_work(a, lane);
     auto work = [&](int g) { return g == 0 ? first : ca_work(a, g + lane); };
     // tiles of a workgroup if all had as many
     uint64_t total = 0;
     for (int g = 0; g < a.S; g += 64) {
         const CaWork w = work(g);
-        total += ca_sum((uint64_t)w.items * (uint64_t)w.tiles);
+        const uint64_t n = (uint64_t)w.items * (uint64_t)w.tiles;  // in two parts: 64 of either fit 32 bits
+        total += (uint64_t)(uint32_t)ca_sum((int)(n & 0xffffff)) + ((uint64_t)(uint32_t)ca_sum((int)(n >> 24)) << 24);
     }
     const int even = (int)min(max((total * a.KV + a.wgs - 1) / a.wgs, (uint64_t)CA_MIN_TILES), (uint64_t)1 << 26);
     // Partitions are whole, so with that many some workgroups are left over, to run alone
@@ -101,47 +119,40 @@ template <bool MERGE> __device__ __forceinline__ CaPlan ca_plan(const CaArgs &a,
     constexpr int TRIES = 5;
     const int eighths[TRIES] = {8, 9, 10, 12, 16};
     int each[TRIES], count[TRIES] = {};
+    float inv[TRIES];
 #pragma unroll
-    for (int i = 0; i < TRIES; ++i) each[i] = (even * eighths[i] + 7) / 8;
+    for (int i = 0; i < TRIES; ++i) each[i] = (even * eighths[i] + 7) / 8, inv[i] = 1.0f / (float)each[i];
     for (int g = 0; g < a.S; g += 64) {
         const CaWork w = work(g);
+        const int n = (int)min((int64_t)w.items * a.KV, (int64_t)1 << 18);
 #pragma unroll
         for (int i = 0; i < TRIES; ++i)
-            count[i] = min(count[i] + ca_sum((int)min((int64_t)w.items * a.KV * ca_parts(w.tiles, each[i]), (int64_t)1 << 18)), 1 << 24);
+            count[i] = min(count[i] + ca_sum(min(n * ca_parts(w.tiles, each[i], inv[i]), 1 << 18)), 1 << 24);
     }
     int take = each[TRIES - 1];
+    float take_inv = inv[TRIES - 1];
     bool all = false;
 #pragma unroll
     for (int i = TRIES - 1; i >= 0; --i)
-        if (count[i] <= a.wgs) take = each[i], all = true;
+        if (count[i] <= a.wgs) take = each[i], take_inv = inv[i], all = true;
 
-    CaPlan p = {-1, 0, 0, 0, 0, 0};
-    int at = 0, slot = 0;
+    CaPlan p = {};
+    p.s = -1;
+    int at = 0, slot = 0, list = 0;
     for (int g = 0; g < a.S; g += 64) {
         const CaWork w = work(g);
-        const int parts = ca_parts(w.tiles, take), n = w.items * a.KV;
-        const int mine = MERGE ? (parts > 1 ? n : 0) : n * parts, slots = parts > 1 ? n * parts : 0;
-        int off = at, soff = slot;  // of the lanes before this one, in the order in which they go
-        if (!MERGE && !all && a.S <= 64) {  // longest workgroups first: one that starts last would end alone
+        const int parts = ca_parts(w.tiles, take, take_inv), n = w.items * a.KV;
+        const int mine = n * parts, slots = parts > 1 ? mine : 0, lists = parts > 1 ? n : 0;
+        const int upto = ca_scan(mine), slots_upto = ca_scan(slots), lists_upto = ca_scan(lists);
+        int off = at + upto - mine;
+        if (!all && a.S <= 64) {  // longest workgroups first: one that starts last would end alone
             const int key = (w.tiles + parts - 1) / parts << w.wide;
+            off = 0;
             for (int j = 0; j < a.S; ++j) {
                 const int kj = __builtin_amdgcn_readlane(key, j), mj = __builtin_amdgcn_readlane(mine, j);
                 if (kj > key || (kj == key && j < lane)) off += mj;
             }
-        } else {
-            int run = mine;
-            for (int o = 1; o < 64; o <<= 1) {
-                const int other = __shfl_up(run, o, 64);
-                run += lane >= o ? other : 0;
-            }
-            off += run - mine;
         }
-        int run = slots;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int other = __shfl_up(run, o, 64);
-            run += lane >= o ? other : 0;
-        }
-        soff += run - slots;
         const uint64_t who = __builtin_amdgcn_ballot_w64(block >= off && block - off < mine);
         if (who != 0) {
             const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
@@ -150,14 +161,20 @@ template <bool MERGE> __device__ __forceinline__ CaPlan ca_plan(const CaArgs &a,
             p.parts = __builtin_amdgcn_readlane(parts, l);
             p.items = __builtin_amdgcn_readlane(w.items, l);
             p.wide = __builtin_amdgcn_readlane(w.wide, l);
-            p.slot = __builtin_amdgcn_readlane(soff, l);
+            p.slot = slot + __builtin_amdgcn_readlane(slots_upto - slots, l);
+            p.list = list + __builtin_amdgcn_readlane(lists_upto - lists, l);
+            p.q.b = __builtin_amdgcn_readlane(w.q.b, l);
+            p.q.n = __builtin_amdgcn_readlane(w.q.n, l);
+            p.q.L = __builtin_amdgcn_readlane(w.q.L, l);
             // sequences whose rows overlap, against the documentation, may ask for more slots than there are
             if (p.parts > 1 && p.slot + p.items * a.KV * p.parts > a.slots) p.s = -1;
-            break;
+            if (block > 0) break;
         }
-        at += ca_sum(mine);
-        slot = __builtin_amdgcn_readlane(slot + run, 63);
+        at += __builtin_amdgcn_readlane(upto, 63);
+        slot += __builtin_amdgcn_readlane(slots_upto, 63);
+        list += __builtin_amdgcn_readlane(lists_upto, 63);
     }
+    p.lists = list;  // (of the whole launch in workgroup 0 only)
     return p;
 }
 
@@ -178,7 +195,13 @@ struct CaJob {
     bool split;
     float *slot;  // where its partial goes
 };
-__device__ __forceinline__ CaJob ca_job(const CaArgs &a, const CaPlan &p, const CaSeq &q, int D) {
+// What the merge needs of a split item: rows first .. end - 1 of the sequence whose first
+// token is `token`. (The list's entry 0 counts the others, in `first`.)
+struct CaItem {
+    int first, end, hk, parts, slot, token, pad[2];
+};
+__device__ __forceinline__ CaJob ca_job(const CaArgs &a, const CaPlan &p, int D) {
+    const CaSeq &q = p.q;
     CaJob j;
     j.s = p.s;
     j.hk = p.local % a.KV;  // with 8 kv heads a head's workgroups share an XCD
@@ -192,7 +215,10 @@ __device__ __forceinline__ CaJob ca_job(const CaArgs &a, const CaPlan &p, const 
     j.k0 = lo + 64 * (int)((int64_t)tiles * part / p.parts);
     j.k1 = min(hi, lo + 64 * (int)((int64_t)tiles * (part + 1) / p.parts));
     j.split = p.parts > 1;
-    j.slot = a.part + (int64_t)(p.slot + (rb * a.KV + j.hk) * p.parts + part) * a.slot_rows * (D + 4);
+    const int slot = p.slot + (rb * a.KV + j.hk) * p.parts;
+    j.slot = a.part + (int64_t)(slot + part) * a.slot_rows * (D + 4);
+    if (j.split && part == 0 && threadIdx.x == 0)
+        a.list[1 + p.list + rb * a.KV + j.hk] = {j.r0, min(j.r0 + per, j.R), j.hk, p.parts, slot, q.b, {}};
     return j;
 }
 __device__ __forceinline__ CaRule ca_rule(const CaArgs &a, const CaSeq &q, int first, int last, int row) {
@@ -505,10 +531,11 @@ template <int D, int BS>
 __global__ void __launch_bounds__(64 * CA_WAVES, D <= 128 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const CaPlan p = ca_plan<false>(a, blockIdx.x, lane);
+    const CaPlan p = ca_plan(a, blockIdx.x, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) a.list[0].first = min(p.lists, a.slots / 2);
     if (p.s < 0) return;
-    const CaSeq sq = ca_seq(a, p.s);
-    const CaJob j = ca_job(a, p, sq, D);
+    const CaSeq &sq = p.q;
+    const CaJob j = ca_job(a, p, D);
     if (p.wide) ca_many<D, BS>(a, sq, j, T0, T1, aux, lane, wave);
     else ca_few<D, BS>(a, sq, j, T0, T1, aux, lane, wave);
 }
@@ -517,17 +544,18 @@ __global__ void __launch_bounds__(64 * CA_WAVES, D <= 128 ? 2 : 1) k_chunk_attn(
 // then take the dims.
 constexpr int CA_MERGE_ROWS = 8;  // of a workgroup
 template <int D> __global__ void __launch_bounds__(256) k_chunk_attn_merge(const CaArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const CaPlan p = ca_plan<true>(a, blockIdx.x, lane);
-    if (p.s < 0) return;
-    const CaSeq sq = ca_seq(a, p.s);
-    const int np = p.parts, hk = p.local % a.KV, rb = p.local / a.KV, per = p.wide ? 128 : 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int count = a.list[0].first;
+    const CaItem it = a.list[1 + blockIdx.x];
+    if ((int)blockIdx.x >= count) return;
+    const CaSeq sq = {it.token, 0, 0};
+    const int np = it.parts;
     const int64_t step = (int64_t)a.slot_rows * (D + 4);
     constexpr int E = (D + 63) / 64, AT_ONCE = 8;
     for (int r = blockIdx.y * CA_MERGE_ROWS + wave; r < (int)(blockIdx.y + 1) * CA_MERGE_ROWS; r += 4) {
-        const int row = per * rb + r;
-        if (r >= per || row >= sq.n * a.G) return;
-        const float *base = a.part + (int64_t)(p.slot + p.local * np) * step + r * (D + 4);
+        const int row = it.first + r;
+        if (row >= it.end) return;
+        const float *base = a.part + it.slot * step + r * (D + 4);
         // the first partitions' sums are on their way while the weights are formed
         float o[AT_ONCE][E];
         auto load = [&](int p0) {
@@ -557,7 +585,7 @@ template <int D> __global__ void __launch_bounds__(256) k_chunk_attn_merge(const
                 for (int e = 0; e < E; ++e) acc[e] += wp * o[i][e];
             }
         }
-        uint16_t *dst = (uint16_t *)ca_out<D>(a, sq, hk, row);
+        uint16_t *dst = (uint16_t *)ca_out<D>(a, sq, it.hk, row);
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (lane + 64 * e < D) dst[lane + 64 * e] = f2h(acc[e] * inv);
@@ -584,9 +612,11 @@ static CaBounds ca_bounds(const tlh_chunk_attention_args &a) {
     return b;
 }
 
+// The list of split items (each has two slots at least), then the slots.
+static int64_t ca_list_bytes(const CaBounds &b) { return b.slots == 0 ? 0 : (int64_t)sizeof(CaItem) * (1 + b.slots / 2); }
 size_t chunk_attention_scratch_bytes(const tlh_chunk_attention_args &a) {
     const CaBounds b = ca_bounds(a);
-    return (size_t)(b.slots * b.slot_rows * (a.head_size + 4) * sizeof(float));
+    return (size_t)(ca_list_bytes(b) + b.slots * b.slot_rows * (a.head_size + 4) * (int64_t)sizeof(float));
 }
 
 template <int D> static void launch_ca(const CaArgs &c, int bs, const CaBounds &b, hipStream_t stream) {
@@ -597,7 +627,7 @@ template <int D> static void launch_ca(const CaArgs &c, int bs, const CaBounds &
     default: hipLaunchKernelGGL((k_chunk_attn<D, 32>), grid, threads, 0, stream, c); break;
     }
     if (b.parts > 1)
-        hipLaunchKernelGGL((k_chunk_attn_merge<D>), dim3((unsigned)std::min(b.items, b.wgs / 2), (unsigned)(b.slot_rows / CA_MERGE_ROWS)),
+        hipLaunchKernelGGL((k_chunk_attn_merge<D>), dim3((unsigned)std::min(b.items, b.slots / 2), (unsigned)(b.slot_rows / CA_MERGE_ROWS)),
                            dim3(256), 0, stream, c);
 }
 
@@ -607,7 +637,8 @@ tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scrat
     c.out = (uint8_t *)a.out, c.q = (const uint8_t *)a.q, c.so = 2 * a.out_stride, c.sq = 2 * a.q_stride;
     c.kc = (const uint16_t *)a.k_cache, c.vc = (const uint16_t *)a.v_cache;
     c.tables = a.block_tables, c.lens = a.context_lens, c.starts = a.row_starts;
-    c.part = (float *)scratch;
+    c.list = (CaItem *)scratch;
+    c.part = (float *)((uint8_t *)scratch + ca_list_bytes(b));
     c.num_blocks = a.num_blocks;
     c.S = a.num_seqs, c.KV = a.num_kv_heads, c.G = a.num_heads / a.num_kv_heads;
     c.rows = a.num_rows, c.max_rows = a.max_rows, c.max_blocks = a.max_blocks_per_seq, c.max_ctx = a.max_context_len;

@@ -36,7 +36,7 @@ template <int D, int BS, class Rule> struct PagedWave {
     const PagedArgs &a;
     const int lane, h, c;
     const int32_t *table;
-    const int64_t page_bytes;
+    const uint32_t page_bytes;  // at most 65535 x 256 x 32 x 2
     const uint8_t *kbase, *vbase;
     const int kappa;  // the key of S^T's row c: bits 2 and 3 of c exchanged
     const int L;  // tokens in the cache
@@ -44,7 +44,7 @@ template <int D, int BS, class Rule> struct PagedWave {
 
     __device__ __forceinline__ PagedWave(const PagedArgs &a_, int lane_, int s, int hk, int L_, const Rule &rule_)
         : a(a_), lane(lane_), h(lane_ >> 5), c(lane_ & 31), table(a_.tables + (int64_t)s * a_.max_blocks),
-          page_bytes((int64_t)a_.KV * D * BS * 2), kbase((const uint8_t *)a_.kc + (int64_t)hk * D * BS * 2),
+          page_bytes((uint32_t)a_.KV * D * BS * 2), kbase((const uint8_t *)a_.kc + (int64_t)hk * D * BS * 2),
           vbase((const uint8_t *)a_.vc + (int64_t)hk * D * BS * 2),
           kappa((c & 0x13) | (c & 4) << 1 | (c & 8) >> 1), L(L_), rule(rule_) {}
 
@@ -76,7 +76,7 @@ template <int D, int BS, class Rule> struct PagedWave {
         int id = p.id[0];
 #pragma unroll
         for (int i = 1; i < PAGES; ++i) id = key / BS == i ? p.id[i] : id;
-        return (int64_t)id * page_bytes;
+        return (int64_t)((uint64_t)(uint32_t)id * page_bytes);
     }
     // this lane's 16 bytes of the keys' step st are k_at() + k_step(st), of the values'
     // keys 16 i + 8 h .. + 7 and dims 32 d .. + 31 v_at(i) + v_step(d)
