@@ -423,58 +423,75 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
         for (int st = 0; st < NS; ++st) qf[st] = w.signed_q(*(const uint4 *)(qr + 32 * st));
     }
     bool careful = false;
-    auto tile = [&](int t, const uint8_t *T, uint8_t *Tn) {
+    auto tile = [&](int t, uint8_t *T, uint8_t *Tn) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): tile t has landed
         lds_barrier();                       // for every wave, and the other buffer is free
-        uint32_t good[SUBS];
+        const int k0 = j.k0 + KT * t;
+        uint32_t good[SUBS], there[SUBS];
+        bool gaps = false;
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u) good[u] = pg[u].good;
+        for (int u = 0; u < SUBS; ++u) {
+            good[u] = pg[u].good;
+            there[u] = w.there(k0 + 32 * u, good[u]);
+            gaps = gaps || there[u] != ~0u;
+        }
         if (t + 1 < ntiles) {
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) pg[u] = w.checked(pn[u]);
             load_tile(pg, Tn);
             ids(t + 2, pn);
         }
-        const int k0 = j.k0 + KT * t;
+        if (gaps) {  // places that hold no token's value may hold anything: zeroed by the waves that loaded them
+#pragma unroll 1
+            for (int f = wave; f < 2 * SUBS * NB; f += CA_WAVES) {
+                uint4 *v = (uint4 *)(T + (KF + f) * 1024) + lane;
+                const int i = f / NB;
+                *v = w.live_v(*v, i & 1, SUBS == 1 || i < 2 ? there[0] : there[SUBS - 1]);
+            }
+            lds_barrier();
+        }
         if (!mine || k0 > any_hi || k0 + KT - 1 < any_lo) return;  // nothing visible to the wave's rows
         f32x16 S[SUBS];
-        PagedSeen see[SUBS];
+        bool whole = true;
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
             S[u] = (f32x16){};
 #pragma unroll
             for (int st = 0; st < NS; ++st)
                 S[u] = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S[u]);
-            see[u] = w.seen(k0 + 32 * u, good[u]);
+            whole = whole && w.rule.whole(k0 + 32 * u) && good[u] == ~0u;
+        }
+        if (!whole) {
+            w.some_masked = true;
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) w.hide(S[u], w.rule.sees(k0 + 32 * u) & there[u]);
         }
         uint4 pf[2 * SUBS];
-        w.softmax(S, see, pf);
+        PagedSeen see[SUBS];
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u) {
-            const uint8_t *V = T + (KF + u * 2 * NB) * 1024;
-            if (careful && !see[u].whole) {
-                uint4 *sp = (uint4 *)aux + 128 * wave;
+        for (int u = 0; u < SUBS; ++u) see[u] = {true, ~0u, ~0u};
+        w.softmax(S, see, pf);
+        if (careful && !whole) {
+            uint4 *sp = (uint4 *)aux + 128 * wave;
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+                see[u].vis = w.rule.sees(k0 + 32 * u) & there[u];
                 __builtin_amdgcn_wave_barrier();
                 sp[lane] = pf[2 * u], sp[64 + lane] = pf[2 * u + 1];
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int d = 0; d < NB; ++d)
-                    w.careful_pv(d, see[u], (const uint32_t *)sp, (const uint32_t *)(V + d * 1024), 256 * NB);
-            } else if (see[u].there != ~0u) {
-#pragma unroll 1
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int d = 0; d < NB; ++d)
-                        w.O[d] = mfma32<false>(w.live_v(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), i, see[u].there),
-                                               i ? pf[2 * u + 1] : pf[2 * u], w.O[d]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int d = 0; d < NB; ++d)
-                        w.O[d] = mfma32<false>(*(const uint4 *)(V + (i * NB + d) * 1024 + 16 * lane), pf[2 * u + i], w.O[d]);
+                    w.careful_pv(d, see[u], (const uint32_t *)sp, (const uint32_t *)(T + (KF + u * 2 * NB + d) * 1024), 256 * NB);
             }
+            return;
         }
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int d = 0; d < NB; ++d)
+                    w.O[d] = mfma32<false>(*(const uint4 *)(T + (KF + (2 * u + i) * NB + d) * 1024 + 16 * lane), pf[2 * u + i], w.O[d]);
     };
     for (;;) {
         w.reset();

@@ -117,26 +117,31 @@ template <int D, int BS, class Rule> struct PagedWave {
         return x;
     }
 
-    // what the wave's rows see of the 32 keys at `base`
+    // which of the 32 keys at `base` are in the cache
+    __device__ __forceinline__ uint32_t there(int base, uint32_t good) const {
+        return L <= base ? 0u : good & (L - base >= 32 ? ~0u : (1u << (L - base)) - 1);
+    }
+    // what the wave's rows see of them
     __device__ __forceinline__ PagedSeen seen(int base, uint32_t good) {
         PagedSeen s = {rule.whole(base) && good == ~0u, ~0u, ~0u};
         if (!s.whole) {
             some_masked = true;
-            s.there = L <= base ? 0u : good & (L - base >= 32 ? ~0u : (1u << (L - base)) - 1);
+            s.there = there(base, good);
             s.vis = rule.sees(base) & s.there;
         }
         return s;
+    }
+    __device__ __forceinline__ void hide(f32x16 &S, uint32_t vis) const {
+        const uint32_t mine = vis >> (8 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[i] = -INFINITY;
     }
     // scores of U x 32 keys -> numerators (f16), the running maximum and sum
     template <int U> __device__ __forceinline__ void softmax(f32x16 (&S)[U], const PagedSeen (&s)[U], uint4 (&pf)[2 * U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (!s[u].whole) {
-                const uint32_t mine = s[u].vis >> (8 * h);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[u][i] = -INFINITY;
-            }
+            if (!s[u].whole) hide(S[u], s[u].vis);
         float mx = S[0][0];
 #pragma unroll
         for (int u = 0; u < U; ++u)
