@@ -500,7 +500,8 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  *                q_stride and out_stride elements from token to token (multiples of 8)
  *   row_starts   i32 [num_seqs + 1]: sequence s has the rows row_starts[s] ..
  *                row_starts[s + 1] - 1, n of them, at most max_rows (starts do not
- *                decrease); rows behind the last sequence are left as they were
+ *                decrease, or nothing is computed); rows behind the last sequence
+ *                are left as they were
  * With L = context_lens[s], row i of the sequence is the token at place L - n + i and
  * sees the tokens up to itself, with window > 0 the last `window` of them. f32 scores,
  * softmax and sums, its numerators rounded to f16 for the product with v (those below
@@ -513,7 +514,9 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  * No row of out may overlap a row of q (other columns of the same rows do not) or the
  * caches. `scratch` holds the partials of split contexts (tlh_chunk_attention_scratch_bytes,
  * which never shrinks as a count grows, 16-byte aligned; it may be NULL when that is
- * 0); calls that share one must be stream-ordered. */
+ * 0). Its first TLH_CHUNK_COUNTER_BYTES must be zero before its first call, and every call
+ * leaves them zero; calls that share one must be stream-ordered. */
+#define TLH_CHUNK_COUNTER_BYTES ((size_t)8192)
 typedef struct tlh_chunk_attention_args {
     void *out;
     const void *q;

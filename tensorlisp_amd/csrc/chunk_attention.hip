@@ -19,8 +19,11 @@
 // Items differ by orders of magnitude in keys, and only the device knows the lengths. So
 // every workgroup works out the same plan from them: how many tiles a workgroup takes
 // so that all run at once, and from that the partitions of every sequence's keys. The
-// partitions are joined in a second launch.
+// last of an item's partitions to arrive joins them, in the order of their keys, whichever
+// it is. (Joined in a second launch, whose code has to come from memory when the keys
+// have gone through the caches, 31 tokens + 600 took 20 us more.)
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_wave.hpp"
 
@@ -28,50 +31,66 @@ namespace tlh {
 
 constexpr int CA_WAVES = 4;
 constexpr int CA_NARROW = 64;      // rows of a (sequence, kv head) up to which a workgroup takes 32
-constexpr int CA_MAX_PARTS = 64;   // a lane each in the merge
-constexpr int CA_MIN_TILES = 2;    // 64-key tiles of a partition, at least: a round of the four waves
+// A partition costs a partial written and read, and the join waits for eight of them at a
+// time. So at most 32 of an item (1 token over 8000, us: 15.4 with 32, 17.5 with 42), each
+// of at least 2 tiles of 64 keys, a round of the four waves, or with more than 8 rows of 8
+// (4 x 16 tokens over 100..3000, us, with 3, 6, 9: 22.0, 21.5, 18.3; 64 tokens over 3000 with
+// 2, 4, 6, 8: 45, 31, 28.5, 29.6; 1 token over 1500 with 3, 6, 9: 10.2, 11.0, 11.9).
+constexpr int CA_MAX_PARTS = 32, CA_MIN_TILES = 2, CA_MIN_TILES_ROWS = 8;
 constexpr int CA_NO_WINDOW = 1 << 30;
+
+// n / d for 0 <= n < 2^31 by a product. What every workgroup runs before its first load is
+// kept short: its code comes from memory where another kernel's was last.
+struct CaDiv {
+    uint32_t mul, shift, by;
+    __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+    __device__ __forceinline__ int rest(int n) const { return n - (*this)(n) * (int)by; }
+};
+static CaDiv ca_div(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return {(uint32_t)((1ull << (31 + s)) / (uint64_t)d + 1), (uint32_t)(31 + s), (uint32_t)d};
+}
 
 struct CaArgs : PagedArgs {
     uint8_t *out;
     const uint8_t *q;
     int64_t so, sq;  // bytes from token to token
     const int32_t *lens, *starts;
-    float *part;     // [slot][slot_rows][m, l, -, -, D]
-    struct CaItem *list;
-    int S, G, rows, max_rows, max_ctx, window, wgs, slots, slot_rows;
+    float *part;     // units of 4 rows of ca_row(D) floats
+    unsigned *counters;  // of an item's partitions that have arrived; 0 before and after a call
+    int S, rows, max_rows, max_ctx, window;
+    int lg_wgs;          // workgroups that fill the machine, a power of two
+    int span_few, span_many;  // keys that some row of a block of 32 and of 128 rows sees
+    CaDiv G, kv;
 };
 
 struct CaSeq {
-    int b, n, L;  // first row, new tokens, tokens in the cache
+    int b, n, L;  // first row, new tokens (below 0: the sequence ends before it starts), tokens in the cache
 };
 __device__ __forceinline__ CaSeq ca_seq(const CaArgs &a, int s) {
     CaSeq q;
     q.b = max(0, min(a.starts[s], a.rows));
-    const int e = max(q.b, min(a.starts[s + 1], a.rows));
-    q.n = min(e - q.b, a.max_rows);
+    q.n = min(max(0, min(a.starts[s + 1], a.rows)) - q.b, a.max_rows);
     q.L = a.num_blocks > 0 ? max(0, min(a.lens[s], a.max_ctx)) : 0;
     return q;
 }
 
 // A sequence's items a kv head and the 64-key tiles that the largest of them sees
 struct CaWork {
-    int items, tiles, wide;
+    int items, tiles, wide, units;  // units of 4 rows of an item's partial
     CaSeq q;
 };
-__host__ __device__ __forceinline__ int ca_tiles(int L, int G, int window, int rows) {
-    const int64_t span = (int64_t)window + (rows - 1) / G + 1;  // keys that some row of a block of `rows` sees
-    return L <= span ? (L + 63) / 64 : (int)((span + 63) / 64) + 1;
-}
+__host__ __device__ __forceinline__ int ca_tiles(int L, int span) { return L <= span ? (L + 63) >> 6 : ((span + 63) >> 6) + 1; }
 __device__ __forceinline__ CaWork ca_work(const CaArgs &a, int s) {
     CaWork w = {};
     if (s >= a.S) return w;
     const CaSeq q = w.q = ca_seq(a, s);
-    const int R = q.n * a.G;
+    const int R = max(q.n, 0) * (int)a.G.by;
     w.wide = R > CA_NARROW;
-    const int per = w.wide ? 128 : 32;
-    w.items = (R + per - 1) / per;
-    w.tiles = ca_tiles(q.L, a.G, a.window, per);
+    w.items = w.wide ? (R + 127) >> 7 : (R + 31) >> 5;
+    w.units = w.wide ? 32 : (min(R, 32) + 3) >> 2;
+    w.tiles = ca_tiles(q.L, w.wide ? a.span_many : a.span_few);
     return w;
 }
 
@@ -87,66 +106,77 @@ __device__ __forceinline__ int ca_scan(int v) {
     return v;
 }
 __device__ __forceinline__ int ca_sum(int v) { return __builtin_amdgcn_readlane(ca_scan(v), 63); }
-// ceil(tiles / each), at least 1 and at most CA_MAX_PARTS
-__device__ __forceinline__ int ca_parts(int tiles, int each, float inv) {
-    if (tiles >= (int64_t)CA_MAX_PARTS * each) return CA_MAX_PARTS;
-    const int q = (int)((float)tiles * inv);  // off by at most 1
-    const int r = tiles - q * each;
-    return max(1, q + (r > 0) + (r > each) - (r <= -each));
+// a sequence's partitions of at most `each` tiles: ceil(tiles / each), within the bounds
+__device__ __forceinline__ int ca_parts(const CaWork &w, int each) {
+    const int n = max(each, w.units > 2 ? CA_MIN_TILES_ROWS : CA_MIN_TILES);
+    if (w.tiles >= (int64_t)CA_MAX_PARTS * n) return CA_MAX_PARTS;
+    const int q = (int)((float)w.tiles * __builtin_amdgcn_rcpf((float)n));  // off by at most 1
+    const int r = w.tiles - q * n;
+    return max(1, q + (r > 0) + (r > n) - (r <= -n));
 }
 
 // What a workgroup does. Every lane calls; a lane looks at one sequence of 64 at a time.
 struct CaPlan {
-    int s, local, parts, items, wide, slot;  // s < 0: nothing; slot: the sequence's first
-    int list, lists;                         // the first of the sequence's split items, and how many there are in all
+    int s, local, parts, items, wide, units;  // s < 0: nothing
+    int unit, counter;  // the first ones of the sequence's
     CaSeq q;
 };
 __device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) {
     const CaWork first = ca_work(a, lane);
     auto work = [&](int g) { return g == 0 ? first : ca_work(a, g + lane); };
-    // tiles of a workgroup if all had as many
-    uint64_t total = 0;
-    for (int g = 0; g < a.S; g += 64) {
-        const CaWork w = work(g);
-        const uint64_t n = (uint64_t)w.items * (uint64_t)w.tiles;  // in two parts: 64 of either fit 32 bits
-        total += (uint64_t)(uint32_t)ca_sum((int)(n & 0xffffff)) + ((uint64_t)(uint32_t)ca_sum((int)(n >> 24)) << 24);
-    }
-    const int even = (int)min(max((total * a.KV + a.wgs - 1) / a.wgs, (uint64_t)CA_MIN_TILES), (uint64_t)1 << 26);
-    // Partitions are whole, so with that many some workgroups are left over, to run alone
-    // after the others: the first of a few larger numbers that leaves none. With more
-    // items than workgroups none does, and the last one splits only what is much longer
-    // than the others.
-    constexpr int TRIES = 5;
-    const int eighths[TRIES] = {8, 9, 10, 12, 16};
-    int each[TRIES], count[TRIES] = {};
-    float inv[TRIES];
-#pragma unroll
-    for (int i = 0; i < TRIES; ++i) each[i] = (even * eighths[i] + 7) / 8, inv[i] = 1.0f / (float)each[i];
-    for (int g = 0; g < a.S; g += 64) {
-        const CaWork w = work(g);
-        const int n = (int)min((int64_t)w.items * a.KV, (int64_t)1 << 18);
-#pragma unroll
-        for (int i = 0; i < TRIES; ++i)
-            count[i] = min(count[i] + ca_sum(min(n * ca_parts(w.tiles, each[i], inv[i]), 1 << 18)), 1 << 24);
-    }
-    int take = each[TRIES - 1];
-    float take_inv = inv[TRIES - 1];
-    bool all = false;
-#pragma unroll
-    for (int i = TRIES - 1; i >= 0; --i)
-        if (count[i] <= a.wgs) take = each[i], take_inv = inv[i], all = true;
-
+    const int KV = (int)a.kv.by, wgs = 1 << a.lg_wgs;
+    // tiles, of the sequences with few rows and of the others
+    uint64_t few = 0, many = 0;
     CaPlan p = {};
     p.s = -1;
-    int at = 0, slot = 0, list = 0;
     for (int g = 0; g < a.S; g += 64) {
         const CaWork w = work(g);
-        const int parts = ca_parts(w.tiles, take, take_inv), n = w.items * a.KV;
-        const int mine = n * parts, slots = parts > 1 ? mine : 0, lists = parts > 1 ? n : 0;
-        const int upto = ca_scan(mine), slots_upto = ca_scan(slots), lists_upto = ca_scan(lists);
+        // Starts that decrease make sequences overlap, and more work than there is room for:
+        // then nothing is computed.
+        if (__builtin_amdgcn_ballot_w64(w.q.n < 0) != 0) return p;
+        const uint64_t n = (uint64_t)w.items * (uint32_t)w.tiles;  // in two parts: 64 of either fit 32 bits
+        const int lo = (int)(n & 0xffffff), hi = (int)(n >> 24);
+        few += (uint64_t)(uint32_t)ca_sum(w.wide ? 0 : lo) + ((uint64_t)(uint32_t)ca_sum(w.wide ? 0 : hi) << 24);
+        many += (uint64_t)(uint32_t)ca_sum(w.wide ? lo : 0) + ((uint64_t)(uint32_t)ca_sum(w.wide ? hi : 0) << 24);
+    }
+    const uint64_t total = (few + many) * KV;
+    auto share = [&](uint64_t tiles, int lg) {  // of one of 2^lg workgroups
+        return (int)min(max((tiles + (1u << lg) - 1) >> lg, (uint64_t)CA_MIN_TILES), (uint64_t)1 << 26);
+    };
+    const int even = share(total, a.lg_wgs);
+    // Few rows: no workgroup takes more than 1.5 even shares. (us with 0.5, 1, 1.5, 2: 32
+    // tokens over 512..8192 120, 123, 113, 117; 8 over 8000 57, 50, 47, 45; 24 over 100..30000
+    // 282, 283, 267, 290; 1 over 100000 85, 85, 90, 79.)
+    const int each_few = (even * 3 + 1) >> 1;
+    // Many rows: partitions are whole, so with an even share some workgroups are left over,
+    // to run alone after the others: the first of a few larger shares, up to twice the even
+    // one, that leaves none. With more items than workgroups none does, and the last one
+    // splits only what is much longer than the others.
+    int each_many = even, count = 0;
+    if (many > 0)
+#pragma unroll 1
+        for (int eighths = 8;; eighths += eighths < 10 ? 1 : eighths == 10 ? 2 : 4) {
+            each_many = (even * eighths + 7) >> 3;
+            count = 0;
+            for (int g = 0; g < a.S; g += 64) {
+                const CaWork w = work(g);
+                const int n = w.wide ? (int)min((int64_t)w.items * KV, (int64_t)1 << 18) : 0;
+                count = min(count + ca_sum(min(n * ca_parts(w, each_many), 1 << 18)), 1 << 24);
+            }
+            if (count <= wgs || eighths == 16) break;
+        }
+    // all run at once: their order does not matter
+    const bool all = few == 0 ? count <= wgs : total <= (uint64_t)(wgs * CA_MIN_TILES);
+
+    int at = 0, unit = 0, counter = 0;
+    for (int g = 0; g < a.S; g += 64) {
+        const CaWork w = work(g);
+        const int parts = ca_parts(w, w.wide ? each_many : each_few), n = w.items * KV;
+        const int mine = n * parts, units = parts > 1 ? mine * w.units : 0, counters = parts > 1 ? n : 0;
+        const int upto = ca_scan(mine), units_upto = ca_scan(units), counters_upto = ca_scan(counters);
         int off = at + upto - mine;
         if (!all && a.S <= 64) {  // longest workgroups first: one that starts last would end alone
-            const int key = (w.tiles + parts - 1) / parts << w.wide;
+            const int key = (int)((float)w.tiles / (float)parts) << w.wide;
             off = 0;
             for (int j = 0; j < a.S; ++j) {
                 const int kj = __builtin_amdgcn_readlane(key, j), mj = __builtin_amdgcn_readlane(mine, j);
@@ -161,20 +191,18 @@ __device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) 
             p.parts = __builtin_amdgcn_readlane(parts, l);
             p.items = __builtin_amdgcn_readlane(w.items, l);
             p.wide = __builtin_amdgcn_readlane(w.wide, l);
-            p.slot = slot + __builtin_amdgcn_readlane(slots_upto - slots, l);
-            p.list = list + __builtin_amdgcn_readlane(lists_upto - lists, l);
+            p.units = __builtin_amdgcn_readlane(w.units, l);
+            p.unit = unit + __builtin_amdgcn_readlane(units_upto - units, l);
+            p.counter = counter + __builtin_amdgcn_readlane(counters_upto - counters, l);
             p.q.b = __builtin_amdgcn_readlane(w.q.b, l);
             p.q.n = __builtin_amdgcn_readlane(w.q.n, l);
             p.q.L = __builtin_amdgcn_readlane(w.q.L, l);
-            // sequences whose rows overlap, against the documentation, may ask for more slots than there are
-            if (p.parts > 1 && p.slot + p.items * a.KV * p.parts > a.slots) p.s = -1;
-            if (block > 0) break;
+            break;
         }
         at += __builtin_amdgcn_readlane(upto, 63);
-        slot += __builtin_amdgcn_readlane(slots_upto, 63);
-        list += __builtin_amdgcn_readlane(lists_upto, 63);
+        unit += __builtin_amdgcn_readlane(units_upto, 63);
+        counter += __builtin_amdgcn_readlane(counters_upto, 63);
     }
-    p.lists = list;  // (of the whole launch in workgroup 0 only)
     return p;
 }
 
@@ -189,48 +217,75 @@ struct CaRule {
     }
 };
 
+// Floats of a row of a partial: of few rows [m, l, -, -, D], of many the lanes' registers as
+// they are (whole blocks of 32 dims), which 64 lanes write and read in one piece.
+__host__ __device__ constexpr int ca_row(int D) { return (D + 31) / 32 * 32 + 4; }
+
 // One partition of an item: rows r0 .. (of R), keys k0 .. k1 - 1, k0 a multiple of 64
 struct CaJob {
     int s, hk, r0, R, k0, k1;
-    bool split;
-    float *slot;  // where its partial goes
-};
-// What the merge needs of a split item: rows first .. end - 1 of the sequence whose first
-// token is `token`. (The list's entry 0 counts the others, in `first`.)
-struct CaItem {
-    int first, end, hk, parts, slot, token, pad[2];
+    int part, parts;
+    float *slots;       // the item's partials, `step` floats apart
+    int step;
+    unsigned *counter;  // the item's
 };
 __device__ __forceinline__ CaJob ca_job(const CaArgs &a, const CaPlan &p, int D) {
     const CaSeq &q = p.q;
     CaJob j;
     j.s = p.s;
-    j.hk = p.local % a.KV;  // with 8 kv heads a head's workgroups share an XCD
-    const int r = p.local / a.KV, rb = p.items - 1 - r % p.items, part = r / p.items;  // last rows first: they see the most
+    const int r = a.kv(p.local);
+    j.hk = p.local - r * a.KV;  // with 8 kv heads a head's workgroups share an XCD
+    const int part = (uint32_t)r / (uint32_t)p.items, rb = p.items - 1 - (r - part * p.items);  // last rows first: they see the most
     const int per = p.wide ? 128 : 32;
-    j.R = q.n * a.G;
+    j.R = q.n * (int)a.G.by;
     j.r0 = per * rb;
-    const int last = (min(j.r0 + per, j.R) - 1) / a.G;  // tokens r0 / G .. last
-    const int lo = max(0, q.L - q.n + j.r0 / a.G - a.window + 1) & ~63, hi = q.L - q.n + last + 1;
-    const int tiles = hi > lo ? (hi - lo + 63) / 64 : 0;
-    j.k0 = lo + 64 * (int)((int64_t)tiles * part / p.parts);
-    j.k1 = min(hi, lo + 64 * (int)((int64_t)tiles * (part + 1) / p.parts));
-    j.split = p.parts > 1;
-    const int slot = p.slot + (rb * a.KV + j.hk) * p.parts;
-    j.slot = a.part + (int64_t)(slot + part) * a.slot_rows * (D + 4);
-    if (j.split && part == 0 && threadIdx.x == 0)
-        a.list[1 + p.list + rb * a.KV + j.hk] = {j.r0, min(j.r0 + per, j.R), j.hk, p.parts, slot, q.b, {}};
+    const int last = a.G(min(j.r0 + per, j.R) - 1);  // tokens r0 / G .. last
+    const int lo = max(0, q.L - q.n + a.G(j.r0) - a.window + 1) & ~63, hi = q.L - q.n + last + 1;
+    const uint32_t tiles = hi > lo ? (hi - lo + 63) >> 6 : 0, parts = p.parts;  // < 2^25, <= 64
+    j.k0 = lo + 64 * (int)(tiles * part / parts);
+    j.k1 = min(hi, lo + 64 * (int)(tiles * (part + 1) / parts));
+    const int item = rb * a.KV + j.hk;
+    j.part = part, j.parts = p.parts;
+    j.step = p.units * 4 * ca_row(D);
+    j.slots = a.part + (int64_t)(p.unit + item * p.parts * p.units) * 4 * ca_row(D);
+    j.counter = a.counters + p.counter + item;
     return j;
+}
+
+// Partials pass between workgroups, which may run on different XCDs: relaxed agent-scope
+// stores and loads, which on gfx950 go past the XCD's L2 (no write-back or invalidation
+// of all of it, which would cost the others the pages that they share).
+__device__ __forceinline__ void ca_put(float *p, float x, float y) {
+    __hip_atomic_store((uint64_t *)p, (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 ca_get(const float *p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+// Whether this workgroup is the last of its item's to have written its partial. That each
+// wave's stores are complete (its wait) before the counter moves (behind the barrier), and
+// that the loads behind it do not look in an older copy, rests on the above.
+__device__ __forceinline__ bool ca_last(const CaJob &j, int *flag) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = __hip_atomic_fetch_add(j.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)j.parts;
+        if (last) __hip_atomic_store(j.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    return *flag != 0;
 }
 __device__ __forceinline__ CaRule ca_rule(const CaArgs &a, const CaSeq &q, int first, int last, int row) {
     const int p = q.L - q.n;
-    const int at = p + row / a.G;
-    return {at - a.window + 1, at, p + last / a.G - a.window + 1, p + first / a.G};
+    const int at = p + a.G(row);
+    return {at - a.window + 1, at, p + a.G(last) - a.window + 1, p + a.G(first)};
 }
 template <int D> __device__ __forceinline__ const uint8_t *ca_q(const CaArgs &a, const CaSeq &q, int hk, int row) {
-    return a.q + (int64_t)(q.b + row / a.G) * a.sq + (int64_t)(hk * a.G + row % a.G) * D * 2;
+    return a.q + (int64_t)(q.b + a.G(row)) * a.sq + (int64_t)(hk * (int)a.G.by + a.G.rest(row)) * D * 2;
 }
 template <int D> __device__ __forceinline__ uint8_t *ca_out(const CaArgs &a, const CaSeq &q, int hk, int row) {
-    return a.out + (int64_t)(q.b + row / a.G) * a.so + (int64_t)(hk * a.G + row % a.G) * D * 2;
+    return a.out + (int64_t)(q.b + a.G(row)) * a.so + (int64_t)(hk * (int)a.G.by + a.G.rest(row)) * D * 2;
 }
 
 // LDS of a workgroup, in two parts that the compiler can tell apart (a tile is loaded
@@ -245,7 +300,7 @@ template <int D> struct CaLds {
 // --------------------------------------------------------------- few rows
 template <int D, int BS>
 __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const CaJob &j, uint8_t *T0, uint8_t *T1, uint8_t *aux,
-                                       int lane, int wave) {
+                                       int *flag, int lane, int wave) {
     using W = PagedWave<D, BS, CaRule>;
     constexpr int NS = W::NS, NB = W::NB, MD = CaLds<D>::MD;
     // Loads a tile ahead, where two waves' registers hold O, the keys and the values; above
@@ -364,24 +419,83 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
                 sum += f * s_l[x][r];
                 o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
             }
-            if (!j.split) {
+            if (j.parts == 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const float x[8] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv, 0, 0, 0, 0};
                 const uint4 v = pack8<false>(x);
                 *(uint2 *)(ca_out<D>(a, sq, j.hk, rr) + 2 * dim) = make_uint2(v.x, v.y);
             } else {
-                float *dst = j.slot + r * (D + 4);
-                *(float4 *)(dst + 4 + dim) = o;
-                if (dim == 0) *(float2 *)dst = make_float2(M, sum);
+                float *dst = j.slots + j.part * j.step + r * ca_row(D);
+                ca_put(dst + 4 + dim, o.x, o.y), ca_put(dst + 6 + dim, o.z, o.w);
+                if (dim == 0) ca_put(dst, M, sum);
             }
         }
+    }
+    if (j.parts == 1 || !ca_last(j, flag)) return;
+    // a thread takes four dims of a row
+#pragma unroll 1
+    for (int e = threadIdx.x; e < min(32, j.R - j.r0) * (D / 4); e += 64 * CA_WAVES) {
+        const int r = e / (D / 4), dim = 4 * (e % (D / 4));
+        const float *src = j.slots + r * ca_row(D);
+        float M = -INFINITY, sum = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        constexpr int AT_ONCE = 8;
+#pragma unroll 1
+        for (int p0 = 0; p0 < j.parts; p0 += AT_ONCE) {
+            float2 ml[AT_ONCE], lo[AT_ONCE], hi[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float *x = src + min(p0 + i, j.parts - 1) * j.step;
+                ml[i] = ca_get(x), lo[i] = ca_get(x + 4 + dim), hi[i] = ca_get(x + 6 + dim);
+            }
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, ml[i].x);
+            const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((M - top) * a.cs);
+            M = top;
+            sum *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                if (p0 + i >= j.parts) break;
+                if (ml[i].x == -INFINITY && !(ml[i].y != 0.0f)) continue;  // saw nothing
+                const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml[i].x - M) * a.cs);
+                sum += w * ml[i].y;
+                o.x += w * lo[i].x, o.y += w * lo[i].y, o.z += w * hi[i].x, o.w += w * hi[i].y;
+            }
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float x[8] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv, 0, 0, 0, 0};
+        const uint4 v = pack8<false>(x);
+        *(uint2 *)(ca_out<D>(a, sq, j.hk, j.r0 + r) + 2 * dim) = make_uint2(v.x, v.y);
     }
 }
 
 // -------------------------------------------------------------- many rows
+// use(f, fragment f) for N 1-KiB fragments in LDS, read BATCH at a time and a batch
+// ahead of their use: left to itself the compiler reads each right before its product.
+template <int N, typename Use> __device__ __forceinline__ void ca_stream(const uint8_t *at, Use use) {
+    constexpr int BATCH = 4;
+    uint4 f[2][BATCH];
+    auto read = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (BATCH * b + i < N) f[b & 1][i] = *(const uint4 *)(at + (BATCH * b + i) * 1024);
+    };
+    read(0);
+#pragma unroll
+    for (int b = 0; BATCH * b < N; ++b) {
+        read(b + 1);
+        __builtin_amdgcn_sched_barrier(0x6);  // vector and scalar arithmetic may pass, reads and products not
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (BATCH * b + i < N) use(BATCH * b + i, f[b & 1][i]);
+        __builtin_amdgcn_sched_barrier(0x6);
+    }
+}
+
 template <int D, int BS>
 __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const CaJob &j, uint8_t *T0, uint8_t *T1, uint8_t *aux,
-                                        int lane, int wave) {
+                                        int *flag, int lane, int wave) {
     using W = PagedWave<D, BS, CaRule>;
     using Sh = PagedTile<D>;
     constexpr int NS = W::NS, NB = W::NB, KT = Sh::KT, SUBS = KT / 32, KF = SUBS * NS;
@@ -422,8 +536,7 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 #pragma unroll
         for (int st = 0; st < NS; ++st) qf[st] = w.signed_q(*(const uint4 *)(qr + 32 * st));
     }
-    bool careful = false;
-    auto tile = [&](int t, uint8_t *T, uint8_t *Tn) {
+    auto tile = [&](auto careful, int t, uint8_t *T, uint8_t *Tn) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): tile t has landed
         lds_barrier();                       // for every wave, and the other buffer is free
         const int k0 = j.k0 + KT * t;
@@ -456,22 +569,22 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
             S[u] = (f32x16){};
-#pragma unroll
-            for (int st = 0; st < NS; ++st)
-                S[u] = mfma32<false>(*(const uint4 *)(T + (u * NS + st) * 1024 + 16 * lane), qf[st], S[u]);
             whole = whole && w.rule.whole(k0 + 32 * u) && good[u] == ~0u;
         }
+        ca_stream<KF>(T + 16 * lane, [&](int f, uint4 k) { S[f / NS] = mfma32<false>(k, qf[f % NS], S[f / NS]); });
         if (!whole) {
             w.some_masked = true;
+            int k = k0;
+            asm volatile("" : "+s"(k));  // the masks formed here, not before every tile
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) w.hide(S[u], w.rule.sees(k0 + 32 * u) & there[u]);
+            for (int u = 0; u < SUBS; ++u) w.hide(S[u], w.rule.sees(k + 32 * u) & there[u]);
         }
         uint4 pf[2 * SUBS];
         PagedSeen see[SUBS];
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) see[u] = {true, ~0u, ~0u};
         w.softmax(S, see, pf);
-        if (careful && !whole) {
+        if (careful() && !whole) {
             uint4 *sp = (uint4 *)aux + 128 * wave;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
@@ -485,15 +598,10 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
             }
             return;
         }
-#pragma unroll
-        for (int u = 0; u < SUBS; ++u)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int d = 0; d < NB; ++d)
-                    w.O[d] = mfma32<false>(*(const uint4 *)(T + (KF + (2 * u + i) * NB + d) * 1024 + 16 * lane), pf[2 * u + i], w.O[d]);
+        ca_stream<2 * SUBS * NB>(T + KF * 1024 + 16 * lane,
+                                 [&](int f, uint4 v) { w.O[f % NB] = mfma32<false>(v, pf[f / NB], w.O[f % NB]); });
     };
-    for (;;) {
+    auto begin = [&] {
         w.reset();
         if (ntiles > 0) {
             int first = 0;
@@ -504,32 +612,66 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
             for (int u = 0; u < SUBS; ++u) pg[u] = w.checked(pg[u]);
             load_tile(pg, T0);
         }
-        for (int t = 0; t < ntiles; t += 2) {
-            tile(t, T0, T1);
-            if (t + 1 < ntiles) tile(t + 1, T1, T0);
-        }
-        if (careful) break;
-        const bool again = mine && w.some_masked && __builtin_amdgcn_ballot_w64(w.bad() && r0 + c < j.R) != 0;
-        if (lane == 0) s_flag[wave] = again;
-        lds_barrier();  // and every wave is done with both buffers
-        careful = (s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3]) != 0;
-        if (!careful) break;
+    };
+    begin();
+    for (int t = 0; t < ntiles; t += 2) {
+        tile(std::false_type(), t, T0, T1);
+        if (t + 1 < ntiles) tile(std::false_type(), t + 1, T1, T0);
+    }
+    const bool again = mine && w.some_masked && __builtin_amdgcn_ballot_w64(w.bad() && r0 + c < j.R) != 0;
+    if (lane == 0) s_flag[wave] = again;
+    lds_barrier();  // and every wave is done with both buffers
+    if ((s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3]) != 0) {
+        // (a loop of its own: with both kinds of tile in one, every tile moved O to other registers)
+        begin();
+#pragma unroll 1
+        for (int t = 0; t < ntiles; ++t) tile(std::true_type(), t, t & 1 ? T1 : T0, t & 1 ? T0 : T1);
     }
     const int rr = r0 + c;
-    const float sum = sum_halves(w.l);
-    if (rr >= j.R) return;
-    if (j.split) {
-        float *dst = j.slot + (32 * wave + c) * (D + 4);
-        if (h == 0) *(float2 *)dst = make_float2(w.m, sum);
+    float sum = sum_halves(w.l);
+    if (j.parts > 1) {
+        // register pair x of lane l at 64 x + l, m and the sum behind the last
+        const int at = 32 * wave * ca_row(D) + 2 * lane;
+        float *dst = j.slots + j.part * j.step + at;
 #pragma unroll
         for (int d = 0; d < NB; ++d)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (32 * d + 8 * x < D)
-                    *(float4 *)(dst + 4 + 32 * d + 8 * x + 4 * h) =
-                        make_float4(w.O[d][4 * x], w.O[d][4 * x + 1], w.O[d][4 * x + 2], w.O[d][4 * x + 3]);
-        return;
+            for (int x = 0; x < 8; ++x) ca_put(dst + 128 * (8 * d + x), w.O[d][2 * x], w.O[d][2 * x + 1]);
+        ca_put(dst + 128 * 8 * NB, w.m, sum);
+        static_assert(128 * (8 * NB + 1) <= 32 * ca_row(D), "a wave's registers");
+        if (!ca_last(j, flag)) return;
+        const float *src = j.slots + at;
+        float M = -INFINITY;
+#pragma unroll 4
+        for (int p = 0; p < j.parts; ++p) M = fmaxf(M, ca_get(src + p * j.step + 128 * 8 * NB).x);
+        f32x16 O[NB];
+#pragma unroll
+        for (int d = 0; d < NB; ++d) O[d] = (f32x16){};
+        float all = 0.0f;
+#pragma unroll 1
+        for (int p = 0; p < j.parts; ++p) {
+            const float *from = src + p * j.step;
+            const float2 ml = ca_get(from + 128 * 8 * NB);
+            const bool none = ml.x == -INFINITY && !(ml.y != 0.0f);  // saw nothing
+            const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - M) * a.cs);
+            all += none ? 0.0f : f * ml.y;
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+                float2 v[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = ca_get(from + 128 * (8 * d + x));
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    O[d][2 * x] += none ? 0.0f : f * v[x].x;
+                    O[d][2 * x + 1] += none ? 0.0f : f * v[x].y;
+                }
+            }
+        }
+        sum = all;
+#pragma unroll
+        for (int d = 0; d < NB; ++d) w.O[d] = O[d];
     }
+    if (rr >= j.R) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint8_t *dst = ca_out<D>(a, sq, j.hk, rr) + 8 * h;
 #pragma unroll
@@ -547,93 +689,48 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * CA_WAVES, D <= 128 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
+    __shared__ int flag;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const CaPlan p = ca_plan(a, blockIdx.x, lane);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) a.list[0].first = min(p.lists, a.slots / 2);
     if (p.s < 0) return;
     const CaSeq &sq = p.q;
     const CaJob j = ca_job(a, p, D);
-    if (p.wide) ca_many<D, BS>(a, sq, j, T0, T1, aux, lane, wave);
-    else ca_few<D, BS>(a, sq, j, T0, T1, aux, lane, wave);
+    if (p.wide) ca_many<D, BS>(a, sq, j, T0, T1, aux, &flag, lane, wave);
+    else ca_few<D, BS>(a, sq, j, T0, T1, aux, &flag, lane, wave);
 }
 
-// Joins an item's partitions, a wave a row: lane p holds partition p's weight, the lanes
-// then take the dims.
-constexpr int CA_MERGE_ROWS = 8;  // of a workgroup
-template <int D> __global__ void __launch_bounds__(256) k_chunk_attn_merge(const CaArgs a) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int count = a.list[0].first;
-    const CaItem it = a.list[1 + blockIdx.x];
-    if ((int)blockIdx.x >= count) return;
-    const CaSeq sq = {it.token, 0, 0};
-    const int np = it.parts;
-    const int64_t step = (int64_t)a.slot_rows * (D + 4);
-    constexpr int E = (D + 63) / 64, AT_ONCE = 8;
-    for (int r = blockIdx.y * CA_MERGE_ROWS + wave; r < (int)(blockIdx.y + 1) * CA_MERGE_ROWS; r += 4) {
-        const int row = it.first + r;
-        if (row >= it.end) return;
-        const float *base = a.part + it.slot * step + r * (D + 4);
-        // the first partitions' sums are on their way while the weights are formed
-        float o[AT_ONCE][E];
-        auto load = [&](int p0) {
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-                for (int e = 0; e < E; ++e)  // (past the last partition or dim: an element that gets no weight, or no place)
-                    o[i][e] = base[min(p0 + i, np - 1) * step + 4 + min(lane + 64 * e, D - 1)];
-        };
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (lane < np) ml = *(const float2 *)(base + lane * step);
-        load(0);
-        float M = ml.x;
-        for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
-        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - M) * a.cs);
-        float sum = w * ml.y;
-        for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i, 64);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        float acc[E] = {};
-        for (int p0 = 0; p0 < np; p0 += AT_ONCE) {
-            if (p0 > 0) load(p0);
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) {
-                if (p0 + i >= np) break;
-                const float wp = __shfl(w, p0 + i, 64);
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += wp * o[i][e];
-            }
-        }
-        uint16_t *dst = (uint16_t *)ca_out<D>(a, sq, it.hk, row);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lane + 64 * e < D) dst[lane + 64 * e] = f2h(acc[e] * inv);
-    }
-}
-
-// What the host knows of the plan: bounds of the items, the partitions, the workgroups
-// and the slots that any lengths and starts within the arguments can lead to.
+// What the host knows of the plan: bounds of the items, the partitions, the workgroups and
+// the partials that any lengths and starts within the arguments can lead to.
+// Of each kind of sequence: a share of t tiles makes a split sequence's partitions fewer
+// than 2 / t of its tiles, and the shares are 1.5 / wgs of all tiles or more (few rows), and
+// 2 / wgs or more if more than wgs partitions would come of less (many rows).
 struct CaBounds {
-    int64_t items, parts, wgs, slots, slot_rows, blocks;
+    int64_t items, parts, wgs, units, blocks;
+    int span_few, span_many;
 };
 static CaBounds ca_bounds(const tlh_chunk_attention_args &a) {
     CaBounds b;
     const int64_t G = a.num_heads / a.num_kv_heads, most = (int64_t)std::min(a.max_rows, a.num_rows) * G;
+    const bool wide = most > CA_NARROW;
     // a sequence's last block of rows may be short, and 33 to 64 rows take two
     b.items = a.num_kv_heads * (std::min<int64_t>(a.num_seqs, a.num_rows) * (most > 32 ? 2 : 1) + a.num_rows * G / 128);
     b.wgs = a.head_size <= 128 ? 512 : 256;  // workgroups that fill the machine
     const int window = a.window > 0 ? std::min(a.window, CA_NO_WINDOW) : CA_NO_WINDOW;
-    const int64_t tiles = ca_tiles(a.max_context_len, (int)G, window, most > CA_NARROW ? 128 : 32);
+    b.span_few = window + 31 / (int)G + 1, b.span_many = window + 127 / (int)G + 1;
+    const int64_t tiles = ca_tiles(a.max_context_len, wide ? b.span_many : b.span_few);
     b.parts = std::max<int64_t>(1, std::min<int64_t>(CA_MAX_PARTS, (tiles + CA_MIN_TILES - 1) / CA_MIN_TILES));
-    b.slots = b.parts == 1 ? 0 : std::min(b.wgs, b.items * b.parts);
-    b.slot_rows = most > CA_NARROW ? 128 : 32;
-    b.blocks = b.parts == 1 ? b.items : std::min(b.items * b.parts, std::max(b.wgs, b.items + b.wgs / 2));
+    const int64_t few = (std::min<int64_t>(most, 32) + 3) / 4, many = wide ? 32 : 0;
+    b.units = b.parts == 1 ? 0 : std::min(2 * b.wgs * few + b.wgs * many, b.items * b.parts * std::max(few, many));
+    b.blocks = b.parts == 1 ? b.items : std::min(b.items * b.parts, 2 * b.wgs + b.items);
     return b;
 }
 
-// The list of split items (each has two slots at least), then the slots.
-static int64_t ca_list_bytes(const CaBounds &b) { return b.slots == 0 ? 0 : (int64_t)sizeof(CaItem) * (1 + b.slots / 2); }
+// The counters, always in the same place and as many as any call may need (a split item has
+// two partitions at least), then the partials.
+static_assert(TLH_CHUNK_COUNTER_BYTES >= 4 * (512 + 512 / 2), "split items");
 size_t chunk_attention_scratch_bytes(const tlh_chunk_attention_args &a) {
     const CaBounds b = ca_bounds(a);
-    return (size_t)(ca_list_bytes(b) + b.slots * b.slot_rows * (a.head_size + 4) * (int64_t)sizeof(float));
+    return b.parts == 1 ? 0 : (size_t)(TLH_CHUNK_COUNTER_BYTES + b.units * 4 * ca_row(a.head_size) * (int64_t)sizeof(float));
 }
 
 template <int D> static void launch_ca(const CaArgs &c, int bs, const CaBounds &b, hipStream_t stream) {
@@ -643,9 +740,6 @@ template <int D> static void launch_ca(const CaArgs &c, int bs, const CaBounds &
     case 16: hipLaunchKernelGGL((k_chunk_attn<D, 16>), grid, threads, 0, stream, c); break;
     default: hipLaunchKernelGGL((k_chunk_attn<D, 32>), grid, threads, 0, stream, c); break;
     }
-    if (b.parts > 1)
-        hipLaunchKernelGGL((k_chunk_attn_merge<D>), dim3((unsigned)std::min(b.items, b.slots / 2), (unsigned)(b.slot_rows / CA_MERGE_ROWS)),
-                           dim3(256), 0, stream, c);
 }
 
 tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scratch, hipStream_t stream) {
@@ -654,13 +748,13 @@ tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scrat
     c.out = (uint8_t *)a.out, c.q = (const uint8_t *)a.q, c.so = 2 * a.out_stride, c.sq = 2 * a.q_stride;
     c.kc = (const uint16_t *)a.k_cache, c.vc = (const uint16_t *)a.v_cache;
     c.tables = a.block_tables, c.lens = a.context_lens, c.starts = a.row_starts;
-    c.list = (CaItem *)scratch;
-    c.part = (float *)((uint8_t *)scratch + ca_list_bytes(b));
+    c.counters = (unsigned *)scratch;
+    c.part = (float *)((uint8_t *)scratch + TLH_CHUNK_COUNTER_BYTES);
     c.num_blocks = a.num_blocks;
-    c.S = a.num_seqs, c.KV = a.num_kv_heads, c.G = a.num_heads / a.num_kv_heads;
+    c.S = a.num_seqs, c.KV = a.num_kv_heads, c.kv = ca_div(a.num_kv_heads), c.G = ca_div(a.num_heads / a.num_kv_heads);
     c.rows = a.num_rows, c.max_rows = a.max_rows, c.max_blocks = a.max_blocks_per_seq, c.max_ctx = a.max_context_len;
     c.window = a.window > 0 ? std::min(a.window, CA_NO_WINDOW) : CA_NO_WINDOW;
-    c.wgs = (int)b.wgs, c.slots = (int)b.slots, c.slot_rows = (int)b.slot_rows;
+    c.lg_wgs = b.wgs == 512 ? 9 : 8, c.span_few = b.span_few, c.span_many = b.span_many;
     set_scale(c, a.scale);
     if (b.blocks >= 1 << 24)  // x 256 threads
         return set_error(TLH_INVALID, "chunk_attention: too many rows and heads for one launch");

@@ -893,6 +893,9 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None):
     return outs
 
 
+CHUNK_COUNTER_BYTES = 8192
+
+
 class ChunkAttention(_ScratchNode):
     """Causal attention of the sequences' new tokens over the paged cache, one or thousands a sequence, with its
     scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. A call takes up to
@@ -911,6 +914,7 @@ class ChunkAttention(_ScratchNode):
         n = C.c_size_t()
         check(lib().tlh_chunk_attention_scratch_bytes(C.byref(a), C.byref(n)))
         self._allocate(n.value, device)
+        self.scratch[:CHUNK_COUNTER_BYTES].zero_()  # and every call leaves them so
 
     def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, row_starts, stream=None):
         """q and out f16 (rows, heads, head size) with rows <= num_rows, tokens at any stride that is a multiple of 8

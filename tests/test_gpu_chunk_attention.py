@@ -142,9 +142,9 @@ def test_lengths_past_the_maximum_are_the_maximum(gpu):
     check(run(c, max_context=50), c, max_context=50)
 
 
-@pytest.mark.parametrize("starts", [[0, 0, 9], [3, 5, 9], [0, 9, 9], [4, 4, 4], [-5, 4, 100], [9, 4, 8]])
+@pytest.mark.parametrize("starts", [[0, 0, 9], [3, 5, 9], [0, 9, 9], [4, 4, 4], [-5, 4, 100], [-5, -9, 4]])
 def test_starts_that_leave_rows_out(gpu, starts):
-    """Gaps, empty sequences, starts outside the rows (taken as the nearer end), an end before its start (empty)."""
+    """Gaps, empty sequences, starts outside the rows (taken as the nearer end)."""
     c = build(8, 2, 128, 16, [40, 90], [3, 6], 39)
     c["starts"] = starts
     clamped = [max(0, min(x, 9)) for x in starts]
@@ -262,9 +262,10 @@ def test_page_shared_by_sequences_and_a_wide_table(gpu):
 def test_the_same_result_every_time_and_a_used_scratch(gpu, cached, new):
     c = build(32, 8, 128, 16, cached, new, 46)
     a, node, dev = run(c), node_of(c), on_gpu(c)
-    node.scratch.fill_(0xff)
+    node.scratch[N.CHUNK_COUNTER_BYTES:].fill_(0xff)
     for _ in range(3):
         assert torch.equal(a, node(torch.empty_like(a), *dev))
+        assert (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
 
 
 def test_a_node_for_more_takes_smaller_calls(gpu):
@@ -358,3 +359,17 @@ def test_one_call_form_on_streams(gpu):
         torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda")  # the allocator may hand out what the call let go
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("starts", [[9, 4, 8], [0, 9, 0], [0, 9, 8]])
+def test_starts_that_decrease_compute_nothing(gpu, starts):
+    """Sequences that overlap would make more work than the scratch has room for; the next call is as ever."""
+    c = build(8, 2, 128, 16, [4000, 2000], [3, 6], 39)
+    node, dev = node_of(c, max_rows=9), list(on_gpu(c))
+    out = torch.full(c["q"].shape, 7.0, dtype=torch.float16, device="cuda")
+    right, dev[5] = dev[5], i32(starts)
+    node(out, *dev)
+    torch.cuda.synchronize()
+    assert (out == 7).all() and (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
+    dev[5] = right
+    check(node(out, *dev), c)
