@@ -5,172 +5,426 @@
 //
 // Everything is f64. A drawn token is the first whose running sum exceeds r times the
 // whole: with f32 terms (off by 2^-24 of themselves) the sums would be off by more than
-// most of a vocabulary's tokens weigh, and the token would depend on the order of additions.
+// most of a vocabulary's tokens weigh, and the token would depend on the order of
+// additions. f64 products run at f32's rate here, so the bound is one read of the logits.
+//
+// Three launches: the sums of chunks of all rows, a chunk a workgroup; then every workgroup
+// of a sequence finds where it stops, and sums its chunk of what the token there is drawn
+// from; then one workgroup a sequence finds the chunk and the token in it.
 #include <algorithm>
 
 #include "kernels.hpp"
 
 namespace tlh {
 
-struct DvRow {  // of a row of logits
-    double sum;  // of exp((x - top) / T); 0 where the row is no distribution
-    float top;   // its largest logit
-    int at;      // the lowest index of that
+constexpr int DV_MAX_CHUNKS = 64;  // of a row: a lane each
+// elements of a chunk: 64 (or 16, for few rows) of each of 256 lanes
+constexpr int DV_CHUNK = 64 * 256, DV_CHUNK_SMALL = 16 * 256;
+
+// Sums of exp((x - ref) / T) need no running maximum: f64 holds 2^900 times a term as well
+// as the term, so `ref` is some early element, and only a chunk with one further above it
+// is taken again.
+constexpr double DV_ABOVE = 900.0;  // powers of 2
+
+struct DvPart {  // of a chunk of a row
+    double sum;  // of exp((x - ref) / T); NaN where the chunk rules a distribution out
+    float ref;   // (greedy: its largest logit; -inf: it holds nothing else)
+    int at;      // greedy: the lowest index of that
+};
+struct DvMass {  // of a chunk of what is drawn from
+    double sum;
+    int last, pad;  // the last index with a weight, -1: none
+};
+struct DvStop {  // of a sequence
+    double zp, zq;    // the sums of the rows drawn from
+    float mp, mq;     // ... and what their exponents are taken from
+    int stop, draws;  // drafts accepted; whether a token is to be drawn
 };
 
-template <int TY> __device__ __forceinline__ float dv_load(const void *p, int64_t i) {
+template <int TY> __device__ __forceinline__ float dv_elem(const void *p, int64_t i) {
     if constexpr (TY == TLH_TYPE_F32) return ((const float *)p)[i];
     else if constexpr (TY == TLH_TYPE_F16) return h2f(((const uint16_t *)p)[i]);
     else return bf16_to_f32(((const uint16_t *)p)[i]);
 }
 
+// exp(d), off by less than 2^-50 of it: 2^k times the Taylor series of the rest, |r| <= ln 2
+// / 2, whose first term left out is below 2^-52.
+__device__ __forceinline__ double dv_exp(double d) {
+    const double t = fmax(d * 1.4426950408889634074, -1100.0);
+    const double k = rint(t), r = (t - k) * 0.69314718055994530942;
+    double e = 1.0 / 479001600.0;
+    e = fma(e, r, 1.0 / 39916800.0);
+    e = fma(e, r, 1.0 / 3628800.0);
+    e = fma(e, r, 1.0 / 362880.0);
+    e = fma(e, r, 1.0 / 40320.0);
+    e = fma(e, r, 1.0 / 5040.0);
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    return ldexp(e, (int)k);
+}
+// exp((x - ref) / T): a masked logit has no weight at any temperature
+__device__ __forceinline__ double dv_weight(float x, float ref, double inv_t) {
+    return x == -INFINITY ? 0.0 : dv_exp(((double)x - (double)ref) * inv_t);
+}
+
+template <typename T> __device__ __forceinline__ T dv_sum(T v, int lanes = 64) {
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ float dv_max(float v, int lanes = 64) {
+    for (int o = 1; o < lanes; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int dv_min(int v, int lanes = 64) {
+    for (int o = 1; o < lanes; o <<= 1) v = min(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
 struct DvSeq {
-    int b, n;  // first draft, drafts
+    int b, n;  // first draft, drafts that are looked at
 };
+__device__ __forceinline__ int dv_start(const tlh_draft_verify_args &a, int s) { return max(0, min(a.draft_starts[s], a.num_drafts)); }
 __device__ __forceinline__ DvSeq dv_seq(const tlh_draft_verify_args &a, int s) {
     DvSeq q;
-    q.b = max(0, min(a.draft_starts[s], a.num_drafts));
-    q.n = min(max(q.b, min(a.draft_starts[s + 1], a.num_drafts)) - q.b, a.max_drafts);
+    q.b = dv_start(a, s);
+    q.n = min(max(q.b, dv_start(a, s + 1)) - q.b, a.max_drafts);
     return q;
 }
-
-// p(x) of element x of a row
-__device__ __forceinline__ double dv_weight(float x, float top, double inv_t) {
-    return x == -INFINITY ? 0.0 : exp(((double)x - (double)top) * inv_t);
+// the last sequence whose first row (of drafts: its first draft, else with one more row a
+// sequence) is `row` or before it; starts are looked at 64 at a time
+__device__ __forceinline__ int dv_find(const tlh_draft_verify_args &a, int row, bool target, int lane) {
+    int lo = 0, len = a.num_seqs;
+    while (len > 1) {
+        const int stride = (len + 63) / 64, s = lo + lane * stride;
+        const bool in = s < lo + len && dv_start(a, s) + (target ? s : 0) <= row;
+        const int n = max(1, (int)__popcll(__builtin_amdgcn_ballot_w64(in)));
+        const int next = lo + (n - 1) * stride;
+        len = min(stride, lo + len - next);
+        lo = next;
+    }
+    return lo;
 }
 
-// One workgroup a (sequence; draft or the row behind them; target or draft row).
+// C consecutive elements of a row in 16 bytes, from element e on; what lies outside it is
+// -inf. Loads are aligned whatever the row's address (`shift` elements past 16 bytes): a
+// chunk's numbering begins up to C - 1 elements before the row.
+template <int TY> struct DvLoad {
+    static constexpr int C = TY == TLH_TYPE_F32 ? 4 : 8, ES = 16 / C;
+    const char *base;
+    int V, shift;
+    __device__ __forceinline__ DvLoad(const void *logits, int64_t row, int64_t stride, int vocab)
+        : base((const char *)logits + row * stride * ES), V(vocab), shift((int)(((uintptr_t)base & 15) / ES)) {}
+    __device__ __forceinline__ void vec(int e, bool aligned, float (&x)[C]) const {
+        if (aligned && e >= 0 && e + C <= V) {
+            const uint4 w = *(const uint4 *)(base + (int64_t)e * ES);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                x[c] = TY == TLH_TYPE_F32   ? __uint_as_float(ws[c % 4])
+                       : TY == TLH_TYPE_F16 ? h2f((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))))
+                                            : bf16_to_f32((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))));
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) x[c] = e + c >= 0 && e + c < V ? dv_elem<TY>(base, e + c) : -INFINITY;
+        }
+    }
+};
+
 template <int TY>
-__global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args a, DvRow *rows) {
-    const int s = blockIdx.y, which = blockIdx.z;
+__global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args a, int r0, int P, int chunk, DvPart *__restrict__ parts) {
+    using L = DvLoad<TY>;
+    constexpr int C = L::C, AT_ONCE = 16 / C;  // vectors on their way at a time
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = blockIdx.x;
+    const int r = r0 + blockIdx.y, targets = a.num_drafts + a.num_seqs;
+    const bool target = r < targets;
+    const int row = target ? r : r - targets;
+    const int s = __builtin_amdgcn_readfirstlane(dv_find(a, row, target, lane));
     const DvSeq q = dv_seq(a, s);
     const float T = a.temperatures[s];
     const bool greedy = !(T > 0.0f);
-    __shared__ float s_m[256];
-    __shared__ int s_at[256];
-    __shared__ double s_s[256];
-    for (int i = blockIdx.x; i < q.n + 1 - which; i += gridDim.x) {
-        const void *logits = which ? a.draft : a.target;
-        const int64_t base = which ? (q.b + i) * a.draft_stride : ((int64_t)q.b + s + i) * a.target_stride;
-        float m = -INFINITY;
-        int at = 0;
-        bool bad = false;
-        for (int e = threadIdx.x; e < a.vocab; e += 256) {
-            const float x = dv_load<TY>(logits, base + e);
-            if (x > m) m = x, at = e;
-            bad |= x != x || (x == INFINITY && !greedy);
+    const int i = row - q.b - (target ? s : 0);
+    if (i < 0 || i >= q.n + (target ? 1 : 0) || (greedy && !target)) return;  // nobody looks at the row
+    const L load(target ? a.target : a.draft, row, target ? a.target_stride : a.draft_stride, a.vocab);
+    const int first = p * chunk - load.shift + threadIdx.x * C, end = min((p + 1) * chunk - load.shift, a.vocab);
+    const double inv_t = greedy ? 0.0 : 1.0 / (double)T;
+    float top = -INFINITY, ref = -INFINITY;
+    int at = 0x7fffffff;
+    double sum = 0.0;
+    bool bad = false;
+    for (;;) {
+#pragma unroll 1
+        for (int e = first; e < end; e += 256 * C * AT_ONCE) {
+            float x[AT_ONCE][C];
+#pragma unroll
+            for (int v = 0; v < AT_ONCE; ++v)
+                if (e + 256 * C * v < end) load.vec(e + 256 * C * v, true, x[v]);
+                else
+#pragma unroll
+                    for (int c = 0; c < C; ++c) x[v][c] = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < AT_ONCE; ++v)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    if (x[v][c] > top) top = x[v][c], at = e + 256 * C * v + c;
+                    bad = bad || (greedy ? x[v][c] != x[v][c] : !(x[v][c] < INFINITY));
+                }
+            if (greedy || top == -INFINITY) continue;
+            if (ref == -INFINITY) ref = top;
+#pragma unroll
+            for (int v = 0; v < AT_ONCE; ++v)
+#pragma unroll
+                for (int c = 0; c < C; ++c) sum += dv_weight(x[v][c], ref, inv_t);
         }
-        __syncthreads();
-        s_m[threadIdx.x] = bad ? NAN : m, s_at[threadIdx.x] = at;
-        __syncthreads();
-        m = -INFINITY, at = 0x7fffffff, bad = false;
-        for (int t = 0; t < 256; ++t) {
-            bad |= s_m[t] != s_m[t];
-            if (s_m[t] > m || (s_m[t] == m && s_at[t] < at)) m = s_m[t], at = s_at[t];
-        }
-        bad |= m == -INFINITY;
-        double sum = 0.0;
-        if (!bad && !greedy)
-            for (int e = threadIdx.x; e < a.vocab; e += 256) sum += dv_weight(dv_load<TY>(logits, base + e), m, 1.0 / (double)T);
-        s_s[threadIdx.x] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            DvRow r = {bad ? 0.0 : 1.0, m, at};
-            if (!bad && !greedy) {
-                r.sum = 0.0;
-                for (int t = 0; t < 256; ++t) r.sum += s_s[t];
-            }
-            rows[which ? a.num_drafts + a.num_seqs + q.b + i : q.b + s + i] = r;
-        }
+        if (greedy || bad || !(((double)top - (double)ref) * inv_t * 1.4426950408889634074 > DV_ABOVE)) break;
+        ref = top;
+        sum = 0.0;
     }
+    __shared__ float s_ref[4];
+    __shared__ double s_sum[4];
+    __shared__ int s_at[4];
+    if (greedy) ref = top;
+    const float all = dv_max(ref);
+    if (lane == 0) s_ref[wave] = all;
+    __syncthreads();
+    const float R = fmaxf(fmaxf(s_ref[0], s_ref[1]), fmaxf(s_ref[2], s_ref[3]));
+    if (greedy) at = dv_min(ref == R ? at : 0x7fffffff);
+    else sum = dv_sum(sum * dv_weight(ref, R, inv_t));  // (no element but -inf: 0)
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) sum = NAN;
+    if (lane == 0) s_sum[wave] = sum, s_at[wave] = at;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        parts[(int64_t)r * P + p] = {(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), R, min(min(s_at[0], s_at[1]), min(s_at[2], s_at[3]))};
 }
 
-// One workgroup a sequence: the tests, then the token.
+// A row's parts joined by `lanes` lanes, one a chunk
+struct DvRow {
+    double z;  // the sum of exp((x - m) / T); NaN: no distribution
+    float m;
+    int at;    // greedy: the likeliest token
+};
+__device__ __forceinline__ DvRow dv_row(const DvPart *parts, int P, int c, int lanes, bool greedy, double inv_t) {
+    DvPart x = {0.0, -INFINITY, 0x7fffffff};
+    if (c < P) x = parts[c];
+    DvRow r;
+    r.m = dv_max(x.ref, lanes);
+    double z = x.ref == -INFINITY ? 0.0 : x.sum * (greedy ? 0.0 : dv_weight(x.ref, r.m, inv_t));
+    if (x.sum != x.sum) z = NAN;
+    r.z = dv_sum(z, lanes);
+    r.at = greedy ? dv_min(x.ref == r.m ? x.at : 0x7fffffff, lanes) : 0;
+    if (r.m == -INFINITY) r.z = NAN;
+    return r;
+}
+
 template <int TY>
-__global__ void __launch_bounds__(256) k_draft_decide(const tlh_draft_verify_args a, const DvRow *rows) {
-    const int s = blockIdx.x;
-    const DvSeq sq = dv_seq(a, s);
+__global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_args a, int P, int chunk, int lanes,
+                                                      const DvPart *__restrict__ parts, DvStop *__restrict__ stops,
+                                                      DvMass *__restrict__ masses) {
+    using L = DvLoad<TY>;
+    constexpr int C = L::C;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.y, p = blockIdx.x;
+    const DvSeq q = dv_seq(a, s);
     const float T = a.temperatures[s];
     const bool greedy = !(T > 0.0f);
     const double inv_t = 1.0 / (double)T;
-    const DvRow *target = rows + sq.b + s, *draft = rows + a.num_drafts + a.num_seqs + sq.b;
-    auto weight = [&](const void *logits, int64_t base, const DvRow &r, int x) {
-        if (x < 0 || x >= a.vocab) return 0.0;
-        if (greedy) return x == r.at ? 1.0 : 0.0;
-        return dv_weight(dv_load<TY>(logits, base + x), r.top, inv_t) / r.sum;
-    };
-    auto p_of = [&](int i, int x) { return weight(a.target, ((int64_t)sq.b + s + i) * a.target_stride, target[i], x); };
-    auto q_of = [&](int i, int x) {
-        if (!a.draft) return x == a.tokens[sq.b + i] && x >= 0 && x < a.vocab ? 1.0 : 0.0;
-        return weight(a.draft, (int64_t)(sq.b + i) * a.draft_stride, draft[i], x);
-    };
-    int stop = sq.n;
-    bool none = false;  // no distribution where it stops
-    for (int i = sq.n - 1; i >= 0; --i) {
-        const int x = a.tokens[sq.b + i];
-        const bool bad = target[i].sum == 0.0 || (a.draft && !greedy && draft[i].sum == 0.0);
-        const double p = bad ? 0.0 : p_of(i, x), q = bad ? 0.0 : greedy ? 1.0 : q_of(i, x);
-        const bool ok = !bad && (greedy ? p == 1.0 : (double)a.accept_at[sq.b + i] * q < p);
-        if (threadIdx.x == 0 && a.accept_probs)
-            a.accept_probs[sq.b + i] = bad ? NAN : q > 0.0 ? (float)fmin(1.0, p / q) : p > 0.0 ? 1.0f : 0.0f;
-        if (!ok) stop = i, none = bad;
+    const int64_t t0 = q.b + s;                                      // the target's first row
+    const DvPart *tp = parts + t0 * P, *dp = parts + ((int64_t)a.num_drafts + a.num_seqs + q.b) * P;
+    __shared__ int s_stop;
+    if (threadIdx.x == 0) s_stop = q.n;
+    __syncthreads();
+    // `lanes` lanes a draft
+    const int each = 256 / lanes, c = threadIdx.x & (lanes - 1);
+    for (int i0 = 0; i0 < q.n; i0 += each) {
+        const int i = min(i0 + (int)threadIdx.x / lanes, q.n - 1);
+        const int x = a.tokens[q.b + i];
+        const bool known = x >= 0 && x < a.vocab, drawn = a.draft && !greedy;
+        const float u = a.accept_at[q.b + i];
+        const float tx = known ? dv_elem<TY>(a.target, (t0 + i) * a.target_stride + x) : -INFINITY;
+        const float dx = known && drawn ? dv_elem<TY>(a.draft, (int64_t)(q.b + i) * a.draft_stride + x) : -INFINITY;
+        const DvRow t = dv_row(tp + (int64_t)i * P, P, c, lanes, greedy, inv_t);
+        const DvRow d = drawn ? dv_row(dp + (int64_t)i * P, P, c, lanes, false, inv_t) : DvRow{1.0, 0.0f, 0};
+        const bool bad = t.z != t.z || d.z != d.z;
+        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? dv_weight(tx, t.m, inv_t) / t.z : 0.0;
+        const double qx = !known ? 0.0 : drawn ? dv_weight(dx, d.m, inv_t) / d.z : 1.0;
+        const bool ok = !bad && (greedy ? px == 1.0 : (double)u * qx < px);
+        if (c == 0 && !ok) atomicMin(&s_stop, i);
+        if (p == 0 && c == 0 && a.accept_probs)
+            a.accept_probs[q.b + i] = bad ? NAN : qx > 0.0 ? (float)fmin(1.0, px / qx) : px > 0.0 ? 1.0f : 0.0f;
     }
-    if (stop == sq.n) none = target[stop].sum == 0.0;
-    int next = -1;
-    if (!none && greedy) next = target[stop].at;
-    if (!none && !greedy) {
-        __shared__ double s_s[256];
-        __shared__ int s_last[256], s_next;
-        const int each = (a.vocab + 255) / 256, e0 = threadIdx.x * each, e1 = min(e0 + each, a.vocab);
-        for (int whole = stop == sq.n; whole < 2; ++whole) {  // from p where p - q has nothing
-            auto mass = [&](int x) { return whole ? p_of(stop, x) : fmax(p_of(stop, x) - q_of(stop, x), 0.0); };
-            double sum = 0.0;
-            int last = -1;
-            for (int e = e0; e < e1; ++e) {
-                const double w = mass(e);
-                sum += w;
-                if (w > 0.0) last = e;
-            }
-            __syncthreads();
-            s_s[threadIdx.x] = sum, s_last[threadIdx.x] = last;
-            if (threadIdx.x == 0) s_next = 0x7fffffff;
-            __syncthreads();
-            double before = 0.0, total = 0.0;
-            last = -1;
-            for (int t = 0; t < 256; ++t) {
-                if (t == threadIdx.x) before = total;
-                total += s_s[t];
-                last = max(last, s_last[t]);
-            }
-            if (total == 0.0) continue;
-            const double reach = (double)a.sample_at[s] * total;
-            if (before + sum > reach) {
-                for (int e = e0; e < e1; ++e) {
-                    before += mass(e);
-                    if (before > reach) {
-                        atomicMin(&s_next, e);
-                        break;
-                    }
-                }
-            }
-            __syncthreads();
-            next = s_next == 0x7fffffff ? last : s_next;
-            break;
+    __syncthreads();
+    const int stop = s_stop;
+    const bool minus = stop < q.n && a.draft && !greedy;  // a refused draft: its drafter's weights are taken off
+    const DvRow t = dv_row(tp + (int64_t)stop * P, P, lane, 64, greedy, inv_t);
+    const DvRow d = minus ? dv_row(dp + (int64_t)stop * P, P, lane, 64, false, inv_t) : DvRow{0.0, 0.0f, 0};
+    const bool bad = t.z != t.z || d.z != d.z;
+    const int outright = stop < q.n && !a.draft && !greedy ? a.tokens[q.b + stop] : -1;  // and of one proposed outright, itself
+    if (p == 0) {
+        int32_t *out = a.out_tokens + (int64_t)s * (a.max_drafts + 1);
+        for (int i = threadIdx.x; i <= a.max_drafts; i += 256)
+            out[i] = i < stop ? a.tokens[q.b + i] : i == stop && greedy && !bad ? t.at : -1;
+        if (threadIdx.x == 0) {
+            a.accepted[s] = stop;
+            stops[s] = {t.z, d.z, t.m, d.m, stop, !greedy && !bad};
         }
     }
-    int32_t *out = a.out_tokens + (int64_t)s * (a.max_drafts + 1);
-    for (int i = threadIdx.x; i <= a.max_drafts; i += 256) out[i] = i < stop ? a.tokens[sq.b + i] : i == stop ? next : -1;
-    if (threadIdx.x == 0) a.accepted[s] = stop;
+    if (greedy || bad) return;
+    const L lt(a.target, t0 + stop, a.target_stride, a.vocab);
+    const L ld(minus ? a.draft : a.target, minus ? (int64_t)q.b + stop : 0, minus ? a.draft_stride : 0, a.vocab);
+    const bool alike = lt.shift == ld.shift;  // else the drafter's row is read element by element
+    const int first = p * chunk - lt.shift + threadIdx.x * C, end = min((p + 1) * chunk - lt.shift, a.vocab);
+    const double ip = 1.0 / t.z, iq = minus ? 1.0 / d.z : 0.0;
+    double sum = 0.0;
+    int last = -1;
+#pragma unroll 1
+    for (int e = first; e < end; e += 256 * C) {
+        float x[C], y[C];
+        lt.vec(e, true, x);
+        if (minus) ld.vec(e, alike, y);
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            double w = dv_weight(x[k], t.m, inv_t) * ip;
+            if (minus) w = fmax(w - dv_weight(y[k], d.m, inv_t) * iq, 0.0);
+            if (e + k == outright) w = 0.0;
+            sum += w;
+            if (w > 0.0) last = e + k;
+        }
+    }
+    sum = dv_sum(sum);
+    last = -dv_min(-last);
+    __shared__ double s_sum[4];
+    __shared__ int s_last[4];
+    if (lane == 0) s_sum[wave] = sum, s_last[wave] = last;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        masses[(int64_t)s * P + p] = {(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3])), 0};
 }
 
+// One workgroup a sequence: the chunk, then the token in it, a thread a run of elements.
+constexpr int DV_DRAW = 1024;
+template <int TY>
+__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int P, int chunk, const DvPart *__restrict__ parts,
+                                                        const DvStop *__restrict__ stops, const DvMass *__restrict__ masses) {
+    constexpr int ES = TY == TLH_TYPE_F32 ? 4 : 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x;
+    const DvStop st = stops[s];
+    if (!st.draws) return;
+    const DvSeq q = dv_seq(a, s);
+    const double inv_t = 1.0 / (double)a.temperatures[s];
+    const int64_t row = q.b + s + st.stop;
+    bool minus = st.stop < q.n && a.draft;
+    int outright = st.stop < q.n && !a.draft ? a.tokens[q.b + st.stop] : -1;
+    DvMass m = {0.0, -1, 0};
+    if (lane < P) m = masses[(int64_t)s * P + lane];
+    if (dv_sum(m.sum) == 0.0) {  // nothing above the drafter's: from p alone
+        minus = false;
+        outright = -1;
+        m = {0.0, -1, 0};
+        if (lane < P) {
+            const DvPart x = parts[row * P + lane];
+            m.sum = x.ref == -INFINITY ? 0.0 : x.sum * dv_weight(x.ref, st.mp, inv_t) / st.zp;
+            m.last = m.sum > 0.0 ? 0x7fffffff : -1;  // (the last one with a weight is found below)
+        }
+    }
+    double run = m.sum;
+    for (int o = 1; o < 64; o <<= 1) {
+        const double before = __shfl_up(run, o, 64);
+        run += lane >= o ? before : 0.0;
+    }
+    const double total = __shfl(run, 63, 64);
+    const double reach = (double)a.sample_at[s] * total;
+    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < P && run > reach), any = __builtin_amdgcn_ballot_w64(m.last >= 0);
+    const int p = over != 0 ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((unsigned long long)any);  // else the last with a weight
+    double from = __shfl(run - m.sum, p, 64);
+
+    const char *base = (const char *)a.target + row * a.target_stride * ES;
+    const int first = p * chunk - (int)(((uintptr_t)base & 15) / ES);
+    const int each = chunk / DV_DRAW, e0 = max(first + (int)threadIdx.x * each, 0), e1 = min(first + ((int)threadIdx.x + 1) * each, a.vocab);
+    const double ip = 1.0 / st.zp, iq = minus ? 1.0 / st.zq : 0.0;
+    auto mass = [&](int e) {
+        double w = dv_weight(dv_elem<TY>(base, e), st.mp, inv_t) * ip;
+        if (minus) w = fmax(w - dv_weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, inv_t) * iq, 0.0);
+        return e == outright ? 0.0 : w;
+    };
+    double sum = 0.0;
+    int last = -1;
+    for (int e = e0; e < e1; ++e) {
+        const double w = mass(e);
+        sum += w;
+        if (w > 0.0) last = e;
+    }
+    __shared__ double s_sum[DV_DRAW / 64];
+    __shared__ int s_last[DV_DRAW / 64], s_next;
+    double upto = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+        const double before = __shfl_up(upto, o, 64);
+        upto += lane >= o ? before : 0.0;
+    }
+    const int wlast = -dv_min(-last);
+    if (lane == 63) s_sum[wave] = upto;
+    if (lane == 0) s_last[wave] = wlast;
+    if (threadIdx.x == 0) s_next = 0x7fffffff;
+    __syncthreads();
+    last = -1;
+    for (int w = 0; w < DV_DRAW / 64; ++w) {
+        if (w < wave) from += s_sum[w];
+        last = max(last, s_last[w]);
+    }
+    from += upto - sum;
+    if (from + sum > reach) {
+        for (int e = e0; e < e1; ++e) {
+            from += mass(e);
+            if (from > reach) {
+                atomicMin(&s_next, e);
+                break;
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.out_tokens[(int64_t)s * (a.max_drafts + 1) + st.stop] = s_next == 0x7fffffff ? last : s_next;
+}
+
+// A small vocabulary's chunk of 64 a lane would be mostly empty; few rows: shorter chunks,
+// so that more CUs share them.
+static bool dv_small(int64_t vocab) { return vocab <= 2 * DV_CHUNK_SMALL; }
+static int dv_ept(int64_t rows, int64_t vocab) {
+    return dv_small(vocab) ||
+                   (rows * ((vocab + DV_CHUNK - 1) / DV_CHUNK) < 256 && vocab + 7 <= (int64_t)DV_CHUNK_SMALL * DV_MAX_CHUNKS)
+               ? 16
+               : 64;
+}
+static int dv_chunks(int64_t vocab, int ept) {
+    return (int)((vocab + 7 + 256 * ept - 1) / (256 * ept));  // up to 7 places before a row that is not aligned
+}
+static int64_t dv_rows(const tlh_draft_verify_args &a) { return (int64_t)a.num_drafts + a.num_seqs + (a.draft ? a.num_drafts : 0); }
+
+// Room for either chunk length, so that the size grows with the rows and one buffer for
+// the largest batch serves every smaller one: the sequences' stops, masses, the rows' parts.
+static size_t dv_most_chunks(int64_t rows, int64_t vocab) {
+    return dv_small(vocab) ? (size_t)rows * dv_chunks(vocab, 16)
+                           : (size_t)rows * dv_chunks(vocab, 64) + (size_t)std::min<int64_t>(rows, 256) * dv_chunks(vocab, 16);
+}
 size_t draft_verify_scratch_bytes(const tlh_draft_verify_args &a) {
-    return sizeof(DvRow) * ((size_t)a.num_drafts + a.num_seqs + (a.draft ? a.num_drafts : 0));
+    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * dv_most_chunks(a.num_seqs, a.vocab) +
+           sizeof(DvPart) * dv_most_chunks(dv_rows(a), a.vocab);
 }
 
 template <int TY> static void launch_dv(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {
-    const int n = std::min(a.max_drafts, a.num_drafts) + 1;
-    hipLaunchKernelGGL((k_draft_rows<TY>), dim3(n, a.num_seqs, a.draft ? 2 : 1), dim3(256), 0, stream, a, (DvRow *)scratch);
-    hipLaunchKernelGGL((k_draft_decide<TY>), dim3(a.num_seqs), dim3(256), 0, stream, a, (const DvRow *)scratch);
+    const int64_t rows = dv_rows(a);
+    const int ept = dv_ept(rows, a.vocab), chunk = 256 * ept, P = dv_chunks(a.vocab, ept);
+    int lanes = 1;
+    while (lanes < P) lanes <<= 1;
+    DvStop *stops = (DvStop *)scratch;
+    DvMass *masses = (DvMass *)(stops + a.num_seqs);
+    DvPart *parts = (DvPart *)(masses + dv_most_chunks(a.num_seqs, a.vocab));
+    for (int64_t r0 = 0; r0 < rows; r0 += 65535)  // grid y
+        hipLaunchKernelGGL((k_draft_rows<TY>), dim3(P, (unsigned)std::min<int64_t>(rows - r0, 65535)), dim3(256), 0, stream, a, (int)r0,
+                           P, chunk, parts);
+    hipLaunchKernelGGL((k_draft_masses<TY>), dim3(P, a.num_seqs), dim3(256), 0, stream, a, P, chunk, lanes, parts, stops, masses);
+    hipLaunchKernelGGL((k_draft_draw<TY>), dim3(a.num_seqs), dim3(DV_DRAW), 0, stream, a, P, chunk, parts, stops, masses);
 }
 
 tlh_status launch_draft_verify(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {
