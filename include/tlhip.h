@@ -622,7 +622,7 @@ tlh_status tlh_head_rope(const tlh_head_rope_args *a, void *stream);
  * Draft i with token x is accepted if accept_at[b + i] * q(x) < p(x) and those before it
  * are; accept_probs[b + i] = min(1, p(x) / q(x)) (NULL: not wanted; p(x) > 0 where q(x)
  * is 0). accepted[s] counts them. The next token is drawn from what p has above q at the first one
- * refused (from p where that is nothing), or from the row behind the drafts: the
+ * refused (from p where that is nothing: less than 2^-40), or from the row behind the drafts: the
  * lowest index where the running sum exceeds sample_at[s] times the whole (the last with
  * a weight above 0 where none does). out_tokens[s], i32 [max_drafts + 1], receives the
  * accepted ones, this one, and -1 behind them. All of it is computed in 64 bits: a running sum over

@@ -32,8 +32,7 @@ struct DvPart {  // of a chunk of a row
     int at;      // greedy: the lowest index of that
 };
 struct DvMass {  // of a chunk of what is drawn from
-    double sum;
-    int last, pad;  // the last index with a weight, -1: none
+    double sum, whole;  // of max(p - q, 0), of p
 };
 struct DvStop {  // of a sequence
     double zp, zq;    // the sums of the rows drawn from
@@ -47,43 +46,73 @@ template <int TY> __device__ __forceinline__ float dv_elem(const void *p, int64_
     else return bf16_to_f32(((const uint16_t *)p)[i]);
 }
 
-// exp(d), off by less than 2^-50 of it: 2^k times the Taylor series of the rest, |r| <= ln 2
-// / 2, whose first term left out is below 2^-52.
-__device__ __forceinline__ double dv_exp(double d) {
-    const double t = fmax(d * 1.4426950408889634074, -1100.0);
-    const double k = rint(t), r = (t - k) * 0.69314718055994530942;
-    double e = 1.0 / 479001600.0;
-    e = fma(e, r, 1.0 / 39916800.0);
-    e = fma(e, r, 1.0 / 3628800.0);
-    e = fma(e, r, 1.0 / 362880.0);
-    e = fma(e, r, 1.0 / 40320.0);
-    e = fma(e, r, 1.0 / 5040.0);
-    e = fma(e, r, 1.0 / 720.0);
-    e = fma(e, r, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    return ldexp(e, (int)k);
+// exp((x - ref) / T) with c = log2(e) / T, off by less than 2^-45 of it (2^-52 times the
+// exponent, 2^-47 from the series): 2^k times the Taylor series of 2^f, |f| <= 1/2, up to
+// f^11. The instructions that convert between f64 and integers, round or scale are slow
+// beside its additions and products: k is the low word of the sum with 1.5 x 2^52, and is
+// added to the result's exponent (32 x 1..8: 57 us with them, ROWS_US without). Nothing is
+// left below 2^-1000, and nothing of a masked logit (-inf), at any temperature.
+__device__ __forceinline__ double dv_weight(float x, float ref, double c) {
+    const double t = ((double)x - (double)ref) * c;
+    const double big = t + 6755399441055744.0, f = t - (big - 6755399441055744.0);
+    // ln(2)^n / n!
+    double e = 4.4455382718708114976e-10;
+    e = fma(e, f, 7.0549116208011233299e-9);
+    e = fma(e, f, 1.0178086009239699728e-7);
+    e = fma(e, f, 1.3215486790144309488e-6);
+    e = fma(e, f, 1.5252733804059840280e-5);
+    e = fma(e, f, 1.5403530393381609954e-4);
+    e = fma(e, f, 1.3333558146428443423e-3);
+    e = fma(e, f, 9.6181291076284771620e-3);
+    e = fma(e, f, 5.5504108664821579953e-2);
+    e = fma(e, f, 2.4022650695910071233e-1);
+    e = fma(e, f, 6.9314718055994530942e-1);
+    e = fma(e, f, 1.0);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, e);
+    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, big) << 20);
+    const bool some = t >= -1000.0;  // (no NaN: 0 times an infinity)
+    return __builtin_bit_cast(double, some ? (uint64_t)hi << 32 | (uint32_t)bits : 0);
 }
-// exp((x - ref) / T): a masked logit has no weight at any temperature
-__device__ __forceinline__ double dv_weight(float x, float ref, double inv_t) {
-    return x == -INFINITY ? 0.0 : dv_exp(((double)x - (double)ref) * inv_t);
+constexpr double DV_LOG2E = 1.4426950408889634074;
+// what p = wp ip has above q = wq iq: of equal distributions exactly 0
+__device__ __forceinline__ double dv_above(double wp, double ip, double wq, double iq) {
+#pragma clang fp contract(off)
+    return fmax(wp * ip - wq * iq, 0.0);
 }
+// ... and a sum of those that equal distributions in another order of additions may leave
+constexpr double DV_NOTHING = 0x1p-40;
 
-template <typename T> __device__ __forceinline__ T dv_sum(T v, int lanes = 64) {
-    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, 64);
+// A lane's value and its partner's in a butterfly of STEP = 1, 2, 4, ..: within the vector
+// unit (4 and 8 mirror groups whose lanes already agree)
+template <int STEP> __device__ __forceinline__ uint32_t dv_other(uint32_t v) {
+    if constexpr (STEP == 1) return __builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true);
+    else if constexpr (STEP == 2) return __builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true);
+    else if constexpr (STEP == 4) return __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true);
+    else if constexpr (STEP == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true);
+    else return __shfl_xor(v, STEP, 64);
+}
+template <int STEP, typename T> __device__ __forceinline__ T dv_swap(T v) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, dv_other<STEP>(__builtin_bit_cast(uint32_t, v)));
+    else {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, (uint64_t)dv_other<STEP>((uint32_t)(b >> 32)) << 32 | dv_other<STEP>((uint32_t)b));
+    }
+}
+// f over the first `lanes` lanes' values (a power of two), in each of them
+template <typename T, typename F> __device__ __forceinline__ T dv_all(T v, int lanes, F f) {
+    if (lanes > 1) v = f(v, dv_swap<1>(v));
+    if (lanes > 2) v = f(v, dv_swap<2>(v));
+    if (lanes > 4) v = f(v, dv_swap<4>(v));
+    if (lanes > 8) v = f(v, dv_swap<8>(v));
+    if (lanes > 16) v = f(v, dv_swap<16>(v));
+    if (lanes > 32) v = f(v, dv_swap<32>(v));
     return v;
 }
-__device__ __forceinline__ float dv_max(float v, int lanes = 64) {
-    for (int o = 1; o < lanes; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+__device__ __forceinline__ double dv_sum(double v, int lanes = 64) {
+    return dv_all(v, lanes, [](double a, double b) { return a + b; });
 }
-__device__ __forceinline__ int dv_min(int v, int lanes = 64) {
-    for (int o = 1; o < lanes; o <<= 1) v = min(v, __shfl_xor(v, o, 64));
-    return v;
-}
+__device__ __forceinline__ float dv_max(float v, int lanes = 64) { return dv_all(v, lanes, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ int dv_min(int v, int lanes = 64) { return dv_all(v, lanes, [](int a, int b) { return min(a, b); }); }
 
 struct DvSeq {
     int b, n;  // first draft, drafts that are looked at
@@ -151,7 +180,7 @@ __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args 
     if (i < 0 || i >= q.n + (target ? 1 : 0) || (greedy && !target)) return;  // nobody looks at the row
     const L load(target ? a.target : a.draft, row, target ? a.target_stride : a.draft_stride, a.vocab);
     const int first = p * chunk - load.shift + threadIdx.x * C, end = min((p + 1) * chunk - load.shift, a.vocab);
-    const double inv_t = greedy ? 0.0 : 1.0 / (double)T;
+    const double c_t = greedy ? 0.0 : DV_LOG2E / (double)T;
     float top = -INFINITY, ref = -INFINITY;
     int at = 0x7fffffff;
     double sum = 0.0;
@@ -178,9 +207,9 @@ __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args 
 #pragma unroll
             for (int v = 0; v < AT_ONCE; ++v)
 #pragma unroll
-                for (int c = 0; c < C; ++c) sum += dv_weight(x[v][c], ref, inv_t);
+                for (int c = 0; c < C; ++c) sum += dv_weight(x[v][c], ref, c_t);
         }
-        if (greedy || bad || !(((double)top - (double)ref) * inv_t * 1.4426950408889634074 > DV_ABOVE)) break;
+        if (greedy || bad || !(((double)top - (double)ref) * c_t > DV_ABOVE)) break;
         ref = top;
         sum = 0.0;
     }
@@ -193,7 +222,7 @@ __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args 
     __syncthreads();
     const float R = fmaxf(fmaxf(s_ref[0], s_ref[1]), fmaxf(s_ref[2], s_ref[3]));
     if (greedy) at = dv_min(ref == R ? at : 0x7fffffff);
-    else sum = dv_sum(sum * dv_weight(ref, R, inv_t));  // (no element but -inf: 0)
+    else sum = dv_sum(sum * dv_weight(ref, R, c_t));  // (no element but -inf: 0)
     if (__builtin_amdgcn_ballot_w64(bad) != 0) sum = NAN;
     if (lane == 0) s_sum[wave] = sum, s_at[wave] = at;
     __syncthreads();
@@ -207,12 +236,12 @@ struct DvRow {
     float m;
     int at;    // greedy: the likeliest token
 };
-__device__ __forceinline__ DvRow dv_row(const DvPart *parts, int P, int c, int lanes, bool greedy, double inv_t) {
+__device__ __forceinline__ DvRow dv_row(const DvPart *parts, int P, int c, int lanes, bool greedy, double c_t) {
     DvPart x = {0.0, -INFINITY, 0x7fffffff};
     if (c < P) x = parts[c];
     DvRow r;
     r.m = dv_max(x.ref, lanes);
-    double z = x.ref == -INFINITY ? 0.0 : x.sum * (greedy ? 0.0 : dv_weight(x.ref, r.m, inv_t));
+    double z = x.ref == -INFINITY ? 0.0 : x.sum * (greedy ? 0.0 : dv_weight(x.ref, r.m, c_t));
     if (x.sum != x.sum) z = NAN;
     r.z = dv_sum(z, lanes);
     r.at = greedy ? dv_min(x.ref == r.m ? x.at : 0x7fffffff, lanes) : 0;
@@ -221,7 +250,7 @@ __device__ __forceinline__ DvRow dv_row(const DvPart *parts, int P, int c, int l
 }
 
 template <int TY>
-__global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_args a, int P, int chunk, int lanes,
+__global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_args a, int P, int M, int chunk, int lanes,
                                                       const DvPart *__restrict__ parts, DvStop *__restrict__ stops,
                                                       DvMass *__restrict__ masses) {
     using L = DvLoad<TY>;
@@ -230,7 +259,7 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
     const DvSeq q = dv_seq(a, s);
     const float T = a.temperatures[s];
     const bool greedy = !(T > 0.0f);
-    const double inv_t = 1.0 / (double)T;
+    const double c_t = DV_LOG2E / (double)T;
     const int64_t t0 = q.b + s;                                      // the target's first row
     const DvPart *tp = parts + t0 * P, *dp = parts + ((int64_t)a.num_drafts + a.num_seqs + q.b) * P;
     __shared__ int s_stop;
@@ -245,11 +274,11 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
         const float u = a.accept_at[q.b + i];
         const float tx = known ? dv_elem<TY>(a.target, (t0 + i) * a.target_stride + x) : -INFINITY;
         const float dx = known && drawn ? dv_elem<TY>(a.draft, (int64_t)(q.b + i) * a.draft_stride + x) : -INFINITY;
-        const DvRow t = dv_row(tp + (int64_t)i * P, P, c, lanes, greedy, inv_t);
-        const DvRow d = drawn ? dv_row(dp + (int64_t)i * P, P, c, lanes, false, inv_t) : DvRow{1.0, 0.0f, 0};
+        const DvRow t = dv_row(tp + (int64_t)i * P, P, c, lanes, greedy, c_t);
+        const DvRow d = drawn ? dv_row(dp + (int64_t)i * P, P, c, lanes, false, c_t) : DvRow{1.0, 0.0f, 0};
         const bool bad = t.z != t.z || d.z != d.z;
-        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? dv_weight(tx, t.m, inv_t) / t.z : 0.0;
-        const double qx = !known ? 0.0 : drawn ? dv_weight(dx, d.m, inv_t) / d.z : 1.0;
+        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? dv_weight(tx, t.m, c_t) / t.z : 0.0;
+        const double qx = !known ? 0.0 : drawn ? dv_weight(dx, d.m, c_t) / d.z : 1.0;
         const bool ok = !bad && (greedy ? px == 1.0 : (double)u * qx < px);
         if (c == 0 && !ok) atomicMin(&s_stop, i);
         if (p == 0 && c == 0 && a.accept_probs)
@@ -258,8 +287,8 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
     __syncthreads();
     const int stop = s_stop;
     const bool minus = stop < q.n && a.draft && !greedy;  // a refused draft: its drafter's weights are taken off
-    const DvRow t = dv_row(tp + (int64_t)stop * P, P, lane, 64, greedy, inv_t);
-    const DvRow d = minus ? dv_row(dp + (int64_t)stop * P, P, lane, 64, false, inv_t) : DvRow{0.0, 0.0f, 0};
+    const DvRow t = dv_row(tp + (int64_t)stop * P, P, lane, 64, greedy, c_t);
+    const DvRow d = minus ? dv_row(dp + (int64_t)stop * P, P, lane, 64, false, c_t) : DvRow{0.0, 0.0f, 0};
     const bool bad = t.z != t.z || d.z != d.z;
     const int outright = stop < q.n && !a.draft && !greedy ? a.tokens[q.b + stop] : -1;  // and of one proposed outright, itself
     if (p == 0) {
@@ -277,8 +306,7 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
     const bool alike = lt.shift == ld.shift;  // else the drafter's row is read element by element
     const int first = p * chunk - lt.shift + threadIdx.x * C, end = min((p + 1) * chunk - lt.shift, a.vocab);
     const double ip = 1.0 / t.z, iq = minus ? 1.0 / d.z : 0.0;
-    double sum = 0.0;
-    int last = -1;
+    double sum = 0.0, whole = 0.0;
 #pragma unroll 1
     for (int e = first; e < end; e += 256 * C) {
         float x[C], y[C];
@@ -286,48 +314,40 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
         if (minus) ld.vec(e, alike, y);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-            double w = dv_weight(x[k], t.m, inv_t) * ip;
-            if (minus) w = fmax(w - dv_weight(y[k], d.m, inv_t) * iq, 0.0);
-            if (e + k == outright) w = 0.0;
-            sum += w;
-            if (w > 0.0) last = e + k;
+            const double w = dv_weight(x[k], t.m, c_t), above = minus ? dv_above(w, ip, dv_weight(y[k], d.m, c_t), iq) : w * ip;
+            whole += w * ip;
+            sum += e + k == outright ? 0.0 : above;
         }
     }
-    sum = dv_sum(sum);
-    last = -dv_min(-last);
-    __shared__ double s_sum[4];
-    __shared__ int s_last[4];
-    if (lane == 0) s_sum[wave] = sum, s_last[wave] = last;
+    sum = dv_sum(sum), whole = dv_sum(whole);
+    __shared__ DvMass s_mass[4];
+    if (lane == 0) s_mass[wave] = {sum, whole};
     __syncthreads();
     if (threadIdx.x == 0)
-        masses[(int64_t)s * P + p] = {(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), max(max(s_last[0], s_last[1]), max(s_last[2], s_last[3])), 0};
+        masses[(int64_t)s * M + p] = {(s_mass[0].sum + s_mass[1].sum) + (s_mass[2].sum + s_mass[3].sum),
+                                      (s_mass[0].whole + s_mass[1].whole) + (s_mass[2].whole + s_mass[3].whole)};
 }
 
 // One workgroup a sequence: the chunk, then the token in it, a thread a run of elements.
 constexpr int DV_DRAW = 1024;
 template <int TY>
-__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int P, int chunk, const DvPart *__restrict__ parts,
-                                                        const DvStop *__restrict__ stops, const DvMass *__restrict__ masses) {
+__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int M, int chunk, const DvStop *__restrict__ stops,
+                                                        const DvMass *__restrict__ masses) {
     constexpr int ES = TY == TLH_TYPE_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x;
     const DvStop st = stops[s];
     if (!st.draws) return;
     const DvSeq q = dv_seq(a, s);
-    const double inv_t = 1.0 / (double)a.temperatures[s];
+    const double c_t = DV_LOG2E / (double)a.temperatures[s];
     const int64_t row = q.b + s + st.stop;
     bool minus = st.stop < q.n && a.draft;
     int outright = st.stop < q.n && !a.draft ? a.tokens[q.b + st.stop] : -1;
-    DvMass m = {0.0, -1, 0};
-    if (lane < P) m = masses[(int64_t)s * P + lane];
-    if (dv_sum(m.sum) == 0.0) {  // nothing above the drafter's: from p alone
+    DvMass m = {};
+    if (lane < M) m = masses[(int64_t)s * M + lane];
+    if (dv_sum(m.sum) <= DV_NOTHING) {  // nothing above the drafter's: from p alone
         minus = false;
         outright = -1;
-        m = {0.0, -1, 0};
-        if (lane < P) {
-            const DvPart x = parts[row * P + lane];
-            m.sum = x.ref == -INFINITY ? 0.0 : x.sum * dv_weight(x.ref, st.mp, inv_t) / st.zp;
-            m.last = m.sum > 0.0 ? 0x7fffffff : -1;  // (the last one with a weight is found below)
-        }
+        m.sum = m.whole;
     }
     double run = m.sum;
     for (int o = 1; o < 64; o <<= 1) {
@@ -336,7 +356,7 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     }
     const double total = __shfl(run, 63, 64);
     const double reach = (double)a.sample_at[s] * total;
-    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < P && run > reach), any = __builtin_amdgcn_ballot_w64(m.last >= 0);
+    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < M && run > reach), any = __builtin_amdgcn_ballot_w64(m.sum > 0.0);
     const int p = over != 0 ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((unsigned long long)any);  // else the last with a weight
     double from = __shfl(run - m.sum, p, 64);
 
@@ -345,9 +365,10 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     const int each = chunk / DV_DRAW, e0 = max(first + (int)threadIdx.x * each, 0), e1 = min(first + ((int)threadIdx.x + 1) * each, a.vocab);
     const double ip = 1.0 / st.zp, iq = minus ? 1.0 / st.zq : 0.0;
     auto mass = [&](int e) {
-        double w = dv_weight(dv_elem<TY>(base, e), st.mp, inv_t) * ip;
-        if (minus) w = fmax(w - dv_weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, inv_t) * iq, 0.0);
-        return e == outright ? 0.0 : w;
+        const double w = dv_weight(dv_elem<TY>(base, e), st.mp, c_t);
+        if (e == outright) return 0.0;
+        if (!minus) return w * ip;
+        return dv_above(w, ip, dv_weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, c_t), iq);
     };
     double sum = 0.0;
     int last = -1;
@@ -399,6 +420,9 @@ static int dv_ept(int64_t rows, int64_t vocab) {
 static int dv_chunks(int64_t vocab, int ept) {
     return (int)((vocab + 7 + 256 * ept - 1) / (256 * ept));  // up to 7 places before a row that is not aligned
 }
+// What is drawn from is one row a sequence: in short chunks wherever a lane each are enough.
+static int dv_mass_ept(int64_t vocab) { return vocab + 7 <= (int64_t)DV_CHUNK_SMALL * DV_MAX_CHUNKS ? 16 : 64; }
+static int dv_mass_chunks(int64_t vocab) { return dv_chunks(vocab, dv_mass_ept(vocab)); }
 static int64_t dv_rows(const tlh_draft_verify_args &a) { return (int64_t)a.num_drafts + a.num_seqs + (a.draft ? a.num_drafts : 0); }
 
 // Room for either chunk length, so that the size grows with the rows and one buffer for
@@ -408,23 +432,24 @@ static size_t dv_most_chunks(int64_t rows, int64_t vocab) {
                            : (size_t)rows * dv_chunks(vocab, 64) + (size_t)std::min<int64_t>(rows, 256) * dv_chunks(vocab, 16);
 }
 size_t draft_verify_scratch_bytes(const tlh_draft_verify_args &a) {
-    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * dv_most_chunks(a.num_seqs, a.vocab) +
+    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * (size_t)a.num_seqs * dv_mass_chunks(a.vocab) +
            sizeof(DvPart) * dv_most_chunks(dv_rows(a), a.vocab);
 }
 
 template <int TY> static void launch_dv(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {
     const int64_t rows = dv_rows(a);
     const int ept = dv_ept(rows, a.vocab), chunk = 256 * ept, P = dv_chunks(a.vocab, ept);
+    const int M = dv_mass_chunks(a.vocab), mass_chunk = 256 * dv_mass_ept(a.vocab);
     int lanes = 1;
     while (lanes < P) lanes <<= 1;
     DvStop *stops = (DvStop *)scratch;
     DvMass *masses = (DvMass *)(stops + a.num_seqs);
-    DvPart *parts = (DvPart *)(masses + dv_most_chunks(a.num_seqs, a.vocab));
+    DvPart *parts = (DvPart *)(masses + (size_t)a.num_seqs * M);
     for (int64_t r0 = 0; r0 < rows; r0 += 65535)  // grid y
         hipLaunchKernelGGL((k_draft_rows<TY>), dim3(P, (unsigned)std::min<int64_t>(rows - r0, 65535)), dim3(256), 0, stream, a, (int)r0,
                            P, chunk, parts);
-    hipLaunchKernelGGL((k_draft_masses<TY>), dim3(P, a.num_seqs), dim3(256), 0, stream, a, P, chunk, lanes, parts, stops, masses);
-    hipLaunchKernelGGL((k_draft_draw<TY>), dim3(a.num_seqs), dim3(DV_DRAW), 0, stream, a, P, chunk, parts, stops, masses);
+    hipLaunchKernelGGL((k_draft_masses<TY>), dim3(M, a.num_seqs), dim3(256), 0, stream, a, P, M, mass_chunk, lanes, parts, stops, masses);
+    hipLaunchKernelGGL((k_draft_draw<TY>), dim3(a.num_seqs), dim3(DV_DRAW), 0, stream, a, M, mass_chunk, stops, masses);
 }
 
 tlh_status launch_draft_verify(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {
