@@ -12,6 +12,7 @@
 // of a sequence finds where it stops, and sums its chunk of what the token there is drawn
 // from; then one workgroup a sequence finds the chunk and the token in it.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 
@@ -46,33 +47,33 @@ template <int TY> __device__ __forceinline__ float dv_elem(const void *p, int64_
     else return bf16_to_f32(((const uint16_t *)p)[i]);
 }
 
-// exp((x - ref) / T) with c = log2(e) / T, off by less than 2^-45 of it (2^-52 times the
-// exponent, 2^-47 from the series): 2^k times the Taylor series of 2^f, |f| <= 1/2, up to
-// f^11. The instructions that convert between f64 and integers, round or scale are slow
+// exp((x - ref) / T) with c = log2(e) / T, off by less than 2^-45 of it (and 2^-52 times the
+// exponent): 2^k times the polynomial that agrees with 2^f, |f| <= 1/2, at the ten Chebyshev
+// nodes. The instructions that convert between f64 and integers, round or scale are slow
 // beside its additions and products: k is the low word of the sum with 1.5 x 2^52, and is
-// added to the result's exponent (32 x 1..8: 57 us with them, ROWS_US without). Nothing is
-// left below 2^-1000, and nothing of a masked logit (-inf), at any temperature.
-__device__ __forceinline__ double dv_weight(float x, float ref, double c) {
-    const double t = ((double)x - (double)ref) * c;
-    const double big = t + 6755399441055744.0, f = t - (big - 6755399441055744.0);
-    // ln(2)^n / n!
-    double e = 4.4455382718708114976e-10;
-    e = fma(e, f, 7.0549116208011233299e-9);
-    e = fma(e, f, 1.0178086009239699728e-7);
-    e = fma(e, f, 1.3215486790144309488e-6);
-    e = fma(e, f, 1.5252733804059840280e-5);
-    e = fma(e, f, 1.5403530393381609954e-4);
-    e = fma(e, f, 1.3333558146428443423e-3);
-    e = fma(e, f, 9.6181291076284771620e-3);
-    e = fma(e, f, 5.5504108664821579953e-2);
-    e = fma(e, f, 2.4022650695910071233e-1);
-    e = fma(e, f, 6.9314718055994530942e-1);
-    e = fma(e, f, 1.0);
-    const uint64_t bits = __builtin_bit_cast(uint64_t, e);
-    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, big) << 20);
-    const bool some = t >= -1000.0;  // (no NaN: 0 times an infinity)
-    return __builtin_bit_cast(double, some ? (uint64_t)hi << 32 | (uint32_t)bits : 0);
-}
+// added to the result's exponent. Nothing is left below 2^-1000, and nothing of a masked
+// logit (-inf), at any temperature. (32 x 1..8, the rows' sums, us: with rint, ldexp and a
+// Taylor series up to f^12 56, up to f^11 without them 43, this 40.)
+struct DvExp {
+    double k[10];  // from f^9 down, in vector registers: else each would be moved there for every use
+    __device__ __forceinline__ DvExp()
+        : k{1.0205905413765595e-07, 1.325964524488711e-06, 1.5252672924850737e-05, 0.0001540343375125101, 0.0013333558200794592,
+            0.009618129193934313, 0.05550410866465167, 0.2402265069564034, 0.6931471805599462, 1.0000000000000135} {
+#pragma unroll
+        for (int i = 0; i < 10; ++i) asm("" : "+v"(k[i]));
+    }
+    __device__ __forceinline__ double operator()(float x, float ref, double c) const {
+        const double t = ((double)x - (double)ref) * c;
+        const double big = t + 6755399441055744.0, f = t - (big - 6755399441055744.0);
+        double e = k[0];
+#pragma unroll
+        for (int i = 1; i < 10; ++i) e = fma(e, f, k[i]);
+        const uint64_t bits = __builtin_bit_cast(uint64_t, e);
+        const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, big) << 20);
+        const bool some = t >= -1000.0;  // (no NaN: 0 times an infinity)
+        return __builtin_bit_cast(double, some ? (uint64_t)hi << 32 | (uint32_t)bits : 0);
+    }
+};
 constexpr double DV_LOG2E = 1.4426950408889634074;
 // what p = wp ip has above q = wq iq: of equal distributions exactly 0
 __device__ __forceinline__ double dv_above(double wp, double ip, double wq, double iq) {
@@ -148,26 +149,31 @@ template <int TY> struct DvLoad {
     int V, shift;
     __device__ __forceinline__ DvLoad(const void *logits, int64_t row, int64_t stride, int vocab)
         : base((const char *)logits + row * stride * ES), V(vocab), shift((int)(((uintptr_t)base & 15) / ES)) {}
-    __device__ __forceinline__ void vec(int e, bool aligned, float (&x)[C]) const {
-        if (aligned && e >= 0 && e + C <= V) {
-            const uint4 w = *(const uint4 *)(base + (int64_t)e * ES);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    __device__ __forceinline__ void whole(int e, float (&x)[C]) const {
+        const uint4 w = *(const uint4 *)(base + (int64_t)e * ES);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                x[c] = TY == TLH_TYPE_F32   ? __uint_as_float(ws[c % 4])
-                       : TY == TLH_TYPE_F16 ? h2f((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))))
-                                            : bf16_to_f32((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))));
-        } else {
+        for (int c = 0; c < C; ++c)
+            x[c] = TY == TLH_TYPE_F32   ? __uint_as_float(ws[c % 4])
+                   : TY == TLH_TYPE_F16 ? h2f((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))))
+                                        : bf16_to_f32((uint16_t)(ws[c / 2 % 4] >> (16 * (c & 1))));
+    }
+    __device__ __forceinline__ void vec(int e, bool aligned, float (&x)[C]) const {
+        if (aligned && e >= 0 && e + C <= V) whole(e, x);
+        else {
 #pragma unroll
             for (int c = 0; c < C; ++c) x[c] = e + c >= 0 && e + c < V ? dv_elem<TY>(base, e + c) : -INFINITY;
         }
     }
 };
 
+// the larger one, or a NaN
+__device__ __forceinline__ float dv_top(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 template <int TY>
 __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args a, int r0, int P, int chunk, DvPart *__restrict__ parts) {
     using L = DvLoad<TY>;
-    constexpr int C = L::C, AT_ONCE = 16 / C;  // vectors on their way at a time
+    constexpr int C = L::C, AT_ONCE = 16 / C, STEP = 256 * C * AT_ONCE;  // vectors on their way at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = blockIdx.x;
     const int r = r0 + blockIdx.y, targets = a.num_drafts + a.num_seqs;
     const bool target = r < targets;
@@ -179,40 +185,63 @@ __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args 
     const int i = row - q.b - (target ? s : 0);
     if (i < 0 || i >= q.n + (target ? 1 : 0) || (greedy && !target)) return;  // nobody looks at the row
     const L load(target ? a.target : a.draft, row, target ? a.target_stride : a.draft_stride, a.vocab);
-    const int first = p * chunk - load.shift + threadIdx.x * C, end = min((p + 1) * chunk - load.shift, a.vocab);
+    const int begin = p * chunk - load.shift, end = min(begin + chunk, a.vocab), first = begin + threadIdx.x * C;
     const double c_t = greedy ? 0.0 : DV_LOG2E / (double)T;
     float top = -INFINITY, ref = -INFINITY;
     int at = 0x7fffffff;
     double sum = 0.0;
-    bool bad = false;
-    for (;;) {
+    // (edge: the chunk reaches past the row)
+    const DvExp weight;
+    auto get = [&](auto edge, int e, float (&x)[AT_ONCE][C]) {
+#pragma unroll
+        for (int v = 0; v < AT_ONCE; ++v) {
+            if constexpr (edge()) load.vec(e + 256 * C * v, true, x[v]);
+            else load.whole(e + 256 * C * v, x[v]);
+        }
+    };
+    auto pass = [&](auto edge) {
+        top = -INFINITY, sum = 0.0;
+        float next[AT_ONCE][C];
+        get(edge, first, next);
 #pragma unroll 1
-        for (int e = first; e < end; e += 256 * C * AT_ONCE) {
+        for (int e = first; e - (int)threadIdx.x * C < end; e += STEP) {
             float x[AT_ONCE][C];
 #pragma unroll
             for (int v = 0; v < AT_ONCE; ++v)
-                if (e + 256 * C * v < end) load.vec(e + 256 * C * v, true, x[v]);
-                else
 #pragma unroll
-                    for (int c = 0; c < C; ++c) x[v][c] = -INFINITY;
+                for (int c = 0; c < C; ++c) x[v][c] = next[v][c];
+            if (e - (int)threadIdx.x * C + STEP < end) get(edge, e + STEP, next);
+            float m = x[0][0];
 #pragma unroll
             for (int v = 0; v < AT_ONCE; ++v)
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    if (x[v][c] > top) top = x[v][c], at = e + 256 * C * v + c;
-                    bad = bad || (greedy ? x[v][c] != x[v][c] : !(x[v][c] < INFINITY));
+                for (int c = 0; c < C; ++c) m = dv_top(m, x[v][c]);
+            if (greedy) {
+                if (m > top) {
+#pragma unroll
+                    for (int v = AT_ONCE - 1; v >= 0; --v)
+#pragma unroll
+                        for (int c = C - 1; c >= 0; --c) at = x[v][c] == m ? e + 256 * C * v + c : at;
                 }
-            if (greedy || top == -INFINITY) continue;
-            if (ref == -INFINITY) ref = top;
+                top = dv_top(top, m);
+                continue;
+            }
+            top = dv_top(top, m);
+            ref = ref == -INFINITY ? top : ref;
+            if (__builtin_amdgcn_ballot_w64(ref != -INFINITY) == 0) continue;  // masked so far
 #pragma unroll
             for (int v = 0; v < AT_ONCE; ++v)
 #pragma unroll
-                for (int c = 0; c < C; ++c) sum += dv_weight(x[v][c], ref, c_t);
+                for (int c = 0; c < C; ++c) sum += weight(x[v][c], ref, c_t);
         }
-        if (greedy || bad || !(((double)top - (double)ref) * c_t > DV_ABOVE)) break;
+    };
+    for (;;) {
+        if (begin < 0 || begin + chunk > a.vocab) pass(std::true_type());
+        else pass(std::false_type());
+        if (greedy || !(((double)top - (double)ref) * c_t > DV_ABOVE)) break;
         ref = top;
-        sum = 0.0;
     }
+    const bool bad = greedy ? top != top : !(top < INFINITY);
     __shared__ float s_ref[4];
     __shared__ double s_sum[4];
     __shared__ int s_at[4];
@@ -222,7 +251,7 @@ __global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args 
     __syncthreads();
     const float R = fmaxf(fmaxf(s_ref[0], s_ref[1]), fmaxf(s_ref[2], s_ref[3]));
     if (greedy) at = dv_min(ref == R ? at : 0x7fffffff);
-    else sum = dv_sum(sum * dv_weight(ref, R, c_t));  // (no element but -inf: 0)
+    else sum = dv_sum(sum * weight(ref, R, c_t));  // (no element but -inf: 0)
     if (__builtin_amdgcn_ballot_w64(bad) != 0) sum = NAN;
     if (lane == 0) s_sum[wave] = sum, s_at[wave] = at;
     __syncthreads();
@@ -236,12 +265,12 @@ struct DvRow {
     float m;
     int at;    // greedy: the likeliest token
 };
-__device__ __forceinline__ DvRow dv_row(const DvPart *parts, int P, int c, int lanes, bool greedy, double c_t) {
+__device__ __forceinline__ DvRow dv_row(const DvExp &weight, const DvPart *parts, int P, int c, int lanes, bool greedy, double c_t) {
     DvPart x = {0.0, -INFINITY, 0x7fffffff};
     if (c < P) x = parts[c];
     DvRow r;
     r.m = dv_max(x.ref, lanes);
-    double z = x.ref == -INFINITY ? 0.0 : x.sum * (greedy ? 0.0 : dv_weight(x.ref, r.m, c_t));
+    double z = x.ref == -INFINITY ? 0.0 : x.sum * (greedy ? 0.0 : weight(x.ref, r.m, c_t));
     if (x.sum != x.sum) z = NAN;
     r.z = dv_sum(z, lanes);
     r.at = greedy ? dv_min(x.ref == r.m ? x.at : 0x7fffffff, lanes) : 0;
@@ -262,6 +291,7 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
     const double c_t = DV_LOG2E / (double)T;
     const int64_t t0 = q.b + s;                                      // the target's first row
     const DvPart *tp = parts + t0 * P, *dp = parts + ((int64_t)a.num_drafts + a.num_seqs + q.b) * P;
+    const DvExp weight;
     __shared__ int s_stop;
     if (threadIdx.x == 0) s_stop = q.n;
     __syncthreads();
@@ -274,11 +304,11 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
         const float u = a.accept_at[q.b + i];
         const float tx = known ? dv_elem<TY>(a.target, (t0 + i) * a.target_stride + x) : -INFINITY;
         const float dx = known && drawn ? dv_elem<TY>(a.draft, (int64_t)(q.b + i) * a.draft_stride + x) : -INFINITY;
-        const DvRow t = dv_row(tp + (int64_t)i * P, P, c, lanes, greedy, c_t);
-        const DvRow d = drawn ? dv_row(dp + (int64_t)i * P, P, c, lanes, false, c_t) : DvRow{1.0, 0.0f, 0};
+        const DvRow t = dv_row(weight, tp + (int64_t)i * P, P, c, lanes, greedy, c_t);
+        const DvRow d = drawn ? dv_row(weight, dp + (int64_t)i * P, P, c, lanes, false, c_t) : DvRow{1.0, 0.0f, 0};
         const bool bad = t.z != t.z || d.z != d.z;
-        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? dv_weight(tx, t.m, c_t) / t.z : 0.0;
-        const double qx = !known ? 0.0 : drawn ? dv_weight(dx, d.m, c_t) / d.z : 1.0;
+        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? weight(tx, t.m, c_t) / t.z : 0.0;
+        const double qx = !known ? 0.0 : drawn ? weight(dx, d.m, c_t) / d.z : 1.0;
         const bool ok = !bad && (greedy ? px == 1.0 : (double)u * qx < px);
         if (c == 0 && !ok) atomicMin(&s_stop, i);
         if (p == 0 && c == 0 && a.accept_probs)
@@ -287,8 +317,8 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
     __syncthreads();
     const int stop = s_stop;
     const bool minus = stop < q.n && a.draft && !greedy;  // a refused draft: its drafter's weights are taken off
-    const DvRow t = dv_row(tp + (int64_t)stop * P, P, lane, 64, greedy, c_t);
-    const DvRow d = minus ? dv_row(dp + (int64_t)stop * P, P, lane, 64, false, c_t) : DvRow{0.0, 0.0f, 0};
+    const DvRow t = dv_row(weight, tp + (int64_t)stop * P, P, lane, 64, greedy, c_t);
+    const DvRow d = minus ? dv_row(weight, dp + (int64_t)stop * P, P, lane, 64, false, c_t) : DvRow{0.0, 0.0f, 0};
     const bool bad = t.z != t.z || d.z != d.z;
     const int outright = stop < q.n && !a.draft && !greedy ? a.tokens[q.b + stop] : -1;  // and of one proposed outright, itself
     if (p == 0) {
@@ -314,7 +344,7 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
         if (minus) ld.vec(e, alike, y);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-            const double w = dv_weight(x[k], t.m, c_t), above = minus ? dv_above(w, ip, dv_weight(y[k], d.m, c_t), iq) : w * ip;
+            const double w = weight(x[k], t.m, c_t), above = minus ? dv_above(w, ip, weight(y[k], d.m, c_t), iq) : w * ip;
             whole += w * ip;
             sum += e + k == outright ? 0.0 : above;
         }
@@ -342,6 +372,7 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     const int64_t row = q.b + s + st.stop;
     bool minus = st.stop < q.n && a.draft;
     int outright = st.stop < q.n && !a.draft ? a.tokens[q.b + st.stop] : -1;
+    const DvExp weight;
     DvMass m = {};
     if (lane < M) m = masses[(int64_t)s * M + lane];
     if (dv_sum(m.sum) <= DV_NOTHING) {  // nothing above the drafter's: from p alone
@@ -365,10 +396,10 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     const int each = chunk / DV_DRAW, e0 = max(first + (int)threadIdx.x * each, 0), e1 = min(first + ((int)threadIdx.x + 1) * each, a.vocab);
     const double ip = 1.0 / st.zp, iq = minus ? 1.0 / st.zq : 0.0;
     auto mass = [&](int e) {
-        const double w = dv_weight(dv_elem<TY>(base, e), st.mp, c_t);
+        const double w = weight(dv_elem<TY>(base, e), st.mp, c_t);
         if (e == outright) return 0.0;
         if (!minus) return w * ip;
-        return dv_above(w, ip, dv_weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, c_t), iq);
+        return dv_above(w, ip, weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, c_t), iq);
     };
     double sum = 0.0;
     int last = -1;
