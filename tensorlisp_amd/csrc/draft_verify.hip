@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "kernels.hpp"
+#include "wave_ops.hpp"
 
 namespace tlh {
 
@@ -83,37 +84,11 @@ __device__ __forceinline__ double dv_above(double wp, double ip, double wq, doub
 // ... and a sum of those that equal distributions in another order of additions may leave
 constexpr double DV_NOTHING = 0x1p-40;
 
-// A lane's value and its partner's in a butterfly of STEP = 1, 2, 4, ..: within the vector
-// unit (4 and 8 mirror groups whose lanes already agree)
-template <int STEP> __device__ __forceinline__ uint32_t dv_other(uint32_t v) {
-    if constexpr (STEP == 1) return __builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true);
-    else if constexpr (STEP == 2) return __builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true);
-    else if constexpr (STEP == 4) return __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true);
-    else if constexpr (STEP == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true);
-    else return __shfl_xor(v, STEP, 64);
-}
-template <int STEP, typename T> __device__ __forceinline__ T dv_swap(T v) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, dv_other<STEP>(__builtin_bit_cast(uint32_t, v)));
-    else {
-        const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        return __builtin_bit_cast(T, (uint64_t)dv_other<STEP>((uint32_t)(b >> 32)) << 32 | dv_other<STEP>((uint32_t)b));
-    }
-}
-// f over the first `lanes` lanes' values (a power of two), in each of them
-template <typename T, typename F> __device__ __forceinline__ T dv_all(T v, int lanes, F f) {
-    if (lanes > 1) v = f(v, dv_swap<1>(v));
-    if (lanes > 2) v = f(v, dv_swap<2>(v));
-    if (lanes > 4) v = f(v, dv_swap<4>(v));
-    if (lanes > 8) v = f(v, dv_swap<8>(v));
-    if (lanes > 16) v = f(v, dv_swap<16>(v));
-    if (lanes > 32) v = f(v, dv_swap<32>(v));
-    return v;
-}
 __device__ __forceinline__ double dv_sum(double v, int lanes = 64) {
-    return dv_all(v, lanes, [](double a, double b) { return a + b; });
+    return wave_all(v, lanes, [](double a, double b) { return a + b; });
 }
-__device__ __forceinline__ float dv_max(float v, int lanes = 64) { return dv_all(v, lanes, [](float a, float b) { return fmaxf(a, b); }); }
-__device__ __forceinline__ int dv_min(int v, int lanes = 64) { return dv_all(v, lanes, [](int a, int b) { return min(a, b); }); }
+__device__ __forceinline__ float dv_max(float v, int lanes = 64) { return wave_all(v, lanes, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ int dv_min(int v, int lanes = 64) { return wave_all(v, lanes, [](int a, int b) { return min(a, b); }); }
 
 struct DvSeq {
     int b, n;  // first draft, drafts that are looked at
