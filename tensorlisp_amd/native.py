@@ -635,7 +635,10 @@ def _token_rows(t, heads: int, hs: int, name: str, device):
     """(address, token stride) of a (tokens, heads, head size) view whose tokens' heads are contiguous."""
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    st, one = t.stride(), heads * hs
+    one = heads * hs
+    if t.is_contiguous():
+        return t.data_ptr(), one
+    st = t.stride()
     if t.shape[0] <= 1:  # the stride of a single token means nothing
         st = (one, st[1], st[2])
     if t.numel() and ((hs > 1 and st[2] != 1) or (heads > 1 and st[1] != hs)):
@@ -1006,6 +1009,11 @@ class HeadRope:
         a.num_axes = max(axes, default=0) + 1
         a.pair_axis = (C.c_uint8 * 128)(*axes)
 
+    def _out(self, t, like, q_out, name: str):
+        if t.dtype != q_out.dtype or t.shape != like.shape:
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not {q_out.dtype} {tuple(like.shape)}")
+        return _token_rows(t, self.args.num_kv_heads, self.args.head_size, name, self.device)
+
     def __call__(self, q, k, v, positions, q_out, q_norm=None, k_norm=None, k_out=None, v_out=None, k_cache=None,
                  v_cache=None, slots=None, stream=None):
         """q (tokens, heads, head size), k and v (tokens, kv heads, head size) f32, f16 or bf16, tokens at any stride
@@ -1023,15 +1031,14 @@ class HeadRope:
         a.q, a.q_stride = _token_rows(q, H, D, "q", dev)
         a.k, a.k_stride = _token_rows(k, KV, D, "k", dev)
         a.v, a.v_stride = _token_rows(v, KV, D, "v", dev)
-        outs = [("q_out", q_out, H, "q_out_stride"), ("k_out", k_out, KV, "k_out_stride"), ("v_out", v_out, KV, "v_out_stride")]
-        for name, t, heads, stride in outs:
-            if t is None:
-                setattr(a, stride, heads * D)
-                continue
-            if t.dtype != q_out.dtype or t.shape != (n, heads, D):
-                raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not {q_out.dtype} {(n, heads, D)}")
-            p, st = _token_rows(t, heads, D, name, dev)
-            setattr(a, name, p), setattr(a, stride, st)
+        a.q_out, a.q_out_stride = _token_rows(q_out, H, D, "q_out", dev)
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out: {tuple(q_out.shape)}, not {tuple(q.shape)}")
+        a.k_out_stride = a.v_out_stride = KV * D
+        if k_out is not None:
+            a.k_out, a.k_out_stride = self._out(k_out, k, q_out, "k_out")
+        if v_out is not None:
+            a.v_out, a.v_out_stride = self._out(v_out, k, q_out, "v_out")
         if a.n_dims:
             one = positions.dim() == 1 and a.num_axes == 1
             a.positions = _tensor(positions, torch.int32, (n,) if one else (a.num_axes, n), "positions", dev)
