@@ -22,6 +22,12 @@
 // last of an item's partitions to arrive joins them, in the order of their keys, whichever
 // it is. (Joined in a second launch, whose code has to come from memory when the keys
 // have gone through the caches, 31 tokens + 600 took 20 us more.)
+//
+// Measured, 32/8 heads of 128 unless said: 1 token over 1500 10.1 us, the plan and one chain of
+// latencies; 32 sequences decoding over 512..8192 113 us (4.9 TB/s over random pages); 31
+// decoding over 100..8000 beside a piece of 600 over 4000 149 to 178 us; 2048 over 16384 722 to
+// 740 us, 810 to 850 TFLOP/s, where the tiles' LDS reads take as long as the products; nine
+// pieces of 13..701 with 4/1 heads of 256 and a window of 1024 48 us (one wave a SIMD).
 #include <algorithm>
 #include <type_traits>
 

@@ -11,6 +11,10 @@
 // Three launches: the sums of chunks of all rows, a chunk a workgroup; then every workgroup
 // of a sequence finds where it stops, and sums its chunk of what the token there is drawn
 // from; then one workgroup a sequence finds the chunk and the token in it.
+// Measured, us (the three launches): 1 x 4 drafts of 128256 f32 5.6 + 7.8 + 5.8, of which
+// 4.5 + 5 + 5 are there with 1000 tokens, chains of latencies; 32 x 1..8 of 128256 f32, 149
+// MB, 39.5 (3.7 TB/s: f64, which the reads nearly hide) + 16.4 + 10.3; 48 x 10 of 32003
+// bf16, proposed outright, 25.5 (f64: half the bytes an element) + 9.3 + 8.7.
 #include <algorithm>
 #include <type_traits>
 
@@ -426,26 +430,35 @@ static int dv_ept(int64_t rows, int64_t vocab) {
 static int dv_chunks(int64_t vocab, int ept) {
     return (int)((vocab + 7 + 256 * ept - 1) / (256 * ept));  // up to 7 places before a row that is not aligned
 }
-// What is drawn from is one row a sequence: in short chunks wherever a lane each are enough.
-static int dv_mass_ept(int64_t vocab) { return vocab + 7 <= (int64_t)DV_CHUNK_SMALL * DV_MAX_CHUNKS ? 16 : 64; }
-static int dv_mass_chunks(int64_t vocab) { return dv_chunks(vocab, dv_mass_ept(vocab)); }
+// What is drawn from is one row a sequence: in short chunks wherever a lane each are enough,
+// and shorter still where that makes four workgroups a CU at most, whose 5 us of reading the
+// rows' parts go unseen. (Sums and draw with 8 and 16, us: 1 x 4 of 128256 13.6, 18.5; 48 of
+// 32003 17.9, 18.8; 32 of 128256, 2016 workgroups with 8, 28.0, 26.7.)
+constexpr int DV_SHORT_WGS = 1024;
+static int dv_mass_ept(int64_t seqs, int64_t vocab) {
+    if (vocab + 7 <= 8 * 256 * DV_MAX_CHUNKS && seqs * dv_chunks(vocab, 8) <= DV_SHORT_WGS) return 8;
+    return vocab + 7 <= (int64_t)DV_CHUNK_SMALL * DV_MAX_CHUNKS ? 16 : 64;
+}
 static int64_t dv_rows(const tlh_draft_verify_args &a) { return (int64_t)a.num_drafts + a.num_seqs + (a.draft ? a.num_drafts : 0); }
 
-// Room for either chunk length, so that the size grows with the rows and one buffer for
+// Room for any chunk length, so that the size grows with the rows and one buffer for
 // the largest batch serves every smaller one: the sequences' stops, masses, the rows' parts.
 static size_t dv_most_chunks(int64_t rows, int64_t vocab) {
     return dv_small(vocab) ? (size_t)rows * dv_chunks(vocab, 16)
                            : (size_t)rows * dv_chunks(vocab, 64) + (size_t)std::min<int64_t>(rows, 256) * dv_chunks(vocab, 16);
 }
 size_t draft_verify_scratch_bytes(const tlh_draft_verify_args &a) {
-    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * (size_t)a.num_seqs * dv_mass_chunks(a.vocab) +
+    // of as many sequences as take short chunks, or of all in longer ones
+    const int64_t longer = (int64_t)a.num_seqs * dv_chunks(a.vocab, dv_mass_ept(DV_SHORT_WGS + 1, a.vocab));
+    const int64_t masses = std::max(longer, std::min<int64_t>((int64_t)a.num_seqs * dv_chunks(a.vocab, 8), DV_SHORT_WGS));
+    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * (size_t)masses +
            sizeof(DvPart) * dv_most_chunks(dv_rows(a), a.vocab);
 }
 
 template <int TY> static void launch_dv(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {
     const int64_t rows = dv_rows(a);
     const int ept = dv_ept(rows, a.vocab), chunk = 256 * ept, P = dv_chunks(a.vocab, ept);
-    const int M = dv_mass_chunks(a.vocab), mass_chunk = 256 * dv_mass_ept(a.vocab);
+    const int mass_ept = dv_mass_ept(a.num_seqs, a.vocab), M = dv_chunks(a.vocab, mass_ept), mass_chunk = 256 * mass_ept;
     int lanes = 1;
     while (lanes < P) lanes <<= 1;
     DvStop *stops = (DvStop *)scratch;

@@ -284,6 +284,18 @@ def test_a_used_scratch_smaller_calls_streams_and_graphs(gpu):
         assert all(torch.equal(a, b) for a, b in zip(outs, other))
 
 
+@pytest.mark.parametrize("vocab", [128256, 131064, 131065])
+def test_one_node_for_few_and_many_sequences(gpu, vocab):
+    """What is drawn from is summed in chunks whose length follows from the sequences of a call (16 of these
+    vocabularies, and 131064 tokens, are the bounds); the node's scratch has room for each."""
+    c = build([2] * 20, vocab, torch.bfloat16, 40)
+    node = node_of(c)
+    for n in (20, 17, 16, 15, 1):
+        check({**c, "target": c["target"][:3 * n], "draft": c["draft"][:2 * n], "tokens": c["tokens"][:2 * n],
+               "starts": c["starts"][:n + 1], "temps": c["temps"][:n], "accept_at": c["accept_at"][:2 * n],
+               "sample_at": c["sample_at"][:n]}, node)
+
+
 def test_one_call_form(gpu):
     c = build([5, 3, 8], 32000, torch.bfloat16, 31)
     want = check(c)
