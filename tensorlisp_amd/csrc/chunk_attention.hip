@@ -24,9 +24,9 @@
 // have gone through the caches, 31 tokens + 600 took 20 us more.)
 //
 // Measured, 32/8 heads of 128 unless said: 1 token over 1500 10.1 us, the plan and one chain of
-// latencies; 32 sequences decoding over 512..8192 113 us (4.9 TB/s over random pages); 31
-// decoding over 100..8000 beside a piece of 600 over 4000 149 to 178 us; 2048 over 16384 722 to
-// 740 us, 810 to 850 TFLOP/s, where the tiles' LDS reads take as long as the products; nine
+// latencies; 32 sequences decoding over 512..8192 113 us (4.9 TB/s over random pages); 31 of
+// those beside a piece of 600 tokens 149 to 178 us; 2048 over 16384 689 to 740 us, 810 to 850
+// TFLOP/s, where the tiles' LDS reads take as long as the products; nine
 // pieces of 13..701 with 4/1 heads of 256 and a window of 1024 48 us (one wave a SIMD).
 #include <algorithm>
 #include <type_traits>
@@ -40,9 +40,11 @@ constexpr int CA_NARROW = 64;      // rows of a (sequence, kv head) up to which 
 // A partition costs a partial written and read, and the join waits for eight of them at a
 // time. So at most 32 of an item (1 token over 8000, us: 15.4 with 32, 17.5 with 42), each
 // of at least 2 tiles of 64 keys, a round of the four waves, or with more than 8 rows of 8
-// (4 x 16 tokens over 100..3000, us, with 3, 6, 9: 22.0, 21.5, 18.3; 64 tokens over 3000 with
-// 2, 4, 6, 8: 45, 31, 28.5, 29.6; 1 token over 1500 with 3, 6, 9: 10.2, 11.0, 11.9).
-constexpr int CA_MAX_PARTS = 32, CA_MIN_TILES = 2, CA_MIN_TILES_ROWS = 8;
+// (4 x 16 tokens over 100..3000, us, with 3, 6, 9: 22.0, 21.5, 18.3; 1 token over 1500 with 3,
+// 6, 9: 10.2, 11.0, 11.9); with more than 64 rows of an eighth of the tiles, from 4 to 8 (32
+// tokens with 4, 6, 8, heads of 128: over 992 20.3, 22.5, 24.0; over 4000 35.4, 32.9, 31.3; heads
+// of 256: over 992 34, 38, 41; over 2016 42, 43, 45; over 4000 57, 54, 53).
+constexpr int CA_MAX_PARTS = 32, CA_MIN_TILES = 2, CA_MIN_TILES_ROWS = 8, CA_MIN_TILES_MANY = 4;
 constexpr int CA_NO_WINDOW = 1 << 30;
 
 // n / d for 0 <= n < 2^31 by a product. What every workgroup runs before its first load is
@@ -114,7 +116,8 @@ __device__ __forceinline__ int ca_scan(int v) {
 __device__ __forceinline__ int ca_sum(int v) { return __builtin_amdgcn_readlane(ca_scan(v), 63); }
 // a sequence's partitions of at most `each` tiles: ceil(tiles / each), within the bounds
 __device__ __forceinline__ int ca_parts(const CaWork &w, int each) {
-    const int n = max(each, w.units > 2 ? CA_MIN_TILES_ROWS : CA_MIN_TILES);
+    const int least = w.wide ? max(CA_MIN_TILES_MANY, min(w.tiles >> 3, CA_MIN_TILES_ROWS)) : w.units > 2 ? CA_MIN_TILES_ROWS : CA_MIN_TILES;
+    const int n = max(each, least);
     if (w.tiles >= (int64_t)CA_MAX_PARTS * n) return CA_MAX_PARTS;
     const int q = (int)((float)w.tiles * __builtin_amdgcn_rcpf((float)n));  // off by at most 1
     const int r = w.tiles - q * n;
@@ -337,8 +340,8 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
         }
     };
     __syncthreads();
-    bool careful = false;
-    for (;;) {
+    // (a loop for each kind of pass: in one, the rare kind's registers spill the other's above 128 dims)
+    auto pass = [&](auto careful) {
         w.reset();
         typename W::Pages pg = {}, pn = {};
         if (wave < ntiles) {
@@ -358,7 +361,10 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
 #pragma unroll
             for (int st = 0; st < NS; ++st) S[0] = mfma32<false>(kf[st], s_q[64 * st + lane], S[0]);
             if (AHEAD) load_k(pn);  // past the last tile: the last page again
-            else load_v(pg);
+            else {
+                __builtin_amdgcn_sched_barrier(0);  // into the keys' registers
+                load_v(pg);
+            }
             const PagedSeen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
             uint4 pf[2];
             w.softmax(S, sees, pf);
@@ -368,7 +374,7 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
 #pragma unroll
                     for (int d = 0; d < NB; ++d) vf[d][i] = w.live_v(vf[d][i], i, see.there);
             }
-            if (careful && !see.whole) {
+            if (careful() && !see.whole) {
                 // through the wave's part of the merge buffer, which is free until the end
                 uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 128;
                 static_assert(256 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
@@ -390,9 +396,9 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
             pg = pn;
             pn = after;
         }
-        if (careful || !w.some_masked || __builtin_amdgcn_ballot_w64(w.bad()) == 0) break;
-        careful = true;
-    }
+    };
+    pass(std::false_type());
+    if (w.some_masked && __builtin_amdgcn_ballot_w64(w.bad()) != 0) pass(std::true_type());
 
     // merge the waves, MD dims at a time
     const float lt = sum_halves(w.l);
@@ -692,8 +698,11 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
         }
 }
 
+// Two workgroups a CU up to 192 dims (there with spills, outside the loops over tiles: heads of
+// 192, 16/4, with one and two, us: 2048 over 16384 882, 514; nine pieces of 13..701 177, 150; 32
+// decoding over 512..8192 93, 91; 8 x 12 tokens 52, 54).
 template <int D, int BS>
-__global__ void __launch_bounds__(64 * CA_WAVES, D <= 128 ? 2 : 1) k_chunk_attn(const CaArgs a) {
+__global__ void __launch_bounds__(64 * CA_WAVES, D <= 192 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
     __shared__ int flag;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -720,7 +729,7 @@ static CaBounds ca_bounds(const tlh_chunk_attention_args &a) {
     const bool wide = most > CA_NARROW;
     // a sequence's last block of rows may be short, and 33 to 64 rows take two
     b.items = a.num_kv_heads * (std::min<int64_t>(a.num_seqs, a.num_rows) * (most > 32 ? 2 : 1) + a.num_rows * G / 128);
-    b.wgs = a.head_size <= 128 ? 512 : 256;  // workgroups that fill the machine
+    b.wgs = a.head_size <= 192 ? 512 : 256;  // workgroups that fill the machine
     const int window = a.window > 0 ? std::min(a.window, CA_NO_WINDOW) : CA_NO_WINDOW;
     b.span_few = window + 31 / (int)G + 1, b.span_many = window + 127 / (int)G + 1;
     const int64_t tiles = ca_tiles(a.max_context_len, wide ? b.span_many : b.span_few);
