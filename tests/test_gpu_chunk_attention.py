@@ -90,6 +90,15 @@ def test_a_window_in_other_geometries(gpu, hs, bs):
     check(run(c), c)
 
 
+@pytest.mark.parametrize("window", [0, 900])
+@pytest.mark.parametrize("bs", [8, 16, 32])
+@pytest.mark.parametrize("hs", [64, 112, 192, 256])
+def test_partitions_of_long_contexts(gpu, hs, bs, window):
+    """A piece of a prompt, single tokens and a few, over contexts that are split, each in its own number of parts."""
+    c = build(8, 2, hs, bs, [2950, 700, 5000, 40, 1030], [40, 1, 3, 1, 33], 70 + hs + bs, window=window)
+    check(run(c), c)
+
+
 def test_one_new_token_is_the_decode_step(gpu):
     """Paged attention's decode step (its own sum carries + 1e-6)."""
     c = build(32, 8, 128, 16, [99, 700, 1500], [1, 1, 1], 31)

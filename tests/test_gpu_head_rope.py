@@ -87,6 +87,19 @@ def test_against_64_bits(gpu, tokens, heads, kv, hs, dtype, norm, axes, rotated,
     check(build(tokens, heads, kv, hs, dtype, 10 + tokens + hs, norm, axes, rotated, mode, bs))
 
 
+@pytest.mark.parametrize("hs,rotated,mode", [(64, None, 2), (80, 78, 2), (128, 34, 2), (192, None, 0), (256, 250, 2)])
+def test_a_tokens_heads_do_not_depend_on_the_others(gpu, hs, rotated, mode):
+    """However many tokens come together, which lays heads and tokens out otherwise; a norm of one of the two."""
+    whole = build(37, 9, 3, hs, torch.float32, 21, axes=2, rotated=rotated, mode=mode)
+    whole["k_norm" if hs % 128 else "q_norm"] = None
+    want = check(whole)
+    for a, b in ((0, 1), (1, 3), (3, 8), (8, 20), (20, 37)):
+        c = {**whole, **{x: whole[x][a:b] for x in ("q", "k", "v", "slots")}, "positions": whole["positions"][:, a:b].contiguous()}
+        got = check(c)
+        for x, y in zip(got[:3], want[:3]):
+            assert torch.equal(x, y[a:b])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_bf16_out_without_a_cache(gpu, dtype):
     """For packed prompts in bf16; also q alone, and a norm of one of the two."""
