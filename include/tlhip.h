@@ -512,7 +512,7 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  * 2^30), starts by num_rows. Of a sequence with more than max_rows rows the first
  * max_rows are computed, as if it had no others, and the rest are left as they were.
  * No row of out may overlap a row of q (other columns of the same rows do not) or the
- * caches. `scratch` holds the partials of split contexts (tlh_chunk_attention_scratch_bytes,
+ * caches. `scratch` holds the partials of split contexts and the plan of many sequences (tlh_chunk_attention_scratch_bytes,
  * which never shrinks as a count grows, 16-byte aligned; it may be NULL when that is
  * 0). Its first TLH_CHUNK_COUNTER_BYTES must be zero before its first call, and every call
  * leaves them zero; calls that share one must be stream-ordered. */

@@ -18,8 +18,8 @@
 //
 // Items differ by orders of magnitude in keys, and only the device knows the lengths. So
 // every workgroup works out the same plan from them: how many tiles a workgroup takes
-// so that all run at once, and from that the partitions of every sequence's keys. The
-// last of an item's partitions to arrive joins them, in the order of their keys, whichever
+// so that all run at once, and from that the partitions of every sequence's keys (with
+// more than 64 sequences a launch before does it, and they look it up). The last of an item's partitions to arrive joins them, in the order of their keys, whichever
 // it is. (Joined in a second launch, whose code has to come from memory when the keys
 // have gone through the caches, 31 tokens + 600 took 20 us more.)
 //
@@ -46,6 +46,9 @@ constexpr int CA_NARROW = 64;      // rows of a (sequence, kv head) up to which 
 // of 256: over 992 34, 38, 41; over 2016 42, 43, 45; over 4000 57, 54, 53).
 constexpr int CA_MAX_PARTS = 32, CA_MIN_TILES = 2, CA_MIN_TILES_ROWS = 8, CA_MIN_TILES_MANY = 4;
 constexpr int CA_NO_WINDOW = 1 << 30;
+// Sequences up to which every workgroup works out the plan; of more, one does in a launch
+// before, and the others look it up.
+constexpr int CA_PLAN_HERE = 64;
 
 // n / d for 0 <= n < 2^31 by a product. What every workgroup runs before its first load is
 // kept short: its code comes from memory where another kernel's was last.
@@ -67,6 +70,7 @@ struct CaArgs : PagedArgs {
     const int32_t *lens, *starts;
     float *part;     // units of 4 rows of ca_row(D) floats
     unsigned *counters;  // of an item's partitions that have arrived; 0 before and after a call
+    int4 *plan;          // of more than CA_PLAN_HERE sequences, else null
     int S, rows, max_rows, max_ctx, window;
     int lg_wgs;          // workgroups that fill the machine, a power of two
     int span_few, span_many;  // keys that some row of a block of 32 and of 128 rows sees
@@ -124,94 +128,176 @@ __device__ __forceinline__ int ca_parts(const CaWork &w, int each) {
     return max(1, q + (r > 0) + (r > n) - (r <= -n));
 }
 
-// What a workgroup does. Every lane calls; a lane looks at one sequence of 64 at a time.
+// What a workgroup does. Every lane calls; a lane looks at one sequence.
 struct CaPlan {
     int s, local, parts, items, wide, units;  // s < 0: nothing
     int unit, counter;  // the first ones of the sequence's
     CaSeq q;
 };
-__device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) {
-    const CaWork first = ca_work(a, lane);
-    auto work = [&](int g) { return g == 0 ? first : ca_work(a, g + lane); };
-    const int KV = (int)a.kv.by, wgs = 1 << a.lg_wgs;
-    // tiles, of the sequences with few rows and of the others
-    uint64_t few = 0, many = 0;
+// how many tiles one of 2^lg workgroups takes of all
+__device__ __forceinline__ int ca_share(uint64_t tiles, int lg) {
+    return (int)min(max((tiles + (1u << lg) - 1) >> lg, (uint64_t)CA_MIN_TILES), (uint64_t)1 << 26);
+}
+// Few rows: no workgroup takes more than 1.5 even shares. (us with 0.5, 1, 1.5, 2: 32
+// tokens over 512..8192 120, 123, 113, 117; 8 over 8000 57, 50, 47, 45; 24 over 100..30000
+// 282, 283, 267, 290; 1 over 100000 85, 85, 90, 79.)
+__device__ __forceinline__ int ca_few_share(int even) { return (even * 3 + 1) >> 1; }
+// Many rows: partitions are whole, so with an even share some workgroups are left over,
+// to run alone after the others: the first of a few larger shares, up to twice the even
+// one, that leaves none. With more items than workgroups none does, and the last one
+// splits only what is much longer than the others. In eighths of the even share: 8, 9, 10, 12, 16.
+__device__ __forceinline__ int ca_next_share(int eighths) { return eighths + (eighths < 10 ? 1 : eighths == 10 ? 2 : 4); }
+__device__ __forceinline__ int ca_many_share(int even, int eighths) { return (even * eighths + 7) >> 3; }
+// a sequence's workgroups, for that choice
+__device__ __forceinline__ int ca_count(const CaArgs &a, const CaWork &w, int each) {
+    return min((w.wide ? (int)min((int64_t)w.items * (int)a.kv.by, (int64_t)1 << 18) : 0) * ca_parts(w, each), 1 << 18);
+}
+
+// The plan of many sequences, by one workgroup: of each its first workgroup, unit and counter
+// and its partitions, and behind them, as if of one more, the number of workgroups. (Worked
+// out by every workgroup, the time grows with the square of the sequences: a token each over
+// 100, us: 256 sequences 47.5, so 43; 1024 336, 155; 4096 3658, 579.)
+constexpr int CA_PLANNERS = 1024;
+// the sum over the workgroup; called by all
+template <typename T> __device__ __forceinline__ T ca_block_sum(T v, T *s_wave) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < CA_PLANNERS / 64; ++w) v += s_wave[w];
+    return v;
+}
+__global__ void __launch_bounds__(CA_PLANNERS) k_chunk_plan(const CaArgs a) {
+    __shared__ uint64_t s_long[CA_PLANNERS / 64];
+    __shared__ int s_upto[3][CA_PLANNERS / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, KV = (int)a.kv.by, wgs = 1 << a.lg_wgs;
+    uint64_t few = 0, many = 0, bad = 0;
+    for (int s = threadIdx.x; s < a.S; s += CA_PLANNERS) {
+        const CaWork w = ca_work(a, s);
+        bad += w.q.n < 0;
+        (w.wide ? many : few) += (uint64_t)w.items * (uint32_t)w.tiles;
+    }
+    bad = ca_block_sum(bad, s_long), few = ca_block_sum(few, s_long), many = ca_block_sum(many, s_long);
+    if (bad != 0) {  // (as in ca_plan)
+        if (threadIdx.x == 0) a.plan[a.S] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    const int even = ca_share((few + many) * KV, a.lg_wgs), each_few = ca_few_share(even);
+    int each_many = even;
+    if (many > 0) {
+        for (int eighths = 8;; eighths = ca_next_share(eighths)) {
+            each_many = ca_many_share(even, eighths);
+            uint64_t count = 0;
+            for (int s = threadIdx.x; s < a.S; s += CA_PLANNERS) count += ca_count(a, ca_work(a, s), each_many);
+            if (ca_block_sum(count, s_long) <= (uint64_t)wgs || eighths == 16) break;
+        }
+    }
+    int at[3] = {0, 0, 0};  // workgroups, units, counters before the next 1024 sequences
+    for (int s0 = 0; s0 < a.S; s0 += CA_PLANNERS) {
+        const int s = s0 + (int)threadIdx.x;
+        const CaWork w = ca_work(a, s);
+        const int parts = ca_parts(w, w.wide ? each_many : each_few), n = w.items * KV;
+        const int mine[3] = {n * parts, parts > 1 ? n * parts * w.units : 0, parts > 1 ? n : 0};
+        int upto[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) upto[i] = ca_scan(mine[i]);
+        __syncthreads();
+        if (lane == 63) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) s_upto[i][wave] = upto[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            upto[i] += at[i] - mine[i];
+            for (int v = 0; v < CA_PLANNERS / 64; ++v) {
+                if (v < wave) upto[i] += s_upto[i][v];
+                at[i] += s_upto[i][v];
+            }
+        }
+        if (s < a.S) a.plan[s] = make_int4(upto[0], upto[1], upto[2], parts);
+    }
+    if (threadIdx.x == 0) a.plan[a.S] = make_int4(at[0], 0, 0, 0);
+}
+__device__ __forceinline__ CaPlan ca_planned(const CaArgs &a, int block, int lane) {
     CaPlan p = {};
     p.s = -1;
-    for (int g = 0; g < a.S; g += 64) {
-        const CaWork w = work(g);
-        // Starts that decrease make sequences overlap, and more work than there is room for:
-        // then nothing is computed.
-        if (__builtin_amdgcn_ballot_w64(w.q.n < 0) != 0) return p;
-        const uint64_t n = (uint64_t)w.items * (uint32_t)w.tiles;  // in two parts: 64 of either fit 32 bits
-        const int lo = (int)(n & 0xffffff), hi = (int)(n >> 24);
-        few += (uint64_t)(uint32_t)ca_sum(w.wide ? 0 : lo) + ((uint64_t)(uint32_t)ca_sum(w.wide ? 0 : hi) << 24);
-        many += (uint64_t)(uint32_t)ca_sum(w.wide ? lo : 0) + ((uint64_t)(uint32_t)ca_sum(w.wide ? hi : 0) << 24);
+    if (block >= __builtin_amdgcn_readfirstlane(a.plan[a.S].x)) return p;
+    int lo = 0, len = a.S;  // the last sequence that begins at `block` or before it
+    while (len > 1) {
+        const int stride = (len + 63) >> 6, s = lo + lane * stride;
+        const bool in = s < lo + len && a.plan[min(s, a.S)].x <= block;
+        const int n = max(1, (int)__popcll(__builtin_amdgcn_ballot_w64(in)));
+        const int next = lo + (n - 1) * stride;
+        len = min(stride, lo + len - next);
+        lo = next;
     }
+    p.s = __builtin_amdgcn_readfirstlane(lo);
+    const int4 x = a.plan[p.s];
+    const CaWork w = ca_work(a, p.s);
+    p.local = block - __builtin_amdgcn_readfirstlane(x.x);
+    p.unit = __builtin_amdgcn_readfirstlane(x.y), p.counter = __builtin_amdgcn_readfirstlane(x.z);
+    p.parts = __builtin_amdgcn_readfirstlane(x.w);
+    p.items = __builtin_amdgcn_readfirstlane(w.items), p.wide = __builtin_amdgcn_readfirstlane(w.wide);
+    p.units = __builtin_amdgcn_readfirstlane(w.units);
+    p.q.b = __builtin_amdgcn_readfirstlane(w.q.b), p.q.n = __builtin_amdgcn_readfirstlane(w.q.n);
+    p.q.L = __builtin_amdgcn_readfirstlane(w.q.L);
+    return p;
+}
+
+__device__ __forceinline__ CaPlan ca_plan(const CaArgs &a, int block, int lane) {
+    if (a.plan) return ca_planned(a, block, lane);
+    const CaWork w = ca_work(a, lane);
+    const int KV = (int)a.kv.by, wgs = 1 << a.lg_wgs;
+    CaPlan p = {};
+    p.s = -1;
+    // Starts that decrease make sequences overlap, and more work than there is room for:
+    // then nothing is computed.
+    if (__builtin_amdgcn_ballot_w64(w.q.n < 0) != 0) return p;
+    // tiles, of the sequences with few rows and of the others, summed in two parts: 64 of either fit 32 bits
+    const uint64_t mine_all = (uint64_t)w.items * (uint32_t)w.tiles;
+    const int lo = (int)(mine_all & 0xffffff), hi = (int)(mine_all >> 24);
+    const uint64_t few = (uint64_t)(uint32_t)ca_sum(w.wide ? 0 : lo) + ((uint64_t)(uint32_t)ca_sum(w.wide ? 0 : hi) << 24);
+    const uint64_t many = (uint64_t)(uint32_t)ca_sum(w.wide ? lo : 0) + ((uint64_t)(uint32_t)ca_sum(w.wide ? hi : 0) << 24);
     const uint64_t total = (few + many) * KV;
-    auto share = [&](uint64_t tiles, int lg) {  // of one of 2^lg workgroups
-        return (int)min(max((tiles + (1u << lg) - 1) >> lg, (uint64_t)CA_MIN_TILES), (uint64_t)1 << 26);
-    };
-    const int even = share(total, a.lg_wgs);
-    // Few rows: no workgroup takes more than 1.5 even shares. (us with 0.5, 1, 1.5, 2: 32
-    // tokens over 512..8192 120, 123, 113, 117; 8 over 8000 57, 50, 47, 45; 24 over 100..30000
-    // 282, 283, 267, 290; 1 over 100000 85, 85, 90, 79.)
-    const int each_few = (even * 3 + 1) >> 1;
-    // Many rows: partitions are whole, so with an even share some workgroups are left over,
-    // to run alone after the others: the first of a few larger shares, up to twice the even
-    // one, that leaves none. With more items than workgroups none does, and the last one
-    // splits only what is much longer than the others.
+    const int even = ca_share(total, a.lg_wgs), each_few = ca_few_share(even);
     int each_many = even, count = 0;
     if (many > 0)
 #pragma unroll 1
-        for (int eighths = 8;; eighths += eighths < 10 ? 1 : eighths == 10 ? 2 : 4) {
-            each_many = (even * eighths + 7) >> 3;
-            count = 0;
-            for (int g = 0; g < a.S; g += 64) {
-                const CaWork w = work(g);
-                const int n = w.wide ? (int)min((int64_t)w.items * KV, (int64_t)1 << 18) : 0;
-                count = min(count + ca_sum(min(n * ca_parts(w, each_many), 1 << 18)), 1 << 24);
-            }
+        for (int eighths = 8;; eighths = ca_next_share(eighths)) {
+            each_many = ca_many_share(even, eighths);
+            count = ca_sum(ca_count(a, w, each_many));
             if (count <= wgs || eighths == 16) break;
         }
     // all run at once: their order does not matter
     const bool all = few == 0 ? count <= wgs : total <= (uint64_t)(wgs * CA_MIN_TILES);
 
-    int at = 0, unit = 0, counter = 0;
-    for (int g = 0; g < a.S; g += 64) {
-        const CaWork w = work(g);
-        const int parts = ca_parts(w, w.wide ? each_many : each_few), n = w.items * KV;
-        const int mine = n * parts, units = parts > 1 ? mine * w.units : 0, counters = parts > 1 ? n : 0;
-        const int upto = ca_scan(mine), units_upto = ca_scan(units), counters_upto = ca_scan(counters);
-        int off = at + upto - mine;
-        if (!all && a.S <= 64) {  // longest workgroups first: one that starts last would end alone
-            const int key = (int)((float)w.tiles / (float)parts) << w.wide;
-            off = 0;
-            for (int j = 0; j < a.S; ++j) {
-                const int kj = __builtin_amdgcn_readlane(key, j), mj = __builtin_amdgcn_readlane(mine, j);
-                if (kj > key || (kj == key && j < lane)) off += mj;
-            }
+    const int parts = ca_parts(w, w.wide ? each_many : each_few), n = w.items * KV;
+    const int mine = n * parts, units = parts > 1 ? mine * w.units : 0, counters = parts > 1 ? n : 0;
+    const int units_upto = ca_scan(units), counters_upto = ca_scan(counters);
+    int off = ca_scan(mine) - mine;
+    if (!all) {  // longest workgroups first: one that starts last would end alone
+        const int key = (int)((float)w.tiles / (float)parts) << w.wide;
+        off = 0;
+        for (int j = 0; j < a.S; ++j) {
+            const int kj = __builtin_amdgcn_readlane(key, j), mj = __builtin_amdgcn_readlane(mine, j);
+            if (kj > key || (kj == key && j < lane)) off += mj;
         }
-        const uint64_t who = __builtin_amdgcn_ballot_w64(block >= off && block - off < mine);
-        if (who != 0) {
-            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
-            p.s = g + l;
-            p.local = block - __builtin_amdgcn_readlane(off, l);
-            p.parts = __builtin_amdgcn_readlane(parts, l);
-            p.items = __builtin_amdgcn_readlane(w.items, l);
-            p.wide = __builtin_amdgcn_readlane(w.wide, l);
-            p.units = __builtin_amdgcn_readlane(w.units, l);
-            p.unit = unit + __builtin_amdgcn_readlane(units_upto - units, l);
-            p.counter = counter + __builtin_amdgcn_readlane(counters_upto - counters, l);
-            p.q.b = __builtin_amdgcn_readlane(w.q.b, l);
-            p.q.n = __builtin_amdgcn_readlane(w.q.n, l);
-            p.q.L = __builtin_amdgcn_readlane(w.q.L, l);
-            break;
-        }
-        at += __builtin_amdgcn_readlane(upto, 63);
-        unit += __builtin_amdgcn_readlane(units_upto, 63);
-        counter += __builtin_amdgcn_readlane(counters_upto, 63);
     }
+    const uint64_t who = __builtin_amdgcn_ballot_w64(block >= off && block - off < mine);
+    if (who == 0) return p;
+    const int l = p.s = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
+    p.local = block - __builtin_amdgcn_readlane(off, l);
+    p.parts = __builtin_amdgcn_readlane(parts, l);
+    p.items = __builtin_amdgcn_readlane(w.items, l);
+    p.wide = __builtin_amdgcn_readlane(w.wide, l);
+    p.units = __builtin_amdgcn_readlane(w.units, l);
+    p.unit = __builtin_amdgcn_readlane(units_upto - units, l);
+    p.counter = __builtin_amdgcn_readlane(counters_upto - counters, l);
+    p.q.b = __builtin_amdgcn_readlane(w.q.b, l);
+    p.q.n = __builtin_amdgcn_readlane(w.q.n, l);
+    p.q.L = __builtin_amdgcn_readlane(w.q.L, l);
     return p;
 }
 
@@ -741,11 +827,15 @@ static CaBounds ca_bounds(const tlh_chunk_attention_args &a) {
 }
 
 // The counters, always in the same place and as many as any call may need (a split item has
-// two partitions at least), then the partials.
+// two partitions at least), then the plan of many sequences and the partials.
 static_assert(TLH_CHUNK_COUNTER_BYTES >= 4 * (512 + 512 / 2), "split items");
+static size_t ca_plan_bytes(const tlh_chunk_attention_args &a) {
+    return a.num_seqs > CA_PLAN_HERE ? sizeof(int4) * ((size_t)a.num_seqs + 1) : 0;
+}
 size_t chunk_attention_scratch_bytes(const tlh_chunk_attention_args &a) {
     const CaBounds b = ca_bounds(a);
-    return b.parts == 1 ? 0 : (size_t)(TLH_CHUNK_COUNTER_BYTES + b.units * 4 * ca_row(a.head_size) * (int64_t)sizeof(float));
+    const size_t plan = ca_plan_bytes(a);
+    return b.parts == 1 && plan == 0 ? 0 : TLH_CHUNK_COUNTER_BYTES + plan + (size_t)b.units * 4 * ca_row(a.head_size) * sizeof(float);
 }
 
 template <int D> static void launch_ca(const CaArgs &c, int bs, const CaBounds &b, hipStream_t stream) {
@@ -764,7 +854,8 @@ tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scrat
     c.kc = (const uint16_t *)a.k_cache, c.vc = (const uint16_t *)a.v_cache;
     c.tables = a.block_tables, c.lens = a.context_lens, c.starts = a.row_starts;
     c.counters = (unsigned *)scratch;
-    c.part = (float *)((uint8_t *)scratch + TLH_CHUNK_COUNTER_BYTES);
+    c.part = (float *)((uint8_t *)scratch + TLH_CHUNK_COUNTER_BYTES + ca_plan_bytes(a));
+    c.plan = a.num_seqs > CA_PLAN_HERE ? (int4 *)((uint8_t *)scratch + TLH_CHUNK_COUNTER_BYTES) : nullptr;
     c.num_blocks = a.num_blocks;
     c.S = a.num_seqs, c.KV = a.num_kv_heads, c.kv = ca_div(a.num_kv_heads), c.G = ca_div(a.num_heads / a.num_kv_heads);
     c.rows = a.num_rows, c.max_rows = a.max_rows, c.max_blocks = a.max_blocks_per_seq, c.max_ctx = a.max_context_len;
@@ -773,6 +864,7 @@ tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scrat
     set_scale(c, a.scale);
     if (b.blocks >= 1 << 24)  // x 256 threads
         return set_error(TLH_INVALID, "chunk_attention: too many rows and heads for one launch");
+    if (c.plan) hipLaunchKernelGGL(k_chunk_plan, dim3(1), dim3(CA_PLANNERS), 0, stream, c);
     switch (a.head_size) {
     case 64: launch_ca<64>(c, a.block_size, b, stream); break;
     case 80: launch_ca<80>(c, a.block_size, b, stream); break;

@@ -299,6 +299,37 @@ def test_many_sequences(gpu, seqs):
     check(run(c), c)
 
 
+def test_more_sequences_than_a_plan_looks_at_once(gpu):
+    """Over a thousand, some without rows or tokens, pieces and contexts that are split among them; and one node for
+    these and for fewer."""
+    r = np.random.default_rng(80)
+    cached = [int(x) for x in r.choice([0, 3, 50, 100], 1100)]
+    new = [int(x) for x in r.choice([0, 0, 1, 2], 1100)]
+    for s, (c, n) in {0: (900, 1), 63: (4000, 1), 64: (700, 60), 1023: (0, 0), 1024: (3000, 1), 1099: (600, 33)}.items():
+        cached[s], new[s] = c, n
+    c = build(4, 2, 64, 16, cached, new, 81)
+    node, dev = node_of(c), on_gpu(c)
+    for S in (1100, 1025, 65, 64, 1100):
+        rows = c["starts"][S]
+        out = torch.full((rows, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+        node(out, dev[0][:rows], dev[1], dev[2], dev[3][:S], dev[4][:S], dev[5][:S + 1])
+        check(out, {**c, "q": c["q"][:rows], "table": c["table"][:S], "lens": c["lens"][:S], "starts": c["starts"][:S + 1]})
+        assert (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
+
+
+@pytest.mark.parametrize("at", [0, 64, 65, 128])
+def test_starts_that_decrease_among_many_compute_nothing(gpu, at):
+    c = build(4, 2, 64, 16, [600] * 130, [2] * 130, 82)
+    node, dev = node_of(c), list(on_gpu(c))
+    out, right = torch.full(c["q"].shape, 7.0, dtype=torch.float16, device="cuda"), dev[5].clone()
+    dev[5][at] = 259
+    node(out, *dev)
+    torch.cuda.synchronize()
+    assert (out == 7).all() and (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
+    dev[5] = right
+    check(node(out, *dev), c)
+
+
 def test_nothing_to_do(gpu):
     c = build(8, 2, 128, 16, [40, 7], [4, 0], 50)
     c["starts"] = [0, 0, 0]
