@@ -1038,9 +1038,9 @@ class HeadRope:
         a.q, a.q_stride = _token_rows(q, H, D, "q", dev)
         a.k, a.k_stride = _token_rows(k, KV, D, "k", dev)
         a.v, a.v_stride = _token_rows(v, KV, D, "v", dev)
-        a.q_out, a.q_out_stride = _token_rows(q_out, H, D, "q_out", dev)
         if q_out.shape != q.shape:
             raise ValueError(f"q_out: {tuple(q_out.shape)}, not {tuple(q.shape)}")
+        a.q_out, a.q_out_stride = _token_rows(q_out, H, D, "q_out", dev)
         a.k_out_stride = a.v_out_stride = KV * D
         if k_out is not None:
             a.k_out, a.k_out_stride = self._out(k_out, k, q_out, "k_out")

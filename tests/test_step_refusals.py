@@ -281,7 +281,7 @@ def test_head_rope_names_the_tensor():
     with pytest.raises(ValueError, match="on the GPU"):
         node(**good)
     for name, bad in (("q", f16(3, 7, 64)), ("k", f16(2, 2, 64)), ("v", f16(3, 2, 64).float()), ("positions", i32(3)),
-                      ("positions", i32(1, 3)), ("q_out", f16(3, 8, 32)), ("q_norm", torch.zeros(32)),
+                      ("positions", i32(1, 3)), ("q_out", f16(3, 8, 32)), ("q_out", f16(3, 16)[:, ::2]), ("q_norm", torch.zeros(32)),
                       ("k_norm", f16(64)), ("k_out", f16(3, 2, 64).bfloat16()), ("v_out", f16(4, 2, 64)),
                       ("k_cache", f16(5, 2, 8, 8, 8)), ("v_cache", f16(4, 2, 64, 16)), ("slots", i32(3)), ("slots", None),
                       ("k_cache", None), ("q", f16(8, 3, 64).transpose(0, 1))):
