@@ -13,6 +13,7 @@
 //    its fraction there and only then taken to f32;
 //  * a value page holds a dim's tokens next to each other: the values pass through LDS, and
 //    consecutive lanes write consecutive tokens.
+// Norms and rotation are f32, and a head is rounded once, to the type it is written in.
 // Measured against a wave for a (token, head), which forms its angles for each and writes
 // values two bytes a page line: 2501 tokens of 28 + 4 + 4 heads of 128 in bf16 37 -> 12.6 us
 // (3.7 TB/s); 8192 tokens of 32 + 8 + 8 of 128 in f32 230 -> 79.5 us (3.8 TB/s, where a
@@ -24,7 +25,11 @@
 
 namespace tlh {
 
-constexpr int HR_WGS = 1024;  // workgroups that the heads are split for
+// Workgroups that the heads are split for: more of them form the same angles more often,
+// fewer leave CUs empty (from memory, us, with 512, 1024, 2048, 4096: 512 tokens of 32 + 8 +
+// 8 heads of 128 in f32 10.9, 9.9, 9.8, 9.8; 2501 31.7, 25.6, 28.5, 27.5; 8192 107, 73, 74, 68;
+// 2501 of 28 + 4 + 4 in bf16 23.8, 19.4, 18.1, 21.6).
+constexpr int HR_WGS = 1024;
 
 struct HrArgs {
     const uint8_t *q, *k, *v;
