@@ -16,6 +16,12 @@
 //    above 128 dims) in LDS, double-buffered and loaded straight from the pages.
 // Both compute S^T = K . Q^T and O^T += V^T . P^T, so a lane holds one row's scores.
 //
+// P meets V in f16, as the matrix cores take it. With few rows a second product adds what that
+// rounding took off (22 bits in all): the tiles wait for HBM, so 32 sequences decoding take 117
+// us with it and without, and a result is off by 2.07e-4 of its size, all of it its own rounding,
+// instead of 2.9e-4. With many rows the products are the bound (2048 over 16384, us, without and
+// with it: heads of 64 385, 536; 128 633, 831; 256 517, 587), so there P stays rounded to f16.
+//
 // Items differ by orders of magnitude in keys, and only the device knows the lengths. So
 // every workgroup works out the same plan from them: how many tiles a workgroup takes
 // so that all run at once, and from that the partitions of every sequence's keys (with
@@ -452,8 +458,8 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
                 load_v(pg);
             }
             const PagedSeen sees[1] = {w.seen(base, pg.good)}, &see = sees[0];
-            uint4 pf[2];
-            w.softmax(S, sees, pf);
+            uint4 pf[2], rest[2];
+            w.template softmax<true>(S, sees, pf, rest);
             if (see.there != ~0u) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -463,20 +469,24 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
             if (careful() && !see.whole) {
                 // through the wave's part of the merge buffer, which is free until the end
                 uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 128;
-                static_assert(256 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
-                sp[lane] = pf[0], sp[64 + lane] = pf[1];
+                static_assert(192 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
 #pragma unroll
-                for (int d = 0; d < NB; ++d) {
-                    __builtin_amdgcn_wave_barrier();
-                    sv[lane] = vf[d][0], sv[64 + lane] = vf[d][1];
-                    __builtin_amdgcn_wave_barrier();
-                    w.careful_pv(d, see, (const uint32_t *)sp, (const uint32_t *)sv, 256);
-                }
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        __builtin_amdgcn_wave_barrier();
+                        sp[lane] = pf[i], sp[64 + lane] = rest[i], sv[lane] = vf[d][i];
+                        __builtin_amdgcn_wave_barrier();
+                        w.careful_pv(d, see, i, (const uint32_t *)sp, (const uint32_t *)sv);
+                    }
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int d = 0; d < NB; ++d) w.O[d] = mfma32<false>(vf[d][i], pf[i], w.O[d]);
+                    for (int d = 0; d < NB; ++d) {
+                        w.O[d] = mfma32<false>(vf[d][i], pf[i], w.O[d]);
+                        w.O[d] = mfma32<false>(careful() ? W::finite_v(vf[d][i]) : vf[d][i], rest[i], w.O[d]);
+                    }
             }
             if (AHEAD) load_v(pn);
             pg = pn;
@@ -484,7 +494,7 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
         }
     };
     pass(std::false_type());
-    if (w.some_masked && __builtin_amdgcn_ballot_w64(w.bad()) != 0) pass(std::true_type());
+    if (__builtin_amdgcn_ballot_w64(w.bad()) != 0) pass(std::true_type());
 
     // merge the waves, MD dims at a time
     const float lt = sum_halves(w.l);

@@ -99,8 +99,9 @@ template <int D, int BS, class Rule> struct PagedWave {
     f32x16 O[NB];
     float m, l;  // the exponents' reference (an unscaled score), this half's sum
     // A value that is not finite would turn the zero weight of a key that a row does
-    // not see into NaN. So where a wave's sums come out not finite, it takes its tiles
-    // again, carefully: in those with masked keys it adds each seen key's product by itself.
+    // not see into NaN, and an infinite one the rest of a weight. So where a wave's sums come
+    // out not finite, it takes its tiles again, carefully: in those with masked keys it adds
+    // each seen key's product by itself, in the others rests meet finite values only.
     bool some_masked = false;
     __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -137,8 +138,10 @@ template <int D, int BS, class Rule> struct PagedWave {
         for (int i = 0; i < 16; ++i)
             if (!((mine >> (16 * (i / 8) + i % 8)) & 1)) S[i] = -INFINITY;
     }
-    // scores of U x 32 keys -> numerators (f16), the running maximum and sum
-    template <int U> __device__ __forceinline__ void softmax(f32x16 (&S)[U], const PagedSeen (&s)[U], uint4 (&pf)[2 * U]) {
+    // scores of U x 32 keys -> numerators (f16), with REST what that rounding took off them (f16
+    // as well: the two add up to 22 bits), the running maximum and sum
+    template <bool REST = false, int U>
+    __device__ __forceinline__ void softmax(f32x16 (&S)[U], const PagedSeen (&s)[U], uint4 (&pf)[2 * U], uint4 *rest = nullptr) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (!s[u].whole) hide(S[u], s[u].vis);
@@ -170,6 +173,12 @@ template <int D, int BS, class Rule> struct PagedWave {
                 for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(S[u][8 * i + e] * a.cs - mc);
                 l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                 pf[2 * u + i] = pack8<false>(p);
+                if (REST) {
+                    const f16x8 f = __builtin_bit_cast(f16x8, pf[2 * u + i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] -= (float)f[e];
+                    rest[2 * u + i] = pack8<false>(p);
+                }
             }
     }
     // places that hold no token's value may hold anything
@@ -178,18 +187,34 @@ template <int D, int BS, class Rule> struct PagedWave {
         auto keep = [&](int e) { return ((on >> e) & 1 ? 0xffffu : 0u) | ((on >> e) & 2 ? 0xffff0000u : 0u); };
         return make_uint4(v.x & keep(0), v.y & keep(2), v.z & keep(4), v.w & keep(6));
     }
+    // the values that are finite: an infinity times a weight's rest would be NaN
+    static __device__ __forceinline__ uint4 finite_v(uint4 v) {
+        auto keep = [](uint32_t w) {
+            return w & (((w & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u));
+        };
+        return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+    }
     // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
     // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
     __device__ __forceinline__ void careful_pv(int d, const PagedSeen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
 #pragma unroll 1
         for (int key = 0; key < 32; ++key) {
-            const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
-            if (!((s.vis >> key) & 1)) continue;
-            const float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                O[d][x] += p * h2f((uint16_t)(sv[sv_step * i + 4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
+            const int i = key >> 4, at = 4 * (32 * ((key >> 3) & 1) + c) + ((key & 7) >> 1), sh = 16 * (key & 1);
+            if ((s.vis >> key) & 1) careful_key(d, key, h2f((uint16_t)(sp[256 * i + at] >> sh)), sv + sv_step * i);
         }
+    }
+    // ... of the keys 16 i .. + 15, with sp's rests behind it
+    __device__ __forceinline__ void careful_pv(int d, const PagedSeen &s, int i, const uint32_t *sp, const uint32_t *sv) {
+#pragma unroll 1
+        for (int key = 16 * i; key < 16 * i + 16; ++key) {
+            const int at = 4 * (32 * ((key >> 3) & 1) + c) + ((key & 7) >> 1), sh = 16 * (key & 1);
+            if ((s.vis >> key) & 1) careful_key(d, key, h2f((uint16_t)(sp[at] >> sh)) + h2f((uint16_t)(sp[256 + at] >> sh)), sv);
+        }
+    }
+    __device__ __forceinline__ void careful_key(int d, int key, float p, const uint32_t *sv) {
+        const int from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) O[d][x] += p * h2f((uint16_t)(sv[4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
     }
 };
 

@@ -413,3 +413,46 @@ def test_starts_that_decrease_compute_nothing(gpu, starts):
     assert (out == 7).all() and (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
     dev[5] = right
     check(node(out, *dev), c)
+
+
+def close_bound(out, A, d, keys, vmax):
+    """Weights of few rows: rounded to f16, plus what that took off rounded to f16, which is off by half a step of half a
+    step, 2^-22 of the weight (below f16's normal range by 2^-25, 2^-32 of the largest, which is at least 2^7)."""
+    eps = torch.finfo(torch.float16).eps
+    return out.abs() * eps / 2 * 1.01 + A * 2.0 ** -22 * 1.01 + 2 * d * A + 2.0 ** -32 * keys * vmax + 2.0 ** -24
+
+
+@pytest.mark.parametrize("heads,hs,bs,new", [(8, 64, 16, 1), (8, 128, 8, 3), (4, 128, 32, 32), (4, 80, 16, 7), (4, 192, 32, 2),
+                                             (2, 256, 16, 64)])
+def test_weights_of_few_rows_keep_what_f16_rounds_off(gpu, heads, hs, bs, new):
+    """Sums that nearly cancel, where the weights' rounding to f16 (2^-11 of each) would be all there is to see."""
+    cached = [1, 2, 3, 5, 9, 40, 300, 1500]
+    c = build(heads, 2, hs, bs, cached, [new] * len(cached), 90 + hs)
+    c["kc"][:, :, 1:], c["scale"] = 0.0, 0.25  # scores of eight dims, whose sums are off by little
+    out = run(c).cpu().double()
+    for s, L in enumerate(c["lens"]):
+        at, pos = slice(c["starts"][s], c["starts"][s + 1]), np.arange(L)
+        page, off = torch.from_numpy(c["table"][s, pos // bs].astype(np.int64)), torch.from_numpy(pos % bs)
+        see = torch.arange(L)[None] <= L - new + torch.arange(new)[:, None]
+        for h in range(heads):
+            g = h // (heads // 2)
+            k, v = c["kc"][page, g, :, off].reshape(L, hs)[:, :8].double(), c["vc"][page, g, :, off].reshape(L, hs).double()
+            want, A, d = attend(c["q"][at, h, :8].double(), k, v, see, c["scale"])
+            err, tol = (out[at, h] - want).abs(), close_bound(want, A, d, L, float(v.abs().max()))
+            assert (err <= tol).all(), (s, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("hs,bs,new", [(128, 16, 1), (64, 8, 5), (256, 32, 20), (192, 16, 2)])
+def test_infinite_values_that_are_seen(gpu, hs, bs, new):
+    """An infinity that a row sees is its result in that dim, whatever its weight's rounding; both signs are NaN."""
+    c = build(4, 2, hs, bs, [400], [new], 95)
+    place = lambda p: (c["table"][0, p // bs], slice(None), p % bs)  # noqa: E731
+    for p, dims, x in ((40, slice(0, 8), float("inf")), (333, slice(8, 16), -float("inf")), (41, slice(16, 20), float("inf")),
+                       (42, slice(16, 20), -float("inf"))):
+        page, g, off = place(p)
+        c["vc"][page, g, dims, off] = x
+    out = run(c).cpu()
+    assert (out[..., :8] == float("inf")).all() and (out[..., 8:16] == -float("inf")).all() and torch.isnan(out[..., 16:20]).all()
+    finite = {**c, "vc": torch.where(torch.isfinite(c["vc"]), c["vc"], torch.zeros_like(c["vc"]))}
+    want, tol = chunk_reference(finite["q"], finite["kc"], finite["vc"], c["table"], c["lens"], c["starts"], c["scale"])
+    assert ((out[..., 20:].double() - want[..., 20:]).abs() <= tol[..., 20:]).all()
