@@ -631,7 +631,9 @@ tlh_status tlh_head_rope(const tlh_head_rope_args *a, void *stream);
  * Logits may be -inf (a mask). A row with a NaN, with +inf at a temperature above 0, or
  * with nothing but -inf is no distribution: a draft that needs it is refused (accept
  * probability NaN), and a token that would be drawn from it is -1. A token outside
- * [0, vocab) has p = q = 0. Of a sequence with more than max_drafts drafts the first max_drafts are
+ * [0, vocab) has p = q = 0. A sequence that ends before it starts has no drafts; one that
+ * shares drafts with another (starts that decrease) is not verified: accepted 0, tokens -1, accept
+ * probabilities NaN. Starts are bounded by num_drafts. Of a sequence with more than max_drafts drafts the first max_drafts are
  * looked at, as if it had no others. Row strides in elements, any alignment of the type;
  * vocab <= 1000000, max_drafts <= 1024. `scratch` (16-byte aligned) holds the rows'
  * sums; calls that share one must be stream-ordered. The outputs must not overlap the

@@ -104,8 +104,9 @@ __device__ __forceinline__ DvSeq dv_seq(const tlh_draft_verify_args &a, int s) {
     q.n = min(max(q.b, dv_start(a, s + 1)) - q.b, a.max_drafts);
     return q;
 }
-// the last sequence whose first row (of drafts: its first draft, else with one more row a
-// sequence) is `row` or before it; starts are looked at 64 at a time
+// The last sequence whose first row (of drafts: its first draft, else with one more row a
+// sequence) is `row` or before it; starts are looked at 64 at a time. Where they decrease it is
+// some sequence, and what follows from it is not used (dv_alone).
 __device__ __forceinline__ int dv_find(const tlh_draft_verify_args &a, int row, bool target, int lane) {
     int lo = 0, len = a.num_seqs;
     while (len > 1) {
@@ -150,11 +151,20 @@ template <int TY> struct DvLoad {
 __device__ __forceinline__ float dv_top(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 template <int TY>
-__global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args a, int r0, int P, int chunk, DvPart *__restrict__ parts) {
+__global__ void __launch_bounds__(256) k_draft_rows(const tlh_draft_verify_args a, int r0, int rows, int P, int chunk, int *__restrict__ odd,
+                                                    DvPart *__restrict__ parts) {
     using L = DvLoad<TY>;
     constexpr int C = L::C, AT_ONCE = 16 / C, STEP = 256 * C * AT_ONCE;  // vectors on their way at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = blockIdx.x;
     const int r = r0 + blockIdx.y, targets = a.num_drafts + a.num_seqs;
+    if (r == rows) {  // behind the rows: whether a start is below the one before it
+        if (p > 0) return;
+        int any = 0;
+        for (int s = threadIdx.x; s < a.num_seqs; s += 256) any |= dv_start(a, s + 1) < dv_start(a, s);
+        any = __syncthreads_or(any);
+        if (threadIdx.x == 0) *odd = any;
+        return;
+    }
     const bool target = r < targets;
     const int row = target ? r : r - targets;
     const int s = __builtin_amdgcn_readfirstlane(dv_find(a, row, target, lane));
@@ -257,6 +267,20 @@ __device__ __forceinline__ DvRow dv_row(const DvExp &weight, const DvPart *parts
     return r;
 }
 
+// Whether draft x is accepted, and the probability of that; tx and dx: its logits
+struct DvTest {
+    bool ok;
+    float prob;
+};
+__device__ __forceinline__ DvTest dv_test(const DvExp &weight, const DvRow &t, const DvRow &d, int x, bool known, bool drawn, float tx, float dx,
+                                          float u, bool greedy, double c_t) {
+    const bool bad = t.z != t.z || d.z != d.z;
+    const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? weight(tx, t.m, c_t) / t.z : 0.0;
+    const double qx = !known ? 0.0 : drawn ? weight(dx, d.m, c_t) / d.z : 1.0;
+    return {!bad && (greedy ? px == 1.0 : (double)u * qx < px),
+            bad ? NAN : qx > 0.0 ? (float)fmin(1.0, px / qx) : px > 0.0 ? 1.0f : 0.0f};
+}
+
 template <int TY>
 __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_args a, int P, int M, int chunk, int lanes,
                                                       const DvPart *__restrict__ parts, DvStop *__restrict__ stops,
@@ -285,13 +309,9 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
         const float dx = known && drawn ? dv_elem<TY>(a.draft, (int64_t)(q.b + i) * a.draft_stride + x) : -INFINITY;
         const DvRow t = dv_row(weight, tp + (int64_t)i * P, P, c, lanes, greedy, c_t);
         const DvRow d = drawn ? dv_row(weight, dp + (int64_t)i * P, P, c, lanes, false, c_t) : DvRow{1.0, 0.0f, 0};
-        const bool bad = t.z != t.z || d.z != d.z;
-        const double px = greedy ? (known && x == t.at ? 1.0 : 0.0) : known ? weight(tx, t.m, c_t) / t.z : 0.0;
-        const double qx = !known ? 0.0 : drawn ? weight(dx, d.m, c_t) / d.z : 1.0;
-        const bool ok = !bad && (greedy ? px == 1.0 : (double)u * qx < px);
-        if (c == 0 && !ok) atomicMin(&s_stop, i);
-        if (p == 0 && c == 0 && a.accept_probs)
-            a.accept_probs[q.b + i] = bad ? NAN : qx > 0.0 ? (float)fmin(1.0, px / qx) : px > 0.0 ? 1.0f : 0.0f;
+        const DvTest test = dv_test(weight, t, d, x, known, drawn, tx, dx, u, greedy, c_t);
+        if (c == 0 && !test.ok) atomicMin(&s_stop, i);
+        if (p == 0 && c == 0 && a.accept_probs) a.accept_probs[q.b + i] = test.prob;
     }
     __syncthreads();
     const int stop = s_stop;
@@ -339,12 +359,108 @@ __global__ void __launch_bounds__(256) k_draft_masses(const tlh_draft_verify_arg
 
 // One workgroup a sequence: the chunk, then the token in it, a thread a run of elements.
 constexpr int DV_DRAW = 1024;
+
+// Starts that decrease: rows and sequences no longer follow from each other, a row may be
+// several sequences', each at its own temperature. Then this workgroup does its sequence from
+// its logits alone, whatever the launches before have left: the slow way, for what no batch
+// that was laid out has. A sequence that shares drafts with another has no answer, so the
+// others' rows are no more than a batch has.
+template <typename T, typename F> __device__ __forceinline__ T dv_block(T v, T *s_wave, F f) {
+    v = wave_all(v, 64, f);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s_wave[0];
+    for (int w = 1; w < DV_DRAW / 64; ++w) v = f(v, s_wave[w]);
+    return v;
+}
 template <int TY>
-__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int M, int chunk, const DvStop *__restrict__ stops,
-                                                        const DvMass *__restrict__ masses) {
+__device__ __forceinline__ DvRow dv_whole(const DvExp &weight, const void *logits, int64_t base, int V, bool greedy, double c_t, void *s_wave) {
+    DvRow r = {0.0, -INFINITY, 0x7fffffff};
+    for (int e = threadIdx.x; e < V; e += DV_DRAW) {
+        const float x = dv_elem<TY>(logits, base + e);
+        if (x > r.m) r.at = e;
+        r.m = dv_top(r.m, x);
+    }
+    const float top = dv_block(r.m, (float *)s_wave, [](float u, float v) { return dv_top(u, v); });
+    r.at = dv_block(r.m == top ? r.at : 0x7fffffff, (int *)s_wave, [](int u, int v) { return min(u, v); });
+    r.m = top;
+    if (!(top > -INFINITY) || (top == INFINITY && !greedy)) r.z = NAN;
+    else if (!greedy) {
+        for (int e = threadIdx.x; e < V; e += DV_DRAW) r.z += weight(dv_elem<TY>(logits, base + e), top, c_t);
+        r.z = dv_block(r.z, (double *)s_wave, [](double u, double v) { return u + v; });
+    }
+    return r;
+}
+template <int TY>
+__device__ __forceinline__ DvStop dv_alone(const tlh_draft_verify_args &a, int s, int M, int chunk, DvMass *s_mass) {
+    constexpr int ES = TY == TLH_TYPE_F32 ? 4 : 2;
+    __shared__ double s_wave[DV_DRAW / 64];
+    const DvSeq q = dv_seq(a, s);
+    const float T = a.temperatures[s];
+    const bool greedy = !(T > 0.0f), drawn = a.draft && !greedy;
+    const double c_t = DV_LOG2E / (double)T;
+    const DvExp weight;
+    int shares = 0;
+    for (int o = threadIdx.x; o < a.num_seqs; o += DV_DRAW) {
+        const DvSeq x = dv_seq(a, o);
+        shares |= o != s && max(x.b, q.b) < min(x.b + x.n, q.b + q.n);
+    }
+    shares = __syncthreads_or(shares);
+    auto target = [&](int i) { return dv_whole<TY>(weight, a.target, ((int64_t)q.b + s + i) * a.target_stride, a.vocab, greedy, c_t, s_wave); };
+    int stop = shares ? 0 : q.n;
+    DvRow t = {NAN, 0.0f, 0}, d = {0.0, 0.0f, 0};
+    for (int i = 0; i < q.n; ++i) {
+        DvTest test = {false, NAN};
+        if (!shares) {
+            const int x = a.tokens[q.b + i];
+            const bool known = x >= 0 && x < a.vocab;
+            const int64_t row = (int64_t)(q.b + i) * a.draft_stride;
+            const DvRow ti = target(i), di = drawn ? dv_whole<TY>(weight, a.draft, row, a.vocab, false, c_t, s_wave) : DvRow{1.0, 0.0f, 0};
+            const float tx = known ? dv_elem<TY>(a.target, ((int64_t)q.b + s + i) * a.target_stride + x) : -INFINITY;
+            const float dx = known && drawn ? dv_elem<TY>(a.draft, row + x) : -INFINITY;
+            test = dv_test(weight, ti, di, x, known, drawn, tx, dx, a.accept_at[q.b + i], greedy, c_t);
+            if (!test.ok && stop == q.n) stop = i, t = ti, d = di;
+        }
+        if (threadIdx.x == 0 && a.accept_probs) a.accept_probs[q.b + i] = test.prob;
+    }
+    if (stop == q.n && !shares) t = target(q.n);
+    const bool bad = t.z != t.z || d.z != d.z, minus = stop < q.n && drawn;
+    int32_t *out = a.out_tokens + (int64_t)s * (a.max_drafts + 1);
+    for (int i = threadIdx.x; i <= a.max_drafts; i += DV_DRAW) out[i] = i < stop ? a.tokens[q.b + i] : i == stop && greedy && !bad ? t.at : -1;
+    if (threadIdx.x == 0) a.accepted[s] = stop;
+    const DvStop st = {t.z, d.z, t.m, d.m, stop, !greedy && !bad};
+    if (!st.draws) return st;
+    // the chunks' sums, as k_draft_masses has them
+    const int64_t row = ((int64_t)q.b + s + stop) * a.target_stride, drow = (int64_t)(q.b + stop) * a.draft_stride;
+    const int shift = (int)(((uintptr_t)((const char *)a.target + row * ES) & 15) / ES);
+    const int outright = stop < q.n && !a.draft ? a.tokens[q.b + stop] : -1;
+    const double ip = 1.0 / t.z, iq = minus ? 1.0 / d.z : 0.0;
+    for (int p = 0; p < M; ++p) {
+        DvMass m = {0.0, 0.0};
+        for (int e = max(p * chunk - shift, 0) + threadIdx.x; e < min((p + 1) * chunk - shift, a.vocab); e += DV_DRAW) {
+            const double w = weight(dv_elem<TY>(a.target, row + e), t.m, c_t);
+            const double above = minus ? dv_above(w, ip, weight(dv_elem<TY>(a.draft, drow + e), d.m, c_t), iq) : w * ip;
+            m.whole += w * ip;
+            m.sum += e == outright ? 0.0 : above;
+        }
+        auto add = [](double u, double v) { return u + v; };
+        m.sum = dv_block(m.sum, s_wave, add), m.whole = dv_block(m.whole, s_wave, add);
+        if (threadIdx.x == 0) s_mass[p] = m;
+    }
+    __syncthreads();
+    return st;
+}
+
+template <int TY>
+__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int M, int chunk, const int *__restrict__ odd,
+                                                        const DvStop *__restrict__ stops, const DvMass *__restrict__ masses) {
     constexpr int ES = TY == TLH_TYPE_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x;
-    const DvStop st = stops[s];
+    __shared__ DvMass s_alone[DV_MAX_CHUNKS];
+    const bool alone = *odd != 0;
+    DvStop st = stops[s];
+    if (alone) st = dv_alone<TY>(a, s, M, chunk, s_alone);
     if (!st.draws) return;
     const DvSeq q = dv_seq(a, s);
     const double c_t = DV_LOG2E / (double)a.temperatures[s];
@@ -353,7 +469,7 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     int outright = st.stop < q.n && !a.draft ? a.tokens[q.b + st.stop] : -1;
     const DvExp weight;
     DvMass m = {};
-    if (lane < M) m = masses[(int64_t)s * M + lane];
+    if (lane < M) m = alone ? s_alone[lane] : masses[(int64_t)s * M + lane];
     if (dv_sum(m.sum) <= DV_NOTHING) {  // nothing above the drafter's: from p alone
         minus = false;
         outright = -1;
@@ -442,7 +558,9 @@ static int dv_mass_ept(int64_t seqs, int64_t vocab) {
 static int64_t dv_rows(const tlh_draft_verify_args &a) { return (int64_t)a.num_drafts + a.num_seqs + (a.draft ? a.num_drafts : 0); }
 
 // Room for any chunk length, so that the size grows with the rows and one buffer for
-// the largest batch serves every smaller one: the sequences' stops, masses, the rows' parts.
+// the largest batch serves every smaller one: whether starts decrease, the sequences' stops,
+// masses, the rows' parts.
+constexpr size_t DV_ODD_BYTES = 16;
 static size_t dv_most_chunks(int64_t rows, int64_t vocab) {
     return dv_small(vocab) ? (size_t)rows * dv_chunks(vocab, 16)
                            : (size_t)rows * dv_chunks(vocab, 64) + (size_t)std::min<int64_t>(rows, 256) * dv_chunks(vocab, 16);
@@ -451,7 +569,7 @@ size_t draft_verify_scratch_bytes(const tlh_draft_verify_args &a) {
     // of as many sequences as take short chunks, or of all in longer ones
     const int64_t longer = (int64_t)a.num_seqs * dv_chunks(a.vocab, dv_mass_ept(DV_SHORT_WGS + 1, a.vocab));
     const int64_t masses = std::max(longer, std::min<int64_t>((int64_t)a.num_seqs * dv_chunks(a.vocab, 8), DV_SHORT_WGS));
-    return sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * (size_t)masses +
+    return DV_ODD_BYTES + sizeof(DvStop) * (size_t)a.num_seqs + sizeof(DvMass) * (size_t)masses +
            sizeof(DvPart) * dv_most_chunks(dv_rows(a), a.vocab);
 }
 
@@ -461,14 +579,15 @@ template <int TY> static void launch_dv(const tlh_draft_verify_args &a, void *sc
     const int mass_ept = dv_mass_ept(a.num_seqs, a.vocab), M = dv_chunks(a.vocab, mass_ept), mass_chunk = 256 * mass_ept;
     int lanes = 1;
     while (lanes < P) lanes <<= 1;
-    DvStop *stops = (DvStop *)scratch;
+    int *odd = (int *)scratch;
+    DvStop *stops = (DvStop *)((uint8_t *)scratch + DV_ODD_BYTES);
     DvMass *masses = (DvMass *)(stops + a.num_seqs);
     DvPart *parts = (DvPart *)(masses + (size_t)a.num_seqs * M);
-    for (int64_t r0 = 0; r0 < rows; r0 += 65535)  // grid y
-        hipLaunchKernelGGL((k_draft_rows<TY>), dim3(P, (unsigned)std::min<int64_t>(rows - r0, 65535)), dim3(256), 0, stream, a, (int)r0,
-                           P, chunk, parts);
+    for (int64_t r0 = 0; r0 <= rows; r0 += 65535)  // grid y
+        hipLaunchKernelGGL((k_draft_rows<TY>), dim3(P, (unsigned)std::min<int64_t>(rows + 1 - r0, 65535)), dim3(256), 0, stream, a, (int)r0,
+                           (int)rows, P, chunk, odd, parts);
     hipLaunchKernelGGL((k_draft_masses<TY>), dim3(M, a.num_seqs), dim3(256), 0, stream, a, P, M, mass_chunk, lanes, parts, stops, masses);
-    hipLaunchKernelGGL((k_draft_draw<TY>), dim3(a.num_seqs), dim3(DV_DRAW), 0, stream, a, M, mass_chunk, stops, masses);
+    hipLaunchKernelGGL((k_draft_draw<TY>), dim3(a.num_seqs), dim3(DV_DRAW), 0, stream, a, M, mass_chunk, odd, stops, masses);
 }
 
 tlh_status launch_draft_verify(const tlh_draft_verify_args &a, void *scratch, hipStream_t stream) {

@@ -305,3 +305,63 @@ def test_one_call_form(gpu):
         got = N.draft_verify(*on_gpu(c), 8, stream=stream)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def each_alone(c, starts, most):
+    """Every sequence as one of its own, its drafts from its start up to its end (none if that is before it); one that
+    shares a draft with another is not verified."""
+    R, S = len(c["tokens"]), len(starts) - 1
+    lo = [max(0, min(x, R)) for x in starts]
+    span = [(lo[s], min(max(lo[s], lo[s + 1]), lo[s] + most)) for s in range(S)]
+    probs, accepted, out = np.full(R, 7.0), [], []
+    for s, (a, b) in enumerate(span):
+        if any(t != s and max(a, x) < min(b, y) for t, (x, y) in enumerate(span)):
+            probs[a:b] = np.nan
+            accepted.append(0), out.append([-1] * (most + 1))
+            continue
+        draft = None if c["draft"] is None else c["draft"][a:b]
+        one = verify_reference(c["target"][a + s:b + s + 1], draft, c["tokens"][a:b], [0, b - a], c["temps"][s:s + 1],
+                               c["accept_at"][a:b], c["sample_at"][s:s + 1], most)
+        accepted.append(one[0][0]), out.append(one[1][0].tolist())
+        probs[a:b] = one[2]
+    return accepted, out, probs
+
+
+def check_alone(c, starts, most, node):
+    node.scratch.fill_(0xff)
+    outs = outputs({**c, "most": most})
+    node(*on_gpu({**c, "starts": starts}), *outs)
+    torch.cuda.synchronize()
+    accepted, out, probs = each_alone(c, starts, most)
+    assert outs[0].tolist() == accepted
+    assert outs[1].tolist() == out
+    got, ok = outs[2].cpu().double().numpy(), ~np.isnan(probs)
+    assert (np.isnan(got) == ~ok).all()
+    assert (np.abs(got[ok] - probs[ok]) <= 2.0 ** -24 * probs[ok] + 1e-11 * probs[ok]).all()
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("starts", [[5, 2, 4], [4, 1, 3], [0, 5, 0], [5, 0, 5], [0, 3, 1, 2], [0, 3, 1, 4, 5], [3, 5, 0, 3, 3],
+                                    [0, 0, 5, 5, 0], [2, 9, -4, 1], [0, 2, 5]])
+def test_starts_that_decrease(gpu, starts, drafter):
+    """Sequences in any order, of either kind beside each other, over a scratch that holds another call's rows or none."""
+    S = len(starts) - 1
+    for most in (5, 2):
+        for seed, temps in enumerate(([0.0, 0.7, 0.0, 0.9], [0.7, 0.0, 1.1, 0.0], [0.4, 1.3, 0.8, 0.6])):
+            c = build([3, 2] + [0] * (S - 2), 9001, torch.float32, 50 + seed, drafter, temps=temps[:S])
+            node = N.DraftVerify(S, 5, most, 9001, drafter=drafter)
+            check_alone(c, starts, most, node)
+            if starts == sorted(starts):
+                assert not np.isnan(each_alone(c, starts, most)[2]).any()
+
+
+@pytest.mark.parametrize("at,to", [(0, 5), (70, 0), (699, 2), (1399, 1000), (1400, 3)])
+def test_one_start_that_decreases_among_many(gpu, at, to):
+    r = np.random.default_rng(60)
+    c = build([int(x) for x in r.integers(0, 3, 1400)], 300, torch.float32, 61, temps=r.choice([0.0, 0.8, 1.2], 1400))
+    node = N.DraftVerify(1400, len(c["tokens"]), 2, 300)
+    starts = list(c["starts"])
+    starts[at] = to
+    check_alone(c, starts, 2, node)
+    c["most"] = 2
+    check(c, node)  # and the next call is as ever
