@@ -482,7 +482,11 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     }
     const double total = __shfl(run, 63, 64);
     const double reach = (double)a.sample_at[s] * total;
-    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < M && run > reach), any = __builtin_amdgcn_ballot_w64(m.sum > 0.0);
+    // Sums in another order may pass `reach` a rounding earlier, at a place without a weight:
+    // it is no answer (but below 0 the first place is, whatever it weighs).
+    const bool first_place = reach < 0.0;
+    const uint64_t any = __builtin_amdgcn_ballot_w64(m.sum > 0.0);
+    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < M && run > reach && (m.sum > 0.0 || first_place));
     const int p = over != 0 ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((unsigned long long)any);  // else the last with a weight
     double from = __shfl(run - m.sum, p, 64);
 
@@ -523,8 +527,9 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     from += upto - sum;
     if (from + sum > reach) {
         for (int e = e0; e < e1; ++e) {
-            from += mass(e);
-            if (from > reach) {
+            const double w = mass(e);
+            from += w;
+            if (from > reach && (w > 0.0 || first_place)) {
                 atomicMin(&s_next, e);
                 break;
             }

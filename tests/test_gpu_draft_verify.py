@@ -365,3 +365,23 @@ def test_one_start_that_decreases_among_many(gpu, at, to):
     check_alone(c, starts, 2, node)
     c["most"] = 2
     check(c, node)  # and the next call is as ever
+
+
+def test_a_token_without_a_weight_is_never_drawn(gpu):
+    """The random number falls between two tokens of different chunks, with masked ones between them: what was summed
+    before a chunk comes out of a difference, which may be above it by a rounding."""
+    S, V = 512, 3 * 4096
+    g = torch.Generator().manual_seed(62)
+    x = torch.full((S, V), -INF)
+    w = torch.randn((S, 4), generator=g)
+    x[:, 100:104] = w                                # the first chunk weighs half of all
+    x[:, 4096 + 2000] = w[:, 0]                      # the second begins with masked tokens
+    x[:, 2 * 4096 + 900:2 * 4096 + 903] = w[:, 1:]
+    f = lambda v: torch.full((S,), v, device="cuda")  # noqa: E731
+    none = torch.empty((0,), dtype=torch.int32, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        accepted, out, _ = N.draft_verify(x.to(dtype).cuda(), None, none, i32([0] * (S + 1)), f(0.7), f(0.5)[:0], f(0.5), 0)
+        assert (accepted == 0).all()
+        drawn = out[:, 0].cpu().long()
+        assert ((drawn >= 0) & (drawn < V)).all()
+        assert (x.gather(1, drawn[:, None]) > -INF).all()
