@@ -198,8 +198,12 @@ template <int TY, bool BF, int LANES, bool PART> __global__ void __launch_bounds
             for (int i = 0; i < 4; ++i) y[i] = x[i] * cs[i] - x[i + 4] * sn[i], y[i + 4] = x[i] * sn[i] + x[i + 4] * cs[i];
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i], y[2 * i + 1] = x[2 * i] * sn[i] + x[2 * i + 1] * cs[i];
+            for (int i = 0; i < 4; ++i) {
+                // (one that is not rotated passes through: 0 times an infinity beside it would be NaN)
+                const bool turns = (i < 2 ? da : db - 4) / 2 + i < a.pairs;
+                y[2 * i] = turns ? x[2 * i] * cs[i] - x[2 * i + 1] * sn[i] : x[2 * i];
+                y[2 * i + 1] = turns ? x[2 * i] * sn[i] + x[2 * i + 1] * cs[i] : x[2 * i + 1];
+            }
         }
         if (!live || h >= h1) continue;
         const uint2 lo = hr_pack4<BF>(y), hi = hr_pack4<BF>(y + 4);

@@ -275,3 +275,26 @@ def test_streams_and_graphs(gpu):
         torch.cuda.synchronize()
         want = check(c)
         assert torch.equal(out, want[0]) and torch.equal(kc, want[3]) and torch.equal(vc, want[4])
+
+
+@pytest.mark.parametrize("mode", [0, 2])
+@pytest.mark.parametrize("hs,rotated", [(128, 64), (80, 34), (192, 0), (256, 250), (64, 2), (112, 104)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_dims_that_are_not_rotated_pass_through(gpu, bad, hs, rotated, mode):
+    """One that is not finite stays in its place, also beside one that is."""
+    c = build(21, 4, 2, hs, torch.float32, 34, norm=False, rotated=rotated, mode=mode)
+    want = check(c)
+    at = [(3, 1, rotated), (5, 0, rotated + 1), (7, 1, hs - 1), (9, 0, hs - 2)]
+    c["q"], c["k"] = c["q"].clone(), c["k"].clone()
+    for t, h, d in at:
+        c["q"][t, h, d] = c["k"][t, h, d] = bad
+    qo, ko = (torch.empty(c[x].shape, dtype=torch.float16, device="cuda") for x in "qk")
+    kc, vc = c["kc"].clone(), c["vc"].clone()
+    node_of(c)(c["q"], c["k"], c["v"], c["positions"], qo, k_out=ko, k_cache=kc, v_cache=vc, slots=c["slots"])
+    wq, wk = want[0].clone(), want[1].clone()
+    for t, h, d in at:
+        wq[t, h, d] = wk[t, h, d] = bad
+    for got, w in ((qo, wq), (ko, wk)):
+        assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(w))
+    wc, _ = into_caches(c["kc"], c["vc"], ko, c["v"].half(), c["slots"].tolist())
+    assert torch.equal(kc.view(torch.int16), wc.view(torch.int16))
