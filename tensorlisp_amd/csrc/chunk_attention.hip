@@ -828,7 +828,9 @@ static CaBounds ca_bounds(const tlh_chunk_attention_args &a) {
     b.wgs = a.head_size <= 192 ? 512 : 256;  // workgroups that fill the machine
     const int window = a.window > 0 ? std::min(a.window, CA_NO_WINDOW) : CA_NO_WINDOW;
     b.span_few = window + 31 / (int)G + 1, b.span_many = window + 127 / (int)G + 1;
-    const int64_t tiles = ca_tiles(a.max_context_len, wide ? b.span_many : b.span_few);
+    // (a context just past what a block sees may count a tile more than one just within; a call
+    // that may hold many rows may hold few)
+    const int64_t tiles = std::max(ca_tiles(a.max_context_len, b.span_few), wide ? ca_tiles(a.max_context_len, b.span_many) : 0);
     b.parts = std::max<int64_t>(1, std::min<int64_t>(CA_MAX_PARTS, (tiles + CA_MIN_TILES - 1) / CA_MIN_TILES));
     const int64_t few = (std::min<int64_t>(most, 32) + 3) / 4, many = wide ? 32 : 0;
     b.units = b.parts == 1 ? 0 : std::min(2 * b.wgs * few + b.wgs * many, b.items * b.parts * std::max(few, many));

@@ -456,3 +456,14 @@ def test_infinite_values_that_are_seen(gpu, hs, bs, new):
     finite = {**c, "vc": torch.where(torch.isfinite(c["vc"]), c["vc"], torch.zeros_like(c["vc"]))}
     want, tol = chunk_reference(finite["q"], finite["kc"], finite["vc"], c["table"], c["lens"], c["starts"], c["scale"])
     assert ((out[..., 20:].double() - want[..., 20:]).abs() <= tol[..., 20:]).all()
+
+
+@pytest.mark.parametrize("window,cached", [(64, 89), (65, 99), (1, 64), (100, 200)])
+def test_a_windowed_node_for_many_rows_takes_few(gpu, window, cached):
+    """Whose contexts count a tile more in blocks of few rows than in those of many."""
+    whole = build(32, 8, 128, 16, [cached - 39, cached], [40, 1], 96, window=window)
+    node = N.ChunkAttention(2, 41, 40, 32, 8, 128, 16, whole["table"].shape[1], cached + 1, whole["scale"], window=window)
+    for new in ([40, 1], [16, 1], [1, 1], [0, 1]):
+        c = {**whole, "starts": new_token_starts(new), "q": whole["q"][:sum(new)]}
+        out = torch.full(c["q"].shape, 7.0, dtype=torch.float16, device="cuda")
+        check(node(out, *on_gpu(c)), c)

@@ -88,6 +88,23 @@ def test_chunk_attention_scratch_never_shrinks():
                 assert s == sorted(s), name
 
 
+def test_chunk_attention_scratch_never_shrinks_under_a_window():
+    """A tile more or less that a block of few or of many rows sees: contexts around the window, counts around where one
+    block becomes the other."""
+    big = dict(max_blocks_per_seq=8192)
+    for window in (1, 16, 64, 65, 100, 1024):
+        for ctx in {1, 50, 90, window, *range(max(1, window - 3), window + 200, 7)}:
+            for G in (1, 4, 8):
+                s = [chunk_size(num_seqs=1, num_rows=r, max_rows=40, max_context_len=ctx, window=window, num_heads=8,
+                                num_kv_heads=8 // G, **big) for r in range(1, 41)]
+                assert s == sorted(s), (window, ctx, G, s)
+                s = [chunk_size(num_seqs=2, num_rows=200, max_rows=m, max_context_len=ctx, window=window, num_heads=8,
+                                num_kv_heads=8 // G, **big) for m in range(1, 101)]
+                assert s == sorted(s), (window, ctx, G, s)
+        s = [chunk_size(num_rows=300, max_rows=300, max_context_len=ctx, window=window, **big) for ctx in range(0, 3000, 13)]
+        assert s == sorted(s), window
+
+
 def test_chunk_attention_out_must_be_apart():
     """(Calls that pass are refused behind that, for want of scratch: more rows than any split leaves without.)"""
     row, n = 8 * 128 * 2, 10
