@@ -903,7 +903,8 @@ class ChunkAttention(_ScratchNode):
     """Causal attention of the sequences' new tokens over the paged cache, one or thousands a sequence, with its
     scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. A call takes up to
     num_seqs sequences and num_rows new tokens in all, at most max_rows of one sequence; calls of one object must be
-    stream-ordered (they share the scratch). One made while a graph is captured is for calls in that graph."""
+    stream-ordered (they share the scratch). One made while a graph is captured is for captured calls alone: each
+    clears the counters in its own graph."""
 
     def __init__(self, num_seqs, num_rows, max_rows, num_heads, num_kv_heads, head_size, block_size,
                  max_blocks_per_seq, max_context_len, scale, window: int = 0, device="cuda"):
@@ -917,8 +918,9 @@ class ChunkAttention(_ScratchNode):
         n = C.c_size_t()
         check(lib().tlh_chunk_attention_scratch_bytes(C.byref(a), C.byref(n)))
         self._allocate(n.value, device)
-        self.scratch[:CHUNK_COUNTER_BYTES].zero_()  # and every call leaves them so
         self._captured = self.device.type == "cuda" and _capturing(_torch_stream(self._home, self.device))
+        if not self._captured:
+            self.scratch[:CHUNK_COUNTER_BYTES].zero_()  # and every call leaves them so
 
     def __call__(self, out, q, k_cache, v_cache, block_tables, context_lens, row_starts, stream=None):
         """q and out f16 (rows, heads, head size) with rows <= num_rows, tokens at any stride that is a multiple of 8
@@ -944,12 +946,14 @@ class ChunkAttention(_ScratchNode):
         a.context_lens = _tensor(context_lens, torch.int32, (S,), "context_lens", dev)
         a.row_starts = _tensor(row_starts, torch.int32, (S + 1,), "row_starts", dev)
         with _on(dev, stream) as s:
-            if self._captured:  # the counters are cleared in the graph
+            if self._captured:
                 side, home = (_torch_stream(n, dev) for n in (s, self._home))
                 if not _capturing(home):
-                    raise ValueError("the node was made while a graph was captured: it is for calls in that graph")
+                    raise ValueError("the node was made while a graph was captured: it is for calls in that graph or in others")
                 if side != home:
                     side.wait_stream(home)
+                with torch.cuda.stream(side):  # in this call's graph: another's clearing may not have been replayed
+                    self.scratch[:CHUNK_COUNTER_BYTES].zero_()
             self._use_scratch(s)
             check(lib().tlh_chunk_attention(C.byref(a), self.scratch_ptr, self.scratch_bytes, s))
         return out

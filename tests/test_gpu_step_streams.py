@@ -227,3 +227,31 @@ def test_two_nodes_at_once(gpu, case):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for got in gots for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("where", ["current", "forked"])
+def test_a_chunk_node_made_in_one_graph_and_called_in_another(gpu, where):
+    """The second graph is replayed first, over counters that hold anything; then both in turn."""
+    make, call, want = chunk_node()
+    call(make(), want, None)
+    gots, graphs, side = [[torch.zeros_like(t) for t in want] for _ in range(2)], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], torch.cuda.Stream()
+    node = None
+    torch.cuda.synchronize()
+    for got, graph in zip(gots, graphs):
+        with torch.cuda.graph(graph):
+            here = torch.cuda.current_stream()
+            if where == "forked":
+                side.wait_stream(here)
+            node = make() if node is None else node
+            call(node, got, side if where == "forked" else None)
+            if where == "forked":
+                here.wait_stream(side)
+    node.scratch.fill_(0xff)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for got, graph in zip(gots[::-1], graphs[::-1]):
+            got[0].zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0])

@@ -112,3 +112,16 @@ def test_a_chunk_node_made_in_a_capture(steps, monkeypatch, captured):
         with pytest.raises(ValueError, match="for calls in that graph"):
             call(77)
         assert steps == []
+
+
+def test_every_captured_call_clears_its_counters(steps, monkeypatch):
+    """Of a node made in a capture: another graph may be captured with it, and be the one that is replayed first."""
+    monkeypatch.setattr(N, "_capturing", lambda stream: True)
+    args, node = chunk_args(), N.ChunkAttention(1, 3, 3, 8, 2, 64, 16, 8192, 131072, 0.1, device="cpu")
+    args = (*args[:3], torch.empty((1, 8192), dtype=torch.int32), *args[4:])
+    node._captured = True
+    for stream in (None, 77, 0):
+        node.scratch.fill_(255)
+        node(args[0], *args, stream=stream)
+        assert steps[-1] == "launch" and (node.scratch[:N.CHUNK_COUNTER_BYTES] == 0).all()
+        assert (node.scratch[N.CHUNK_COUNTER_BYTES:] == 255).all()
