@@ -512,8 +512,9 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  * of a page outside it are not seen. Lengths are bounded by max_context_len (at most
  * 2^30), starts by num_rows. Of a sequence with more than max_rows rows the first
  * max_rows are computed, as if it had no others, and the rest are left as they were.
- * No row of out may overlap a row of q (other columns of the same rows do not) or the
- * caches. `scratch` holds the partials of split contexts and the plan of many sequences (tlh_chunk_attention_scratch_bytes,
+ * No row of out may overlap a row of q (other columns of the same rows do not), and out not
+ * the caches, tables, lengths or starts; nothing may overlap the scratch. `scratch` holds the
+ * partials of split contexts and the plan of many sequences (tlh_chunk_attention_scratch_bytes,
  * which never shrinks as a count grows, 16-byte aligned; it may be NULL when that is
  * 0). Its first TLH_CHUNK_COUNTER_BYTES must be zero before its first call, and every call
  * leaves them zero; calls that share one must be stream-ordered. */
@@ -637,7 +638,7 @@ tlh_status tlh_head_rope(const tlh_head_rope_args *a, void *stream);
  * looked at, as if it had no others. Row strides in elements, any alignment of the type;
  * vocab <= 1000000, max_drafts <= 1024. `scratch` (16-byte aligned) holds the rows'
  * sums; calls that share one must be stream-ordered. The outputs must not overlap the
- * inputs or each other. */
+ * inputs or each other, and nothing the scratch. */
 typedef struct tlh_draft_verify_args {
     const void *target;
     const void *draft;

@@ -1314,9 +1314,27 @@ tlh_status tlh_chunk_attention(const tlh_chunk_attention_args *a, void *scratch,
     if (rows_overlap(a->out, 2 * a->out_stride, 2 * row, a->q, 2 * a->q_stride, 2 * row, a->num_rows) ||
         overlap(a->out, all, a->k_cache, pool) || overlap(a->out, all, a->v_cache, pool))
         return set_error(TLH_INVALID, "chunk_attention: out overlaps q or the caches");
+    // read by workgroups that start while others already write
+    const struct {
+        const char *name;
+        const void *p;
+        __int128 bytes;
+    } rest[] = {{"block_tables", a->block_tables, (__int128)4 * a->num_seqs * a->max_blocks_per_seq},
+                {"context_lens", a->context_lens, (__int128)4 * a->num_seqs},
+                {"row_starts", a->row_starts, (__int128)4 * (a->num_seqs + 1)},
+                {"out", a->out, all},
+                {"q", a->q, ((__int128)(a->num_rows - 1) * a->q_stride + row) * 2},
+                {"k_cache", a->k_cache, pool},
+                {"v_cache", a->v_cache, pool}};
+    for (int i = 0; i < 3; ++i)
+        if (rest[i].bytes > 0 && overlap(a->out, all, rest[i].p, rest[i].bytes))
+            return set_error(TLH_INVALID, "chunk_attention: out overlaps %s", rest[i].name);
     const size_t need = chunk_attention_scratch_bytes(*a);
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return set_error(TLH_INVALID, "chunk_attention: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    for (const auto &x : rest)
+        if (need > 0 && x.bytes > 0 && overlap(scratch, need, x.p, x.bytes))
+            return set_error(TLH_INVALID, "chunk_attention: %s overlaps the scratch", x.name);
     return launch_chunk_attention(*a, scratch, (hipStream_t)stream);
 }
 
@@ -1464,6 +1482,10 @@ tlh_status tlh_draft_verify(const tlh_draft_verify_args *a, void *scratch, size_
     const size_t need = draft_verify_scratch_bytes(*a);
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return set_error(TLH_INVALID, "draft_verify: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
+    for (const Range &r : in)
+        if (r.bytes > 0 && overlap(scratch, need, r.p, r.bytes)) return set_error(TLH_INVALID, "draft_verify: an input overlaps the scratch");
+    for (const Range &r : out)
+        if (r.bytes > 0 && overlap(scratch, need, r.p, r.bytes)) return set_error(TLH_INVALID, "draft_verify: an output overlaps the scratch");
     return launch_draft_verify(*a, scratch, (hipStream_t)stream);
 }
 

@@ -131,6 +131,27 @@ def test_chunk_attention_out_must_be_apart():
     assert refused(at + 8192 - row + 16, **wide)
 
 
+def test_chunk_attention_out_and_scratch_must_be_apart_from_what_is_read():
+    """Workgroups read the tables, lengths and starts while others write out already, and partials while others write
+    theirs. (Every call here is refused: those that are apart, for want of scratch.)"""
+    big = dict(max_context_len=8192, max_blocks_per_seq=512)
+    need, n = chunk_size(**big), 10 * 8 * 128 * 2
+    size = dict(out=n, q=n, k_cache=100 * 2 * 128 * 32, v_cache=100 * 2 * 128 * 32, block_tables=2 * 512 * 4, context_lens=8,
+                row_starts=12)
+    at = {f: P + i * FAR for i, f in enumerate(size)}
+    for x in ("block_tables", "context_lens", "row_starts"):
+        for place in (at[x] - n + 16, at[x], at[x] + (size[x] - 1) // 16 * 16):
+            st, text = status(N.lib().tlh_chunk_attention, C.byref(chunk(**{**big, "out": place})), None, 0, None)
+            assert st == "INVALID" and "overlaps" in text, (x, text)
+        for place in (at[x] - n, at[x] + (size[x] + 15) // 16 * 16):
+            st, text = status(N.lib().tlh_chunk_attention, C.byref(chunk(**{**big, "out": place})), None, 0, None)
+            assert st == "INVALID" and "overlaps" not in text, (x, text)
+    for x in size:
+        for place in ((at[x] - need + 16) // 16 * 16, at[x], at[x] + (size[x] - 1) // 16 * 16):
+            st, text = status(N.lib().tlh_chunk_attention, C.byref(chunk(**big)), place, need, None)
+            assert st == "INVALID" and "overlaps the scratch" in text, (x, text)
+
+
 # --------------------------------------------------------------- head rope
 ROPE = ("q", "k", "v", "positions", "freqs", "q_norm", "k_norm", "q_out", "k_out", "v_out", "k_cache", "v_cache", "slots")
 
@@ -255,6 +276,16 @@ def test_draft_verify_outputs_must_be_apart():
             for place in (at[x] - size[o], at[x] + size[x]):
                 st, text = status(N.lib().tlh_draft_verify, C.byref(verify(**{o: place})), None, 0, None)
                 assert st == "INVALID" and "scratch" in text, (o, x, place - at[x])
+
+
+def test_draft_verify_scratch_must_be_apart():
+    size = dict(target=9 * 4000, draft=7 * 4000, tokens=28, draft_starts=12, temperatures=8, accept_at=28, sample_at=8,
+                accepted=8, out_tokens=48, accept_probs=28)
+    need, at = verify_size(), {f: P + i * FAR for i, f in enumerate(VERIFY)}
+    for x in VERIFY:
+        for place in ((at[x] - need + 16) // 16 * 16, at[x], at[x] + (size[x] - 1) // 16 * 16):
+            st, text = status(N.lib().tlh_draft_verify, C.byref(verify()), place, need, None)
+            assert st == "INVALID" and "overlaps the scratch" in text, (x, text)
 
 
 # ------------------------------------------------- the Python entry points
