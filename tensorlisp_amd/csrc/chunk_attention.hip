@@ -468,17 +468,16 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
             }
             if (careful() && !see.whole) {
                 // through the wave's part of the merge buffer, which is free until the end
-                uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 128;
-                static_assert(192 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
+                uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 256;
+                static_assert(384 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
+                sp[lane] = pf[0], sp[64 + lane] = pf[1], sp[128 + lane] = rest[0], sp[192 + lane] = rest[1];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        __builtin_amdgcn_wave_barrier();
-                        sp[lane] = pf[i], sp[64 + lane] = rest[i], sv[lane] = vf[d][i];
-                        __builtin_amdgcn_wave_barrier();
-                        w.careful_pv(d, see, i, (const uint32_t *)sp, (const uint32_t *)sv);
-                    }
+                for (int d = 0; d < NB; ++d) {
+                    __builtin_amdgcn_wave_barrier();
+                    sv[lane] = vf[d][0], sv[64 + lane] = vf[d][1];
+                    __builtin_amdgcn_wave_barrier();
+                    w.template careful_pv<true>(d, see, (const uint32_t *)sp, (const uint32_t *)sv, 256);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)

@@ -195,26 +195,19 @@ template <int D, int BS, class Rule> struct PagedWave {
         return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
     }
     // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
-    // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
+    // ([i][lane], 16 bytes each, sv's parts sv_step words apart), with REST sp's rests behind.
+    template <bool REST = false>
     __device__ __forceinline__ void careful_pv(int d, const PagedSeen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
 #pragma unroll 1
         for (int key = 0; key < 32; ++key) {
-            const int i = key >> 4, at = 4 * (32 * ((key >> 3) & 1) + c) + ((key & 7) >> 1), sh = 16 * (key & 1);
-            if ((s.vis >> key) & 1) careful_key(d, key, h2f((uint16_t)(sp[256 * i + at] >> sh)), sv + sv_step * i);
-        }
-    }
-    // ... of the keys 16 i .. + 15, with sp's rests behind it
-    __device__ __forceinline__ void careful_pv(int d, const PagedSeen &s, int i, const uint32_t *sp, const uint32_t *sv) {
-#pragma unroll 1
-        for (int key = 16 * i; key < 16 * i + 16; ++key) {
-            const int at = 4 * (32 * ((key >> 3) & 1) + c) + ((key & 7) >> 1), sh = 16 * (key & 1);
-            if ((s.vis >> key) & 1) careful_key(d, key, h2f((uint16_t)(sp[at] >> sh)) + h2f((uint16_t)(sp[256 + at] >> sh)), sv);
-        }
-    }
-    __device__ __forceinline__ void careful_key(int d, int key, float p, const uint32_t *sv) {
-        const int from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
+            const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
+            if (!((s.vis >> key) & 1)) continue;
+            float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
+            if (REST) p += h2f((uint16_t)(sp[512 + 256 * i + 4 * (from + c) + w] >> sh));
 #pragma unroll
-        for (int x = 0; x < 16; ++x) O[d][x] += p * h2f((uint16_t)(sv[4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
+            for (int x = 0; x < 16; ++x)
+                O[d][x] += p * h2f((uint16_t)(sv[sv_step * i + 4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
+        }
     }
 };
 
