@@ -580,8 +580,7 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
 // -------------------------------------------------------------- many rows
 // use(f, fragment f) for N 1-KiB fragments in LDS, read BATCH at a time and a batch
 // ahead of their use: left to itself the compiler reads each right before its product.
-template <int N, typename Use> __device__ __forceinline__ void ca_stream(const uint8_t *at, Use use) {
-    constexpr int BATCH = 4;
+template <int N, int BATCH, typename Use> __device__ __forceinline__ void ca_stream(const uint8_t *at, Use use) {
     uint4 f[2][BATCH];
     auto read = [&](int b) {
 #pragma unroll
@@ -606,6 +605,10 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
     using W = PagedWave<D, BS, CaRule>;
     using Sh = PagedTile<D>;
     constexpr int NS = W::NS, NB = W::NB, KT = Sh::KT, SUBS = KT / 32, KF = SUBS * NS;
+    // At 192 dims a batch of four leaves O and Q four registers too few, and reading those back
+    // from memory waits for the next tile's loads, which are before it in line (2048 over 16384,
+    // 16/4 heads, with four and two: 737, 485 us).
+    constexpr int BATCH = D == 192 ? 2 : 4;
     __shared__ int s_flag[CA_WAVES];
     const int c = lane & 31, h = lane >> 5;
     const int r0 = j.r0 + 32 * wave, row = min(r0 + c, j.R - 1);
@@ -678,7 +681,7 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
             S[u] = (f32x16){};
             whole = whole && w.rule.whole(k0 + 32 * u) && good[u] == ~0u;
         }
-        ca_stream<KF>(T + 16 * lane, [&](int f, uint4 k) { S[f / NS] = mfma32<false>(k, qf[f % NS], S[f / NS]); });
+        ca_stream<KF, BATCH>(T + 16 * lane, [&](int f, uint4 k) { S[f / NS] = mfma32<false>(k, qf[f % NS], S[f / NS]); });
         if (!whole) {
             w.some_masked = true;
             int k = k0;
@@ -705,7 +708,7 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
             }
             return;
         }
-        ca_stream<2 * SUBS * NB>(T + KF * 1024 + 16 * lane,
+        ca_stream<2 * SUBS * NB, BATCH>(T + KF * 1024 + 16 * lane,
                                  [&](int f, uint4 v) { w.O[f % NB] = mfma32<false>(v, pf[f / NB], w.O[f % NB]); });
     };
     auto begin = [&] {
@@ -793,9 +796,11 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
         }
 }
 
-// Two workgroups a CU up to 192 dims (there with spills, outside the loops over tiles: heads of
-// 192, 16/4, with one and two, us: 2048 over 16384 882, 514; nine pieces of 13..701 177, 150; 32
-// decoding over 512..8192 93, 91; 8 x 12 tokens 52, 54).
+// Two workgroups a CU up to 192 dims (there with spills, around the loops over tiles and in those
+// of the careful pass: heads of 192, 16/4, with one and two, us: 2048 over 16384 861, 485; nine
+// pieces of 13..701 behind up to 5000 256, 182; 32 decoding over 512..8192 110, 91; 8 x 12 tokens
+// over 2000 34, 32). Pages of 8 keep a tile's page ids in memory of the lane's own, in the loops
+// too: 2048 over 16384, heads of 128, 763 us where pages of 16 take 635; 32 decoding 147 and 113.
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * CA_WAVES, D <= 192 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
