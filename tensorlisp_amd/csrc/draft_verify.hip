@@ -453,14 +453,9 @@ __device__ __forceinline__ DvStop dv_alone(const tlh_draft_verify_args &a, int s
 }
 
 template <int TY>
-__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int M, int chunk, const int *__restrict__ odd,
-                                                        const DvStop *__restrict__ stops, const DvMass *__restrict__ masses) {
+__device__ __forceinline__ void dv_draw(const tlh_draft_verify_args &a, int s, int M, int chunk, const DvStop &st, const DvMass *masses) {
     constexpr int ES = TY == TLH_TYPE_F32 ? 4 : 2;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x;
-    __shared__ DvMass s_alone[DV_MAX_CHUNKS];
-    const bool alone = *odd != 0;
-    DvStop st = stops[s];
-    if (alone) st = dv_alone<TY>(a, s, M, chunk, s_alone);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (!st.draws) return;
     const DvSeq q = dv_seq(a, s);
     const double c_t = DV_LOG2E / (double)a.temperatures[s];
@@ -469,7 +464,7 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     int outright = st.stop < q.n && !a.draft ? a.tokens[q.b + st.stop] : -1;
     const DvExp weight;
     DvMass m = {};
-    if (lane < M) m = alone ? s_alone[lane] : masses[(int64_t)s * M + lane];
+    if (lane < M) m = masses[lane];
     if (dv_sum(m.sum) <= DV_NOTHING) {  // nothing above the drafter's: from p alone
         minus = false;
         outright = -1;
@@ -501,12 +496,13 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
         return dv_above(w, ip, weight(dv_elem<TY>(a.draft, (int64_t)(q.b + st.stop) * a.draft_stride + e), st.mq, c_t), iq);
     };
     double sum = 0.0;
-    int last = -1;
+    int lead = 0x7fffffff, last = -1;  // the first and the last with a weight
     for (int e = e0; e < e1; ++e) {
         const double w = mass(e);
         sum += w;
-        if (w > 0.0) last = e;
+        if (w > 0.0) lead = min(lead, e), last = e;
     }
+    if (first_place && e0 < e1) lead = e0;
     __shared__ double s_sum[DV_DRAW / 64];
     __shared__ int s_last[DV_DRAW / 64], s_next;
     double upto = sum;
@@ -525,11 +521,11 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
         last = max(last, s_last[w]);
     }
     from += upto - sum;
-    if (from + sum > reach) {
+    if (from > reach) atomicMin(&s_next, lead);
+    else if (from + sum > reach) {
         for (int e = e0; e < e1; ++e) {
-            const double w = mass(e);
-            from += w;
-            if (from > reach && (w > 0.0 || first_place)) {
+            from += mass(e);
+            if (from > reach) {
                 atomicMin(&s_next, e);
                 break;
             }
@@ -537,6 +533,16 @@ __global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_a
     }
     __syncthreads();
     if (threadIdx.x == 0) a.out_tokens[(int64_t)s * (a.max_drafts + 1) + st.stop] = s_next == 0x7fffffff ? last : s_next;
+}
+template <int TY>
+__global__ void __launch_bounds__(DV_DRAW) k_draft_draw(const tlh_draft_verify_args a, int M, int chunk, const int *__restrict__ odd,
+                                                        const DvStop *__restrict__ stops, const DvMass *__restrict__ masses) {
+    __shared__ DvMass s_alone[DV_MAX_CHUNKS];
+    const int s = blockIdx.x;
+    const bool alone = *odd != 0;
+    DvStop st = stops[s];
+    if (alone) st = dv_alone<TY>(a, s, M, chunk, s_alone);
+    dv_draw<TY>(a, s, M, chunk, st, alone ? s_alone : masses + (int64_t)s * M);
 }
 
 // A small vocabulary's chunk of 64 a lane would be mostly empty; few rows: shorter chunks,
