@@ -504,9 +504,10 @@ tlh_status tlh_token_logprobs(const tlh_token_logprobs_args *a, void *scratch, s
  *                are left as they were
  * With L = context_lens[s], row i of the sequence is the token at place L - n + i and
  * sees the tokens up to itself, with window > 0 the last `window` of them. f32 scores,
- * softmax and sums. For the product with v its numerators keep 22 bits where a sequence has
- * up to 64 rows of q a kv head (those below 2^-10 of the row's largest change by up to 2^-32
- * of it), and are rounded to f16 where it has more (those below 2^-21); a row that sees nothing (a
+ * softmax and sums; for the product with v its numerators keep 22 bits (those below 2^-10 of
+ * the row's largest change by up to 2^-32 of it). With f16_weights 1 (else 0) they are rounded
+ * to f16 (those below 2^-21 alike) where a sequence has more than 64 rows of q a kv head, which
+ * saves one of three products there. A row that sees nothing (a
  * place below 0, pages that are not there) gives zeros, and what a row does not see does
  * not reach it, whatever it holds. num_blocks is the pools' length in blocks: tokens
  * of a page outside it are not seen. Lengths are bounded by max_context_len (at most
@@ -541,6 +542,7 @@ typedef struct tlh_chunk_attention_args {
     int32_t max_context_len;
     int32_t window;
     float scale;
+    int32_t f16_weights;
 } tlh_chunk_attention_args;
 
 tlh_status tlh_chunk_attention_scratch_bytes(const tlh_chunk_attention_args *a, size_t *bytes);

@@ -16,24 +16,28 @@
 //    above 128 dims) in LDS, double-buffered and loaded straight from the pages.
 // Both compute S^T = K . Q^T and O^T += V^T . P^T, so a lane holds one row's scores.
 //
-// P meets V in f16, as the matrix cores take it. With few rows a second product adds what that
-// rounding took off (22 bits in all): the tiles wait for HBM, so 32 sequences decoding take 117
-// us with it and without, and a result is off by 2.07e-4 of its size, all of it its own rounding,
-// instead of 2.9e-4. With many rows the products are the bound (2048 over 16384, us, without and
-// with it: heads of 64 385, 536; 128 633, 831; 256 517, 587), so there P stays rounded to f16.
+// P meets V in f16, as the matrix cores take it, and a second product adds what that rounding
+// took off (22 bits in all): a result is off by 2.07e-4 of its size, all of it its own rounding,
+// instead of 2.9e-4. With few rows the tiles wait for HBM, and 32 sequences decoding take 113 us
+// with it and without. With many the products are the bound, so there a caller may choose to do
+// without (us, with it and without: 2048 over 16384 with heads of 64 544, 387; 128 840, 643; 192
+// 636, 482; 256 590, 514; 31 tokens + 600 148, 143; 9 x 13..701 52.3, 47.7).
 //
 // Items differ by orders of magnitude in keys, and only the device knows the lengths. So
 // every workgroup works out the same plan from them: how many tiles a workgroup takes
 // so that all run at once, and from that the partitions of every sequence's keys (with
-// more than 64 sequences a launch before does it, and they look it up). The last of an item's partitions to arrive joins them, in the order of their keys, whichever
-// it is. (Joined in a second launch, whose code has to come from memory when the keys
+// more than 64 sequences a launch before does it, and they look it up; there the workgroups go
+// in the order of the sequences, not longest first: 65 over 512..8192 take 226 to 239 us, 64 of
+// them 212). The last of an item's partitions to arrive joins them, in the order of their keys,
+// whichever it is. (Joined in a second launch, whose code has to come from memory when the keys
 // have gone through the caches, 31 tokens + 600 took 20 us more.)
 //
-// Measured, 32/8 heads of 128 unless said: 1 token over 1500 10.1 us, the plan and one chain of
-// latencies; 32 sequences decoding over 512..8192 113 us (4.9 TB/s over random pages); 31 of
-// those beside a piece of 600 tokens 149 to 178 us; 2048 over 16384 689 to 740 us, 810 to 850
-// TFLOP/s, where the tiles' LDS reads take as long as the products; nine
-// pieces of 13..701 with 4/1 heads of 256 and a window of 1024 48 us (one wave a SIMD).
+// Measured, 32/8 heads of 128 unless said, with inputs that were just used and with others each
+// time: 1 token over 1500 10.3 and 13.4 us, the plan and one chain of latencies; 32 sequences
+// decoding over 512..8192 113 us (4.9 TB/s over random pages); 31 of those beside a piece of 600
+// tokens 148 to 160 and 199 us; 2048 over 16384 840 to 863 and 886 us, the three products at 1.02
+// to 1.04 PFLOP/s, nearly a large library product's rate (1.09); nine pieces of 13..701 with 4/1
+// heads of 256 and a window of 1024 52 to 54 and 56 us (one wave a SIMD).
 #include <algorithm>
 #include <type_traits>
 
@@ -80,6 +84,7 @@ struct CaArgs : PagedArgs {
     int S, rows, max_rows, max_ctx, window;
     int lg_wgs;          // workgroups that fill the machine, a power of two
     int span_few, span_many;  // keys that some row of a block of 32 and of 128 rows sees
+    int f16_weights;
     CaDiv G, kv;
 };
 
@@ -342,7 +347,7 @@ __device__ __forceinline__ CaJob ca_job(const CaArgs &a, const CaPlan &p, int D)
     j.r0 = per * rb;
     const int last = a.G(min(j.r0 + per, j.R) - 1);  // tokens r0 / G .. last
     const int lo = max(0, q.L - q.n + a.G(j.r0) - a.window + 1) & ~63, hi = q.L - q.n + last + 1;
-    const uint32_t tiles = hi > lo ? (hi - lo + 63) >> 6 : 0, parts = p.parts;  // < 2^25, <= 64
+    const uint32_t tiles = hi > lo ? (hi - lo + 63) >> 6 : 0, parts = p.parts;  // < 2^25, <= CA_MAX_PARTS
     j.k0 = lo + 64 * (int)(tiles * part / parts);
     j.k1 = min(hi, lo + 64 * (int)(tiles * (part + 1) / parts));
     const int item = rb * a.KV + j.hk;
@@ -468,16 +473,17 @@ __device__ __forceinline__ void ca_few(const CaArgs &a, const CaSeq &sq, const C
             }
             if (careful() && !see.whole) {
                 // through the wave's part of the merge buffer, which is free until the end
-                uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 256;
-                static_assert(384 * 16 <= CaLds<D>::WAVE, "operands of one dim block");
-                sp[lane] = pf[0], sp[64 + lane] = pf[1], sp[128 + lane] = rest[0], sp[192 + lane] = rest[1];
+                uint4 *sp = (uint4 *)merge_at(wave), *sv = sp + 128;
+                static_assert(192 * 16 <= CaLds<D>::WAVE, "operands of 16 keys and a dim block");
 #pragma unroll
-                for (int d = 0; d < NB; ++d) {
-                    __builtin_amdgcn_wave_barrier();
-                    sv[lane] = vf[d][0], sv[64 + lane] = vf[d][1];
-                    __builtin_amdgcn_wave_barrier();
-                    w.template careful_pv<true>(d, see, (const uint32_t *)sp, (const uint32_t *)sv, 256);
-                }
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        __builtin_amdgcn_wave_barrier();
+                        sp[lane] = pf[i], sp[64 + lane] = rest[i], sv[lane] = vf[d][i];
+                        __builtin_amdgcn_wave_barrier();
+                        w.careful_rest_pv(d, see, i, (const uint32_t *)sp, (const uint32_t *)sv);
+                    }
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -607,7 +613,7 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
     constexpr int NS = W::NS, NB = W::NB, KT = Sh::KT, SUBS = KT / 32, KF = SUBS * NS;
     // At 192 dims a batch of four leaves O and Q four registers too few, and reading those back
     // from memory waits for the next tile's loads, which are before it in line (2048 over 16384,
-    // 16/4 heads, with four and two: 737, 485 us).
+    // 16/4 heads, f16_weights, with four and two: 737, 485 us).
     constexpr int BATCH = D == 192 ? 2 : 4;
     __shared__ int s_flag[CA_WAVES];
     const int c = lane & 31, h = lane >> 5;
@@ -646,7 +652,7 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 #pragma unroll
         for (int st = 0; st < NS; ++st) qf[st] = w.signed_q(*(const uint4 *)(qr + 32 * st));
     }
-    auto tile = [&](auto careful, int t, uint8_t *T, uint8_t *Tn) {
+    auto tile = [&](auto careful, auto rests, int t, uint8_t *T, uint8_t *Tn) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): tile t has landed
         lds_barrier();                       // for every wave, and the other buffer is free
         const int k0 = j.k0 + KT * t;
@@ -664,7 +670,9 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
             load_tile(pg, Tn);
             ids(t + 2, pn);
         }
-        if (gaps) {  // places that hold no token's value may hold anything: zeroed by the waves that loaded them
+        // Places that hold no token's value may hold anything: zeroed, by whichever wave, since behind
+        // the barrier above every wave's loads of this tile have landed.
+        if (gaps) {
 #pragma unroll 1
             for (int f = wave; f < 2 * SUBS * NB; f += CA_WAVES) {
                 uint4 *v = (uint4 *)(T + (KF + f) * 1024) + lane;
@@ -689,27 +697,32 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) w.hide(S[u], w.rule.sees(k + 32 * u) & there[u]);
         }
-        uint4 pf[2 * SUBS];
+        uint4 pf[2 * SUBS], rest[2 * SUBS];
         PagedSeen see[SUBS];
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) see[u] = {true, ~0u, ~0u};
-        w.softmax(S, see, pf);
+        w.template softmax<rests()>(S, see, pf, rest);
         if (careful() && !whole) {
             uint4 *sp = (uint4 *)aux + 128 * wave;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
                 see[u].vis = w.rule.sees(k0 + 32 * u) & there[u];
-                __builtin_amdgcn_wave_barrier();
-                sp[lane] = pf[2 * u], sp[64 + lane] = pf[2 * u + 1];
-                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int d = 0; d < NB; ++d)
-                    w.careful_pv(d, see[u], (const uint32_t *)sp, (const uint32_t *)(T + (KF + u * 2 * NB + d) * 1024), 256 * NB);
+                for (int i = 0; i < 2; ++i) {
+                    __builtin_amdgcn_wave_barrier();
+                    sp[lane] = pf[2 * u + i], sp[64 + lane] = rest[2 * u + i];
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int d = 0; d < NB; ++d)
+                        w.careful_rest_pv(d, see[u], i, (const uint32_t *)sp, (const uint32_t *)(T + (KF + (2 * u + i) * NB + d) * 1024));
+                }
             }
             return;
         }
-        ca_stream<2 * SUBS * NB, BATCH>(T + KF * 1024 + 16 * lane,
-                                 [&](int f, uint4 v) { w.O[f % NB] = mfma32<false>(v, pf[f / NB], w.O[f % NB]); });
+        ca_stream<2 * SUBS * NB, BATCH>(T + KF * 1024 + 16 * lane, [&](int f, uint4 v) {
+            w.O[f % NB] = mfma32<false>(v, pf[f / NB], w.O[f % NB]);
+            if (rests()) w.O[f % NB] = mfma32<false>(careful() ? W::finite_v(v) : v, rest[f / NB], w.O[f % NB]);
+        });
     };
     auto begin = [&] {
         w.reset();
@@ -724,18 +737,22 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
         }
     };
     begin();
-    for (int t = 0; t < ntiles; t += 2) {
-        tile(std::false_type(), t, T0, T1);
-        if (t + 1 < ntiles) tile(std::false_type(), t + 1, T1, T0);
-    }
-    const bool again = mine && w.some_masked && __builtin_amdgcn_ballot_w64(w.bad() && r0 + c < j.R) != 0;
+    auto all = [&](auto rests) {
+        for (int t = 0; t < ntiles; t += 2) {
+            tile(std::false_type(), rests, t, T0, T1);
+            if (t + 1 < ntiles) tile(std::false_type(), rests, t + 1, T1, T0);
+        }
+    };
+    if (a.f16_weights) all(std::false_type());
+    else all(std::true_type());
+    const bool again = mine && __builtin_amdgcn_ballot_w64(w.bad() && r0 + c < j.R) != 0;
     if (lane == 0) s_flag[wave] = again;
     lds_barrier();  // and every wave is done with both buffers
     if ((s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3]) != 0) {
         // (a loop of its own: with both kinds of tile in one, every tile moved O to other registers)
         begin();
 #pragma unroll 1
-        for (int t = 0; t < ntiles; ++t) tile(std::true_type(), t, t & 1 ? T1 : T0, t & 1 ? T0 : T1);
+        for (int t = 0; t < ntiles; ++t) tile(std::true_type(), std::true_type(), t, t & 1 ? T1 : T0, t & 1 ? T0 : T1);
     }
     const int rr = r0 + c;
     float sum = sum_halves(w.l);
@@ -797,10 +814,12 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 }
 
 // Two workgroups a CU up to 192 dims (there with spills, around the loops over tiles and in those
-// of the careful pass: heads of 192, 16/4, with one and two, us: 2048 over 16384 861, 485; nine
-// pieces of 13..701 behind up to 5000 256, 182; 32 decoding over 512..8192 110, 91; 8 x 12 tokens
-// over 2000 34, 32). Pages of 8 keep a tile's page ids in memory of the lane's own, in the loops
-// too: 2048 over 16384, heads of 128, 763 us where pages of 16 take 635; 32 decoding 147 and 113.
+// of the careful pass: heads of 192, 16/4, f16_weights, with one and two, us: 2048 over 16384 861,
+// 485; nine pieces of 13..701 behind up to 5000 256, 182; 32 decoding over 512..8192 110, 91; 8 x
+// 12 tokens over 2000 34, 32). Pages of 8 keep a tile's page ids in memory of the lane's own, in
+// the loops too: 2048 over 16384, heads of 128, 922 us where pages of 16 take 840; 32 decoding 151
+// and 113. (Three workgroups a CU at 64 dims: 2048 over 16384 525 instead of 544, but 451 instead
+// of 387 with f16_weights.)
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * CA_WAVES, D <= 192 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
@@ -877,6 +896,7 @@ tlh_status launch_chunk_attention(const tlh_chunk_attention_args &a, void *scrat
     c.rows = a.num_rows, c.max_rows = a.max_rows, c.max_blocks = a.max_blocks_per_seq, c.max_ctx = a.max_context_len;
     c.window = a.window > 0 ? std::min(a.window, CA_NO_WINDOW) : CA_NO_WINDOW;
     c.lg_wgs = b.wgs == 512 ? 9 : 8, c.span_few = b.span_few, c.span_many = b.span_many;
+    c.f16_weights = a.f16_weights;
     set_scale(c, a.scale);
     if (b.blocks >= 1 << 24)  // x 256 threads
         return set_error(TLH_INVALID, "chunk_attention: too many rows and heads for one launch");

@@ -11,10 +11,12 @@
 // Three launches: the sums of chunks of all rows, a chunk a workgroup; then every workgroup
 // of a sequence finds where it stops, and sums its chunk of what the token there is drawn
 // from; then one workgroup a sequence finds the chunk and the token in it.
-// Measured, us (the three launches): 1 x 4 drafts of 128256 f32 5.6 + 7.8 + 5.8, of which
-// 4.5 + 5 + 5 are there with 1000 tokens, chains of latencies; 32 x 1..8 of 128256 f32, 149
-// MB, 39.5 (3.7 TB/s: f64, which the reads nearly hide) + 16.4 + 10.3; 48 x 10 of 32003
-// bf16, proposed outright, 25.5 (f64: half the bytes an element) + 9.3 + 8.7.
+// Measured, us (the three launches, with the same logits again): 1 x 4 drafts of 128256 f32 5.6
+// + 7.9 + 5.7, of which 4.5 + 5 + 5 are there with 1000 tokens, chains of latencies; 32 x 1..8
+// of 128256 f32, 149 MB, 40.2 (f64, as long as a read from memory) + 16.5 + 10.0; 48 x 10 of
+// 32003 bf16, proposed outright, 25.4 (f64: half the bytes an element) + 9.4 + 8.4. With logits
+// that no cache holds the calls take 24, 75 and 48 us, with the same ones 19.4, 65 and 41; all
+// greedy, 1 x 4 and 32 x 1..8 15 and 34 (26 with the same).
 #include <algorithm>
 #include <type_traits>
 

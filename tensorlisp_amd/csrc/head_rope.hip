@@ -15,9 +15,12 @@
 //    consecutive lanes write consecutive tokens.
 // Norms and rotation are f32, and a head is rounded once, to the type it is written in.
 // Measured against a wave for a (token, head), which forms its angles for each and writes
-// values two bytes a page line: 2501 tokens of 28 + 4 + 4 heads of 128 in bf16 37 -> 12.6 us
-// (3.7 TB/s); 8192 tokens of 32 + 8 + 8 of 128 in f32 230 -> 79.5 us (3.8 TB/s, where a
-// large copy reaches 4.9).
+// values two bytes a page line, with the same inputs again: 2501 tokens of 28 + 4 + 4 heads of
+// 128 in bf16 (46 MB) 37 -> 13 us; 8192 tokens of 32 + 8 + 8 of 128 in f32 (302 MB) 230 -> 74 us.
+// With inputs that no cache holds 19 us (2.4 TB/s: the angles, formed anew for each group of
+// heads, are not hidden) and 86 us (3.5 TB/s, where a large copy reaches 4.9). 2048 tokens of
+// 32 + 8 + 8 in bf16 take 15 and 22 us, rotating half of a head in mode 2, where each of a
+// pair's lanes forms its angle, 17 and 23.
 #include <algorithm>
 
 #include "kernels.hpp"

@@ -195,18 +195,28 @@ template <int D, int BS, class Rule> struct PagedWave {
         return make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
     }
     // One dim block's products key by key: sp and sv hold the lanes' P and V^T operands
-    // ([i][lane], 16 bytes each, sv's parts sv_step words apart), with REST sp's rests behind.
-    template <bool REST = false>
+    // ([i][lane], 16 bytes each, sv's parts sv_step words apart).
     __device__ __forceinline__ void careful_pv(int d, const PagedSeen &s, const uint32_t *sp, const uint32_t *sv, int sv_step) {
 #pragma unroll 1
         for (int key = 0; key < 32; ++key) {
             const int i = key >> 4, from = 32 * ((key >> 3) & 1), w = (key & 7) >> 1, sh = 16 * (key & 1);
             if (!((s.vis >> key) & 1)) continue;
-            float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
-            if (REST) p += h2f((uint16_t)(sp[512 + 256 * i + 4 * (from + c) + w] >> sh));
+            const float p = h2f((uint16_t)(sp[256 * i + 4 * (from + c) + w] >> sh));
 #pragma unroll
             for (int x = 0; x < 16; ++x)
                 O[d][x] += p * h2f((uint16_t)(sv[sv_step * i + 4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
+        }
+    }
+    // ... of the keys 16 i .. + 15 alone, the weights' rests behind P
+    __device__ __forceinline__ void careful_rest_pv(int d, const PagedSeen &s, int i, const uint32_t *sp, const uint32_t *sv) {
+#pragma unroll 1
+        for (int key = 0; key < 16; ++key) {
+            const int from = 32 * (key >> 3), w = (key & 7) >> 1, sh = 16 * (key & 1);
+            if (!((s.vis >> (16 * i + key)) & 1)) continue;
+            const uint32_t *at = sp + 4 * (from + c) + w;
+            const float p = h2f((uint16_t)(at[0] >> sh)) + h2f((uint16_t)(at[256] >> sh));
+#pragma unroll
+            for (int x = 0; x < 16; ++x) O[d][x] += p * h2f((uint16_t)(sv[4 * (from + 8 * (x / 4) + 4 * h + x % 4) + w] >> sh));
         }
     }
 };

@@ -1280,6 +1280,8 @@ static tlh_status check_chunk(const tlh_chunk_attention_args *a) {
         return set_error(TLH_INVALID, "chunk_attention: bad counts (at most 65535 sequences)");
     if (a->max_context_len > 1 << 30)  // the kernels look a few tiles past it, in 32 bits
         return set_error(TLH_INVALID, "chunk_attention: max_context_len %d above 2^30", a->max_context_len);
+    if (a->f16_weights != 0 && a->f16_weights != 1)
+        return set_error(TLH_INVALID, "chunk_attention: f16_weights %d is neither 0 nor 1", a->f16_weights);
     if ((int64_t)a->max_blocks_per_seq * a->block_size < a->max_context_len)
         return set_error(TLH_INVALID, "chunk_attention: max_blocks_per_seq * block_size < max_context_len");
     if ((int64_t)a->num_rows * a->num_heads > 1 << 30)

@@ -120,7 +120,7 @@ class TlhChunkArgs(C.Structure):
                 ("out_stride", C.c_int64), ("q_stride", C.c_int64), ("num_blocks", C.c_int64), ("num_seqs", C.c_int32),
                 ("num_rows", C.c_int32), ("max_rows", C.c_int32), ("num_heads", C.c_int32), ("num_kv_heads", C.c_int32),
                 ("head_size", C.c_int32), ("block_size", C.c_int32), ("max_blocks_per_seq", C.c_int32),
-                ("max_context_len", C.c_int32), ("window", C.c_int32), ("scale", C.c_float)]
+                ("max_context_len", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("f16_weights", C.c_int32)]
 
 
 class TlhHeadRopeArgs(C.Structure):
@@ -901,20 +901,22 @@ CHUNK_COUNTER_BYTES = 8192
 
 class ChunkAttention(_ScratchNode):
     """Causal attention of the sequences' new tokens over the paged cache, one or thousands a sequence, with its
-    scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. A call takes up to
+    scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. f16_weights: sequences
+    with more than 64 rows of q a kv head round the softmax's weights to f16 before they meet v, as packed and tree
+    attention do (less exact, and a quarter faster where many rows see long contexts). A call takes up to
     num_seqs sequences and num_rows new tokens in all, at most max_rows of one sequence; calls of one object must be
     stream-ordered (they share the scratch). One made while a graph is captured is for captured calls alone: each
     clears the counters in its own graph."""
 
     def __init__(self, num_seqs, num_rows, max_rows, num_heads, num_kv_heads, head_size, block_size,
-                 max_blocks_per_seq, max_context_len, scale, window: int = 0, device="cuda"):
+                 max_blocks_per_seq, max_context_len, scale, window: int = 0, device="cuda", f16_weights: bool = False):
         a = self.args = TlhChunkArgs()
         counts = dict(num_seqs=num_seqs, num_rows=num_rows, max_rows=max_rows, num_heads=num_heads,
                       num_kv_heads=num_kv_heads, head_size=head_size, block_size=block_size,
                       max_blocks_per_seq=max_blocks_per_seq, max_context_len=max_context_len, window=window)
         for name, value in counts.items():
             setattr(a, name, _int32(value, name))
-        a.scale = scale
+        a.scale, a.f16_weights = scale, bool(f16_weights)
         n = C.c_size_t()
         check(lib().tlh_chunk_attention_scratch_bytes(C.byref(a), C.byref(n)))
         self._allocate(n.value, device)
@@ -960,14 +962,14 @@ class ChunkAttention(_ScratchNode):
 
 
 def chunk_attention(q, k_cache, v_cache, block_tables, context_lens, row_starts, max_rows: int, max_context_len: int,
-                    scale: float, window: int = 0, stream=None):
+                    scale: float, window: int = 0, stream=None, f16_weights: bool = False):
     """One ChunkAttention call: q f16 (rows, heads, head size) -> out alike, contiguous (zeros in rows behind the last
     sequence). `stream` waits for the current stream's work."""
     import torch
 
     rows, heads, hs = q.shape
     node = ChunkAttention(block_tables.shape[0], rows, max_rows, heads, v_cache.shape[1], hs, v_cache.shape[3],
-                          block_tables.shape[1], max_context_len, scale, window, device=q.device)
+                          block_tables.shape[1], max_context_len, scale, window, device=q.device, f16_weights=f16_weights)
     out = torch.zeros((rows, heads, hs), dtype=q.dtype, device=q.device)
     # the zeros come from the current stream; the copy is the call's, on its own
     with torch.cuda.stream(_behind_current(stream, q.device)):

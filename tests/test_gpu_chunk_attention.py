@@ -467,3 +467,67 @@ def test_a_windowed_node_for_many_rows_takes_few(gpu, window, cached):
         c = {**whole, "starts": new_token_starts(new), "q": whole["q"][:sum(new)]}
         out = torch.full(c["q"].shape, 7.0, dtype=torch.float16, device="cuda")
         check(node(out, *on_gpu(c)), c)
+
+
+def close(c, out, heads, kv, hs, bs, new):
+    for s, L in enumerate(c["lens"]):
+        at, pos = slice(c["starts"][s], c["starts"][s + 1]), np.arange(L)
+        page, off = torch.from_numpy(c["table"][s, pos // bs].astype(np.int64)), torch.from_numpy(pos % bs)
+        see = torch.arange(L)[None] <= L - new + torch.arange(new)[:, None]
+        for h in range(heads):
+            g = h // (heads // kv)
+            k, v = c["kc"][page, g, :, off].reshape(L, hs)[:, :8].double(), c["vc"][page, g, :, off].reshape(L, hs).double()
+            want, A, d = attend(c["q"][at, h, :8].double(), k, v, see, c["scale"])
+            err, tol = (out[at, h] - want).abs(), close_bound(want, A, d, L, float(v.abs().max()))
+            yield bool((err <= tol).all())
+
+
+@pytest.mark.parametrize("heads,hs,bs,new", [(8, 64, 16, 33), (8, 128, 8, 90), (4, 128, 32, 130), (4, 80, 16, 70), (4, 112, 16, 40),
+                                             (4, 96, 32, 200), (4, 192, 32, 50), (4, 192, 16, 140), (2, 256, 16, 65)])
+def test_weights_of_many_rows_keep_what_f16_rounds_off(gpu, heads, hs, bs, new):
+    """As those of few, unless the caller asks for weights in f16; contexts that are split among them."""
+    cached = [1, 40, 300, 2500]
+    c = build(heads, 2 if heads < 8 else 1, hs, bs, cached, [new] * len(cached), 97 + hs)
+    kv = c["vc"].shape[1]
+    c["kc"][:, :, 1:], c["scale"] = 0.0, 0.25
+    out = run(c).cpu().double()
+    assert all(close(c, out, heads, kv, hs, bs, new))
+    fast = N.ChunkAttention(4, c["q"].shape[0], new, heads, kv, hs, bs, c["table"].shape[1], max(c["lens"]), 0.25, f16_weights=True)
+    fast = fast(torch.empty_like(c["q"], device="cuda"), *on_gpu(c))
+    assert not all(close(c, fast.cpu().double(), heads, kv, hs, bs, new))  # the test can see it
+    check(fast, c)
+
+
+@pytest.mark.parametrize("heads,kv,hs,bs,cached,new", [x for x in CASES if max(x[5]) * x[0] // x[1] > 64])
+def test_f16_weights_against_64_bits(gpu, heads, kv, hs, bs, cached, new):
+    """Few rows beside many are what they are without; the one-call form takes it too."""
+    c = build(heads, kv, hs, bs, cached, new, 20 + heads + hs + bs + sum(new))
+    want, dev = run(c), on_gpu(c)
+    out = N.chunk_attention(*dev, max(new), max(c["lens"]), c["scale"], f16_weights=True)
+    check(out, c)
+    for s, n in enumerate(new):
+        at = slice(c["starts"][s], c["starts"][s + 1])
+        if n * heads // kv <= 64:
+            assert torch.equal(out[at], want[at])
+        if n * heads // kv > 64:
+            assert not torch.equal(out[at], want[at])
+
+
+@pytest.mark.parametrize("f16_weights", [False, True])
+@pytest.mark.parametrize("hs,bs,new", [(128, 16, 40), (64, 8, 70), (256, 32, 90), (192, 16, 70), (80, 32, 50)])
+def test_infinite_values_that_many_rows_see(gpu, hs, bs, new, f16_weights):
+    """An infinity that a row sees is its result in that dim, both signs are NaN, and the other dims are as ever; rows
+    before it do not see it."""
+    c = build(4, 1, hs, bs, [400], [new], 98)
+    for p, dims, x in ((40, slice(0, 8), float("inf")), (333, slice(8, 16), -float("inf")), (41, slice(16, 20), float("inf")),
+                       (42, slice(16, 20), -float("inf")), (420, slice(24, 28), float("inf"))):
+        c["vc"][c["table"][0, p // bs], :, dims, p % bs] = x
+    node = N.ChunkAttention(1, new, new, 4, 1, hs, bs, c["table"].shape[1], 400 + new, c["scale"], f16_weights=f16_weights)
+    out = node(torch.empty_like(c["q"], device="cuda"), *on_gpu(c)).cpu()
+    assert (out[..., :8] == float("inf")).all() and (out[..., 8:16] == -float("inf")).all() and torch.isnan(out[..., 16:20]).all()
+    assert (out[20:, :, 24:28] == float("inf")).all() and torch.isfinite(out[:20, :, 24:28]).all()
+    finite = {**c, "vc": torch.where(torch.isfinite(c["vc"]), c["vc"], torch.zeros_like(c["vc"]))}
+    want, tol = chunk_reference(finite["q"], finite["kc"], finite["vc"], c["table"], c["lens"], c["starts"], c["scale"])
+    for dims in (slice(20, 24), slice(28, hs)):
+        assert ((out[..., dims].double() - want[..., dims]).abs() <= tol[..., dims]).all()
+    assert ((out[:20, :, 24:28].double() - want[:20, :, 24:28]).abs() <= tol[:20, :, 24:28]).all()

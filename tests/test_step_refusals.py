@@ -51,6 +51,15 @@ def test_chunk_attention_refusals(kw, want):
     assert status(N.lib().tlh_chunk_attention, C.byref(chunk(**kw)), P, BIG, None)[0] == want
 
 
+@pytest.mark.parametrize("value", [-1, 2, 1 << 30])
+def test_f16_weights_is_one_or_the_other(value):
+    st, text = status(N.lib().tlh_chunk_attention, C.byref(chunk(f16_weights=value)), P, BIG, None)
+    assert st == "INVALID" and "f16_weights" in text
+    n = C.c_size_t()
+    assert status(N.lib().tlh_chunk_attention_scratch_bytes, C.byref(chunk(f16_weights=value)), C.byref(n))[0] == "INVALID"
+    assert chunk_size(f16_weights=1) == chunk_size(f16_weights=0)
+
+
 def chunk_size(**kw):
     n = C.c_size_t()
     assert status(N.lib().tlh_chunk_attention_scratch_bytes, C.byref(chunk(**kw)), C.byref(n))[0] == "OK"
