@@ -20,8 +20,8 @@
 // took off (22 bits in all): a result is off by 2.07e-4 of its size, all of it its own rounding,
 // instead of 2.9e-4. With few rows the tiles wait for HBM, and 32 sequences decoding take 113 us
 // with it and without. With many the products are the bound, so there a caller may choose to do
-// without (us, with it and without: 2048 over 16384 with heads of 64 544, 387; 128 840, 643; 192
-// 636, 482; 256 590, 514; 31 tokens + 600 148, 143; 9 x 13..701 52.3, 47.7).
+// without (us, with it and without: 2048 over 16384 with heads of 64 513, 386; 128 826, 644; 192
+// 627, 481; 256 577, 514; 31 tokens + 600 150, 144; 9 x 13..701 51.6, 47.5).
 //
 // Items differ by orders of magnitude in keys, and only the device knows the lengths. So
 // every workgroup works out the same plan from them: how many tiles a workgroup takes
@@ -35,9 +35,9 @@
 // Measured, 32/8 heads of 128 unless said, with inputs that were just used and with others each
 // time: 1 token over 1500 10.3 and 13.4 us, the plan and one chain of latencies; 32 sequences
 // decoding over 512..8192 113 us (4.9 TB/s over random pages); 31 of those beside a piece of 600
-// tokens 148 to 160 and 199 us; 2048 over 16384 840 to 863 and 886 us, the three products at 1.02
-// to 1.04 PFLOP/s, nearly a large library product's rate (1.09); nine pieces of 13..701 with 4/1
-// heads of 256 and a window of 1024 52 to 54 and 56 us (one wave a SIMD).
+// tokens 150 to 162 and 198 us; 2048 over 16384 826 to 835 and 879 us, the three products at 1.0
+// to 1.06 PFLOP/s, nearly a large library product's rate (1.09); nine pieces of 13..701 with 4/1
+// heads of 256 and a window of 1024 52 to 53 and 56 us (one wave a SIMD).
 #include <algorithm>
 #include <type_traits>
 
@@ -691,7 +691,6 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
         }
         ca_stream<KF, BATCH>(T + 16 * lane, [&](int f, uint4 k) { S[f / NS] = mfma32<false>(k, qf[f % NS], S[f / NS]); });
         if (!whole) {
-            w.some_masked = true;
             int k = k0;
             asm volatile("" : "+s"(k));  // the masks formed here, not before every tile
 #pragma unroll
@@ -817,9 +816,9 @@ __device__ __forceinline__ void ca_many(const CaArgs &a, const CaSeq &sq, const 
 // of the careful pass: heads of 192, 16/4, f16_weights, with one and two, us: 2048 over 16384 861,
 // 485; nine pieces of 13..701 behind up to 5000 256, 182; 32 decoding over 512..8192 110, 91; 8 x
 // 12 tokens over 2000 34, 32). Pages of 8 keep a tile's page ids in memory of the lane's own, in
-// the loops too: 2048 over 16384, heads of 128, 922 us where pages of 16 take 840; 32 decoding 151
-// and 113. (Three workgroups a CU at 64 dims: 2048 over 16384 525 instead of 544, but 451 instead
-// of 387 with f16_weights.)
+// the loops too: 2048 over 16384, heads of 128, 893 us where pages of 16 take 826; 32 decoding 151
+// and 113. (Three workgroups a CU at 64 dims gained 4% of 2048 over 16384 and lost 16% of it with
+// f16_weights.)
 template <int D, int BS>
 __global__ void __launch_bounds__(64 * CA_WAVES, D <= 192 ? 2 : 1) k_chunk_attn(const CaArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t T0[CaLds<D>::HALF], T1[CaLds<D>::HALF], aux[CaLds<D>::AUX];
