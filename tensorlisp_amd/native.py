@@ -902,8 +902,8 @@ CHUNK_COUNTER_BYTES = 8192
 class ChunkAttention(_ScratchNode):
     """Causal attention of the sequences' new tokens over the paged cache, one or thousands a sequence, with its
     scratch, launched many times; window > 0: a token sees the last `window` tokens up to itself. f16_weights: sequences
-    with more than 64 rows of q a kv head round the softmax's weights to f16 before they meet v, as packed and tree
-    attention do (less exact, and a quarter faster where many rows see long contexts). A call takes up to
+    with more than 64 rows of q a kv head round the softmax's weights to f16 before they meet v, as tree
+    attention does (less exact, and a quarter faster where many rows see long contexts). A call takes up to
     num_seqs sequences and num_rows new tokens in all, at most max_rows of one sequence; calls of one object must be
     stream-ordered (they share the scratch). One made while a graph is captured is for captured calls alone: each
     clears the counters in its own graph."""
@@ -1103,7 +1103,8 @@ class DraftVerify(_ScratchNode):
     def __call__(self, target, draft, tokens, draft_starts, temperatures, accept_at, sample_at, accepted, out_tokens,
                  accept_probs=None, stream=None):
         """target (drafts + sequences, vocab): sequence s has the rows of its n drafted tokens and one more, from
-        draft_starts[s] + s on; draft (drafts, vocab) or None; tokens i32 (drafts,), draft_starts i32 (sequences + 1,),
+        draft_starts[s] + s on; draft (drafts, vocab) or None; tokens i32 (drafts,), draft_starts i32 (sequences + 1,)
+        (a sequence that shares drafts with another is not verified: 0 accepted, tokens -1, probabilities NaN),
         temperatures f32 (sequences,) (0: greedy), accept_at f32 (drafts,) and sample_at f32 (sequences,) uniform in
         [0, 1) -> accepted i32 (sequences,), out_tokens i32 (sequences, max_drafts + 1): the accepted tokens, the next
         one, -1 behind; accept_probs f32 (drafts,) or None."""
