@@ -1329,13 +1329,13 @@ tlh_status tlh_chunk_attention(const tlh_chunk_attention_args *a, void *scratch,
                 {"k_cache", a->k_cache, pool},
                 {"v_cache", a->v_cache, pool}};
     for (int i = 0; i < 3; ++i)
-        if (rest[i].bytes > 0 && overlap(a->out, all, rest[i].p, rest[i].bytes))
+        if (rest[i].p && rest[i].bytes > 0 && overlap(a->out, all, rest[i].p, rest[i].bytes))
             return set_error(TLH_INVALID, "chunk_attention: out overlaps %s", rest[i].name);
     const size_t need = chunk_attention_scratch_bytes(*a);
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return set_error(TLH_INVALID, "chunk_attention: scratch of %zu bytes, need %zu, 16-byte aligned", scratch_bytes, need);
     for (const auto &x : rest)
-        if (need > 0 && x.bytes > 0 && overlap(scratch, need, x.p, x.bytes))
+        if (need > 0 && x.p && x.bytes > 0 && overlap(scratch, need, x.p, x.bytes))
             return set_error(TLH_INVALID, "chunk_attention: %s overlaps the scratch", x.name);
     return launch_chunk_attention(*a, scratch, (hipStream_t)stream);
 }
